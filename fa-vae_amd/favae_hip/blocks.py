@@ -1,0 +1,350 @@
+"""The operators of a residual block: group norm with an activation (channels last), matrix product with bias, activation and
+residual in its epilogue, both with their gradients, and activations kept for the backward pass in 8 bits (csrc/groupnorm.hip,
+linear.hip, ckpt8.hip).
+
+    y, mean, rstd, x8 = group_norm_act(x, groups, gamma, beta, act="silu", ckpt=True)
+    out, pre          = linear_act(y, w, bias, act="gelu_tanh", residual=r, save_pre=True)
+    y8, pre8          = ckpt8_pack(y), ckpt8_pack(pre)                       # y and pre need not be kept
+    dy, dw, db        = linear_act_bwd(dout, y8, w, act="gelu_tanh", pre=pre8)   # the gradient of r is dout
+    dx, dgamma, dbeta = group_norm_act_bwd(dy, x8, groups, gamma, beta, mean, rstd, act="silu")
+
+Tensors are fp32 or bf16 (one type per call), scale, shift, bias and statistics fp32.  Every call is asynchronous on the current
+stream of its tensors' device, may be captured into a graph, and takes its workspace from torch's allocator on that stream.
+Activations: "none", "lrelu" (slope 0.01), "silu", "gelu_tanh".  Wrong arguments raise ValueError or TypeError before anything is
+launched; there is no CPU fallback.
+"""
+import ctypes
+
+import torch
+
+from . import lib as L
+
+_raw = L.raw()
+_p, _ll, _i, _sz = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_size_t
+_raw.favae_ckpt8_pack.argtypes = [_p, _ll, _ll, _i, _p, _ll, _p, _ll, _i, _p]
+_raw.favae_ckpt8_unpack.argtypes = [_p, _ll, _p, _ll, _ll, _i, _p, _ll, _i, _p]
+_raw.favae_gn_act_scratch.argtypes = [_ll, _ll, _i, _i, _i, _i]
+_raw.favae_gn_act_scratch.restype = _sz
+_raw.favae_gn_act_fwd.argtypes = [_p, _ll, _ll, _ll, _ll, _i, _i, _p, _p, ctypes.c_float, _i, _p, _ll, _ll, _p, _p, _p, _sz, _i, _p]
+_raw.favae_gn_act_bwd.argtypes = [_p, _ll, _ll, _p, _ll, _ll, _p, _p, _ll, _ll, _i, _i, _p, _p, _p, _p, _i, _p, _ll, _ll, _p, _p, _p, _sz,
+                                  _i, _p]
+_raw.favae_linear_act_fwd_scratch.argtypes = [_ll, _i, _i, _i]
+_raw.favae_linear_act_fwd_scratch.restype = _sz
+_raw.favae_linear_act_fwd.argtypes = [_p, _ll, _p, _ll, _p, _p, _ll, _p, _ll, _p, _ll, _ll, _i, _i, _i, _p, _sz, _i, _p]
+_raw.favae_linear_act_bwd_scratch.argtypes = [_ll, _i, _i, _i, _i]
+_raw.favae_linear_act_bwd_scratch.restype = _sz
+_raw.favae_linear_act_bwd.argtypes = [_p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _ll, _ll, _i, _i, _i, _p, _ll, _p, _ll, _i, _p, _p, _sz,
+                                      _i, _p]
+
+ACTS = {"none": 0, "lrelu": 1, "silu": 2, "gelu_tanh": 3}
+CKPT_BLOCK = 32
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+class Ckpt8:
+    """An activation in 8 bits: q int8 [..., C] and e uint8 [..., ceil(C / 32)], value = q * 2^(e - 127); dtype is the type it was
+    packed from.  A decoded value is exact in bf16.  A block of 32 channels that held an infinity or a NaN decodes to NaN."""
+
+    __slots__ = ("q", "e", "dtype")
+
+    def __init__(self, q, e, dtype):
+        if q.dtype != torch.int8 or e.dtype != torch.uint8:
+            raise TypeError("Ckpt8: q is int8 and e is uint8")
+        if dtype not in (F32, BF16):
+            raise TypeError("Ckpt8: dtype is float32 or bfloat16")
+        if q.dim() < 1 or e.shape != q.shape[:-1] + ((q.shape[-1] + CKPT_BLOCK - 1) // CKPT_BLOCK,):
+            raise ValueError("Ckpt8: e has the shape of q with ceil(C / 32) in place of C")
+        if q.device != e.device or not (q.is_contiguous() and e.is_contiguous()):
+            raise ValueError("Ckpt8: q and e are contiguous and on one device")
+        self.q, self.e, self.dtype = q, e, dtype
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    @property
+    def device(self):
+        return self.q.device
+
+
+# ---- arguments -----------------------------------------------------------------------------------------------------------
+def _code(t, name):
+    if t.dtype == F32:
+        return L.F32
+    if t.dtype == BF16:
+        return L.BF16
+    raise TypeError("%s: float32 or bfloat16, not %s" % (name, t.dtype))
+
+
+def _act(name):
+    if name not in ACTS:
+        raise ValueError("act: one of %s, not %r" % (", ".join(sorted(ACTS)), name))
+    return ACTS[name]
+
+
+def _rows(t, name):
+    """Stride between the rows of t seen as [R, C]; its leading dimensions must collapse and its last one be contiguous."""
+    if t.dim() < 1:
+        raise ValueError("%s: a tensor of at least one dimension" % name)
+    if t.is_contiguous():
+        return t.shape[-1]
+    sh, st = t.shape, t.stride()
+    if 0 in sh:
+        return sh[-1]
+    if sh[-1] > 1 and st[-1] != 1:
+        raise ValueError("%s: the last dimension must be contiguous" % name)
+    ld, span = None, 1
+    for n, s in zip(reversed(sh[:-1]), reversed(st[:-1])):
+        if n == 1:
+            continue
+        if ld is None:
+            ld = s
+        elif s != ld * span:
+            raise ValueError("%s: its leading dimensions are not one run of rows" % name)
+        span *= n
+    if ld is None:
+        return sh[-1]
+    if ld < sh[-1]:
+        raise ValueError("%s: its rows overlap" % name)
+    return ld
+
+
+def _maps(t, name):
+    """(sample stride, position stride) of t [N, ..., C]; the middle dimensions must be one run of positions."""
+    c = t.shape[-1]
+    if t.is_contiguous() or t.numel() == 0:
+        s = 1
+        for n in t.shape[1:-1]:
+            s *= n
+        return s * c, c
+    pos = _rows(t[0], name)
+    return (t.stride(0) if t.shape[0] > 1 else 0), pos
+
+
+def _vec(t, n, name, dev):
+    if t.dtype != F32 or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError("%s: float32 [%d]" % (name, n))
+    if t.device != dev or not t.is_contiguous():
+        raise ValueError("%s: contiguous and on the device of the call" % name)
+    return t.data_ptr()
+
+
+def _on(dev, **tensors):
+    if dev.type != "cuda":
+        raise ValueError("tensors must be on the GPU; there is no CPU fallback")
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError("%s is on %s, the call is on %s" % (name, t.device, dev))
+
+
+def _span(t):
+    """First and one-past-last byte that t can touch."""
+    if t.numel() == 0:
+        return 0, 0
+    n = 1 + sum((k - 1) * s for k, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _same_place(a, b):
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
+
+
+def _apart(out, name, ins, may_be=None):
+    """`out` shares no memory with the inputs, but that it may be `may_be` itself."""
+    lo, hi = _span(out)
+    for t in ins:
+        if t is None or (t is may_be and _same_place(out, t)):
+            continue
+        a, b = _span(t)
+        if lo < b and a < hi:
+            raise ValueError("%s overlaps an input" % name)
+
+
+def _out(out, name, shape, dtype, dev, ins, may_be=None):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if out.dtype != dtype or out.shape != torch.Size(shape) or out.device != dev:
+        raise ValueError("%s: %s %s on %s" % (name, dtype, list(shape), dev))
+    _apart(out, name, ins, may_be)
+    return out
+
+
+def _call(dev, fn, *args):
+    """fn(*args, stream) on the current stream of `dev`, whichever device is current."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    L.check(rc)
+
+
+def _scratch(nbytes, dev):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# ---- 8-bit activations ---------------------------------------------------------------------------------------------------
+def ckpt8_pack(x):
+    """x [..., C] (fp32 or bf16, rows of any stride) -> Ckpt8."""
+    code, ld, dev = _code(x, "x"), _rows(x, "x"), x.device
+    _on(dev)
+    c = x.shape[-1]
+    nb = (c + CKPT_BLOCK - 1) // CKPT_BLOCK
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    e = torch.empty(x.shape[:-1] + (nb,), dtype=torch.uint8, device=dev)
+    if x.numel():
+        _call(dev, _raw.favae_ckpt8_pack, x.data_ptr(), ld, x.numel() // c, c, q.data_ptr(), c, e.data_ptr(), nb, code)
+    return Ckpt8(q, e, x.dtype)
+
+
+def ckpt8_unpack(ck, dtype=None, out=None):
+    """The values of a checkpoint, in the type it was packed from or in `dtype`; out: rows of any stride."""
+    dtype = ck.dtype if dtype is None and out is None else out.dtype if dtype is None else dtype
+    if dtype not in (F32, BF16):
+        raise TypeError("dtype: float32 or bfloat16")
+    dev = ck.device
+    _on(dev)
+    out = _out(out, "out", ck.shape, dtype, dev, (ck.q, ck.e))
+    c = ck.shape[-1]
+    if out.numel():
+        _call(dev, _raw.favae_ckpt8_unpack, ck.q.data_ptr(), c, ck.e.data_ptr(), ck.e.shape[-1], out.numel() // c, c, out.data_ptr(),
+              _rows(out, "out"), _code(out, "out"))
+    return out
+
+
+# ---- group norm ----------------------------------------------------------------------------------------------------------
+def _gn_sizes(shape, groups):
+    if len(shape) < 2:
+        raise ValueError("x: [N, ..., C]")
+    n, c = shape[0], shape[-1]
+    if not isinstance(groups, int) or groups < 1 or c < 1 or c % groups:
+        raise ValueError("groups: a divisor of the %d channels, not %r" % (c, groups))
+    s = 1
+    for k in shape[1:-1]:
+        s *= k
+    return n, s, c
+
+
+def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out=None):
+    """y = act(gamma * (x - mean) * rstd + beta) over x [N, ..., C], channels last, per sample and group of C / groups neighbouring
+    channels.  Returns y, mean [N, groups], rstd [N, groups] (fp32) and, with ckpt, x as a Ckpt8.  A sample of no positions has mean
+    0 and variance 0.  out may be x (without ckpt)."""
+    n, s, c = _gn_sizes(x.shape, groups)
+    code, a, dev = _code(x, "x"), _act(act), x.device
+    _on(dev)
+    g, b = _vec(gamma, c, "gamma", dev), _vec(beta, c, "beta", dev)
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError("eps: not negative")
+    xn, xs = _maps(x, "x")
+    y = _out(out, "out", x.shape, x.dtype, dev, (x, gamma, beta), None if ckpt else x)
+    yn, ys = _maps(y, "out")
+    stats = torch.empty(2, n, groups, dtype=F32, device=dev)
+    mean, rstd = stats[0], stats[1]
+    if n:
+        nbytes = _raw.favae_gn_act_scratch(n, s, c, groups, 0, code)
+        ws = _scratch(nbytes, dev)
+        _call(dev, _raw.favae_gn_act_fwd, x.data_ptr(), xn, xs, n, s, c, groups, g, b, eps, a, y.data_ptr(), yn, ys, mean.data_ptr(),
+              rstd.data_ptr(), _ptr(ws), nbytes, code)
+    return (y, mean, rstd, ckpt8_pack(x)) if ckpt else (y, mean, rstd)
+
+
+def group_norm_act_bwd(dy, x, groups, gamma, beta, mean, rstd, act="none", out=None):
+    """Gradients of group_norm_act: dx (dy's type), dgamma, dbeta (fp32 [C]).  x: the forward's input or its Ckpt8; mean and rstd as
+    the forward returned them.  out may be dy."""
+    n, s, c = _gn_sizes(dy.shape, groups)
+    code, a, dev = _code(dy, "dy"), _act(act), dy.device
+    ck = isinstance(x, Ckpt8)
+    if x.shape != dy.shape or x.dtype != dy.dtype:
+        raise ValueError("x: %s %s, as dy" % (dy.dtype, list(dy.shape)))
+    _on(dev, x=x, mean=mean, rstd=rstd)
+    g, b = _vec(gamma, c, "gamma", dev), _vec(beta, c, "beta", dev)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t.dtype != F32 or t.shape != (n, groups) or not t.is_contiguous():
+            raise ValueError("%s: contiguous float32 [%d, %d]" % (name, n, groups))
+    dn, ds = _maps(dy, "dy")
+    xn, xs = (0, 0) if ck else _maps(x, "x")
+    dx = _out(out, "out", dy.shape, dy.dtype, dev, (dy, x.q, x.e, gamma, beta, mean, rstd) if ck else (dy, x, gamma, beta, mean, rstd), dy)
+    dxn, dxs = _maps(dx, "out")
+    grads = torch.empty(2, c, dtype=F32, device=dev)
+    nbytes = _raw.favae_gn_act_scratch(n, s, c, groups, 1, code)
+    ws = _scratch(nbytes, dev)
+    _call(dev, _raw.favae_gn_act_bwd, dy.data_ptr(), dn, ds, None if ck else x.data_ptr(), xn, xs, x.q.data_ptr() if ck else None,
+          x.e.data_ptr() if ck else None, n, s, c, groups, g, b, mean.data_ptr(), rstd.data_ptr(), a, dx.data_ptr(), dxn, dxs,
+          grads[0].data_ptr(), grads[1].data_ptr(), _ptr(ws), nbytes, code)
+    return dx, grads[0], grads[1]
+
+
+# ---- matrix product ------------------------------------------------------------------------------------------------------
+def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=None):
+    """act(x w^T + bias) + residual: x [..., K], w [N, K], bias fp32 [N], residual and the result [..., N] of x's type, rows of any
+    stride.  Sums, bias, activation and residual are fp32, the result is rounded once.  With save_pre returns (y, pre), pre = x w^T +
+    bias rounded to x's type, for linear_act_bwd.  out may be residual."""
+    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError("x [..., K] and w [N, K], not %s and %s" % (list(x.shape), list(w.shape)))
+    code, a, dev = _code(x, "x"), _act(act), x.device
+    if w.dtype != x.dtype:
+        raise TypeError("w: %s, as x" % x.dtype)
+    _on(dev, w=w, residual=residual)
+    n, k = w.shape
+    m = 1
+    for v in x.shape[:-1]:
+        m *= v
+    shape = x.shape[:-1] + (n,)
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
+        raise ValueError("residual: %s %s" % (x.dtype, list(shape)))
+    bp = None if bias is None else _vec(bias, n, "bias", dev)
+    y = _out(out, "out", shape, x.dtype, dev, (x, w, bias, residual), residual)
+    pre = torch.empty(shape, dtype=x.dtype, device=dev) if save_pre else None
+    if m and n:
+        nbytes = _raw.favae_linear_act_fwd_scratch(m, n, k, code)
+        ws = _scratch(nbytes, dev)
+        _call(dev, _raw.favae_linear_act_fwd, x.data_ptr(), _rows(x, "x"), w.data_ptr(), _rows(w, "w"), bp, _ptr(residual),
+              0 if residual is None else _rows(residual, "residual"), _ptr(pre), n, y.data_ptr(), _rows(y, "out"), m, n, k, a, _ptr(ws), nbytes,
+              code)
+    return (y, pre) if save_pre else y
+
+
+def linear_act_bwd(dy, x, w, act="none", pre=None, need=("x", "w", "b"), dw=None):
+    """Gradients of linear_act: (dx, dw, db), None for what `need` leaves out.  x and pre: tensors or Ckpt8; pre is needed unless act
+    is "none".  dx [..., K] is of dy's type, dw [N, K] of w's type or, into a float32 `dw`, unrounded, db fp32 [N].  The gradient of
+    the residual is dy."""
+    code, a, dev = _code(dy, "dy"), _act(act), dy.device
+    if w.dim() != 2 or dy.dim() < 1 or dy.shape[-1] != w.shape[0] or x.shape != dy.shape[:-1] + (w.shape[1],):
+        raise ValueError("dy [..., N], x [..., K], w [N, K], not %s, %s, %s" % (list(dy.shape), list(x.shape), list(w.shape)))
+    if w.dtype != dy.dtype or x.dtype != dy.dtype:
+        raise TypeError("x and w: %s, as dy" % dy.dtype)
+    if not set(need) <= {"x", "w", "b"}:
+        raise ValueError("need: of 'x', 'w', 'b'")
+    if act == "none":
+        pre = None
+    elif pre is None:
+        raise ValueError("pre: the gradient of %s needs the pre-activation" % act)
+    elif pre.shape != dy.shape or pre.dtype != dy.dtype:
+        raise ValueError("pre: %s %s, as dy" % (dy.dtype, list(dy.shape)))
+    _on(dev, x=x, w=w, pre=pre)
+    n, k = w.shape
+    m = 1
+    for v in dy.shape[:-1]:
+        m *= v
+    xck, pck = isinstance(x, Ckpt8), isinstance(pre, Ckpt8)
+    if dw is not None and "w" in need:
+        if dw.dtype not in (F32, w.dtype) or dw.shape != w.shape or dw.device != dev:
+            raise ValueError("dw: float32 or %s, %s" % (w.dtype, list(w.shape)))
+        _apart(dw, "dw", (dy, w) + ((x.q, x.e) if xck else (x,)) + ((pre.q, pre.e) if pck else (pre,)))
+    dx = torch.empty(x.shape, dtype=dy.dtype, device=dev) if "x" in need else None
+    dw = None if "w" not in need else torch.empty(n, k, dtype=w.dtype, device=dev) if dw is None else dw
+    db = torch.empty(n, dtype=F32, device=dev) if "b" in need else None
+    nbytes = _raw.favae_linear_act_bwd_scratch(m, n, k, a, code)
+    ws = _scratch(nbytes, dev)
+    xp = x.q if xck else x
+    pp = pre.q if pck else pre
+    _call(dev, _raw.favae_linear_act_bwd, dy.data_ptr(), _rows(dy, "dy"), xp.data_ptr(), _rows(xp, "x"), x.e.data_ptr() if xck else None,
+          x.e.shape[-1] if xck else 0, w.data_ptr(), _rows(w, "w"), _ptr(pp), 0 if pp is None else _rows(pp, "pre"),
+          pre.e.data_ptr() if pck else None, pre.e.shape[-1] if pck else 0, m, n, k, a, _ptr(dx), k, _ptr(dw), k if dw is None else _rows(dw, "dw"),
+          L.F32 if dw is not None and dw.dtype == F32 else code, _ptr(db), _ptr(ws), nbytes, code)
+    return dx, dw, db

@@ -597,6 +597,53 @@ int favae_axpby(long long n, double a, const double* x, double b, const double* 
 /* out[N][Kn] = in[N][K][:, sel] (pruning of q.Z['mean'], cA/favae.py:507). */
 int favae_gather_cols(const double* in, int K, const int* sel, int Kn, double* out, long long N, void* stream);
 
+/* ---- residual block: group norm with an activation, linear with an epilogue, activations kept in 8 bits (no counterpart in the
+ * reference, whose blocks are BatchNorm + LeakyReLU and plain nn.Linear).  Nothing is allocated or synchronised; scratch comes from
+ * the caller, sized by the *_scratch function (bytes) for the same arguments, and belongs to one call at a time. ---------------- */
+#define FAVAE_ACT_NONE 0
+#define FAVAE_ACT_LRELU 1        /* slope 0.01 */
+#define FAVAE_ACT_SILU 2         /* z sigmoid(z) */
+#define FAVAE_ACT_GELU_TANH 3    /* z sigmoid(sqrt(8 / pi) (z + 0.044715 z^3)) */
+
+/* Activations in 8 bits: q [R][C] int8 and one byte e [R][ceil(C / 32)] per 32 channels of a row; value = q * 2^(e - 127).  The step
+ * is the least power of two >= 2^-126 on which no value of the block passes 127 steps (2^121 at most), q = round-half-even(x / step).
+ * A decoded value is exact in bf16.  A block that holds an infinity or a NaN has e = 255, q = 0 and decodes to NaN throughout.
+ * Row strides in elements (of e: bytes); dtype FAVAE_F32 or FAVAE_BF16 is that of x / out. */
+int favae_ckpt8_pack(const void* x, long long ldx, long long R, int C, void* q, long long ldq, void* e, long long lde, int dtype,
+                     void* stream);
+int favae_ckpt8_unpack(const void* q, long long ldq, const void* e, long long lde, long long R, int C, void* out, long long ldo,
+                       int dtype, void* stream);
+
+/* y = act(gamma (x - mean) rstd + beta) over x [N][S][C] in G groups of C / G neighbouring channels; mean, rstd [N][G] fp32 out,
+ * rstd = (population variance + eps)^-1/2.  Strides of a sample and of a position in elements, channels contiguous.  S = 0: mean 0,
+ * variance 0.  y may be x. */
+size_t favae_gn_act_scratch(long long N, long long S, int C, int G, int backward, int dtype);
+int favae_gn_act_fwd(const void* x, long long xn, long long xs, long long N, long long S, int C, int G, const float* gamma,
+                     const float* beta, float eps, int act, void* y, long long yn, long long ys, float* mean, float* rstd, void* scratch,
+                     size_t scratch_bytes, int dtype, void* stream);
+/* Its gradients from dy and either x or its checkpoint (q, e as above with R = N * S contiguous rows; mean and rstd stay those of the
+ * forward pass): dx (dtype; may be dy), dgamma and dbeta [C] fp32 (NULL to skip).  Deterministic. */
+int favae_gn_act_bwd(const void* dy, long long dn, long long ds, const void* x, long long xn, long long xs, const void* q, const void* e,
+                     long long N, long long S, int C, int G, const float* gamma, const float* beta, const float* mean, const float* rstd,
+                     int act, void* dx, long long dxn, long long dxs, float* dgamma, float* dbeta, void* scratch, size_t scratch_bytes,
+                     int dtype, void* stream);
+
+/* y = act(u) + residual, u = x w^T + bias: x [M][K], w [N][K], y, residual and pre [M][N] of dtype, bias [N] fp32; bias, residual and
+ * pre may be NULL.  pre receives u rounded to dtype.  Accumulation, bias, activation and residual in fp32, one rounding.  residual may
+ * be y.  Row strides in elements. */
+size_t favae_linear_act_fwd_scratch(long long M, int N, int K, int dtype);
+int favae_linear_act_fwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias, const void* residual,
+                         long long ldr, void* pre, long long ldpre, void* y, long long ldy, long long M, int N, int K, int act,
+                         void* scratch, size_t scratch_bytes, int dtype, void* stream);
+/* Its gradients: du = dy act'(pre) rounded to dtype, dx [M][K] = du w (dtype), dw [N][K] = du^T x (dw_dtype: fp32 or dtype), db [N]
+ * fp32 = column sums of du before its rounding; any of the three NULL to skip.  x and pre are tensors of dtype, or, with xe / pe
+ * given, 8-bit checkpoints (x / pre point to q).  pre is not read with act none.  The gradient of residual is dy.  Deterministic. */
+size_t favae_linear_act_bwd_scratch(long long M, int N, int K, int act, int dtype);
+int favae_linear_act_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* xe, long long ldxe, const void* w,
+                         long long ldw, const void* pre, long long ldpre, const void* pe, long long ldpe, long long M, int N, int K,
+                         int act, void* dx, long long lddx, void* dw, long long lddw, int dw_dtype, float* db, void* scratch,
+                         size_t scratch_bytes, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

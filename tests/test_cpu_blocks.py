@@ -1,0 +1,102 @@
+"""Refusals of the residual-block operators (favae_hip/blocks.py): wrong arguments raise before anything is launched, so they are
+checked here without a GPU; the C entry points report theirs through favae_last_error."""
+import pytest
+import torch
+
+
+def _b():
+    from favae_hip import blocks
+    return blocks
+
+
+def _gn(b, **kw):
+    a = dict(x=torch.zeros(2, 3, 8), groups=2, gamma=torch.ones(8), beta=torch.zeros(8))
+    a.update(kw)
+    return b.group_norm_act(**a)
+
+
+@pytest.mark.parametrize("kw,err", [
+    (dict(groups=3), ValueError), (dict(groups=0), ValueError), (dict(groups=2.0), ValueError), (dict(act="relu6"), ValueError),
+    (dict(x=torch.zeros(8)), ValueError), (dict(x=torch.zeros(2, 3, 8, dtype=torch.float16)), TypeError),
+    (dict(x=torch.zeros(2, 3, 8, dtype=torch.float64)), TypeError), (dict(), ValueError)])
+def test_group_norm_refusals(kw, err):
+    with pytest.raises(err):
+        _gn(_b(), **kw)
+
+
+def test_group_norm_bwd_refusals():
+    b = _b()
+    dy, g, st = torch.zeros(2, 3, 8), torch.ones(8), torch.zeros(2, 2)
+    for x in (torch.zeros(2, 4, 8), torch.zeros(2, 3, 8, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="as dy"):
+            b.group_norm_act_bwd(dy, x, 2, g, g, st, st)
+    ck = b.Ckpt8(torch.zeros(2, 3, 8, dtype=torch.int8), torch.zeros(2, 3, 1, dtype=torch.uint8), torch.bfloat16)
+    with pytest.raises(ValueError, match="as dy"):
+        b.group_norm_act_bwd(dy, ck, 2, g, g, st, st)
+
+
+def test_linear_refusals():
+    b = _b()
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    with pytest.raises(ValueError, match="GPU"):
+        b.linear_act(x, w)
+    for bad in (torch.zeros(6, 7), torch.zeros(8), torch.zeros(2, 6, 8)):
+        with pytest.raises(ValueError):
+            b.linear_act(x, bad)
+    with pytest.raises(TypeError):
+        b.linear_act(x, w.bfloat16())
+    with pytest.raises(ValueError, match="act"):
+        b.linear_act(x, w, act="tanh")
+    dy = torch.zeros(4, 6)
+    with pytest.raises(ValueError, match="pre"):
+        b.linear_act_bwd(dy, x, w, act="silu")
+    with pytest.raises(ValueError, match="pre"):
+        b.linear_act_bwd(dy, x, w, act="silu", pre=torch.zeros(4, 5))
+    with pytest.raises(ValueError, match="need"):
+        b.linear_act_bwd(dy, x, w, need=("r",))
+    with pytest.raises(ValueError):
+        b.linear_act_bwd(dy, torch.zeros(3, 8), w)
+    with pytest.raises(ValueError, match="GPU"):
+        b.linear_act_bwd(dy, x, w)
+
+
+def test_ckpt8_refusals():
+    b = _b()
+    i8, u8 = torch.int8, torch.uint8
+    q, e = torch.zeros(4, 40, dtype=i8), torch.zeros(4, 2, dtype=u8)
+    assert b.Ckpt8(q, e, torch.float32).shape == (4, 40)
+    for args, err in (((q.to(u8), e, torch.float32), TypeError), ((q, e, torch.float16), TypeError), ((q, e[:, :1], torch.float32), ValueError),
+                      ((q[:, :33].clone()[:, :32], e[:, :1], torch.float32), ValueError), ((q, torch.zeros(2, 4, dtype=u8).t(), torch.float32), ValueError)):
+        with pytest.raises(err):
+            b.Ckpt8(*args)
+    with pytest.raises(TypeError):
+        b.ckpt8_pack(torch.zeros(4, 8, dtype=torch.int32))
+    with pytest.raises(ValueError, match="GPU"):
+        b.ckpt8_pack(torch.zeros(4, 8))
+    with pytest.raises(TypeError):
+        b.ckpt8_unpack(b.Ckpt8(q, e, torch.float32), torch.float64)
+
+
+def test_row_strides():
+    b = _b()
+    t = torch.zeros(4, 6, 10)
+    assert b._rows(t, "t") == 10 and b._rows(t[:, :, :7], "t") == 10 and b._rows(t[:, 2, :5], "t") == 60 and b._rows(t[:1, :, 3:], "t") == 10
+    assert b._rows(t[0, 0, 2:5], "t") == 3 and b._maps(t[:, 1:4, :8], "t") == (60, 10) and b._maps(t[2:3, :, :8], "t") == (0, 10)
+    for bad in (t[:, :3], t.transpose(1, 2), t[:, :, ::2], torch.zeros(10).expand(4, 10), t.permute(1, 0, 2)):
+        with pytest.raises(ValueError):
+            b._rows(bad, "t")
+
+
+def test_c_entry_points_refuse_without_a_gpu():
+    b = _b()
+    from favae_hip import lib as L
+    r = b._raw
+    for call, text in ((lambda: r.favae_ckpt8_pack(None, 8, 4, 8, None, 8, None, 1, 0, None), "favae_ckpt8_pack"),
+                       (lambda: r.favae_ckpt8_pack(None, 8, -1, 8, None, 8, None, 1, 0, None), "bad sizes"),
+                       (lambda: r.favae_ckpt8_unpack(None, 8, None, 1, 4, 8, None, 8, 7, None), "dtype"),
+                       (lambda: r.favae_gn_act_fwd(None, 8, 8, 1, 1, 8, 3, None, None, 1e-5, 0, None, 8, 8, None, None, None, 0, 0, None), "groups"),
+                       (lambda: r.favae_gn_act_fwd(None, 8, 8, 1, 1, 8, 2, None, None, 1e-5, 9, None, 8, 8, None, None, None, 0, 0, None), "activation"),
+                       (lambda: r.favae_gn_act_bwd(None, 8, 8, None, 8, 8, None, None, 1, 1, 8, 2, None, None, None, None, 0, None, 8, 8, None, None, None, 0, 0, None), "null"),
+                       (lambda: r.favae_linear_act_fwd(None, 8, None, 8, None, None, 0, None, 0, None, 6, 4, 6, 8, 0, None, 0, 5, None), "dtype"),
+                       (lambda: r.favae_linear_act_bwd(None, 6, None, 8, None, 0, None, 8, None, 0, None, 0, 4, 6, 8, 0, None, 8, None, 8, 0, None, None, 0, 0, None), "dy")):
+        assert call() < 0 and text in L.last_error(), L.last_error()

@@ -1,0 +1,606 @@
+"""Residual-block operators (favae_hip/blocks.py) against plain fp64 formulas: group norm with an activation, matrix product with bias,
+activation and residual, their gradients, and 8-bit activation checkpoints.
+
+Bounds.  u = 2^-24 (half a step of fp32).  A stored value is off by half a step of its type.  Sums inside the kernels are trees over
+runs of at most a few hundred terms, so that a sum of t terms is off by at most SUM * u * sum|term| with SUM = 400 + (t's share of one
+lane, stated where it is larger); matrix products accumulate K terms in one chain: (K + 8) u sum|x w|.  The activations have slope at
+most 1.13 and curvature at most 1.2; their exp and reciprocal add (|z| + 8) 4 u of relative error."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+SUM = 400 * U
+F32, BF16, F64 = torch.float32, torch.bfloat16, torch.float64
+ACTS = ["none", "lrelu", "silu", "gelu_tanh"]
+SLOPE, CURVE = 1.13, 1.2
+
+
+def B():
+    from favae_hip import blocks
+    return blocks
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def act64(z, act):
+    if act == "none":
+        return z, torch.ones_like(z)
+    if act == "lrelu":
+        return torch.where(z > 0, z, 0.01 * z), torch.where(z > 0, 1.0, 0.01).to(z)
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    c = math.sqrt(8 / math.pi)
+    s = torch.sigmoid(c * (z + 0.044715 * z ** 3))
+    return z * s, s * (1 + z * (1 - s) * c * (1 + 0.134145 * z * z))
+
+
+def close(got, want, bound, dtype=None):
+    """|got - want| <= half a step of the stored type + bound, everywhere."""
+    assert got.shape == want.shape
+    lim = bound + half(dtype or got.dtype) * (want.abs() + bound) + 1e-37
+    bad = (got.double() - want).abs() - lim
+    assert not torch.isnan(got).any()
+    assert bad.numel() == 0 or bad.max() <= 0, (bad.max().item(), (got.double() - want).abs().max().item())
+
+
+def rnd(gen, *shape, dtype=F32, scale=1.0, shift=0.0):
+    return (torch.randn(*shape, generator=gen, device=DEV) * scale + shift).to(dtype)
+
+
+def gen(*key):
+    return torch.Generator(device=DEV).manual_seed(hash(tuple(int(k) for k in key)) % (1 << 31))
+
+
+# ---- 8-bit activations ---------------------------------------------------------------------------------------------------
+def ref_pack(x):
+    """The format from its definition, block by block, in fp64 on the host."""
+    x = x.double().cpu()
+    R, C = x.shape
+    nb = (C + 31) // 32
+    q, e = torch.zeros(R, C, dtype=torch.int8), torch.zeros(R, nb, dtype=torch.uint8)
+    for b in range(nb):
+        blk = x[:, 32 * b:32 * b + 32]
+        for r in range(R):
+            v = blk[r]
+            if not torch.isfinite(v).all():
+                e[r, b] = 255
+                continue
+            k = -126
+            while k < 121 and torch.round(v.abs().max() * 2.0 ** -k) > 127:
+                k += 1
+            q[r, 32 * b:32 * b + 32] = torch.round(v * 2.0 ** -k).clamp(-127, 127).to(torch.int8)
+            e[r, b] = k + 127
+    return q, e
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("R,C", [(1, 1), (3, 31), (5, 32), (2, 33), (7, 40), (4, 64), (3, 129), (33, 8), (2, 1024)])
+def test_ckpt8_is_the_format_bit_for_bit(R, C, dtype):
+    b = B()
+    x = rnd(gen(R, C), R, C, dtype=dtype) * torch.exp2(torch.randint(-40, 40, (R, 1), generator=gen(C, R), device=DEV).float()).to(dtype)
+    x[0, :min(C, 32)] = 0                                   # a block of zeros
+    ck = b.ckpt8_pack(x)
+    q, e = ref_pack(x)
+    assert torch.equal(ck.q.cpu(), q) and torch.equal(ck.e.cpu(), e)
+    want = q.double() * torch.exp2(e.double() - 127).repeat_interleave(32, 1)[:, :C]
+    for t in (F32, BF16):
+        assert torch.equal(b.ckpt8_unpack(ck, t).cpu().double(), want)      # decoded values are exact in both types
+    # no value is further than half a step of its block from what was packed, nor a step above 2^-6 of the block's largest
+    step = torch.exp2(e.double() - 127).repeat_interleave(32, 1)[:, :C]
+    assert ((want - x.double().cpu()).abs() <= 0.5 * step).all()
+
+
+def test_ckpt8_extremes_and_faults():
+    b = B()
+    big, tiny = torch.finfo(F32).max, 2.0 ** -149
+    x = torch.zeros(8, 64, device=DEV)
+    x[0, 3], x[0, 5] = big, -big
+    x[1, 0] = tiny
+    x[2, 0], x[2, 1] = 2.0 ** -126, 2.0 ** -127
+    x[3, 7] = float("inf")
+    x[4, 40] = float("nan")
+    x[5, 0], x[5, 1] = 127.5, 1.0                           # rounds to 128 steps of 1: the step is 2
+    x[6, 0], x[6, 1], x[6, 2] = 127.0, 0.5, 1.5             # ties to even: 0 and 2
+    x[7, 0] = -float("inf")
+    ck = b.ckpt8_pack(x)
+    q, e = ref_pack(x)
+    assert torch.equal(ck.q.cpu(), q) and torch.equal(ck.e.cpu(), e)
+    v = b.ckpt8_unpack(ck)
+    assert torch.isnan(v[3, :32]).all() and (v[3, 32:] == 0).all() and torch.isnan(v[4, 32:]).all() and torch.isnan(v[7, :32]).all()
+    assert torch.isfinite(v[0]).all() and v[0, 3] == 127 * 2.0 ** 121 and v[5, 0] == 128 and v[6, 1] == 0 and v[6, 2] == 2
+    assert torch.isfinite(b.ckpt8_unpack(ck, BF16)[0]).all()
+
+
+def test_ckpt8_strides_and_empty():
+    b = B()
+    wide = rnd(gen(1), 9, 100)
+    for x in (wide[:, 3:67], wide[:, 4:36], wide[::2, 8:72], wide.to(BF16)[:, 1:34], wide.view(3, 3, 100)[:, :, :64]):
+        ck, ref = b.ckpt8_pack(x), b.ckpt8_pack(x.contiguous())
+        assert torch.equal(ck.q, ref.q) and torch.equal(ck.e, ref.e)
+        out = torch.full(x.shape[:-1] + (x.shape[-1] + 5,), 7.0, device=DEV, dtype=x.dtype)
+        b.ckpt8_unpack(ck, out=out[..., 2:-3])
+        assert torch.equal(out[..., 2:-3], b.ckpt8_unpack(ref)) and (out[..., :2] == 7).all() and (out[..., -3:] == 7).all()
+    for shape in ((0, 8), (4, 0), (0,)):
+        x = torch.empty(shape, device=DEV)
+        assert b.ckpt8_unpack(b.ckpt8_pack(x)).shape == x.shape
+
+
+# ---- group norm ----------------------------------------------------------------------------------------------------------
+GN = [(1, 1, 1, 1), (2, 1, 8, 2), (3, 7, 10, 5), (1, 4, 1024, 32), (3, 64, 64, 8), (2, 4096, 64, 16), (5, 195, 210, 30), (700, 1, 64, 8),
+      (3, 2, 24, 24), (2, 9000, 16, 2), (1, 70000, 8, 1), (2, 5, 8192, 1), (1, 3, 4099, 1), (2, 300, 2050, 2), (4, 33, 33, 3), (130, 16, 256, 4)]
+
+
+def gn_ref(x, gamma, beta, G, act, eps=1e-5):
+    """y, mean, rstd in fp64, the bound of z's error, and z and xh."""
+    n, c = x.shape[0], x.shape[-1]
+    xg = x.double().reshape(n, -1, G, c // G)
+    mean = xg.mean((1, 3))
+    var = (xg - mean[:, None, :, None]).square().mean((1, 3))
+    rstd = (var + eps).rsqrt()
+    xh = ((xg - mean[:, None, :, None]) * rstd[:, None, :, None]).reshape(n, -1, c)
+    z = xh * gamma.double() + beta.double()
+    mean_err = SUM * xg.abs().mean((1, 3)) + U * mean.abs()
+    # the squared distances: relative SUM, and twice the mean's rounding against the spread
+    rstd_rel = SUM + 4 * U + mean_err.square() * rstd.square()
+    xh_err = (mean_err * rstd)[:, None, :, None].expand(xg.shape).reshape(n, -1, c) + xh.abs() * (rstd_rel[:, None, :, None].expand(xg.shape).reshape(n, -1, c) + 2 * U)
+    z_err = gamma.double().abs() * xh_err + 4 * U * (z.abs() + beta.double().abs())
+    return act64(z, act)[0], mean, rstd, z, z_err, mean_err, rstd_rel
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,S,C,G", GN)
+def test_group_norm_act(N, S, C, G, dtype):
+    b = B()
+    g = gen(N, S, C, G)
+    x = rnd(g, N, S, C, dtype=dtype, scale=1.7, shift=3.0)
+    gamma, beta = rnd(g, C, scale=0.3, shift=1.0), rnd(g, C, scale=0.5)
+    for act in ACTS:
+        y, mean, rstd = b.group_norm_act(x, G, gamma, beta, act=act)
+        want, m, r, z, z_err, m_err, r_rel = gn_ref(x, gamma, beta, G, act)
+        close(mean, m, m_err)
+        close(rstd, r, r * r_rel)
+        close(y, want, SLOPE * z_err + (z.abs() + 8) * 4 * U * want.abs())
+        assert y.dtype == dtype and mean.dtype == rstd.dtype == F32
+
+
+def gn_bwd_check(b, N, S, C, G, dtype, act, ck, g):
+    x = rnd(g, N, S, C, dtype=dtype, scale=1.7, shift=3.0)
+    dy = rnd(g, N, S, C, dtype=dtype)
+    gamma, beta = rnd(g, C, scale=0.3, shift=1.0), rnd(g, C, scale=0.5)
+    _, mean, rstd = b.group_norm_act(x, G, gamma, beta, act=act)
+    src = b.ckpt8_pack(x) if ck else x
+    xv = b.ckpt8_unpack(src, F32) if ck else x
+    dx, dg, db = b.group_norm_act_bwd(dy, src, G, gamma, beta, mean, rstd, act=act)
+    rep = lambda t: t.double().repeat_interleave(C // G, 1)[:, None, :]
+    ga, be = gamma.double(), beta.double()
+    d = xv.double() - rep(mean)
+    xh = d * rep(rstd)
+    xh_err = 2 * U * xh.abs()
+    z = xh * ga + be
+    z_err = ga.abs() * xh_err + 2 * U * (z.abs() + be.abs())
+    _, slope = act64(z, act)
+    dz = dy.double() * slope
+    dz_err = dy.double().abs() * (CURVE * z_err + (z.abs() + 8) * 4 * U) if act != "none" else torch.zeros_like(dz)
+    if act == "lrelu":                                       # within the rounding of z the kink may fall on either side
+        dz_err = dz_err + torch.where(z.abs() <= z_err, 0.99 * dy.double().abs(), 0.0)
+    close(db, dz.sum((0, 1)), dz_err.sum((0, 1)) + SUM * dz.abs().sum((0, 1)))
+    close(dg, (dz * xh).sum((0, 1)), (dz_err * xh.abs() + dz.abs() * xh_err).sum((0, 1)) + SUM * (dz * xh).abs().sum((0, 1)))
+    grp = lambda t: t.sum(1).reshape(N, G, C // G).sum(2)
+    m = S * (C // G)
+    s1, s2 = grp(ga * dz), grp(ga * dz * xh)
+    s1_err = grp(ga.abs() * dz_err) + SUM * grp((ga * dz).abs())
+    s2_err = grp(ga.abs() * (dz_err * xh.abs() + dz.abs() * xh_err)) + SUM * grp((ga * dz * xh).abs())
+    want = rep(rstd) * (ga * dz - (rep(s1) + xh * rep(s2)) / m)
+    size = rep(rstd) * ((ga * dz).abs() + (rep(s1).abs() + (xh * rep(s2)).abs()) / m)
+    err = rep(rstd) * (ga.abs() * dz_err + (rep(s1_err) + xh.abs() * rep(s2_err) + xh_err * rep(s2).abs()) / m) + 6 * U * size
+    close(dx, want, err)
+    assert dx.dtype == dtype and dg.dtype == db.dtype == F32
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,S,C,G", GN)
+def test_group_norm_act_bwd(N, S, C, G, dtype):
+    for act in ACTS:
+        for ck in (False, True):
+            gn_bwd_check(B(), N, S, C, G, dtype, act, ck, gen(N, S, C, G, ck))
+
+
+def test_group_norm_gradients_against_differences():
+    """dx, dgamma, dbeta of the kernels against central differences of the fp64 forward formula along random directions."""
+    b = B()
+    g = gen(42)
+    N, S, C, G = 2, 12, 24, 4
+    x, dy = rnd(g, N, S, C), rnd(g, N, S, C)
+    gamma, beta = rnd(g, C, scale=0.3, shift=1.0), rnd(g, C, scale=0.5)
+    for act in ("none", "silu", "gelu_tanh"):
+        _, mean, rstd = b.group_norm_act(x, G, gamma, beta, act=act)
+        grads = b.group_norm_act_bwd(dy, x, G, gamma, beta, mean, rstd, act=act)
+        f = lambda t: (gn_ref(t[0], t[1], t[2], G, act)[0] * dy.double()).sum()
+        args = [x.double(), gamma.double(), beta.double()]
+        for k in range(3):
+            v = torch.randn(args[k].shape, generator=g, device=DEV, dtype=F64)
+            up, dn = list(args), list(args)
+            h = 1e-5
+            up[k], dn[k] = args[k] + h * v, args[k] - h * v
+            diff = (f(up) - f(dn)) / (2 * h)
+            # third derivative times h^2 is below 1e-8; the kernels' fp32 sums: SUM of the absolute terms
+            assert abs((grads[k].double() * v).sum() - diff) <= 1e-7 * (grads[k].double() * v).abs().sum() + SUM * (dy.double().abs().sum() * v.abs().max())
+
+
+def test_group_norm_layouts_in_place_and_empty():
+    b = B()
+    g = gen(7)
+    big = rnd(g, 3, 10, 12, 48, dtype=BF16)
+    gamma, beta = rnd(g, 32), rnd(g, 32)
+    for x in (big[:, :, :, :32], big[:, :, :, 5:37], big[:, 2:3, :, 8:40], big[1:2, :, :, 16:48]):
+        dy = rnd(g, *x.shape, dtype=BF16)
+        y, m, r = b.group_norm_act(x, 4, gamma, beta, act="silu")
+        y2, m2, r2 = b.group_norm_act(x.contiguous(), 4, gamma, beta, act="silu")
+        close(y, y2.double(), half(BF16) * y2.double().abs())        # another vector width sums in another order
+        out = torch.full(x.shape[:-1] + (40,), 9.0, dtype=BF16, device=DEV)
+        b.group_norm_act(x, 4, gamma, beta, act="silu", out=out[..., 4:36])
+        assert torch.equal(out[..., 4:36], y) or (out[..., 4:36].float() - y.float()).abs().max() <= 2 ** -7 * y.float().abs().max()
+        assert (out[..., :4] == 9).all() and (out[..., 36:] == 9).all()
+        dx = b.group_norm_act_bwd(dy, x, 4, gamma, beta, m, r, act="silu")[0]
+        dx2 = b.group_norm_act_bwd(dy, x.contiguous(), 4, gamma, beta, m, r, act="silu")[0]
+        assert (dx.float() - dx2.float()).abs().max() <= 2 ** -7 * dx2.float().abs().max()
+    # a channels_last convolution output is a view of this layout
+    nchw = rnd(g, 2, 32, 5, 6).to(memory_format=torch.channels_last)
+    y, _, _ = b.group_norm_act(nchw.permute(0, 2, 3, 1), 8, gamma, beta, act="lrelu")
+    want = gn_ref(nchw.permute(0, 2, 3, 1).contiguous(), gamma, beta, 8, "lrelu")
+    close(y.reshape(2, 30, 32), want[0], SLOPE * want[4] + 8 * U * want[0].abs())
+    # in place, forward and backward
+    x = rnd(g, 4, 50, 32)
+    dy = rnd(g, 4, 50, 32)
+    y, m, r = b.group_norm_act(x, 4, gamma, beta, act="gelu_tanh")
+    xi, di = x.clone(), dy.clone()
+    assert b.group_norm_act(xi, 4, gamma, beta, act="gelu_tanh", out=xi)[0] is xi and torch.equal(xi, y)
+    dx = b.group_norm_act_bwd(dy, x, 4, gamma, beta, m, r, act="gelu_tanh")[0]
+    assert torch.equal(b.group_norm_act_bwd(di, x, 4, gamma, beta, m, r, act="gelu_tanh", out=di)[0], dx)
+    # nothing in, nothing out
+    y, m, r = b.group_norm_act(torch.empty(0, 5, 32, device=DEV), 4, gamma, beta)
+    assert y.shape == (0, 5, 32) and m.shape == (0, 4)
+    e = torch.empty(3, 0, 32, device=DEV)
+    y, m, r = b.group_norm_act(e, 4, gamma, beta)
+    assert y.shape == e.shape and (m == 0).all() and torch.allclose(r, torch.full_like(r, 1e-5 ** -0.5))
+    for t in (e, torch.empty(0, 5, 32, device=DEV)):
+        st = torch.zeros(t.shape[0], 4, device=DEV)
+        dx, dg, db = b.group_norm_act_bwd(t, t, 4, gamma, beta, st, st)
+        assert dx.shape == t.shape and (dg == 0).all() and (db == 0).all()
+    # a constant group: variance 0
+    y, m, r = b.group_norm_act(torch.full((2, 9, 32), 5.0, device=DEV), 4, gamma, beta)
+    assert (m == 5).all() and torch.equal(y, beta.expand(2, 9, 32))
+
+
+def test_group_norm_far_mean_and_nan_stays_in_its_group():
+    b = B()
+    g = gen(8)
+    x = rnd(g, 2, 500, 32, scale=0.01, shift=1000.0)         # spread 1e-5 of the mean: squares minus square of the mean would be noise
+    gamma, beta = torch.ones(32, device=DEV), torch.zeros(32, device=DEV)
+    y, m, r = b.group_norm_act(x, 4, gamma, beta, eps=0.0)
+    xg = x.double().reshape(2, 500, 4, 8)
+    sd = xg.var((1, 3), unbiased=False).sqrt()
+    m_err = (SUM + U) * xg.abs().mean((1, 3))
+    assert ((r.double() * sd - 1).abs() <= SUM + (m_err / sd) ** 2).all()
+    x[0, 3, 9] = float("nan")
+    x[1, 4, 0] = float("inf")
+    y, m, r = b.group_norm_act(x, 4, gamma, beta)
+    bad = torch.zeros(2, 500, 32, dtype=torch.bool, device=DEV)
+    bad[0, :, 8:16] = True
+    bad[1, :, 0:8] = True
+    assert torch.isnan(y[bad]).all() and torch.isfinite(y[~bad]).all()
+
+
+def test_group_norm_forward_checkpoint_is_the_input_packed():
+    b = B()
+    x = rnd(gen(3), 5, 65, 96, dtype=BF16)
+    gamma, beta = torch.ones(96, device=DEV), torch.zeros(96, device=DEV)
+    y, m, r, ck = b.group_norm_act(x, 8, gamma, beta, act="silu", ckpt=True)
+    y2, m2, r2 = b.group_norm_act(x, 8, gamma, beta, act="silu")
+    ref = b.ckpt8_pack(x)
+    assert torch.equal(ck.q, ref.q) and torch.equal(ck.e, ref.e) and torch.equal(y, y2) and torch.equal(m, m2) and torch.equal(r, r2)
+
+
+# ---- matrix product ------------------------------------------------------------------------------------------------------
+LIN = [(1, 1, 1), (1, 4096, 64), (3, 7, 5), (2, 20, 200), (64, 128, 4096), (129, 130, 65), (200, 33, 523), (130, 256, 64), (256, 384, 192), (1000, 8, 16),
+       (17, 300, 8), (5, 1000, 1031), (16, 512, 1024), (40, 264, 520)]      # M, N, K
+
+
+def lin_bound(x, w, bias):
+    k = x.shape[-1]
+    return (k + 8) * U * (x.double().abs() @ w.double().abs().t()) + 2 * U * bias.double().abs()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", LIN)
+def test_linear_act(M, N, K, dtype):
+    b = B()
+    g = gen(M, N, K)
+    x, w = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype, scale=K ** -0.5)
+    bias, res = rnd(g, N, scale=0.3), rnd(g, M, N, dtype=dtype)
+    for act in ACTS:
+        for with_bias, with_res, save in ((True, True, True), (False, False, False), (True, False, False)):
+            bb = bias if with_bias else torch.zeros_like(bias)
+            got = b.linear_act(x, w, bias if with_bias else None, act=act, residual=res if with_res else None, save_pre=save)
+            u = x.double() @ w.double().t() + bb.double()
+            u_err = lin_bound(x, w, bb)
+            v = act64(u, act)[0]
+            err = SLOPE * u_err + (u.abs() + 8) * 4 * U * v.abs()
+            if with_res:
+                v = v + res.double()
+                err = err + U * v.abs()
+            if save:
+                got, pre = got
+                close(pre, u, u_err)
+            close(got, v, err)
+            assert got.dtype == dtype
+
+
+def lin_bwd_check(b, M, N, K, dtype, act, ck, g, dw_dtype=None):
+    x, w, dy = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype, scale=K ** -0.5), rnd(g, M, N, dtype=dtype)
+    pre = rnd(g, M, N, dtype=dtype, scale=2.0)
+    xs, ps = (b.ckpt8_pack(x), b.ckpt8_pack(pre)) if ck else (x, pre)
+    xv, pv = (b.ckpt8_unpack(xs, F32).double(), b.ckpt8_unpack(ps, F32).double()) if ck else (x.double(), pre.double())
+    buf = torch.full((N, K), float("nan"), dtype=dw_dtype, device=DEV) if dw_dtype else None
+    dx, dw, db = b.linear_act_bwd(dy, xs, w, act=act, pre=None if act == "none" else ps, dw=buf)
+    slope = act64(pv, act)[1]
+    du = dy.double() * slope
+    du_err = dy.double().abs() * (pv.abs() + 8) * 4 * U if act != "none" else torch.zeros_like(du)
+    close(db, du.sum(0), du_err.sum(0) + (SUM + (M / 256 / 4 + 16) * U) * du.abs().sum(0))
+    du_r = du_err + (half(dtype) * du.abs() if act != "none" else 0.0)        # du as the products read it
+    close(dx, du @ w.double(), du_r @ w.double().abs() + (N + 8) * U * (du.abs() @ w.double().abs()))
+    close(dw, du.t() @ xv, du_r.t() @ xv.abs() + (M + 300) * U * (du.abs().t() @ xv.abs()))
+    assert dx.dtype == dtype and dw.dtype == (dw_dtype or dtype) and db.dtype == F32 and (buf is None or dw is buf)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", LIN)
+def test_linear_act_bwd(M, N, K, dtype):
+    for act in ACTS:
+        for ck in (False, True):
+            lin_bwd_check(B(), M, N, K, dtype, act, ck, gen(M, N, K, ck), F32 if act == "lrelu" else None)
+
+
+def test_linear_act_bwd_long_reduction():
+    lin_bwd_check(B(), 9001, 72, 136, BF16, "silu", True, gen(5), F32)
+    lin_bwd_check(B(), 20000, 64, 64, F32, "none", False, gen(6))
+
+
+def test_linear_gradients_against_differences():
+    b = B()
+    g = gen(43)
+    M, N, K = 6, 10, 14
+    x, w, bias, dy, res = rnd(g, M, K), rnd(g, N, K, scale=0.3), rnd(g, N), rnd(g, M, N), rnd(g, M, N)
+    for act in ("none", "silu", "gelu_tanh"):
+        y, pre = b.linear_act(x, w, bias, act=act, residual=res, save_pre=True)
+        grads = b.linear_act_bwd(dy, x, w, act=act, pre=pre)
+        f = lambda t: ((act64(t[0] @ t[1].t() + t[2], act)[0] + res.double()) * dy.double()).sum()
+        args = [x.double(), w.double(), bias.double()]
+        for k in range(3):
+            v = torch.randn(args[k].shape, generator=g, device=DEV, dtype=F64)
+            up, dn = list(args), list(args)
+            h = 1e-5
+            up[k], dn[k] = args[k] + h * v, args[k] - h * v
+            diff = (f(up) - f(dn)) / (2 * h)
+            assert abs((grads[k].double() * v).sum() - diff) <= 1e-7 * (grads[k].double() * v).abs().sum() + 40 * U * (dy.double().abs().sum() * v.abs().max() * 10)
+
+
+def test_linear_layouts():
+    b = B()
+    g = gen(11)
+    M, N, K = 70, 96, 72
+    xw, ww, rw = rnd(g, M, K + 24, dtype=BF16), rnd(g, N, K + 8, dtype=BF16, scale=0.1), rnd(g, M, N + 16, dtype=BF16)
+    bias = rnd(g, N)
+    for off in (0, 1, 8):
+        x, w, r = xw[:, off:off + K], ww[:, off % 8:off % 8 + K], rw[:, off:off + N]
+        want, wpre = b.linear_act(x.contiguous(), w.contiguous(), bias, act="silu", residual=r.contiguous(), save_pre=True)
+        out = torch.full((M, N + 16), 5.0, dtype=BF16, device=DEV)
+        got, pre = b.linear_act(x, w, bias, act="silu", residual=r, save_pre=True, out=out[:, off:off + N])
+        assert torch.equal(got, want) and torch.equal(pre, wpre)
+        assert (out[:, :off] == 5).all() and (out[:, off + N:] == 5).all()
+        dyw = rnd(g, M, N + 16, dtype=BF16)
+        dy = dyw[:, off:off + N]
+        a = b.linear_act_bwd(dy, x, w, act="silu", pre=r)
+        c = b.linear_act_bwd(dy.contiguous(), x.contiguous(), w.contiguous(), act="silu", pre=r.contiguous())
+        for s, t in zip(a, c):
+            assert (s.float() - t.float()).abs().max() <= 2 ** -7 * t.float().abs().max()
+        dww = torch.full((N, K + 16), 5.0, device=DEV)
+        dw = b.linear_act_bwd(dy, x, w, act="silu", pre=r, need=("w",), dw=dww[:, off:off + K])[1]
+        assert (dw.to(BF16).float() - c[1].float()).abs().max() <= 2 ** -7 * c[1].float().abs().max()
+        assert (dww[:, :off] == 5).all() and (dww[:, off + K:] == 5).all()
+    # the result over the residual, leading dimensions, a single row
+    x, w, r = xw[:, :K].contiguous(), ww[:, :K].contiguous(), rw[:, :N].contiguous()
+    want = b.linear_act(x, w, bias, act="gelu_tanh", residual=r)
+    ri = r.clone()
+    assert torch.equal(b.linear_act(x, w, bias, act="gelu_tanh", residual=ri, out=ri), want)
+    assert torch.equal(b.linear_act(x.view(7, 10, K), w, bias, act="gelu_tanh", residual=r.view(7, 10, N)), want.view(7, 10, N))
+    one = b.linear_act(x[3], w, bias, act="gelu_tanh", residual=r[3])
+    assert one.shape == (N,) and (one.float() - want[3].float()).abs().max() <= 2 ** -7 * want[3].float().abs().max()
+    # parts of the gradients
+    dy = rnd(g, M, N, dtype=BF16)
+    full = b.linear_act_bwd(dy, x, w)
+    assert torch.equal(b.linear_act_bwd(dy, x, w, need=("x",))[0], full[0]) and b.linear_act_bwd(dy, x, w, need=("x",))[1:] == (None, None)
+    assert torch.equal(b.linear_act_bwd(dy, x, w, need=("b",))[2], full[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_empty(dtype):
+    b = B()
+    e = lambda *s: torch.empty(*s, dtype=dtype, device=DEV)
+    z = lambda *s: torch.randn(*s, device=DEV).to(dtype)
+    bias = torch.randn(6, device=DEV)
+    assert b.linear_act(e(0, 4), z(6, 4), bias).shape == (0, 6)
+    assert b.linear_act(z(3, 4), e(0, 4)).shape == (3, 0)
+    assert torch.equal(b.linear_act(e(3, 0), e(6, 0), bias, act="lrelu"), act64(bias.double(), "lrelu")[0].to(F32).to(dtype).expand(3, 6))
+    dx, dw, db = b.linear_act_bwd(e(0, 6), e(0, 4), z(6, 4), act="silu", pre=e(0, 6))
+    assert dx.shape == (0, 4) and (dw == 0).all() and (db == 0).all()
+    dx, dw, db = b.linear_act_bwd(e(3, 0), z(3, 4), e(0, 4))
+    assert (dx == 0).all() and dx.shape == (3, 4) and dw.shape == (0, 4) and db.shape == (0,)
+    dx, dw, db = b.linear_act_bwd(z(3, 6), e(3, 0), e(6, 0))
+    assert dx.shape == (3, 0) and dw.shape == (6, 0) and db.shape == (6,)
+
+
+def test_linear_special_values_stay_in_their_rows():
+    b = B()
+    g = gen(12)
+    x, w = rnd(g, 40, 64, dtype=BF16), rnd(g, 48, 64, dtype=BF16)
+    want = b.linear_act(x, w)
+    x[5, 9], x[7, 0] = float("nan"), float("inf")
+    y = b.linear_act(x, w)
+    keep = torch.ones(40, dtype=torch.bool, device=DEV)
+    keep[5] = keep[7] = False
+    assert torch.equal(y[keep], want[keep]) and torch.isnan(y[5]).all() and not torch.isfinite(y[7]).any()
+    # large pre-activations: the gates saturate without a NaN
+    for act in ("silu", "gelu_tanh"):
+        t = torch.tensor([[3e38, -3e38, 1e20, -1e20, 200.0, -200.0, 0.0, -0.0]], device=DEV)
+        eye = torch.eye(8, device=DEV)
+        v = b.linear_act(t, eye, act=act)
+        assert torch.equal(v[0, :5], torch.tensor([3e38, 0, 1e20, 0, 200.0], device=DEV)) and (v[0, 5:].abs() < 1e-30).all()
+        dx = b.linear_act_bwd(torch.ones(1, 8, device=DEV), t, eye, act=act, pre=t)[0]
+        assert torch.equal(dx[0, [0, 2, 4]], torch.ones(3, device=DEV)) and (dx[0, [1, 3, 5]].abs() < 1e-30).all() and (dx[0, 6:] == 0.5).all()
+
+
+# ---- together ------------------------------------------------------------------------------------------------------------
+def block_step(b, x, p, dout):
+    """A pre-norm residual block with everything kept in 8 bits, forward and backward."""
+    y, mean, rstd, x8 = b.group_norm_act(x, 8, p["gamma"], p["beta"], act="silu", ckpt=True)
+    h, pre = b.linear_act(y, p["w1"], p["b1"], act="gelu_tanh", save_pre=True)
+    out = b.linear_act(h, p["w2"], p["b2"], residual=x)
+    y8, h8, pre8 = b.ckpt8_pack(y), b.ckpt8_pack(h), b.ckpt8_pack(pre)
+    dh, dw2, db2 = b.linear_act_bwd(dout, h8, p["w2"])
+    dy, dw1, db1 = b.linear_act_bwd(dh, y8, p["w1"], act="gelu_tanh", pre=pre8)
+    dx, dg, dbt = b.group_norm_act_bwd(dy, x8, 8, p["gamma"], p["beta"], mean, rstd, act="silu")
+    return [out, dx + dout, dg, dbt, dw1, db1, dw2, db2]
+
+
+def block_inputs(seed, dtype, n=6, s=16, c=64):
+    g = gen(seed)
+    p = dict(gamma=rnd(g, c, scale=0.2, shift=1.0), beta=rnd(g, c, scale=0.2), w1=rnd(g, 2 * c, c, dtype=dtype, scale=c ** -0.5), b1=rnd(g, 2 * c, scale=0.1),
+             w2=rnd(g, c, 2 * c, dtype=dtype, scale=(2 * c) ** -0.5), b2=rnd(g, c, scale=0.1))
+    return rnd(g, n, s, c, dtype=dtype), p, rnd(g, n, s, c, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_block_with_8_bit_checkpoints_against_autograd(dtype):
+    """The whole block against fp64 autograd.  What the checkpoints add: a value is off by half a step, at most 2^-7 of its block's
+    largest, so a gradient is off by about 2^-7 / sqrt(3) of itself per kept tensor it passes (three of them), bf16 a further 2^-8 per
+    rounding; errors of single values add with mixed signs.  2 % of the gradient's norm holds both with room."""
+    b = B()
+    x, p, dout = block_inputs(1, dtype)
+    got = block_step(b, x, p, dout)
+    leaf = {k: v.double().requires_grad_(True) for k, v in dict(p, x=x).items()}
+    n, s, c = x.shape
+    xg = leaf["x"].view(n, s, 8, c // 8)
+    xh = ((xg - xg.mean((1, 3), keepdim=True)) / (xg.var((1, 3), unbiased=False, keepdim=True) + 1e-5).sqrt()).view(n, s, c)
+    y = act64(xh * leaf["gamma"] + leaf["beta"], "silu")[0]
+    h = act64(y @ leaf["w1"].t() + leaf["b1"], "gelu_tanh")[0]
+    out = h @ leaf["w2"].t() + leaf["b2"] + leaf["x"]
+    out.backward(dout.double())
+    want = [out.detach()] + [leaf[k].grad for k in ("x", "gamma", "beta", "w1", "b1", "w2", "b2")]
+    for a, t in zip(got, want):
+        assert (a.double() - t).norm() <= 0.02 * t.norm()
+
+
+def test_block_is_deterministic_and_runs_on_other_streams():
+    b = B()
+    x, p, dout = block_inputs(2, BF16, n=40)
+    first = block_step(b, x, p, dout)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for st in (s1, s2, s1):
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            outs.append(block_step(b, x, p, dout))
+    torch.cuda.synchronize()
+    for o in outs:
+        for a, t in zip(o, first):
+            assert torch.equal(a, t)
+
+
+def test_two_captured_blocks_replayed_in_turn():
+    b = B()
+    sets = [block_inputs(k, BF16) for k in (3, 4)]
+    eager = [block_step(b, *t) for t in sets]
+    graphs = []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for t in sets:
+            block_step(b, *t)
+    torch.cuda.current_stream().wait_stream(side)
+    for t in sets:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = block_step(b, *t)
+        graphs.append((gr, out))
+    for k in (0, 1, 1, 0, 1):
+        gr, out = graphs[k]
+        for o in out:
+            o.fill_(float("nan"))
+        gr.replay()
+        again = block_step(b, *sets[1 - k])                  # eager work beside the replays
+        torch.cuda.synchronize()
+        for a, t in zip(out, eager[k]):
+            assert torch.equal(a, t)
+        for a, t in zip(again, eager[1 - k]):
+            assert torch.equal(a, t)
+
+
+def test_offsets_past_32_bits():
+    """Row strides that put the last rows more than 2^32 bytes behind the first: one tensor of 5 GiB, few of its rows used."""
+    b = B()
+    ld = (1 << 31) // 8 + 8                                  # elements; 9 rows of bf16 span 4.8 GB
+    big = torch.empty(9 * ld + 64, dtype=BF16, device=DEV)
+    x = big.as_strided((10, 64), (ld, 1))
+    g = gen(21)
+    val = rnd(g, 10, 64, dtype=BF16)
+    x.copy_(val)
+    w, bias = rnd(g, 72, 64, dtype=BF16, scale=0.1), rnd(g, 72)
+    assert torch.equal(b.linear_act(x, w, bias, act="silu"), b.linear_act(val, w, bias, act="silu"))
+    dy = rnd(g, 10, 72, dtype=BF16)
+    for a, t in zip(b.linear_act_bwd(dy, x, w), b.linear_act_bwd(dy, val, w)):
+        assert torch.equal(a, t)
+    ck, ref = b.ckpt8_pack(x), b.ckpt8_pack(val)
+    assert torch.equal(ck.q, ref.q) and torch.equal(ck.e, ref.e)
+    gamma, beta = rnd(g, 64), rnd(g, 64)
+    a, t = b.group_norm_act(x.view(10, 1, 64), 8, gamma, beta), b.group_norm_act(val.view(10, 1, 64), 8, gamma, beta)
+    for s, v in zip(a, t):
+        assert torch.equal(s, v)
+    d = rnd(g, 10, 1, 64, dtype=BF16)
+    for s, v in zip(b.group_norm_act_bwd(d, x.view(10, 1, 64), 8, gamma, beta, t[1], t[2]), b.group_norm_act_bwd(d, val.view(10, 1, 64), 8, gamma, beta, t[1], t[2])):
+        assert torch.equal(s, v)
+    y = torch.empty(9 * ld + 64, dtype=BF16, device=DEV).as_strided((10, 64), (ld, 1))
+    assert torch.equal(b.ckpt8_unpack(ck, out=y), b.ckpt8_unpack(ck))
+
+
+def test_refusals_on_the_gpu():
+    b = B()
+    x, w = torch.randn(4, 8, device=DEV), torch.randn(6, 8, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        b.linear_act(x, torch.randn(8, 8, device=DEV), out=x)
+    big = torch.randn(5, 6, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        b.linear_act(x, w, residual=big[:4], out=big[1:])
+    with pytest.raises(ValueError, match="overlaps"):
+        b.group_norm_act(x, 2, torch.ones(8, device=DEV), torch.zeros(8, device=DEV), ckpt=True, out=x)
+    with pytest.raises(ValueError, match="device"):
+        b.linear_act(x, w, bias=torch.randn(6))
+    with pytest.raises(ValueError, match="contiguous"):
+        b.linear_act(x, torch.randn(8, 6, device=DEV).t())
+    with pytest.raises(ValueError, match="rows overlap"):
+        b.linear_act(torch.randn(8, device=DEV).expand(4, 8), w)
+    from favae_hip import lib as L
+    raw = L.raw()
+    y = torch.empty(2000, 64, device=DEV)
+    rc = b._raw.favae_linear_act_fwd(y.data_ptr(), 64, y.data_ptr(), 64, None, None, 0, None, 0, y.data_ptr(), 64, 64, 64, 100000, 0, None, 0, 0, None)
+    assert rc < 0 and "row stride" in L.last_error()
+    rc = b._raw.favae_linear_act_fwd(y.data_ptr(), 4096, y.data_ptr(), 4096, None, None, 0, None, 0, y.data_ptr(), 64, 64, 64, 4096, 0, None, 0, 0, None)
+    assert rc < 0 and "scratch" in L.last_error()
