@@ -105,4 +105,5 @@ __device__ __forceinline__ int ck_round(float x, unsigned code) {
     const float q = rintf(x * __uint_as_float((254u - code) << 23));
     return (int)fminf(fmaxf(q, -127.f), 127.f);
 }
-__device__ __forceinline__ float ck_byte(unsigned w, int j) { return (float)(signed char)(w >> (8 * j)); }
+// value of byte j of w at step s: a conversion that selects and sign-extends its byte, and a product
+__device__ __forceinline__ float ck_value(unsigned w, int j, float s) { return (float)(signed char)(w >> (8 * j)) * s; }

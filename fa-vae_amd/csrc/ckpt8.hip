@@ -117,7 +117,7 @@ template <class T, int U> __global__ __launch_bounds__(256) void ck_unpack_wide(
         const float s = ck_scale(code[u]);
         float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = ck_byte(j < 4 ? w[u].x : w[u].y, j & 3) * s;
+        for (int j = 0; j < 8; ++j) f[j] = ck_value(j < 4 ? w[u].x : w[u].y, j & 3, s);
         T* o = (T*)p.out + row[u] * p.ldo + c[u];
         if constexpr (sizeof(T) == 2) { uint4 r; vec_put(r, f); *(uint4*)o = r; }
         else { *(float4*)o = make_float4(f[0], f[1], f[2], f[3]); *(float4*)(o + 4) = make_float4(f[4], f[5], f[6], f[7]); }

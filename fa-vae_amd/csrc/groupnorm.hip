@@ -124,7 +124,7 @@ template <int VEC> struct CkData {
     }
     __device__ __forceinline__ void get(float (&f)[VEC]) const {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = ck_byte(w[j >> 2], j & 3) * s;
+        for (int j = 0; j < VEC; ++j) f[j] = ck_value(w[j >> 2], j & 3, s);
     }
 };
 

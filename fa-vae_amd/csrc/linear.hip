@@ -10,6 +10,7 @@
 // transposed tile (Q rows x P columns): a lane then holds 4 neighbouring output columns of one row.
 #include "act8.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -56,17 +57,20 @@ struct GemmP {
 //   CM bf16: [BKE][ROWS]; the transposing load reads, per half wave, one 64-byte piece of 4 consecutive rows: the piece index is XORed
 //       with row & 3 so that the four lie in different quarters of the 256-byte bank row.
 //   CM fp32: [BKE][ROWS]; the two halves of a wave read rows k and k + 8: the 128-byte half is XORed with bit 3 of the row.
-template <class T, int ROWS, bool CM> struct TileImg {
-    static constexpr int BKE = 128 / sizeof(T);                       // 64 bf16, 32 fp32
+template <class T, int ROWS, bool CM, int BKE_ = 128 / (int)sizeof(T)> struct TileImg {
+    static constexpr int BKE = BKE_;
+    static constexpr int RB = BKE * (int)sizeof(T);                   // bytes of a KC row: 64 or 128
     static constexpr int VE = 16 / sizeof(T);
     static constexpr int CPR = CM ? ROWS / VE : BKE / VE;             // chunks of a row
     static constexpr int CHUNKS = ROWS * BKE / VE;
     static constexpr int BYTES = CHUNKS * 16;
     __device__ static __forceinline__ int off(int row, int ch) {
-        if constexpr (!CM) return row * 128 + ((ch ^ ((row >> 1) & 7)) << 4);
+        if constexpr (!CM) return row * RB + ((ch ^ ((row / (256 / RB)) & (CPR - 1))) << 4);
         else if constexpr (sizeof(T) == 2) return row * (ROWS * 2) + ((((ch >> 2) ^ (row & 3)) << 2 | (ch & 3)) << 4);
         else return row * (ROWS * 4) + ((ch ^ (row & 8)) << 4);
     }
+    // inverse: which chunk of its row the 16-byte slot `slot` of that row holds
+    __device__ static __forceinline__ int chunk_at(int row, int slot) { return (off(row, slot) - row * (CM ? ROWS * (int)sizeof(T) : RB)) >> 4; }
     // fragment: output row rb + (lane & 31), reduction elements k0 + 8 (lane >> 5) ..
     __device__ static __forceinline__ void frag(Frag<T>& f, const char* lds, int rb, int k0, int lane) {
         const int r = lane & 31, h = lane >> 5;
@@ -95,8 +99,8 @@ template <class T, int ROWS, bool CM> struct TileImg {
 // Staging of one operand's tile.  REG: through registers, any alignment, any tail; CKPT: the operand is an 8-bit checkpoint.
 enum { S_REG = 0, S_CKPT = 1 };
 
-template <class T, int ROWS, bool CM, int MODE, int NT> struct Stager {
-    typedef TileImg<T, ROWS, CM> Img;
+template <class T, int ROWS, bool CM, int MODE, int NT, int BKE = 128 / (int)sizeof(T)> struct Stager {
+    typedef TileImg<T, ROWS, CM, BKE> Img;
     static constexpr int NC = Img::CHUNKS / NT;
     static_assert(Img::CHUNKS % NT == 0, "whole chunks per thread");
     uint4 v[NC];
@@ -143,12 +147,12 @@ template <class T, int ROWS, bool CM, int MODE, int NT> struct Stager {
                 if constexpr (sizeof(T) == 2) {
                     float f[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = ck_byte(j < 4 ? t.x : t.y, j & 3) * s;
+                    for (int j = 0; j < 8; ++j) f[j] = ck_value(j < 4 ? t.x : t.y, j & 3, s);
                     vec_put(t, f);
                 } else {
                     float f[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) f[j] = ck_byte(t.x, j) * s;
+                    for (int j = 0; j < 4; ++j) f[j] = ck_value(t.x, j, s);
                     t = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
                 }
             }
@@ -157,45 +161,153 @@ template <class T, int ROWS, bool CM, int MODE, int NT> struct Stager {
     }
 };
 
-// 8 neighbouring output columns of one row: bias, activation, residual, store
-template <class T, class OT> __device__ __forceinline__ void epilogue8(const GemmP& p, float (&f)[8], long long i, int j) {
-    const int left = p.J - j;
-    if (p.bias) {
+// 8 neighbouring output columns of a row, `left` of which exist: bias, activation, residual, store.  oo, op, orr: element offsets in out, pre and
+// res.  FAST: all 8 exist and 16-byte accesses are allowed.
+template <class T, class OT, bool FAST> __device__ __forceinline__ void epilogue8(const GemmP& p, float (&f)[8], const float (&bias)[8], int left, long long oo, long long op, long long orr) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] += k < left ? p.bias[j + k] : 0.f;
-    }
-    if (p.pre) {
-        OT* o = (OT*)p.pre + i * p.ldpre + j;
-        if (p.vec && left >= 8) {
+    for (int k = 0; k < 8; ++k) f[k] += bias[k];
+    const auto put = [&](OT* o) __attribute__((always_inline)) {
+        if constexpr (FAST) {
             if constexpr (sizeof(OT) == 2) { uint4 r; vec_put(r, f); *(uint4*)o = r; }
             else { ((float4*)o)[0] = make_float4(f[0], f[1], f[2], f[3]); ((float4*)o)[1] = make_float4(f[4], f[5], f[6], f[7]); }
-        } else
+        } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) if (k < left) o[k] = from_f32<OT>(f[k]);
-    }
+        }
+    };
+    if (p.pre) put((OT*)p.pre + op);
     act_apply<T>(f, p.act);
     if (p.res) {
-        const T* a = (const T*)p.res + i * p.ldr + j;
+        const T* a = (const T*)p.res + orr;
         float t[8];
-        if (p.vec && left >= 8) {
+        if constexpr (FAST) {
             if constexpr (sizeof(T) == 2) vec_get(t, *(const uint4*)a);
             else {
                 const float4 lo = ((const float4*)a)[0], hi = ((const float4*)a)[1];
                 t[0] = lo.x; t[1] = lo.y; t[2] = lo.z; t[3] = lo.w; t[4] = hi.x; t[5] = hi.y; t[6] = hi.z; t[7] = hi.w;
             }
-        } else
+        } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) t[k] = k < left ? to_f32<T>(a[k]) : 0.f;
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) f[k] += t[k];
     }
-    OT* o = (OT*)p.out + i * p.ldo + j;
-    if (p.vec && left >= 8) {
-        if constexpr (sizeof(OT) == 2) { uint4 r; vec_put(r, f); *(uint4*)o = r; }
-        else { ((float4*)o)[0] = make_float4(f[0], f[1], f[2], f[3]); ((float4*)o)[1] = make_float4(f[4], f[5], f[6], f[7]); }
-    } else
+    put((OT*)p.out + oo);
+}
+__device__ __forceinline__ void load_bias(const GemmP& p, float (&b)[8], int j) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) if (k < left) o[k] = from_f32<OT>(f[k]);
+    for (int k = 0; k < 8; ++k) b[k] = p.bias && j + k < p.J ? p.bias[j + k] : 0.f;
+}
+
+// Staging by DMA: 16-byte chunks go from memory into LDS without registers in between.  A wave's load instruction fills 64
+// neighbouring 16-byte slots, so the swizzle is applied to the addresses: the lane that fills slot s of a row loads the chunk that
+// belongs there.  The buffer descriptor's range check turns what lies outside the operand into zeros: lanes whose output row (or
+// column) does not exist, or whose chunk lies past the end of the reduction, carry an offset with bit 31 set.
+typedef unsigned v4u_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+template <class T, int ROWS, bool CM, int BKE, int NT> struct Dma {
+    typedef TileImg<T, ROWS, CM, BKE> Img;
+    static constexpr int NC = Img::CHUNKS / NT;
+    static_assert(Img::CHUNKS % NT == 0, "whole chunks per thread");
+    unsigned voff[NC];
+    const char* base;                 // element (o0, first reduction element of this split), KC; (first, o0), CM
+    long long step;                   // bytes between steps
+    __device__ __forceinline__ void init(const char* p, long long ld, long long o0, long long no, long long c0) {
+        base = p + ((CM ? c0 * ld + o0 : o0 * ld + c0) * (long long)sizeof(T));
+        step = CM ? (long long)BKE * ld * (long long)sizeof(T) : (long long)Img::RB;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int c = (int)threadIdx.x + i * NT, row = c / Img::CPR, slot = c - row * Img::CPR, ch = Img::chunk_at(row, slot);
+            const bool ok = CM ? o0 + ch * Img::VE < no : o0 + row < no;
+            voff[i] = ok ? (unsigned)row * (unsigned)(ld * (int)sizeof(T)) + (unsigned)ch * 16u : 0x80000000u;
+        }
+    }
+    // FULL: BKE reduction elements are left; otherwise `left` of them, the rest reads as zero
+    template <bool FULL> __device__ __forceinline__ void issue(char* lds, int wave, int left) {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            unsigned v = voff[i];
+            if constexpr (!FULL) {
+                const int c = (int)threadIdx.x + i * NT, row = c / Img::CPR, slot = c - row * Img::CPR;
+                v = (CM ? row : Img::chunk_at(row, slot) * Img::VE) < left ? v : 0x80000000u;
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (wave * 64 + i * NT) * 16), 16, (int)v, 0, 0, 0);
+        }
+        base += step;
+    }
+};
+
+// block -> (split, tile): blocks are dealt to the 8 XCDs in turn; each XCD takes a contiguous run of tiles, bands of 8 tile rows walked
+// column by column, so that the tiles running at one time share operand rows in one L2
+__device__ __forceinline__ void gemm_tile(const GemmP& p, int& split, int& ti, int& tj) {
+    const long long n = (long long)p.ti * p.tj * p.splits, per = n / 8, b = blockIdx.x;
+    long long lb = b < per * 8 ? (b & 7) * per + (b >> 3) : b;
+    split = (int)(lb / ((long long)p.ti * p.tj));
+    lb -= (long long)split * p.ti * p.tj;
+    const int band = (int)(lb / (8 * p.tj)), in_band = (int)(lb - (long long)band * 8 * p.tj), bh = min(8, p.ti - band * 8);
+    tj = in_band / bh;
+    ti = band * 8 + in_band - tj * bh;
+}
+
+// Output tile of a wave through LDS: 32 rows at a time in a region of its own, [32][NJ * 32 + 4] fp32, so that a lane ends up with 8
+// neighbouring columns of a row, 16 bytes of bf16; its columns are the same in every row it takes
+template <class T, class OT, bool FAST, int NJ, int EL>
+__device__ __forceinline__ void epilogue_rows(const GemmP& p, const float* tile, const float (&bias)[8], long long i_lo, int j, int split, int lane) {
+    constexpr int WC = NJ * 32, RS = WC + 4, LPR = WC / 8, STEP = 64 / LPR;
+    const int r0 = lane / LPR;
+    const float* src = tile + r0 * RS + (lane % LPR) * 8;
+    const long long i0 = i_lo + r0;
+    long long oo = i0 * p.ldo + j, op = i0 * p.ldpre + j, orr = i0 * p.ldr + j;
+    if (p.splits > 1) {
+        float* o = p.part + ((long long)split * p.I + i0) * p.J + j;
+#pragma unroll FAST ? 4 : 1
+        for (int e = 0; e < EL; ++e) {
+            const float4 lo = *(const float4*)src, hi = *(const float4*)(src + 4);
+            if constexpr (FAST) { ((float4*)o)[0] = lo; ((float4*)o)[1] = hi; }
+            else {
+                const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                if (i0 + e * STEP < p.I)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) if (j + k < p.J) o[k] = f[k];
+            }
+            src += STEP * RS;
+            o += (long long)STEP * p.J;
+        }
+        return;
+    }
+#pragma unroll FAST ? 2 : 1
+    for (int e = 0; e < EL; ++e) {
+        const float4 lo = *(const float4*)src, hi = *(const float4*)(src + 4);
+        float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (FAST || (i0 + e * STEP < p.I && j < p.J)) epilogue8<T, OT, FAST>(p, f, bias, p.J - j, oo, op, orr);
+        src += STEP * RS;
+        oo += STEP * p.ldo; op += STEP * p.ldpre; orr += STEP * p.ldr;
+    }
+}
+template <class T, class OT, int TI, int TJ, int WI, int WJ, int NI, int NJ>
+__device__ __forceinline__ void gemm_epilogue(const GemmP& p, f32x16 (&acc)[NI][NJ], char* smem, long long i0, int j0, int split, int lane, int wi, int wj, int wave) {
+    constexpr int WC = NJ * 32, RS = WC + 4, LPR = WC / 8, EL = 32 * LPR / 64;
+    float* tile = (float*)smem + wave * 32 * RS;
+    const int j = j0 + wj * WC + (lane % LPR) * 8;
+    float bias[8];
+    load_bias(p, bias, j);
+    const bool fast = p.vec && i0 + TI <= p.I && j0 + TJ <= p.J && (p.splits == 1 || p.J % 8 == 0);
+    __syncthreads();
+#pragma unroll
+    for (int a = 0; a < NI; ++a) {
+#pragma unroll
+        for (int c = 0; c < NJ; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *(float4*)(tile + (lane & 31) * RS + c * 32 + 8 * e + 4 * (lane >> 5)) = make_float4(acc[a][c][4 * e], acc[a][c][4 * e + 1], acc[a][c][4 * e + 2], acc[a][c][4 * e + 3]);
+        __builtin_amdgcn_wave_barrier();
+        const long long i_lo = i0 + wi * (TI / WI) + a * 32;
+        if (fast) epilogue_rows<T, OT, true, NJ, EL>(p, tile, bias, i_lo, j, split, lane);
+        else epilogue_rows<T, OT, false, NJ, EL>(p, tile, bias, i_lo, j, split, lane);
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 // T: type of the operands and the residual, OT: of the output (and pre).  TI x TJ output tile, WI x WJ waves.
@@ -208,14 +320,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmP p) {
     constexpr int NI = TI / WI / 32, NJ = TJ / WJ / 32;
     extern __shared__ char smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / WJ, wj = wave - wi * WJ;
-    // block -> (split, tile): blocks are dealt to the 8 XCDs in turn; each XCD takes a contiguous run of tiles, bands of 8 tile rows
-    // walked column by column, so that the tiles running at one time share operand rows in one L2
-    const long long n = (long long)p.ti * p.tj * p.splits, per = n / 8, b = blockIdx.x;
-    long long lb = b < per * 8 ? (b & 7) * per + (b >> 3) : b;
-    const int split = (int)(lb / ((long long)p.ti * p.tj));
-    lb -= (long long)split * p.ti * p.tj;
-    const int band = (int)(lb / (8 * p.tj)), in_band = (int)(lb - (long long)band * 8 * p.tj), bh = min(8, p.ti - band * 8);
-    const int tj = in_band / bh, ti = band * 8 + in_band - tj * bh;
+    int split, ti, tj;
+    gemm_tile(p, split, ti, tj);
     const long long i0 = (long long)ti * TI;
     const int j0 = tj * TJ;
     const long long cb = split * p.cchunk, ce = min(p.Cn, cb + p.cchunk);
@@ -262,35 +368,127 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmP p) {
             sq.store(nxt + PI::BYTES);
         }
     }
-    // epilogue: 32 output rows of the wave at a time through a region of LDS of its own, [32][NJ * 32 + 4] fp32, so that a lane ends up with 8 neighbouring columns
-    __syncthreads();
-    constexpr int WC = NJ * 32, RS = WC + 4, LPR = WC / 8;
-    float* tile = (float*)smem + wave * 32 * RS;
+    gemm_epilogue<T, OT, TI, TJ, WI, WJ>(p, acc, smem, i0, j0, split, lane, wi, wj, wave);
+}
+
+// Instruction order of a slice of M MFMAs with R LDS reads and `v` (0 or more) DMA loads: spread between the MFMAs
+template <int M, int R> __device__ __forceinline__ void slice_order(const int v) {
 #pragma unroll
-    for (int a = 0; a < NI; ++a) {
+    for (int i = 0; i < M; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        constexpr int per = (R + M - 1) / M;
+        if (i * per < R) __builtin_amdgcn_sched_group_barrier(0x100, per, 0);
+        if (i < v) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    }
+}
+
+// The same product with P (and Q, unless it is an 8-bit checkpoint) staged by DMA into a ring of STAGES tiles of BKE reduction
+// elements.  At the top of step t one barrier makes tile t + 1 visible and frees tile t - 1, whose slot takes the DMA of tile
+// t + STAGES - 1; loads stay in flight over STAGES - 2 steps.  Fragments are read one 16-deep slice ahead of their MFMAs, across the
+// step border too, so that no MFMA waits for LDS behind a barrier.
+template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int QMODE, int WPE>
+__global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP p) {
+    constexpr int NT = 64 * WI * WJ;
+    typedef TileImg<T, TI, PCM, BKE> PI;
+    typedef TileImg<T, TJ, QCM, BKE> QI;
+    constexpr int STAGE = PI::BYTES + QI::BYTES, SL = BKE / 16;
+    constexpr int NI = TI / WI / 32, NJ = TJ / WJ / 32;
+    constexpr bool CK = QMODE == S_CKPT;
+    constexpr int LOADS = Dma<T, TI, PCM, BKE, NT>::NC + (CK ? 0 : Dma<T, TJ, QCM, BKE, NT>::NC);   // DMA instructions of a wave per step
+    static_assert(STAGES >= (CK ? 4 : 3) && SL >= 2 && SL % 2 == 0, "ring and slices");
+    extern __shared__ char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wi = wave / WJ, wj = wave - wi * WJ;
+    int split, ti, tj;
+    gemm_tile(p, split, ti, tj);
+    const long long i0 = (long long)ti * TI;
+    const int j0 = tj * TJ;
+    const long long cb = split * p.cchunk, ce = min(p.Cn, cb + p.cchunk);
+
+    f32x16 acc[NI][NJ];
+#pragma unroll
+    for (int a = 0; a < NI; ++a)
 #pragma unroll
         for (int c = 0; c < NJ; ++c)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                *(float4*)(tile + (lane & 31) * RS + c * 32 + 8 * e + 4 * (lane >> 5)) = make_float4(acc[a][c][4 * e], acc[a][c][4 * e + 1], acc[a][c][4 * e + 2], acc[a][c][4 * e + 3]);
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int e = 0; e < 32 * LPR / 64; ++e) {
-            const int row = (lane + 64 * e) / LPR, cc = ((lane + 64 * e) - row * LPR) * 8;
-            const float4 lo = *(const float4*)(tile + row * RS + cc), hi = *(const float4*)(tile + row * RS + cc + 4);
-            float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-            const long long i = i0 + wi * (TI / WI) + a * 32 + row;
-            const int j = j0 + wj * WC + cc;
-            if (i < p.I && j < p.J) {
-                if (p.splits > 1) {
-                    float* o = p.part + ((long long)split * p.I + i) * p.J + j;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) if (j + k < p.J) o[k] = f[k];
-                } else epilogue8<T, OT>(p, f, i, j);
-            }
+            for (int e = 0; e < 16; ++e) acc[a][c][e] = 0.f;
+
+    Dma<T, TI, PCM, BKE, NT> dp;
+    Dma<T, TJ, QCM, BKE, NT> dq;
+    Stager<T, TJ, QCM, QMODE, NT, BKE> sq;
+    dp.init(p.P, p.ldp, i0, p.I, cb);
+    if constexpr (!CK) dq.init(p.Q, p.ldq, j0, p.J, cb);
+    const int steps = (int)((ce - cb + BKE - 1) / BKE);
+    const int pb = wi * (TI / WI), qb = wj * (TJ / WJ);
+    const int last = (int)(ce - cb - (long long)(steps - 1) * BKE);       // reduction elements of the last step
+    const auto issue = [&](char* s, int t) __attribute__((always_inline)) {
+        if (t + 1 < steps) {
+            dp.template issue<true>(s, wave, BKE);
+            if constexpr (!CK) dq.template issue<true>(s + PI::BYTES, wave, BKE);
+        } else {
+            dp.template issue<false>(s, wave, last);
+            if constexpr (!CK) dq.template issue<false>(s + PI::BYTES, wave, last);
         }
-        __builtin_amdgcn_wave_barrier();
+    };
+    if (steps > 0) {
+        for (int t = 0; t < STAGES - 1 && t < steps; ++t) {
+            if constexpr (CK) {
+                sq.load(p, p.Q, p.ldq, j0, p.J, cb + (long long)t * BKE, ce);
+                if (t < STAGES - 2) sq.store(smem + t * STAGE + PI::BYTES);   // the last one stays in registers until the first step
+            }
+            issue(smem + t * STAGE, t);
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        Frag<T> fp[2][NI], fq[2][NJ];
+#pragma unroll
+        for (int a = 0; a < NI; ++a) PI::frag(fp[0][a], smem, pb + a * 32, 0, lane);
+#pragma unroll
+        for (int c = 0; c < NJ; ++c) QI::frag(fq[0][c], smem + PI::BYTES, qb + c * 32, 0, lane);
+        int cur = 0, fill = (STAGES - 1) * STAGE;                            // byte offsets of the slots of tile t and of tile t + STAGES - 1
+        // FULL: another whole step to load; NONE: nothing left to load
+        const auto step = [&](int t, auto full) __attribute__((always_inline)) {
+            constexpr bool FULL = decltype(full)::value;
+            const int nxt = cur + STAGE == STAGES * STAGE ? 0 : cur + STAGE;
+            __builtin_amdgcn_sched_barrier(0);
+            // tile t + 1 has landed (younger loads may be under way), and every wave's reads of tile t - 1 are behind it
+            if (FULL || t + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 3) * LOADS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if constexpr (CK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            asm volatile("s_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (CK) {
+                const int mid = fill == 0 ? (STAGES - 1) * STAGE : fill - STAGE;   // slot of tile t + STAGES - 2
+                if (FULL || t + STAGES - 2 < steps) sq.store(smem + mid + PI::BYTES);
+                if (FULL || t + STAGES - 1 < steps) sq.load(p, p.Q, p.ldq, j0, p.J, cb + (long long)(t + STAGES - 1) * BKE, ce);
+            }
+            if constexpr (FULL) {
+                dp.template issue<true>(smem + fill, wave, BKE);
+                if constexpr (!CK) dq.template issue<true>(smem + fill + PI::BYTES, wave, BKE);
+            } else if (t + STAGES - 1 < steps) issue(smem + fill, t + STAGES - 1);
+#pragma unroll
+            for (int k = 0; k < SL; ++k) {
+                const char* s = smem + (k + 1 < SL ? cur : nxt);
+                const int k1 = k + 1 < SL ? (k + 1) * 16 : 0;
+                // (past the last tile this reads a slot that holds older values, and nothing uses them)
+#pragma unroll
+                for (int c = 0; c < NJ; ++c) QI::frag(fq[(k + 1) & 1][c], s + PI::BYTES, qb + c * 32, k1, lane);
+#pragma unroll
+                for (int a = 0; a < NI; ++a) PI::frag(fp[(k + 1) & 1][a], s, pb + a * 32, k1, lane);
+#pragma unroll
+                for (int a = 0; a < NI; ++a)
+#pragma unroll
+                    for (int c = 0; c < NJ; ++c) mma(acc[a][c], fq[k & 1][c], fp[k & 1][a]);
+                // order of the slice: an MFMA, then a share of the LDS reads and (first slice) of the DMA instructions, and so on
+                if constexpr (sizeof(T) == 2) slice_order<NI * NJ, (PCM ? 2 : 1) * NI + (QCM ? 2 : 1) * NJ>(k == 0 && FULL ? LOADS : 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            cur = nxt;
+            fill = fill + STAGE == STAGES * STAGE ? 0 : fill + STAGE;
+        };
+        int t = 0;
+        for (; t + STAGES < steps; ++t) step(t, std::true_type());
+        for (; t < steps; ++t) step(t, std::false_type());
     }
+    gemm_epilogue<T, OT, TI, TJ, WI, WJ>(p, acc, smem, i0, j0, split, lane, wi, wj, wave);
 }
 
 // Sum of the splits, then the epilogue
@@ -305,10 +503,19 @@ template <class T, class OT> __global__ __launch_bounds__(256) void gemm_join_ke
     for (int k = 0; k < 8; ++k) f[k] = 0.f;
     for (int s = 0; s < p.splits; ++s) {
         const float* a = p.part + ((long long)s * p.I + i) * p.J + j;
+        if (p.J % 8 == 0) {
+            const float4 lo = ((const float4*)a)[0], hi = ((const float4*)a)[1];
+            f[0] += lo.x; f[1] += lo.y; f[2] += lo.z; f[3] += lo.w; f[4] += hi.x; f[5] += hi.y; f[6] += hi.z; f[7] += hi.w;
+        } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) if (j + k < p.J) f[k] += a[k];
+            for (int k = 0; k < 8; ++k) if (j + k < p.J) f[k] += a[k];
+        }
     }
-    epilogue8<T, OT>(p, f, i, j);
+    float bias[8];
+    load_bias(p, bias, j);
+    const long long oo = i * p.ldo + j, op = i * p.ldpre + j, orr = i * p.ldr + j;
+    if (p.vec && j + 8 <= p.J) epilogue8<T, OT, true>(p, f, bias, 8, oo, op, orr);
+    else epilogue8<T, OT, false>(p, f, bias, p.J - j, oo, op, orr);
 }
 
 // ---- du = dy act'(u) and the column sums of du ---------------------------------------------------------------------------
@@ -347,7 +554,7 @@ template <class T, int V, int SRC> __global__ __launch_bounds__(256) void act_bw
                     unsigned wd[2] = {0u, 0u};
                     __builtin_memcpy(wd, a, V);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) z[k] = ck_byte(wd[k >> 2], k & 3) * sc;
+                    for (int k = 0; k < V; ++k) z[k] = ck_value(wd[k >> 2], k & 3, sc);
                 }
                 act_grad_mul<T>(d, z, p.act);
                 vec_put(rd, d);
@@ -385,32 +592,65 @@ __global__ __launch_bounds__(512) void col_join_kernel(const float* __restrict__
 // ---- host ----------------------------------------------------------------------------------------------------------------
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
-constexpr long long CUS = 256;
-// Splits of the reduction: as many as bring the launch to about two blocks per CU, each at least 4 steps long
-int plan_splits(long long I, int J, long long Cn, int es) {
-    const long long tiles = cdivll(I, 128) * cdivll(J, 128), bke = 128 / es;
-    if (tiles >= CUS) return 1;
-    long long s = std::min((2 * CUS) / tiles, cdivll(Cn, 4 * bke));
-    return (int)std::max<long long>(1, std::min<long long>(s, 256));
+// Tiles of the product kernels.  WIDE for long reductions of KC operands with a tile for every CU; TALL where two workgroups of 8 waves
+// share a CU, so that the epilogue of one runs beside the MFMAs of the other; SMALL where tiles are few.
+// Measured, bf16 (us, WIDE / TALL): x w^T 16384 x 4096 x 4096 452 / 513, 65536 x 1024 x 1024 with gelu and residual 197 / 188; du w 65536 x 1024
+// x 1024 156 / 137; du^T x 1024 x 1024 x 65536 in 16 splits 172 / 151.
+enum Tile { WIDE = 0, TALL = 1, SMALL = 2 };
+constexpr int TILE_I[3] = {256, 128, 128}, TILE_J[3] = {256, 256, 128}, TILE_SLOTS[3] = {256, 512, 512};   // slots: workgroups the chip holds
+struct GemmPlan { Tile tile; int splits; };
+GemmPlan plan_gemm(long long I, int J, long long Cn, int es, bool both_kc) {
+    const auto tiles = [&](Tile t) { return cdivll(I, TILE_I[t]) * cdivll(J, TILE_J[t]); };
+    GemmPlan pl;
+    pl.tile = es == 2 && both_kc && Cn >= 2048 && tiles(WIDE) >= TILE_SLOTS[WIDE] ? WIDE : SMALL;
+    // a reduction is split over as many workgroups as fill the chip, at least 8 steps of 128 bytes each
+    const long long most = std::max<long long>(1, Cn * es / 1024);
+    if (pl.tile == SMALL && I >= 128 && J >= 256 && tiles(TALL) * most >= TILE_SLOTS[TALL]) pl.tile = TALL;
+    const long long n = std::max<long long>(1, tiles(pl.tile));
+    pl.splits = n >= TILE_SLOTS[pl.tile] ? 1 : (int)std::min<long long>(std::min<long long>(TILE_SLOTS[pl.tile] / n, most), 256);
+    return pl;
 }
-long long split_chunk(long long Cn, int splits, int es) {
-    const long long bke = 128 / es;
-    return cdivll(cdivll(Cn, bke), splits) * bke;
+
+template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int QMODE, int WPE>
+void gemm_launch(const GemmP& p, unsigned blocks, hipStream_t st) {
+    constexpr size_t ring = STAGES * (size_t)(TileImg<T, TI, PCM, BKE>::BYTES + TileImg<T, TJ, QCM, BKE>::BYTES);
+    constexpr size_t lds = std::max(ring, (size_t)WI * WJ * 32 * (TJ / WJ + 4) * sizeof(float));
+    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    gemm_dma_kernel<T, OT, TI, TJ, WI, WJ, BKE, STAGES, PCM, QCM, QMODE, WPE><<<blocks, 64 * WI * WJ, lds, st>>>(p);
 }
 
 template <class T, class OT, bool PCM, bool QCM, int QMODE> int gemm_run(GemmP p, hipStream_t st) {
     if (p.I == 0 || p.J == 0) return FAVAE_OK;
-    constexpr int es = sizeof(T);
-    p.ti = (int)cdivll(p.I, 128);
-    p.tj = cdiv(p.J, 128);
-    p.splits = plan_splits(p.I, p.J, p.Cn, es);
-    p.cchunk = split_chunk(p.Cn, p.splits, es);
+    constexpr int es = sizeof(T), VE = 16 / es;
+    GemmPlan pl = plan_gemm(p.I, p.J, p.Cn, es, !PCM && !QCM);
+    // DMA takes whole 16-byte chunks at 16-byte addresses, with 32-bit offsets inside a tile
+    const auto chunks = [&](const char* a, long long ld, bool cm, long long outs) {
+        return aligned(a, 16) && ld % VE == 0 && ld * es <= (1 << 22) && (cm ? outs : p.Cn) % VE == 0;
+    };
+    const bool dma = chunks(p.P, p.ldp, PCM, p.I) && (QMODE == S_CKPT || chunks(p.Q, p.ldq, QCM, p.J));
+    if (!dma) pl.tile = SMALL;                   // (the split count of the planned tile stays: scratch is sized for it)
+    p.ti = (int)cdivll(p.I, TILE_I[pl.tile]);
+    p.tj = cdiv(p.J, TILE_J[pl.tile]);
+    const long long unit = 128 / es;
+    p.cchunk = cdivll(cdivll(p.Cn, unit), pl.splits) * unit;
     p.splits = (int)std::max<long long>(1, cdivll(p.Cn, std::max<long long>(1, p.cchunk)));
     p.vec = p.ldo % 8 == 0 && aligned(p.out, 16) && (!p.res || (p.ldr % 8 == 0 && aligned(p.res, 16))) && (!p.pre || (p.ldpre % 8 == 0 && aligned(p.pre, 16)));
     const long long blocks = (long long)p.ti * p.tj * p.splits;
     FAVAE_CHECK_ARG(blocks <= 0x7fffffffLL, "favae_linear_act: too many rows for one launch");
-    constexpr size_t lds = std::max<size_t>(2 * (size_t)(TileImg<T, 128, PCM>::BYTES + TileImg<T, 128, QCM>::BYTES), 4 * 32 * (64 + 4) * 4);
-    gemm_kernel<T, OT, 128, 128, 2, 2, PCM, QCM, QMODE><<<(unsigned)blocks, 256, lds, st>>>(p);
+    const unsigned g = (unsigned)blocks;
+    constexpr int ST = QMODE == S_CKPT ? 4 : 3;
+    if (!dma) {
+        gemm_kernel<T, OT, 128, 128, 2, 2, PCM, QCM, QMODE><<<g, 256, 2 * (size_t)(TileImg<T, 128, PCM>::BYTES + TileImg<T, 128, QCM>::BYTES), st>>>(p);
+    } else if constexpr (es == 4) {
+        // fp32 MFMA runs at a sixteenth of the bf16 rate: the plain ring feeds it
+        gemm_launch<T, OT, 128, 128, 2, 2, 32, ST, PCM, QCM, QMODE, 1>(p, g, st);
+    } else if (pl.tile == WIDE) {
+        if constexpr (!PCM && !QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, QMODE, 2>(p, g, st);
+    } else if (pl.tile == TALL) {
+        gemm_launch<T, OT, 128, 256, 2, 4, 32, ST, PCM, QCM, QMODE, 2>(p, g, st);
+    } else {
+        gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, QMODE, 2>(p, g, st);
+    }
     FAVAE_LAUNCH_CHECK();
     if (p.splits > 1) {
         gemm_join_kernel<T, OT><<<(unsigned)cdivll(p.I * ((p.J + 7) / 8), 256), 256, 0, st>>>(p);
@@ -420,9 +660,9 @@ template <class T, class OT, bool PCM, bool QCM, int QMODE> int gemm_run(GemmP p
 }
 
 size_t round256(size_t a) { return (a + 255) & ~(size_t)255; }
-size_t split_bytes(long long I, int J, long long Cn, int es) {
+size_t split_bytes(long long I, int J, long long Cn, int es, bool both_kc) {
     if (I == 0 || J == 0) return 0;
-    const int s = plan_splits(I, J, Cn, es);
+    const int s = plan_gemm(I, J, Cn, es, both_kc).splits;
     return s > 1 ? round256((size_t)s * I * J * sizeof(float)) : 0;
 }
 constexpr int DU_RUNS = 256;
@@ -441,7 +681,7 @@ BwdScratch bwd_scratch(long long M, int N, int K, int act, int dtype) {
     BwdScratch s;
     s.du = act == FAVAE_ACT_NONE ? 0 : round256((size_t)M * N * es);
     s.colp = M > 0 ? round256((size_t)cdivll(M, du_rows(M)) * N * sizeof(float)) : 0;
-    s.split = std::max(split_bytes(M, K, N, es), split_bytes(N, K, M, es));    // the two products run one after the other
+    s.split = std::max(split_bytes(M, K, N, es, false), split_bytes(N, K, M, es, false));    // the two products run one after the other
     s.total = s.du + s.colp + s.split;
     return s;
 }
@@ -501,7 +741,7 @@ template <class T> int lin_bwd(const void* dy, long long lddy, const void* x, lo
 
 extern "C" size_t favae_linear_act_fwd_scratch(long long M, int N, int K, int dtype) {
     if (lin_sizes("favae_linear_act_fwd_scratch", M, N, K, FAVAE_ACT_NONE, dtype) != FAVAE_OK) return 0;
-    return split_bytes(M, N, K, dtype == FAVAE_F32 ? 4 : 2);
+    return split_bytes(M, N, K, dtype == FAVAE_F32 ? 4 : 2, true);
 }
 
 extern "C" int favae_linear_act_fwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias, const void* residual,
@@ -514,7 +754,7 @@ extern "C" int favae_linear_act_fwd(const void* x, long long ldx, const void* w,
     FAVAE_CHECK_ARG(y && (K == 0 || (x && w)), "favae_linear_act_fwd: null pointer");
     FAVAE_CHECK_ARG(ldy >= N && ldx >= K && ldw >= K && (!residual || ldr >= N) && (!pre || ldpre >= N), "favae_linear_act_fwd: a row stride is below the row's length");
     FAVAE_CHECK_ARG(aligned(x, es) && aligned(w, es) && aligned(y, es) && aligned(residual, es) && aligned(pre, es), "favae_linear_act_fwd: a pointer is not aligned to its type");
-    const size_t need = split_bytes(M, N, K, es);
+    const size_t need = split_bytes(M, N, K, es, true);
     FAVAE_CHECK_ARG(need <= scratch_bytes && (need == 0 || scratch), "favae_linear_act_fwd: scratch of %zu bytes, %zu needed", scratch_bytes, need);
     GemmP p = {};
     p.P = (const char*)x; p.ldp = ldx; p.Q = (const char*)w; p.ldq = ldw; p.I = M; p.J = N; p.Cn = K;

@@ -368,6 +368,24 @@ def test_linear_act_bwd(M, N, K, dtype):
             lin_bwd_check(B(), M, N, K, dtype, act, ck, gen(M, N, K, ck), F32 if act == "lrelu" else None)
 
 
+@pytest.mark.parametrize("M,N,K,dtype", [(4100, 4104, 2056, BF16), (2000, 1024, 520, BF16), (300, 264, 4096, BF16), (1000, 520, 264, F32), (33000, 264, 8, BF16)])
+def test_linear_act_large_tiles(M, N, K, dtype):
+    b = B()
+    g = gen(M, N, K)
+    x, w = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype, scale=K ** -0.5)
+    bias, res = rnd(g, N, scale=0.3), rnd(g, M, N, dtype=dtype)
+    y, pre = b.linear_act(x, w, bias, act="gelu_tanh", residual=res, save_pre=True)
+    u = x.double() @ w.double().t() + bias.double()
+    u_err = lin_bound(x, w, bias)
+    v = act64(u, "gelu_tanh")[0]
+    err = SLOPE * u_err + (u.abs() + 8) * 4 * U * v.abs()
+    v = v + res.double()
+    close(pre, u, u_err)
+    close(y, v, err + U * v.abs())
+    lin_bwd_check(b, M, N, K, dtype, "silu", True, gen(M, N, K, 2), F32)
+    lin_bwd_check(b, M, N, K, dtype, "none", False, gen(M, N, K, 3))
+
+
 def test_linear_act_bwd_long_reduction():
     lin_bwd_check(B(), 9001, 72, 136, BF16, "silu", True, gen(5), F32)
     lin_bwd_check(B(), 20000, 64, 64, F32, "none", False, gen(6))
