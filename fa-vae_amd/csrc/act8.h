@@ -1,6 +1,7 @@
 // Device helpers shared by the residual-block operators (groupnorm.hip, linear.hip, ckpt8.hip): vectors of 1 to 8 elements, the
 // activations with their derivatives, and the 8-bit activation format.
 #pragma once
+#include <type_traits>
 #include "common.h"
 #include "favae_hip.h"
 
@@ -49,38 +50,48 @@ template <class T> __device__ __forceinline__ float sigmoid_of(float t) {
 }
 constexpr float GELU_C = 1.59576912160573081f;        // sqrt(8 / pi): gelu_tanh(z) = z sigmoid(GELU_C (z + 0.044715 z^3))
 
-template <class T, int N> __device__ __forceinline__ void act_apply(float (&z)[N], int act) {
-    if (act == FAVAE_ACT_SILU) {
+template <class T, int ACT, int N> __device__ __forceinline__ void act_apply(float (&z)[N]) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = z[j] * sigmoid_of<T>(z[j]);
-    } else if (act == FAVAE_ACT_GELU_TANH) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = z[j] * sigmoid_of<T>(GELU_C * z[j] * fmaf(0.044715f * z[j], z[j], 1.f));
-    } else if (act == FAVAE_ACT_LRELU) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = z[j] > 0.f ? z[j] : 0.01f * z[j];
+    for (int j = 0; j < N; ++j) {
+        if constexpr (ACT == FAVAE_ACT_SILU) z[j] = z[j] * sigmoid_of<T>(z[j]);
+        if constexpr (ACT == FAVAE_ACT_GELU_TANH) z[j] = z[j] * sigmoid_of<T>(GELU_C * z[j] * fmaf(0.044715f * z[j], z[j], 1.f));
+        if constexpr (ACT == FAVAE_ACT_LRELU) z[j] = z[j] > 0.f ? z[j] : 0.01f * z[j];
     }
 }
 // d[j] *= act'(z[j])
-template <class T, int N> __device__ __forceinline__ void act_grad_mul(float (&d)[N], const float (&z)[N], int act) {
-    if (act == FAVAE_ACT_SILU) {
+template <class T, int ACT, int N> __device__ __forceinline__ void act_grad_mul(float (&d)[N], const float (&z)[N]) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
+    for (int j = 0; j < N; ++j) {
+        if constexpr (ACT == FAVAE_ACT_SILU) {
             const float s = sigmoid_of<T>(z[j]);
             d[j] *= s * fmaf(z[j], 1.f - s, 1.f);
         }
-    } else if (act == FAVAE_ACT_GELU_TANH) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
+        if constexpr (ACT == FAVAE_ACT_GELU_TANH) {
             const float s = sigmoid_of<T>(GELU_C * z[j] * fmaf(0.044715f * z[j], z[j], 1.f));
             // past |z| = 20 s is 0 or 1 to the last bit and the second term vanishes; the bound keeps z^3 from overflowing there
             const float c = fminf(fmaxf(z[j], -20.f), 20.f);
             d[j] *= s * fmaf(c * (1.f - s), GELU_C * fmaf(0.134145f * c, c, 1.f), 1.f);
         }
-    } else if (act == FAVAE_ACT_LRELU) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) d[j] = z[j] > 0.f ? d[j] : 0.01f * d[j];
+        if constexpr (ACT == FAVAE_ACT_LRELU) d[j] = z[j] > 0.f ? d[j] : 0.01f * d[j];
     }
+}
+// f(std::integral_constant<int, act>): the choice is made once, outside the loops
+template <class F> __device__ __forceinline__ void with_act(int act, F&& f) {
+    if (act == FAVAE_ACT_SILU) f(std::integral_constant<int, FAVAE_ACT_SILU>());
+    else if (act == FAVAE_ACT_GELU_TANH) f(std::integral_constant<int, FAVAE_ACT_GELU_TANH>());
+    else if (act == FAVAE_ACT_LRELU) f(std::integral_constant<int, FAVAE_ACT_LRELU>());
+    else f(std::integral_constant<int, FAVAE_ACT_NONE>());
+}
+
+template <int ACT, class F> __device__ __forceinline__ void act_choice(int act, F&& f) {
+    if constexpr (ACT >= 0) f(std::integral_constant<int, ACT>());
+    else with_act(act, f);
+}
+template <class F> void with_act_host(int act, F&& f) {
+    if (act == FAVAE_ACT_SILU) f(std::integral_constant<int, FAVAE_ACT_SILU>());
+    else if (act == FAVAE_ACT_GELU_TANH) f(std::integral_constant<int, FAVAE_ACT_GELU_TANH>());
+    else if (act == FAVAE_ACT_LRELU) f(std::integral_constant<int, FAVAE_ACT_LRELU>());
+    else f(std::integral_constant<int, FAVAE_ACT_NONE>());
 }
 
 // ---- 8-bit activations ---------------------------------------------------------------------------------------------------

@@ -1,0 +1,4 @@
+// Backward of group norm with an activation, bf16
+#include "groupnorm_bwd.h"
+
+int gn_bwd_bf16(const GnP& p, const GnPlan& pl, hipStream_t st) { return p.q ? gn_bwd<bf16_t, true>(p, pl, st) : gn_bwd<bf16_t, false>(p, pl, st); }

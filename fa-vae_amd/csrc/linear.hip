@@ -176,7 +176,7 @@ template <class T, class OT, bool FAST> __device__ __forceinline__ void epilogue
         }
     };
     if (p.pre) put((OT*)p.pre + op);
-    act_apply<T>(f, p.act);
+    with_act(p.act, [&](auto a) __attribute__((always_inline)) { act_apply<T, decltype(a)::value>(f); });
     if (p.res) {
         const T* a = (const T*)p.res + orr;
         float t[8];
@@ -538,32 +538,33 @@ template <class T, int V, int SRC> __global__ __launch_bounds__(256) void act_bw
     float s[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) s[k] = 0.f;
-    if (j < p.N) {
+    if (j < p.N)
+        with_act(SRC == 0 ? FAVAE_ACT_NONE : p.act, [&](auto a) __attribute__((always_inline)) {
 #pragma unroll 4
-        for (long long i = r0 + w; i < r1; i += 4) {
-            typename VecOf<T, V>::raw rd;
-            float d[V];
-            rd = *(const typename VecOf<T, V>::raw*)((const T*)p.dy + i * p.lddy + j);
-            vec_get(d, rd);
-            if constexpr (SRC > 0) {
-                float z[V];
-                if constexpr (SRC == 1) vec_get(z, *(const typename VecOf<T, V>::raw*)((const T*)p.pre + i * p.ldpre + j));
-                else {
-                    const float sc = ck_scale(p.pe[i * p.ldpe + (j >> 5)]);
-                    const unsigned char* a = p.pq + i * p.ldpre + j;
-                    unsigned wd[2] = {0u, 0u};
-                    __builtin_memcpy(wd, a, V);
+            for (long long i = r0 + w; i < r1; i += 4) {
+                typename VecOf<T, V>::raw rd;
+                float d[V];
+                rd = *(const typename VecOf<T, V>::raw*)((const T*)p.dy + i * p.lddy + j);
+                vec_get(d, rd);
+                if constexpr (SRC > 0) {
+                    float z[V];
+                    if constexpr (SRC == 1) vec_get(z, *(const typename VecOf<T, V>::raw*)((const T*)p.pre + i * p.ldpre + j));
+                    else {
+                        const float sc = ck_scale(p.pe[i * p.ldpe + (j >> 5)]);
+                        const unsigned char* a8 = p.pq + i * p.ldpre + j;
+                        unsigned wd[2] = {0u, 0u};
+                        __builtin_memcpy(wd, a8, V);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) z[k] = ck_value(wd[k >> 2], k & 3, sc);
+                        for (int k = 0; k < V; ++k) z[k] = ck_value(wd[k >> 2], k & 3, sc);
+                    }
+                    act_grad_mul<T, decltype(a)::value>(d, z);
+                    vec_put(rd, d);
+                    *(typename VecOf<T, V>::raw*)((T*)p.du + i * (long long)p.N + j) = rd;
                 }
-                act_grad_mul<T>(d, z, p.act);
-                vec_put(rd, d);
-                *(typename VecOf<T, V>::raw*)((T*)p.du + i * (long long)p.N + j) = rd;
-            }
 #pragma unroll
-            for (int k = 0; k < V; ++k) s[k] += d[k];
-        }
-    }
+                for (int k = 0; k < V; ++k) s[k] += d[k];
+            }
+        });
     if (!p.part) return;
 #pragma unroll
     for (int k = 0; k < V; ++k) red[w][lane * V + k] = s[k];

@@ -25,7 +25,7 @@ _raw.favae_ckpt8_pack.argtypes = [_p, _ll, _ll, _i, _p, _ll, _p, _ll, _i, _p]
 _raw.favae_ckpt8_unpack.argtypes = [_p, _ll, _p, _ll, _ll, _i, _p, _ll, _i, _p]
 _raw.favae_gn_act_scratch.argtypes = [_ll, _ll, _i, _i, _i, _i]
 _raw.favae_gn_act_scratch.restype = _sz
-_raw.favae_gn_act_fwd.argtypes = [_p, _ll, _ll, _ll, _ll, _i, _i, _p, _p, ctypes.c_float, _i, _p, _ll, _ll, _p, _p, _p, _sz, _i, _p]
+_raw.favae_gn_act_fwd.argtypes = [_p, _ll, _ll, _ll, _ll, _i, _i, _p, _p, ctypes.c_float, _i, _p, _ll, _ll, _p, _p, _p, _p, _p, _sz, _i, _p]
 _raw.favae_gn_act_bwd.argtypes = [_p, _ll, _ll, _p, _ll, _ll, _p, _p, _ll, _ll, _i, _i, _p, _p, _p, _p, _i, _p, _ll, _ll, _p, _p, _p, _sz,
                                   _i, _p]
 _raw.favae_linear_act_fwd_scratch.argtypes = [_ll, _i, _i, _i]
@@ -160,27 +160,33 @@ def _apart(out, name, ins, may_be=None):
             raise ValueError("%s overlaps an input" % name)
 
 
-def _out(out, name, shape, dtype, dev, ins, may_be=None):
+def _out(out, name, like, shape, dtype, ins, may_be=None):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
+        return like.new_empty(shape, dtype=dtype)
+    dev = like.device
     if out.dtype != dtype or out.shape != torch.Size(shape) or out.device != dev:
         raise ValueError("%s: %s %s on %s" % (name, dtype, list(shape), dev))
     _apart(out, name, ins, may_be)
     return out
 
 
+_stream_of, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice    # torch.cuda.current_stream builds an object: 2 us
+
+
 def _call(dev, fn, *args):
     """fn(*args, stream) on the current stream of `dev`, whichever device is current."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    i = dev.index
+    if i == _current():
+        rc = fn(*args, _stream_of(i))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    L.check(rc)
+            rc = fn(*args, _stream_of(i))
+    if rc:
+        L.check(rc)
 
 
-def _scratch(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _scratch(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def _ptr(t):
@@ -188,17 +194,24 @@ def _ptr(t):
 
 
 # ---- 8-bit activations ---------------------------------------------------------------------------------------------------
+def _new_ckpt(x):
+    shape = x.shape
+    ck = Ckpt8.__new__(Ckpt8)                                # right by construction
+    ck.q = x.new_empty(shape, dtype=torch.int8)
+    ck.e = x.new_empty(shape[:-1] + ((shape[-1] + CKPT_BLOCK - 1) // CKPT_BLOCK,), dtype=torch.uint8)
+    ck.dtype = x.dtype
+    return ck
+
+
 def ckpt8_pack(x):
     """x [..., C] (fp32 or bf16, rows of any stride) -> Ckpt8."""
     code, ld, dev = _code(x, "x"), _rows(x, "x"), x.device
     _on(dev)
     c = x.shape[-1]
-    nb = (c + CKPT_BLOCK - 1) // CKPT_BLOCK
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    e = torch.empty(x.shape[:-1] + (nb,), dtype=torch.uint8, device=dev)
+    ck = _new_ckpt(x)
     if x.numel():
-        _call(dev, _raw.favae_ckpt8_pack, x.data_ptr(), ld, x.numel() // c, c, q.data_ptr(), c, e.data_ptr(), nb, code)
-    return Ckpt8(q, e, x.dtype)
+        _call(dev, _raw.favae_ckpt8_pack, x.data_ptr(), ld, x.numel() // c, c, ck.q.data_ptr(), c, ck.e.data_ptr(), ck.e.shape[-1], code)
+    return ck
 
 
 def ckpt8_unpack(ck, dtype=None, out=None):
@@ -208,7 +221,7 @@ def ckpt8_unpack(ck, dtype=None, out=None):
         raise TypeError("dtype: float32 or bfloat16")
     dev = ck.device
     _on(dev)
-    out = _out(out, "out", ck.shape, dtype, dev, (ck.q, ck.e))
+    out = _out(out, "out", ck.q, ck.shape, dtype, (ck.q, ck.e))
     c = ck.shape[-1]
     if out.numel():
         _call(dev, _raw.favae_ckpt8_unpack, ck.q.data_ptr(), c, ck.e.data_ptr(), ck.e.shape[-1], out.numel() // c, c, out.data_ptr(),
@@ -241,16 +254,19 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
     if not eps >= 0.0:
         raise ValueError("eps: not negative")
     xn, xs = _maps(x, "x")
-    y = _out(out, "out", x.shape, x.dtype, dev, (x, gamma, beta), None if ckpt else x)
+    y = _out(out, "out", x, x.shape, x.dtype, (x, gamma, beta), None if ckpt else x)
     yn, ys = _maps(y, "out")
-    stats = torch.empty(2, n, groups, dtype=F32, device=dev)
-    mean, rstd = stats[0], stats[1]
+    mean, rstd = x.new_empty((2, n, groups), dtype=F32).unbind()
+    ck = _new_ckpt(x) if ckpt else None
+    if ckpt and xn != s * xs and n > 1 and s > 1:
+        x = x.contiguous()                                   # a checkpoint is of one run of rows
+        xn, xs = s * c, c
     if n:
         nbytes = _raw.favae_gn_act_scratch(n, s, c, groups, 0, code)
-        ws = _scratch(nbytes, dev)
+        ws = _scratch(nbytes, x)
         _call(dev, _raw.favae_gn_act_fwd, x.data_ptr(), xn, xs, n, s, c, groups, g, b, eps, a, y.data_ptr(), yn, ys, mean.data_ptr(),
-              rstd.data_ptr(), _ptr(ws), nbytes, code)
-    return (y, mean, rstd, ckpt8_pack(x)) if ckpt else (y, mean, rstd)
+              rstd.data_ptr(), ck.q.data_ptr() if ckpt else None, ck.e.data_ptr() if ckpt else None, _ptr(ws), nbytes, code)
+    return (y, mean, rstd, ck) if ckpt else (y, mean, rstd)
 
 
 def group_norm_act_bwd(dy, x, groups, gamma, beta, mean, rstd, act="none", out=None):
@@ -268,15 +284,15 @@ def group_norm_act_bwd(dy, x, groups, gamma, beta, mean, rstd, act="none", out=N
             raise ValueError("%s: contiguous float32 [%d, %d]" % (name, n, groups))
     dn, ds = _maps(dy, "dy")
     xn, xs = (0, 0) if ck else _maps(x, "x")
-    dx = _out(out, "out", dy.shape, dy.dtype, dev, (dy, x.q, x.e, gamma, beta, mean, rstd) if ck else (dy, x, gamma, beta, mean, rstd), dy)
+    dx = _out(out, "out", dy, dy.shape, dy.dtype, (dy, x.q, x.e, gamma, beta, mean, rstd) if ck else (dy, x, gamma, beta, mean, rstd), dy)
     dxn, dxs = _maps(dx, "out")
-    grads = torch.empty(2, c, dtype=F32, device=dev)
+    dgamma, dbeta = dy.new_empty((2, c), dtype=F32).unbind()
     nbytes = _raw.favae_gn_act_scratch(n, s, c, groups, 1, code)
-    ws = _scratch(nbytes, dev)
+    ws = _scratch(nbytes, dy)
     _call(dev, _raw.favae_gn_act_bwd, dy.data_ptr(), dn, ds, None if ck else x.data_ptr(), xn, xs, x.q.data_ptr() if ck else None,
           x.e.data_ptr() if ck else None, n, s, c, groups, g, b, mean.data_ptr(), rstd.data_ptr(), a, dx.data_ptr(), dxn, dxs,
-          grads[0].data_ptr(), grads[1].data_ptr(), _ptr(ws), nbytes, code)
-    return dx, grads[0], grads[1]
+          dgamma.data_ptr(), dbeta.data_ptr(), _ptr(ws), nbytes, code)
+    return dx, dgamma, dbeta
 
 
 # ---- matrix product ------------------------------------------------------------------------------------------------------
@@ -298,11 +314,11 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("residual: %s %s" % (x.dtype, list(shape)))
     bp = None if bias is None else _vec(bias, n, "bias", dev)
-    y = _out(out, "out", shape, x.dtype, dev, (x, w, bias, residual), residual)
-    pre = torch.empty(shape, dtype=x.dtype, device=dev) if save_pre else None
+    y = _out(out, "out", x, shape, x.dtype, (x, w, bias, residual), residual)
+    pre = x.new_empty(shape) if save_pre else None
     if m and n:
         nbytes = _raw.favae_linear_act_fwd_scratch(m, n, k, code)
-        ws = _scratch(nbytes, dev)
+        ws = _scratch(nbytes, x)
         _call(dev, _raw.favae_linear_act_fwd, x.data_ptr(), _rows(x, "x"), w.data_ptr(), _rows(w, "w"), bp, _ptr(residual),
               0 if residual is None else _rows(residual, "residual"), _ptr(pre), n, y.data_ptr(), _rows(y, "out"), m, n, k, a, _ptr(ws), nbytes,
               code)
@@ -336,11 +352,11 @@ def linear_act_bwd(dy, x, w, act="none", pre=None, need=("x", "w", "b"), dw=None
         if dw.dtype not in (F32, w.dtype) or dw.shape != w.shape or dw.device != dev:
             raise ValueError("dw: float32 or %s, %s" % (w.dtype, list(w.shape)))
         _apart(dw, "dw", (dy, w) + ((x.q, x.e) if xck else (x,)) + ((pre.q, pre.e) if pck else (pre,)))
-    dx = torch.empty(x.shape, dtype=dy.dtype, device=dev) if "x" in need else None
-    dw = None if "w" not in need else torch.empty(n, k, dtype=w.dtype, device=dev) if dw is None else dw
-    db = torch.empty(n, dtype=F32, device=dev) if "b" in need else None
+    dx = dy.new_empty(x.shape) if "x" in need else None
+    dw = None if "w" not in need else w.new_empty((n, k)) if dw is None else dw
+    db = dy.new_empty(n, dtype=F32) if "b" in need else None
     nbytes = _raw.favae_linear_act_bwd_scratch(m, n, k, a, code)
-    ws = _scratch(nbytes, dev)
+    ws = _scratch(nbytes, dy)
     xp = x.q if xck else x
     pp = pre.q if pck else pre
     _call(dev, _raw.favae_linear_act_bwd, dy.data_ptr(), _rows(dy, "dy"), xp.data_ptr(), _rows(xp, "x"), x.e.data_ptr() if xck else None,

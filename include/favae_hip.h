@@ -616,11 +616,11 @@ int favae_ckpt8_unpack(const void* q, long long ldq, const void* e, long long ld
 
 /* y = act(gamma (x - mean) rstd + beta) over x [N][S][C] in G groups of C / G neighbouring channels; mean, rstd [N][G] fp32 out,
  * rstd = (population variance + eps)^-1/2.  Strides of a sample and of a position in elements, channels contiguous.  S = 0: mean 0,
- * variance 0.  y may be x. */
+ * variance 0.  y may be x.  q, e: x as an 8-bit checkpoint (contiguous, R = N * S rows), or both NULL. */
 size_t favae_gn_act_scratch(long long N, long long S, int C, int G, int backward, int dtype);
 int favae_gn_act_fwd(const void* x, long long xn, long long xs, long long N, long long S, int C, int G, const float* gamma,
-                     const float* beta, float eps, int act, void* y, long long yn, long long ys, float* mean, float* rstd, void* scratch,
-                     size_t scratch_bytes, int dtype, void* stream);
+                     const float* beta, float eps, int act, void* y, long long yn, long long ys, float* mean, float* rstd, void* q, void* e,
+                     void* scratch, size_t scratch_bytes, int dtype, void* stream);
 /* Its gradients from dy and either x or its checkpoint (q, e as above with R = N * S contiguous rows; mean and rstd stay those of the
  * forward pass): dx (dtype; may be dy), dgamma and dbeta [C] fp32 (NULL to skip).  Deterministic. */
 int favae_gn_act_bwd(const void* dy, long long dn, long long ds, const void* x, long long xn, long long xs, const void* q, const void* e,

@@ -94,8 +94,8 @@ def test_c_entry_points_refuse_without_a_gpu():
     for call, text in ((lambda: r.favae_ckpt8_pack(None, 8, 4, 8, None, 8, None, 1, 0, None), "favae_ckpt8_pack"),
                        (lambda: r.favae_ckpt8_pack(None, 8, -1, 8, None, 8, None, 1, 0, None), "bad sizes"),
                        (lambda: r.favae_ckpt8_unpack(None, 8, None, 1, 4, 8, None, 8, 7, None), "dtype"),
-                       (lambda: r.favae_gn_act_fwd(None, 8, 8, 1, 1, 8, 3, None, None, 1e-5, 0, None, 8, 8, None, None, None, 0, 0, None), "groups"),
-                       (lambda: r.favae_gn_act_fwd(None, 8, 8, 1, 1, 8, 2, None, None, 1e-5, 9, None, 8, 8, None, None, None, 0, 0, None), "activation"),
+                       (lambda: r.favae_gn_act_fwd(None, 8, 8, 1, 1, 8, 3, None, None, 1e-5, 0, None, 8, 8, None, None, None, None, None, 0, 0, None), "groups"),
+                       (lambda: r.favae_gn_act_fwd(None, 8, 8, 1, 1, 8, 2, None, None, 1e-5, 9, None, 8, 8, None, None, None, None, None, 0, 0, None), "activation"),
                        (lambda: r.favae_gn_act_bwd(None, 8, 8, None, 8, 8, None, None, 1, 1, 8, 2, None, None, None, None, 0, None, 8, 8, None, None, None, 0, 0, None), "null"),
                        (lambda: r.favae_linear_act_fwd(None, 8, None, 8, None, None, 0, None, 0, None, 6, 4, 6, 8, 0, None, 0, 5, None), "dtype"),
                        (lambda: r.favae_linear_act_bwd(None, 6, None, 8, None, 0, None, 8, None, 0, None, 0, 4, 6, 8, 0, None, 8, None, 8, 0, None, None, 0, 0, None), "dy")):
