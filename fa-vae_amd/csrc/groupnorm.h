@@ -5,7 +5,7 @@
 #include <type_traits>
 
 
-constexpr int GT = 512;                 // threads of a workgroup
+constexpr int GTF = 512, GTB = 256;     // threads of a workgroup, forward and backward
 constexpr int U = 4;                    // positions a thread has under way in the chunked form's second pass
 
 struct GnP {
@@ -55,7 +55,7 @@ __device__ __forceinline__ float wave_total(float v) {
 }
 
 // lanes (a power of two up to 64) that add the `per` values of each of `pairs` sums side by side
-__device__ __forceinline__ int pair_lanes(int pairs, int per) {
+template <int GT> __device__ __forceinline__ int pair_lanes(int pairs, int per) {
     int L = 64;
     while (L > 1 && (pairs * L > GT || L / 2 >= per)) L >>= 1;
     return L;
@@ -72,7 +72,7 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
         for (int o = p.LV; o < 64; o <<= 1)
 #pragma unroll
             for (int j = 0; j < NV; ++j) v[j] += __shfl_xor(v[j], o, 64);
-        rows = GT / 64;
+        rows = GTF / 64;
         if ((int)(threadIdx.x & 63) < p.LV)
 #pragma unroll
             for (int j = 0; j < NV; ++j) red[(threadIdx.x >> 6) * cols + lv * NV + j] = v[j];
@@ -82,8 +82,8 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
     }
     __syncthreads();
     // L lanes take a pair: as many as there are threads for every pair at once, at most its values
-    const int pairs = p.NSUB * ng, per = rows * cpg, L = pair_lanes(pairs, per), l = (int)threadIdx.x & (L - 1);
-    for (int k = (int)threadIdx.x / L; k < pairs; k += GT / L) {
+    const int pairs = p.NSUB * ng, per = rows * cpg, L = pair_lanes<GTF>(pairs, per), l = (int)threadIdx.x & (L - 1);
+    for (int k = (int)threadIdx.x / L; k < pairs; k += GTF / L) {
         const int sub = k / ng, g = k - sub * ng;
         float s = 0.f;
         for (int i = l; i < per; i += L) {
@@ -165,9 +165,9 @@ template <int VEC, bool GS> struct GnStat {
         else { if ((vec) == 8) F(T, 8) else if ((vec) == 2) F(T, 2) else F(T, 1) }     \
     } while (0)
 
-template <class K> int gn_launch(K k, const GnP& p, size_t lds, hipStream_t st) {
+template <class K> int gn_launch(K k, const GnP& p, int threads, size_t lds, hipStream_t st) {
     FAVAE_CHECK_ARG(p.blocks <= 0x7fffffffLL, "favae_gn_act: too many samples for one launch");
-    if (p.blocks > 0) k<<<(unsigned)p.blocks, GT, lds, st>>>(p);
+    if (p.blocks > 0) k<<<(unsigned)p.blocks, threads, lds, st>>>(p);
     FAVAE_LAUNCH_CHECK();
     return FAVAE_OK;
 }

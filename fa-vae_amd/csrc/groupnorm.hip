@@ -19,7 +19,7 @@ namespace {
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
 // STATS: leave (mean, sum of squared distances) of this chunk in part[((n G + g) nchunk + chunk) pieces + piece] and stop.
-template <class T, int VEC, int ITEMS, bool GS, bool STATS> __global__ __launch_bounds__(GT) void gn_fwd_kernel(const GnP p) {
+template <class T, int VEC, int ITEMS, bool GS, bool STATS> __global__ __launch_bounds__(GTF) void gn_fwd_kernel(const GnP p) {
     extern __shared__ float lds[];
     constexpr int NV = GS ? 1 : VEC;
     const long long lb = xcd_order(blockIdx.x, p.blocks);
@@ -35,7 +35,7 @@ template <class T, int VEC, int ITEMS, bool GS, bool STATS> __global__ __launch_
     const int s_lo = chunk * p.chunk, s_hi = min(p.S, s_lo + p.chunk);
     const bool active = sub < p.NSUB && n < p.N && c0 < b.c_hi;
     float* red = lds;
-    float* grp = lds + GT * NV;
+    float* grp = lds + GTF * NV;
 
     GnData<T, VEC> d[ITEMS];
 #pragma unroll
@@ -69,9 +69,9 @@ template <class T, int VEC, int ITEMS, bool GS, bool STATS> __global__ __launch_
     }
     float keep_mean = 0.f;                       // a pair's mean, by the thread that stores it
     const int pairs = p.NSUB * b.ng;
-    if ((int)threadIdx.x < pairs && pairs <= GT) keep_mean = grp[threadIdx.x] * inv;
-    if (pairs > GT)                              // more pairs than threads: through memory at once (grp is reused below)
-        for (int k = threadIdx.x; k < pairs; k += GT) {
+    if ((int)threadIdx.x < pairs && pairs <= GTF) keep_mean = grp[threadIdx.x] * inv;
+    if (pairs > GTF)                              // more pairs than threads: through memory at once (grp is reused below)
+        for (int k = threadIdx.x; k < pairs; k += GTF) {
             const long long nn = nb0 * p.NSUB + k / b.ng;
             if (nn < p.N) {
                 if constexpr (STATS) p.part[((nn * p.G + b.g_lo + k % b.ng) * p.nchunk + chunk) * p.pieces + b.piece].x = grp[k] * inv;
@@ -89,16 +89,16 @@ template <class T, int VEC, int ITEMS, bool GS, bool STATS> __global__ __launch_
         }
     }
     gn_reduce<NV>(p, v, red, grp, lv, r, b.ng, cpg);
-    for (int k = threadIdx.x; k < pairs; k += GT) {
+    for (int k = threadIdx.x; k < pairs; k += GTF) {
         const long long nn = nb0 * p.NSUB + k / b.ng;
         const int g = b.g_lo + k % b.ng;
         if (nn < p.N) {
             if constexpr (STATS) {
                 float2* o = p.part + ((nn * p.G + g) * p.nchunk + chunk) * p.pieces + b.piece;
-                if (pairs <= GT) o->x = keep_mean;
+                if (pairs <= GTF) o->x = keep_mean;
                 o->y = grp[k];
             } else {
-                if (pairs <= GT) p.mean[nn * p.G + g] = keep_mean;
+                if (pairs <= GTF) p.mean[nn * p.G + g] = keep_mean;
                 p.rstd[nn * p.G + g] = 1.f / sqrtf(grp[k] * inv + p.eps);
             }
         }
@@ -143,7 +143,7 @@ template <class T, int VEC, int ITEMS, bool GS, bool STATS> __global__ __launch_
 }
 
 // Chunked form, second launch: join the chunks of this block's groups (mean of means, and sums of squared distances moved to it), normalise.
-template <class T, int VEC, bool GS> __global__ __launch_bounds__(GT) void gn_apply_kernel(const GnP p) {
+template <class T, int VEC, bool GS> __global__ __launch_bounds__(GTF) void gn_apply_kernel(const GnP p) {
     extern __shared__ float lds[];
     const long long lb = xcd_order(blockIdx.x, p.blocks);
     const int cb = (int)(lb % p.ncb);
@@ -153,7 +153,7 @@ template <class T, int VEC, bool GS> __global__ __launch_bounds__(GT) void gn_ap
     const GnBlock b = gn_block(p, cb);
     const int parts = p.nchunk * p.pieces;
     float2* stat = (float2*)lds;                 // [ng] (mean, rstd)
-    for (int g = threadIdx.x >> 6; g < b.ng; g += GT / 64) {
+    for (int g = threadIdx.x >> 6; g < b.ng; g += GTF / 64) {
         const float2* a = p.part + (n * p.G + b.g_lo + g) * parts;
         const float m = (float)p.S * (float)p.Cg;
         float s = 0.f, q = 0.f;
@@ -239,6 +239,7 @@ __global__ __launch_bounds__(512) void gn_param_grad_kernel(const float2* __rest
 
 GnPlan gn_plan(GnP& p, int es, int vec_max, bool backward) {
     GnPlan pl;
+    const int GT = backward ? GTB : GTF;
     // widest vector whose whole-group blocks (or pieces of one group) start on vector borders
     int vec = vec_max;
     for (;; vec = vec > 2 ? 2 : 1) {
@@ -270,9 +271,10 @@ GnPlan gn_plan(GnP& p, int es, int vec_max, bool backward) {
         p.shuf = p.NSUB == 1 && p.LV <= 32 && (p.LV & (p.LV - 1)) == 0 && p.P * p.LV == GT;
     };
     lanes();
-    // a run of groups that does not fit a workgroup's registers may fit with fewer channels side by side (the blocks that share its
-    // cache lines run on one XCD): down to 32 bytes
-    while (p.pieces == 1 && cdiv(p.S, p.P) > ITEMS_MAX && p.CB % 2 == 0 && (p.CB / 2) % unit == 0 && p.CB / 2 * es >= 32) {
+    // fewer channels side by side, down to 32 bytes, where a run of groups does not fit a workgroup's registers or where there would be
+    // fewer workgroups than CUs (the blocks that share a cache line run on one XCD)
+    while (p.pieces == 1 && p.CB % 2 == 0 && (p.CB / 2) % unit == 0 && p.CB / 2 * es >= 32 &&
+           (cdiv(p.S, p.P) > ITEMS_MAX || (p.S * (long long)p.CB > 16 * vec * 64 && cdivll(p.N, p.NSUB) * p.ncb < 512))) {
         p.CB /= 2;
         p.ncb = cdiv(p.C, p.CB);
         lanes();
@@ -288,13 +290,15 @@ GnPlan gn_plan(GnP& p, int es, int vec_max, bool backward) {
         pl.blocks = backward ? std::min<long long>(cdivll(p.N, p.NSUB), std::max(1, 2048 / p.ncb)) * p.ncb : held_blocks;
         pl.part = backward ? (size_t)(pl.blocks / p.ncb) * p.C : 0;
     } else {
+        while (p.pieces == 1 && p.CB * es < 128 && p.CB * 2 <= std::min(cap, p.C)) p.CB *= 2;   // whole cache lines again
+        if (p.pieces == 1) { p.ncb = cdiv(p.C, p.CB); p.LV = cdiv(p.CB, vec); }
         p.NSUB = 1;
         p.P = std::max(1, GT / p.LV);
         p.shuf = p.LV <= 32 && (p.LV & (p.LV - 1)) == 0 && p.P * p.LV == GT;
         pl.items = ITEMS_MAX;
-        // chunks of what a workgroup holds, shorter where that leaves the chip empty
-        long long chunk = (long long)p.P * ITEMS_MAX;
-        while (chunk > 4 * p.P && (long long)p.N * p.ncb * cdivll(p.S, chunk) < 512) chunk /= 2;
+        // forward: chunks of what a workgroup holds, shorter where that leaves the chip empty; backward: about 4096 workgroups
+        long long chunk = backward ? cdivll(cdivll((long long)p.N * p.ncb * p.S, 4096), 4 * p.P) * 4 * p.P : (long long)p.P * ITEMS_MAX;
+        while (chunk > 4 * p.P && (long long)p.N * p.ncb * cdivll(p.S, chunk) < 512) chunk = cdivll(chunk / 2, p.P) * p.P;
         p.chunk = (int)std::min<long long>(chunk, std::max(1, p.S));
         p.nchunk = std::max(1, cdiv(p.S, p.chunk));
         pl.blocks = (long long)p.N * p.ncb * p.nchunk;
@@ -322,12 +326,12 @@ int vec_of(const GnP& p, int es, bool backward) {
 }
 
 template <class T, int VEC, bool GS> int gn_fwd_t(const GnP& p, const GnPlan& pl, hipStream_t st) {
-    const size_t lds = sizeof(float) * ((size_t)GT * (GS ? 1 : VEC) + (size_t)p.NSUB * cdiv(p.CB, std::min(p.Cg, p.CB)));
+    const size_t lds = sizeof(float) * ((size_t)GTF * (GS ? 1 : VEC) + (size_t)p.NSUB * cdiv(p.CB, std::min(p.Cg, p.CB)));
     if (pl.held)
-        return pl.items <= 4 ? gn_launch(gn_fwd_kernel<T, VEC, 4, GS, false>, p, lds, st) : gn_launch(gn_fwd_kernel<T, VEC, ITEMS_MAX, GS, false>, p, lds, st);
-    const int rc = gn_launch(gn_fwd_kernel<T, VEC, ITEMS_MAX, GS, true>, p, lds, st);
+        return pl.items <= 4 ? gn_launch(gn_fwd_kernel<T, VEC, 4, GS, false>, p, GTF, lds, st) : gn_launch(gn_fwd_kernel<T, VEC, ITEMS_MAX, GS, false>, p, GTF, lds, st);
+    const int rc = gn_launch(gn_fwd_kernel<T, VEC, ITEMS_MAX, GS, true>, p, GTF, lds, st);
     if (rc != FAVAE_OK) return rc;
-    return gn_launch(gn_apply_kernel<T, VEC, GS>, p, sizeof(float2) * cdiv(p.CB, std::min(p.Cg, p.CB)), st);
+    return gn_launch(gn_apply_kernel<T, VEC, GS>, p, GTF, sizeof(float2) * cdiv(p.CB, std::min(p.Cg, p.CB)), st);
 }
 template <class T> int gn_fwd(const GnP& p, const GnPlan& pl, hipStream_t st) {
 #define GN_F(T_, V) { if constexpr (V == 1) return gn_fwd_t<T_, V, true>(p, pl, st); else return pl.gs ? gn_fwd_t<T_, V, true>(p, pl, st) : gn_fwd_t<T_, V, false>(p, pl, st); }

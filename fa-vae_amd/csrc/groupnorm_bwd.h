@@ -4,6 +4,7 @@
 
 namespace {
 
+
 // ---- backward ------------------------------------------------------------------------------------------------------------
 // Column sums (dz, dz xh) of a block's threads into tot[sub][CB] (float2).  red: [rows][CB] float2.
 template <int VEC>
@@ -14,7 +15,7 @@ __device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float 
         for (int o = p.LV; o < 64; o <<= 1)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) { a[j] += __shfl_xor(a[j], o, 64); bq[j] += __shfl_xor(bq[j], o, 64); }
-        rows = GT / 64;
+        rows = GTB / 64;
         if ((int)(threadIdx.x & 63) < p.LV)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) red[(threadIdx.x >> 6) * cols + lv * VEC + j] = make_float2(a[j], bq[j]);
@@ -23,7 +24,7 @@ __device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float 
         for (int j = 0; j < VEC; ++j) red[r * cols + lv * VEC + j] = make_float2(a[j], bq[j]);
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < p.NSUB * cols; k += GT) {
+    for (int k = threadIdx.x; k < p.NSUB * cols; k += GTB) {
         const int sub = k / cols, c = k - sub * cols;
         float2 s = make_float2(0.f, 0.f);
         for (int i = 0; i < rows; ++i) {
@@ -35,34 +36,30 @@ __device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float 
     __syncthreads();
 }
 
-// ACT: the activation, or -1: p.act (a choice inside the kernel costs the wide held form its last registers).
-// SUMS: leave the column sums of the chunk in part[(n nchunk + chunk) C + c] and stop.  Otherwise the block takes samples blockIdx,
-// + gridDim, ...: dx, and its column sums over all of them in part[blockIdx C + c].
+// Held form: the block takes samples blockIdx, + gridDim, ...: dx, and its column sums over all of them in part[blockIdx C + c].
+// ACT: the activation, or -1: p.act (a choice inside the kernel costs the wide form its last registers).
 // Lanes without a channel, a sample or a position read the last valid one instead and count for nothing, so that only stores are
 // under a lane mask.  Items are kept one after the other: interleaved by the compiler they would need the registers of all at once.
-template <class T, int VEC, int ITEMS, bool GS, bool CK, bool SUMS, int ACT> __global__ __launch_bounds__(GT) void gn_bwd_kernel(const GnP p) {
+template <class T, int VEC, int ITEMS, bool GS, bool CK, int ACT> __global__ __launch_bounds__(GTB) void gn_bwd_kernel(const GnP p) {
     extern __shared__ float lds[];
     const int cols = p.LV * VEC;
     float2* red = (float2*)lds;
-    float2* tot = red + (p.shuf ? (GT / 64) * cols : p.P * p.NSUB * cols);
+    float2* tot = red + (p.shuf ? (GTB / 64) * cols : p.P * p.NSUB * cols);
     float2* grp = tot + p.NSUB * cols;           // [NSUB][ng]
     float2* acc = grp + p.NSUB * cols;           // [cols] (held form)
     const long long lb = xcd_order(blockIdx.x, p.blocks);
     const int cb = (int)(lb % p.ncb);
     const long long t_ = lb / p.ncb;
-    const int chunk = SUMS ? (int)(t_ % p.nchunk) : 0;
-    const long long first = SUMS ? t_ / p.nchunk : t_;
-    const long long stride = SUMS ? p.N : p.blocks / p.ncb;
+    const long long first = t_, stride = p.blocks / p.ncb;
     const GnBlock b = gn_block(p, cb);
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
     const int sub = r / p.P;
     int pos = r - sub * p.P;
-    const int s_lo = chunk * p.chunk, last = min(p.S, s_lo + p.chunk) - 1;
+    const int last = p.S - 1;
     const bool col_ok = sub < p.NSUB && b.c_lo + lv * VEC < b.c_hi;
     const int c0 = min(b.c_lo + lv * VEC, b.c_hi - VEC);
-    const int gl = p.pieces == 1 ? (c0 - b.c_lo) / p.Cg : 0;
-    if constexpr (!SUMS)
-        for (int k = threadIdx.x; k < cols; k += GT) acc[k] = make_float2(0.f, 0.f);
+    const int gl = (c0 - b.c_lo) / p.Cg;
+    for (int k = threadIdx.x; k < cols; k += GTB) acc[k] = make_float2(0.f, 0.f);
     const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
     for (long long nb0 = first; nb0 * p.NSUB < p.N; nb0 += stride) {
         const long long n0 = nb0 * p.NSUB + sub, n = min(n0, (long long)p.N - 1);
@@ -72,19 +69,19 @@ template <class T, int VEC, int ITEMS, bool GS, bool CK, bool SUMS, int ACT> __g
         typename std::conditional<CK, CkData<VEC>, GnData<T, VEC>>::type xv[ITEMS];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int s = min(s_lo + pos + i * p.P, last);
+            const int s = min(pos + i * p.P, last);
             if constexpr (CK) xv[i].load(p.q, p.e, n * p.S + s, p.C, p.nb, c0);
             else xv[i].load(p.x, n * p.xn + s * p.xs + c0);
             d[i].load(p.dy, n * p.dn + s * p.ds + c0);
         }
         GnStat<VEC, GS> st;
         float a[VEC];                                // gamma rstd
-        float dz[SUMS ? 1 : ITEMS][VEC];             // held: its exp and reciprocal are half the work of a pass
+        float dz[ITEMS][VEC];             // held: its exp and reciprocal are half the work of a pass
         {
             float be[VEC], sa[VEC], sb[VEC];
 #pragma unroll
             for (int j = 0; j < (GS ? 1 : VEC); ++j) {
-                const int g = b.g_lo + (GS ? gl : p.pieces == 1 ? (c0 - b.c_lo + j) / p.Cg : 0);
+                const int g = b.g_lo + (GS ? gl : (c0 - b.c_lo + j) / p.Cg);
                 st.m[j] = p.mean[n * p.G + g];
                 st.r[j] = p.rstd[n * p.G + g];
             }
@@ -94,7 +91,7 @@ template <class T, int VEC, int ITEMS, bool GS, bool CK, bool SUMS, int ACT> __g
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) {
                     float x[VEC], z[VEC], g[VEC];
-                    if (!(active && s_lo + pos + i * p.P <= last)) d[i].v = typename VecOf<T, VEC>::raw{};
+                    if (!(active && pos + i * p.P <= last)) d[i].v = typename VecOf<T, VEC>::raw{};
                     xv[i].get(x);
                     d[i].get(g);
 #pragma unroll
@@ -103,7 +100,7 @@ template <class T, int VEC, int ITEMS, bool GS, bool CK, bool SUMS, int ACT> __g
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
                         sa[j] += g[j]; sb[j] = fmaf(g[j], x[j], sb[j]);
-                        if constexpr (!SUMS) dz[i][j] = g[j];
+                        dz[i][j] = g[j];
                     }
                     xv[i].keep();
                     __builtin_amdgcn_sched_barrier(0);
@@ -113,57 +110,125 @@ template <class T, int VEC, int ITEMS, bool GS, bool CK, bool SUMS, int ACT> __g
             for (int j = 0; j < VEC; ++j) sb[j] *= st.rstd(j);
             gn_columns<VEC>(p, sa, sb, red, tot, lv, r);
         }
-        if constexpr (SUMS) {
-            for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GT) p.part[(nb0 * p.nchunk + chunk) * p.C + b.c_lo + k] = tot[k];
-        } else {
-            for (int k = threadIdx.x; k < cols; k += GT) {
-                float2 t = acc[k];
-                for (int u = 0; u < p.NSUB; ++u) { t.x += tot[u * cols + k].x; t.y += tot[u * cols + k].y; }
-                acc[k] = t;
+        for (int k = threadIdx.x; k < cols; k += GTB) {
+            float2 t = acc[k];
+            for (int u = 0; u < p.NSUB; ++u) { t.x += tot[u * cols + k].x; t.y += tot[u * cols + k].y; }
+            acc[k] = t;
+        }
+        const int pairs = p.NSUB * b.ng;
+        const int L = pair_lanes<GTB>(pairs, b.cw), l = (int)threadIdx.x & (L - 1);
+        for (int k = (int)threadIdx.x / L; k < pairs; k += GTB / L) {
+            const int u = k / b.ng, g = k - u * b.ng;
+            float2 s = make_float2(0.f, 0.f);
+            for (int c = g * b.cw + l; c < (g + 1) * b.cw; c += L) {
+                const float2 t = tot[u * cols + c];
+                const float w = p.gamma[b.c_lo + c];
+                s.x = fmaf(w, t.x, s.x); s.y = fmaf(w, t.y, s.y);
             }
-            const int pairs = p.NSUB * b.ng;
-            const int L = pair_lanes(pairs, b.cw), l = (int)threadIdx.x & (L - 1);
-            for (int k = (int)threadIdx.x / L; k < pairs; k += GT / L) {
-                const int u = k / b.ng, g = k - u * b.ng;
-                float2 s = make_float2(0.f, 0.f);
-                for (int c = g * b.cw + l; c < (g + 1) * b.cw; c += L) {
-                    const float2 t = tot[u * cols + c];
-                    const float w = p.gamma[b.c_lo + c];
-                    s.x = fmaf(w, t.x, s.x); s.y = fmaf(w, t.y, s.y);
-                }
-                for (int o = L >> 1; o > 0; o >>= 1) { s.x += __shfl_xor(s.x, o, 64); s.y += __shfl_xor(s.y, o, 64); }
-                if (l == 0) grp[k] = s;
-            }
-            __syncthreads();
-            asm volatile("" : "+v"(pos));
-            GnStat<VEC, GS> cc;                      // c1, c2 of the groups
+            for (int o = L >> 1; o > 0; o >>= 1) { s.x += __shfl_xor(s.x, o, 64); s.y += __shfl_xor(s.y, o, 64); }
+            if (l == 0) grp[k] = s;
+        }
+        __syncthreads();
+        asm volatile("" : "+v"(pos));
+        GnStat<VEC, GS> cc;                      // c1, c2 of the groups
 #pragma unroll
-            for (int j = 0; j < (GS ? 1 : VEC); ++j) {
-                const float2 t = grp[min(sub, p.NSUB - 1) * b.ng + (GS ? gl : (c0 - b.c_lo + j) / p.Cg)];
-                cc.m[j] = st.r[j] * t.x * inv_m;
-                cc.r[j] = st.r[j] * st.r[j] * (t.y * inv_m);
-            }
+        for (int j = 0; j < (GS ? 1 : VEC); ++j) {
+            const float2 t = grp[min(sub, p.NSUB - 1) * b.ng + (GS ? gl : (c0 - b.c_lo + j) / p.Cg)];
+            cc.m[j] = st.r[j] * t.x * inv_m;
+            cc.r[j] = st.r[j] * st.r[j] * (t.y * inv_m);
+        }
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                const int s = s_lo + pos + i * p.P;
+        for (int i = 0; i < ITEMS; ++i) {
+            const int s = pos + i * p.P;
+            float x[VEC], g[VEC];
+            xv[i].get(x);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) g[j] = fmaf(st.mean(j) - x[j], cc.rstd(j), fmaf(a[j], dz[i][j], -cc.mean(j)));
+            typename VecOf<T, VEC>::raw o;
+            vec_put(o, g);
+            if (active && s <= last) *(typename VecOf<T, VEC>::raw*)((T*)p.y + n * p.yn + s * p.ys + c0) = o;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();                              // red, tot and grp are free again
+    }
+    for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTB) p.part[first * p.C + b.c_lo + k] = acc[k];
+}
+
+// f(x, dy, s) for positions s, s + P, ... below s_hi, U of them loaded at a time
+template <class T, int VEC, bool CK, class F> __device__ __forceinline__ void gn_walk(const GnP& p, long long n, int s, int s_hi, int c0, F&& f) {
+    for (; s < s_hi; s += U * p.P) {
+        typename std::conditional<CK, CkData<VEC>, GnData<T, VEC>>::type xv[U];
+        GnData<T, VEC> d[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int t = s + u * p.P;
+            if (t < s_hi) {
+                if constexpr (CK) xv[u].load(p.q, p.e, n * p.S + t, p.C, p.nb, c0);
+                else xv[u].load(p.x, n * p.xn + t * p.xs + c0);
+                d[u].load(p.dy, n * p.dn + t * p.ds + c0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int t = s + u * p.P;
+            if (t < s_hi) {
                 float x[VEC], g[VEC];
-                xv[i].get(x);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) g[j] = fmaf(st.mean(j) - x[j], cc.rstd(j), fmaf(a[j], dz[i][j], -cc.mean(j)));
-                typename VecOf<T, VEC>::raw o;
-                vec_put(o, g);
-                if (active && s <= last) *(typename VecOf<T, VEC>::raw*)((T*)p.y + n * p.yn + s * p.ys + c0) = o;
-                __builtin_amdgcn_sched_barrier(0);
+                xv[u].get(x);
+                d[u].get(g);
+                f(x, g, t);
             }
-            __syncthreads();                          // red, tot and grp are free again
         }
     }
-    if constexpr (!SUMS)
-        for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GT) p.part[first * p.C + b.c_lo + k] = acc[k];
+}
+
+// Chunked form, first launch: column sums of a chunk of positions in part[(n nchunk + chunk) C + c].
+template <class T, int VEC, bool GS, bool CK> __global__ __launch_bounds__(GTB) void gn_bwd_sums_kernel(const GnP p) {
+    extern __shared__ float lds[];
+    const int cols = p.LV * VEC;
+    float2* red = (float2*)lds;
+    float2* tot = red + (p.shuf ? GTB / 64 : p.P) * cols;
+    const long long lb = xcd_order(blockIdx.x, p.blocks);
+    const int cb = (int)(lb % p.ncb);
+    const long long t_ = lb / p.ncb;
+    const int chunk = (int)(t_ % p.nchunk);
+    const long long n = t_ / p.nchunk;
+    const GnBlock b = gn_block(p, cb);
+    const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
+    const int c0 = b.c_lo + lv * VEC;
+    float sa[VEC], sb[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sa[j] = sb[j] = 0.f;
+    if (r < p.P && c0 < b.c_hi) {
+        GnStat<VEC, GS> st;
+        float a[VEC], be[VEC];
+#pragma unroll
+        for (int j = 0; j < (GS ? 1 : VEC); ++j) {
+            const int g = b.g_lo + (p.pieces == 1 ? (lv * VEC + j) / p.Cg : 0);
+            st.m[j] = p.mean[n * p.G + g];
+            st.r[j] = p.rstd[n * p.G + g];
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { a[j] = p.gamma[c0 + j] * st.rstd(j); be[j] = p.beta[c0 + j]; }
+        const int s_hi = min(p.S, (chunk + 1) * p.chunk);
+        with_act(p.act, [&](auto act) __attribute__((always_inline)) {
+            gn_walk<T, VEC, CK>(p, n, chunk * p.chunk + r, s_hi, c0, [&](float (&x)[VEC], float (&g)[VEC], int s) __attribute__((always_inline)) {
+                float z[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) { x[j] -= st.mean(j); z[j] = fmaf(x[j], a[j], be[j]); }
+                act_grad_mul<T, decltype(act)::value>(g, z);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) { sa[j] += g[j]; sb[j] = fmaf(g[j], x[j], sb[j]); }
+            });
+        });
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sb[j] *= st.rstd(j);
+    }
+    gn_columns<VEC>(p, sa, sb, red, tot, lv, r);
+    for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTB) p.part[(n * p.nchunk + chunk) * p.C + b.c_lo + k] = tot[k];
 }
 
 // Chunked form, second launch: s1 and s2 of this block's groups from the column sums of every chunk, then dx.
-template <class T, int VEC, bool GS, bool CK> __global__ __launch_bounds__(GT) void gn_bwd_apply_kernel(const GnP p) {
+template <class T, int VEC, bool GS, bool CK> __global__ __launch_bounds__(GTB) void gn_bwd_apply_kernel(const GnP p) {
     extern __shared__ float lds[];
     float2* grp = (float2*)lds;
     const long long lb = xcd_order(blockIdx.x, p.blocks);
@@ -173,7 +238,7 @@ template <class T, int VEC, bool GS, bool CK> __global__ __launch_bounds__(GT) v
     const long long n = t_ / p.nchunk;
     const GnBlock b = gn_block(p, cb);
     const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
-    for (int g = threadIdx.x >> 6; g < b.ng; g += GT / 64) {
+    for (int g = threadIdx.x >> 6; g < b.ng; g += GTB / 64) {
         float2 s = make_float2(0.f, 0.f);
         for (int i = threadIdx.x & 63; i < p.nchunk * p.Cg; i += 64) {
             const int ch = i / p.Cg, c = (b.g_lo + g) * p.Cg + (i - ch * p.Cg);
@@ -201,59 +266,40 @@ template <class T, int VEC, bool GS, bool CK> __global__ __launch_bounds__(GT) v
     for (int j = 0; j < VEC; ++j) { a[j] = p.gamma[c0 + j] * st.rstd(j); be[j] = p.beta[c0 + j]; }
     const int s_hi = min(p.S, (chunk + 1) * p.chunk);
     with_act(p.act, [&](auto act) __attribute__((always_inline)) {
-        for (int s0 = chunk * p.chunk + r; s0 < s_hi; s0 += U * p.P) {
-            typename std::conditional<CK, CkData<VEC>, GnData<T, VEC>>::type xv[U];
-            GnData<T, VEC> d[U];
+        gn_walk<T, VEC, CK>(p, n, chunk * p.chunk + r, s_hi, c0, [&](float (&x)[VEC], float (&g)[VEC], int s) __attribute__((always_inline)) {
+            float z[VEC];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int s = s0 + u * p.P;
-                if (s < s_hi) {
-                    if constexpr (CK) xv[u].load(p.q, p.e, n * p.S + s, p.C, p.nb, c0);
-                    else xv[u].load(p.x, n * p.xn + s * p.xs + c0);
-                    d[u].load(p.dy, n * p.dn + s * p.ds + c0);
-                }
-            }
+            for (int j = 0; j < VEC; ++j) { x[j] -= st.mean(j); z[j] = fmaf(x[j], a[j], be[j]); }
+            act_grad_mul<T, decltype(act)::value>(g, z);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int s = s0 + u * p.P;
-                if (s < s_hi) {
-                    float x[VEC], z[VEC], g[VEC];
-                    xv[u].get(x);
-                    d[u].get(g);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) { x[j] -= st.mean(j); z[j] = fmaf(x[j], a[j], be[j]); }
-                    act_grad_mul<T, decltype(act)::value>(g, z);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) g[j] = fmaf(-x[j], cc.rstd(j), fmaf(a[j], g[j], -cc.mean(j)));
-                    typename VecOf<T, VEC>::raw o;
-                    vec_put(o, g);
-                    *(typename VecOf<T, VEC>::raw*)((T*)p.y + n * p.yn + s * p.ys + c0) = o;
-                }
-            }
-        }
+            for (int j = 0; j < VEC; ++j) g[j] = fmaf(-x[j], cc.rstd(j), fmaf(a[j], g[j], -cc.mean(j)));
+            typename VecOf<T, VEC>::raw o;
+            vec_put(o, g);
+            *(typename VecOf<T, VEC>::raw*)((T*)p.y + n * p.yn + s * p.ys + c0) = o;
+        });
     });
 }
 
 template <class T, int VEC, bool GS, bool CK> int gn_bwd_t(const GnP& p, const GnPlan& pl, hipStream_t st) {
     const int cols = p.LV * VEC;
-    const size_t lds = sizeof(float2) * ((size_t)(p.shuf ? GT / 64 : p.P * p.NSUB) * cols + 2 * (size_t)p.NSUB * cols + cols);
+    const size_t lds = sizeof(float2) * ((size_t)(p.shuf ? GTB / 64 : p.P * p.NSUB) * cols + 2 * (size_t)p.NSUB * cols + cols);
     if (!pl.held) {
-        const int rc = gn_launch(gn_bwd_kernel<T, VEC, ITEMS_MAX, GS, CK, true, -1>, p, lds, st);
+        const int rc = gn_launch(gn_bwd_sums_kernel<T, VEC, GS, CK>, p, GTB, lds, st);
         if (rc != FAVAE_OK) return rc;
-        return gn_launch(gn_bwd_apply_kernel<T, VEC, GS, CK>, p, sizeof(float2) * cdiv(p.CB, std::min(p.Cg, p.CB)), st);
+        return gn_launch(gn_bwd_apply_kernel<T, VEC, GS, CK>, p, GTB, sizeof(float2) * cdiv(p.CB, std::min(p.Cg, p.CB)), st);
     }
     if constexpr (VEC * sizeof(T) == 16) {
         int rc = FAVAE_OK;
         with_act_host(p.act, [&](auto act) {
             constexpr int A = decltype(act)::value;
-            if (pl.items <= 4) rc = gn_launch(gn_bwd_kernel<T, VEC, 4, GS, CK, false, A>, p, lds, st);
-            else if (pl.items <= 8) rc = gn_launch(gn_bwd_kernel<T, VEC, 8, GS, CK, false, A>, p, lds, st);
-            else rc = gn_launch(gn_bwd_kernel<T, VEC, ITEMS_MAX, GS, CK, false, A>, p, lds, st);
+            if (pl.items <= 4) rc = gn_launch(gn_bwd_kernel<T, VEC, 4, GS, CK, A>, p, GTB, lds, st);
+            else if (pl.items <= 8) rc = gn_launch(gn_bwd_kernel<T, VEC, 8, GS, CK, A>, p, GTB, lds, st);
+            else rc = gn_launch(gn_bwd_kernel<T, VEC, ITEMS_MAX, GS, CK, A>, p, GTB, lds, st);
         });
         return rc;
     } else {
-        return pl.items <= 4 ? gn_launch(gn_bwd_kernel<T, VEC, 4, GS, CK, false, -1>, p, lds, st)
-                             : gn_launch(gn_bwd_kernel<T, VEC, ITEMS_MAX, GS, CK, false, -1>, p, lds, st);
+        return pl.items <= 4 ? gn_launch(gn_bwd_kernel<T, VEC, 4, GS, CK, -1>, p, GTB, lds, st)
+                             : gn_launch(gn_bwd_kernel<T, VEC, ITEMS_MAX, GS, CK, -1>, p, GTB, lds, st);
     }
 }
 template <class T, bool CK> int gn_bwd(const GnP& p, const GnPlan& pl, hipStream_t st) {

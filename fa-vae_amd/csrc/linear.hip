@@ -33,8 +33,6 @@ typedef unsigned v4u __attribute__((ext_vector_type(4)));
 struct GemmP {
     const char *P, *Q;                    // operands
     long long ldp, ldq;                   // elements
-    const unsigned char* qe;              // exponents of Q where it is an 8-bit checkpoint
-    long long ldqe;
     long long I, Cn;                      // output rows, reduction length
     int J;                                // output columns
     long long cchunk;                     // reduction elements of a split (a multiple of BK)
@@ -96,16 +94,15 @@ template <class T, int ROWS, bool CM, int BKE_ = 128 / (int)sizeof(T)> struct Ti
     }
 };
 
-// Staging of one operand's tile.  REG: through registers, any alignment, any tail; CKPT: the operand is an 8-bit checkpoint.
-enum { S_REG = 0, S_CKPT = 1 };
+// Staging of one operand's tile through registers: any alignment, any tail
 
-template <class T, int ROWS, bool CM, int MODE, int NT, int BKE = 128 / (int)sizeof(T)> struct Stager {
+template <class T, int ROWS, bool CM, int NT, int BKE = 128 / (int)sizeof(T)> struct Stager {
     typedef TileImg<T, ROWS, CM, BKE> Img;
     static constexpr int NC = Img::CHUNKS / NT;
     static_assert(Img::CHUNKS % NT == 0, "whole chunks per thread");
     uint4 v[NC];
     // o0: first output row of the tile, no: output rows that exist; c0: first reduction element, cn: end of this split
-    __device__ __forceinline__ void load(const GemmP& p, const char* base, long long ld, long long o0, long long no, long long c0, long long cn) {
+    __device__ __forceinline__ void load(const char* base, long long ld, long long o0, long long no, long long c0, long long cn) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             const int c = (int)threadIdx.x + i * NT, row = c / Img::CPR, ch = c - row * Img::CPR;
@@ -114,24 +111,13 @@ template <class T, int ROWS, bool CM, int MODE, int NT, int BKE = 128 / (int)siz
             const long long cc = (CM ? o0 : c0) + ch * Img::VE, ce = CM ? no : cn;
             uint4 t = make_uint4(0u, 0u, 0u, 0u);
             if (rr < rn && cc < ce) {
-                if constexpr (MODE == S_REG) {
-                    const T* a = (const T*)base + rr * ld + cc;
-                    if (cc + Img::VE <= ce) __builtin_memcpy(&t, a, 16);
-                    else {
-                        T tmp[Img::VE];
+                const T* a = (const T*)base + rr * ld + cc;
+                if (cc + Img::VE <= ce) __builtin_memcpy(&t, a, 16);
+                else {
+                    T tmp[Img::VE];
 #pragma unroll
-                        for (int j = 0; j < Img::VE; ++j) tmp[j] = cc + j < ce ? a[j] : (T)0;
-                        __builtin_memcpy(&t, tmp, 16);
-                    }
-                } else {
-                    const unsigned char* a = (const unsigned char*)base + rr * ld + cc;
-                    unsigned w[2] = {0u, 0u};
-                    if (cc + Img::VE <= ce) __builtin_memcpy(w, a, Img::VE);
-                    else
-#pragma unroll
-                        for (int j = 0; j < Img::VE; ++j) if (cc + j < ce) w[j >> 2] |= (unsigned)a[j] << (8 * (j & 3));
-                    t.x = w[0]; t.y = w[1];
-                    t.z = p.qe[rr * p.ldqe + (cc >> 5)];
+                    for (int j = 0; j < Img::VE; ++j) tmp[j] = cc + j < ce ? a[j] : (T)0;
+                    __builtin_memcpy(&t, tmp, 16);
                 }
             }
             v[i] = t;
@@ -141,22 +127,7 @@ template <class T, int ROWS, bool CM, int MODE, int NT, int BKE = 128 / (int)siz
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             const int c = (int)threadIdx.x + i * NT, row = c / Img::CPR, ch = c - row * Img::CPR;
-            uint4 t = v[i];
-            if constexpr (MODE == S_CKPT) {
-                const float s = ck_scale(t.z);
-                if constexpr (sizeof(T) == 2) {
-                    float f[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = ck_value(j < 4 ? t.x : t.y, j & 3, s);
-                    vec_put(t, f);
-                } else {
-                    float f[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) f[j] = ck_value(t.x, j, s);
-                    t = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-                }
-            }
-            *(uint4*)(lds + Img::off(row, ch)) = t;
+            *(uint4*)(lds + Img::off(row, ch)) = v[i];
         }
     }
 };
@@ -311,7 +282,7 @@ __device__ __forceinline__ void gemm_epilogue(const GemmP& p, f32x16 (&acc)[NI][
 }
 
 // T: type of the operands and the residual, OT: of the output (and pre).  TI x TJ output tile, WI x WJ waves.
-template <class T, class OT, int TI, int TJ, int WI, int WJ, bool PCM, bool QCM, int QMODE>
+template <class T, class OT, int TI, int TJ, int WI, int WJ, bool PCM, bool QCM>
 __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmP p) {
     constexpr int NT = 64 * WI * WJ;
     typedef TileImg<T, TI, PCM> PI;
@@ -334,12 +305,12 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmP p) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[a][c][e] = 0.f;
 
-    Stager<T, TI, PCM, S_REG, NT> sp;
-    Stager<T, TJ, QCM, QMODE, NT> sq;
+    Stager<T, TI, PCM, NT> sp;
+    Stager<T, TJ, QCM, NT> sq;
     const int steps = (int)((ce - cb + BKE - 1) / BKE);
     if (steps > 0) {
-        sp.load(p, p.P, p.ldp, i0, p.I, cb, ce);
-        sq.load(p, p.Q, p.ldq, j0, p.J, cb, ce);
+        sp.load(p.P, p.ldp, i0, p.I, cb, ce);
+        sq.load(p.Q, p.ldq, j0, p.J, cb, ce);
         sp.store(smem);
         sq.store(smem + PI::BYTES);
     }
@@ -347,8 +318,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmP p) {
         char* cur = smem + (t & 1) * STAGE;
         __syncthreads();
         if (t + 1 < steps) {
-            sp.load(p, p.P, p.ldp, i0, p.I, cb + (long long)(t + 1) * BKE, ce);
-            sq.load(p, p.Q, p.ldq, j0, p.J, cb + (long long)(t + 1) * BKE, ce);
+            sp.load(p.P, p.ldp, i0, p.I, cb + (long long)(t + 1) * BKE, ce);
+            sq.load(p.Q, p.ldq, j0, p.J, cb + (long long)(t + 1) * BKE, ce);
         }
 #pragma unroll
         for (int k = 0; k < BKE; k += 16) {
@@ -382,20 +353,19 @@ template <int M, int R> __device__ __forceinline__ void slice_order(const int v)
     }
 }
 
-// The same product with P (and Q, unless it is an 8-bit checkpoint) staged by DMA into a ring of STAGES tiles of BKE reduction
+// The same product with both operands staged by DMA into a ring of STAGES tiles of BKE reduction
 // elements.  At the top of step t one barrier makes tile t + 1 visible and frees tile t - 1, whose slot takes the DMA of tile
 // t + STAGES - 1; loads stay in flight over STAGES - 2 steps.  Fragments are read one 16-deep slice ahead of their MFMAs, across the
 // step border too, so that no MFMA waits for LDS behind a barrier.
-template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int QMODE, int WPE>
+template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int WPE>
 __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP p) {
     constexpr int NT = 64 * WI * WJ;
     typedef TileImg<T, TI, PCM, BKE> PI;
     typedef TileImg<T, TJ, QCM, BKE> QI;
     constexpr int STAGE = PI::BYTES + QI::BYTES, SL = BKE / 16;
     constexpr int NI = TI / WI / 32, NJ = TJ / WJ / 32;
-    constexpr bool CK = QMODE == S_CKPT;
-    constexpr int LOADS = Dma<T, TI, PCM, BKE, NT>::NC + (CK ? 0 : Dma<T, TJ, QCM, BKE, NT>::NC);   // DMA instructions of a wave per step
-    static_assert(STAGES >= (CK ? 4 : 3) && SL >= 2 && SL % 2 == 0, "ring and slices");
+    constexpr int LOADS = Dma<T, TI, PCM, BKE, NT>::NC + Dma<T, TJ, QCM, BKE, NT>::NC;   // DMA instructions of a wave per step
+    static_assert(STAGES >= 3 && SL >= 2 && SL % 2 == 0, "ring and slices");
     extern __shared__ char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wi = wave / WJ, wj = wave - wi * WJ;
     int split, ti, tj;
@@ -414,27 +384,22 @@ __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP
 
     Dma<T, TI, PCM, BKE, NT> dp;
     Dma<T, TJ, QCM, BKE, NT> dq;
-    Stager<T, TJ, QCM, QMODE, NT, BKE> sq;
     dp.init(p.P, p.ldp, i0, p.I, cb);
-    if constexpr (!CK) dq.init(p.Q, p.ldq, j0, p.J, cb);
+    dq.init(p.Q, p.ldq, j0, p.J, cb);
     const int steps = (int)((ce - cb + BKE - 1) / BKE);
     const int pb = wi * (TI / WI), qb = wj * (TJ / WJ);
     const int last = (int)(ce - cb - (long long)(steps - 1) * BKE);       // reduction elements of the last step
     const auto issue = [&](char* s, int t) __attribute__((always_inline)) {
         if (t + 1 < steps) {
             dp.template issue<true>(s, wave, BKE);
-            if constexpr (!CK) dq.template issue<true>(s + PI::BYTES, wave, BKE);
+            dq.template issue<true>(s + PI::BYTES, wave, BKE);
         } else {
             dp.template issue<false>(s, wave, last);
-            if constexpr (!CK) dq.template issue<false>(s + PI::BYTES, wave, last);
+            dq.template issue<false>(s + PI::BYTES, wave, last);
         }
     };
     if (steps > 0) {
         for (int t = 0; t < STAGES - 1 && t < steps; ++t) {
-            if constexpr (CK) {
-                sq.load(p, p.Q, p.ldq, j0, p.J, cb + (long long)t * BKE, ce);
-                if (t < STAGES - 2) sq.store(smem + t * STAGE + PI::BYTES);   // the last one stays in registers until the first step
-            }
             issue(smem + t * STAGE, t);
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -452,17 +417,11 @@ __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP
             // tile t + 1 has landed (younger loads may be under way), and every wave's reads of tile t - 1 are behind it
             if (FULL || t + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 3) * LOADS) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if constexpr (CK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             asm volatile("s_barrier" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (CK) {
-                const int mid = fill == 0 ? (STAGES - 1) * STAGE : fill - STAGE;   // slot of tile t + STAGES - 2
-                if (FULL || t + STAGES - 2 < steps) sq.store(smem + mid + PI::BYTES);
-                if (FULL || t + STAGES - 1 < steps) sq.load(p, p.Q, p.ldq, j0, p.J, cb + (long long)(t + STAGES - 1) * BKE, ce);
-            }
             if constexpr (FULL) {
                 dp.template issue<true>(smem + fill, wave, BKE);
-                if constexpr (!CK) dq.template issue<true>(smem + fill + PI::BYTES, wave, BKE);
+                dq.template issue<true>(smem + fill + PI::BYTES, wave, BKE);
             } else if (t + STAGES - 1 < steps) issue(smem + fill, t + STAGES - 1);
 #pragma unroll
             for (int k = 0; k < SL; ++k) {
@@ -612,15 +571,15 @@ GemmPlan plan_gemm(long long I, int J, long long Cn, int es, bool both_kc) {
     return pl;
 }
 
-template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int QMODE, int WPE>
+template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int WPE>
 void gemm_launch(const GemmP& p, unsigned blocks, hipStream_t st) {
     constexpr size_t ring = STAGES * (size_t)(TileImg<T, TI, PCM, BKE>::BYTES + TileImg<T, TJ, QCM, BKE>::BYTES);
     constexpr size_t lds = std::max(ring, (size_t)WI * WJ * 32 * (TJ / WJ + 4) * sizeof(float));
     static_assert(lds <= 160 * 1024, "LDS of a CU");
-    gemm_dma_kernel<T, OT, TI, TJ, WI, WJ, BKE, STAGES, PCM, QCM, QMODE, WPE><<<blocks, 64 * WI * WJ, lds, st>>>(p);
+    gemm_dma_kernel<T, OT, TI, TJ, WI, WJ, BKE, STAGES, PCM, QCM, WPE><<<blocks, 64 * WI * WJ, lds, st>>>(p);
 }
 
-template <class T, class OT, bool PCM, bool QCM, int QMODE> int gemm_run(GemmP p, hipStream_t st) {
+template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, hipStream_t st) {
     if (p.I == 0 || p.J == 0) return FAVAE_OK;
     constexpr int es = sizeof(T), VE = 16 / es;
     GemmPlan pl = plan_gemm(p.I, p.J, p.Cn, es, !PCM && !QCM);
@@ -628,7 +587,7 @@ template <class T, class OT, bool PCM, bool QCM, int QMODE> int gemm_run(GemmP p
     const auto chunks = [&](const char* a, long long ld, bool cm, long long outs) {
         return aligned(a, 16) && ld % VE == 0 && ld * es <= (1 << 22) && (cm ? outs : p.Cn) % VE == 0;
     };
-    const bool dma = chunks(p.P, p.ldp, PCM, p.I) && (QMODE == S_CKPT || chunks(p.Q, p.ldq, QCM, p.J));
+    const bool dma = chunks(p.P, p.ldp, PCM, p.I) && chunks(p.Q, p.ldq, QCM, p.J);
     if (!dma) pl.tile = SMALL;                   // (the split count of the planned tile stays: scratch is sized for it)
     p.ti = (int)cdivll(p.I, TILE_I[pl.tile]);
     p.tj = cdiv(p.J, TILE_J[pl.tile]);
@@ -639,18 +598,17 @@ template <class T, class OT, bool PCM, bool QCM, int QMODE> int gemm_run(GemmP p
     const long long blocks = (long long)p.ti * p.tj * p.splits;
     FAVAE_CHECK_ARG(blocks <= 0x7fffffffLL, "favae_linear_act: too many rows for one launch");
     const unsigned g = (unsigned)blocks;
-    constexpr int ST = QMODE == S_CKPT ? 4 : 3;
     if (!dma) {
-        gemm_kernel<T, OT, 128, 128, 2, 2, PCM, QCM, QMODE><<<g, 256, 2 * (size_t)(TileImg<T, 128, PCM>::BYTES + TileImg<T, 128, QCM>::BYTES), st>>>(p);
+        gemm_kernel<T, OT, 128, 128, 2, 2, PCM, QCM><<<g, 256, 2 * (size_t)(TileImg<T, 128, PCM>::BYTES + TileImg<T, 128, QCM>::BYTES), st>>>(p);
     } else if constexpr (es == 4) {
         // fp32 MFMA runs at a sixteenth of the bf16 rate: the plain ring feeds it
-        gemm_launch<T, OT, 128, 128, 2, 2, 32, ST, PCM, QCM, QMODE, 1>(p, g, st);
+        gemm_launch<T, OT, 128, 128, 2, 2, 32, 3, PCM, QCM, 1>(p, g, st);
     } else if (pl.tile == WIDE) {
-        if constexpr (!PCM && !QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, QMODE, 2>(p, g, st);
+        if constexpr (!PCM && !QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, 2>(p, g, st);
     } else if (pl.tile == TALL) {
-        gemm_launch<T, OT, 128, 256, 2, 4, 32, ST, PCM, QCM, QMODE, 2>(p, g, st);
+        gemm_launch<T, OT, 128, 256, 2, 4, 32, 3, PCM, QCM, 2>(p, g, st);
     } else {
-        gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, QMODE, 2>(p, g, st);
+        gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
     }
     FAVAE_LAUNCH_CHECK();
     if (p.splits > 1) {
@@ -676,14 +634,15 @@ int lin_sizes(const char* who, long long M, int N, int K, int act, int dtype) {
     return FAVAE_OK;
 }
 
-struct BwdScratch { size_t du, colp, split, total; };
-BwdScratch bwd_scratch(long long M, int N, int K, int act, int dtype) {
+struct BwdScratch { size_t du, colp, split, x, total; };
+BwdScratch bwd_scratch(long long M, int N, int K, int act, bool x_ckpt, int dtype) {
     const int es = dtype == FAVAE_F32 ? 4 : 2;
     BwdScratch s;
     s.du = act == FAVAE_ACT_NONE ? 0 : round256((size_t)M * N * es);
     s.colp = M > 0 ? round256((size_t)cdivll(M, du_rows(M)) * N * sizeof(float)) : 0;
     s.split = std::max(split_bytes(M, K, N, es, false), split_bytes(N, K, M, es, false));    // the two products run one after the other
-    s.total = s.du + s.colp + s.split;
+    s.x = x_ckpt ? round256((size_t)M * ((K + 7) & ~7) * es) : 0;
+    s.total = s.du + s.colp + s.split + s.x;
     return s;
 }
 
@@ -723,17 +682,27 @@ template <class T> int lin_bwd(const void* dy, long long lddy, const void* x, lo
         GemmP p = {};
         p.P = (const char*)du; p.ldp = lddu; p.Q = (const char*)w; p.ldq = ldw; p.I = M; p.J = K; p.Cn = N;
         p.out = dx; p.ldo = lddx; p.part = part; p.act = FAVAE_ACT_NONE;
-        const int rc = gemm_run<T, T, false, true, S_REG>(p, st);
+        const int rc = gemm_run<T, T, false, true>(p, st);
         if (rc != FAVAE_OK) return rc;
     }
     if (dw) {
+        if (xe && M > 0 && K > 0) {
+            // a checkpoint is decoded into the workspace first: 2 + 1 bytes a value, against decoding in the product's staging, which
+            // made du^T x 283 us instead of 12 + 135 (4096 x 1024 x 16384)
+            T* xt = (T*)(scratch + sz.du + sz.colp + sz.split);
+            const long long ldt = (K + 16 / es - 1) / (16 / es) * (16 / es);
+            const int rc = favae_ckpt8_unpack(x, ldx, xe, ldxe, M, K, xt, ldt, es == 4 ? FAVAE_F32 : FAVAE_BF16, st);
+            if (rc != FAVAE_OK) return rc;
+            x = xt;
+            ldx = ldt;
+        }
         GemmP p = {};
-        p.P = (const char*)du; p.ldp = lddu; p.Q = (const char*)x; p.ldq = ldx; p.qe = xe; p.ldqe = ldxe; p.I = N; p.J = K; p.Cn = M;
+        p.P = (const char*)du; p.ldp = lddu; p.Q = (const char*)x; p.ldq = ldx; p.I = N; p.J = K; p.Cn = M;
         p.out = dw; p.ldo = lddw; p.part = part; p.act = FAVAE_ACT_NONE;
         if constexpr (es == 2) {
-            if (dw_f32) return xe ? gemm_run<T, float, true, true, S_CKPT>(p, st) : gemm_run<T, float, true, true, S_REG>(p, st);
+            if (dw_f32) return gemm_run<T, float, true, true>(p, st);
         }
-        return xe ? gemm_run<T, T, true, true, S_CKPT>(p, st) : gemm_run<T, T, true, true, S_REG>(p, st);
+        return gemm_run<T, T, true, true>(p, st);
     }
     return FAVAE_OK;
 }
@@ -760,13 +729,13 @@ extern "C" int favae_linear_act_fwd(const void* x, long long ldx, const void* w,
     GemmP p = {};
     p.P = (const char*)x; p.ldp = ldx; p.Q = (const char*)w; p.ldq = ldw; p.I = M; p.J = N; p.Cn = K;
     p.out = y; p.ldo = ldy; p.part = (float*)scratch; p.bias = bias; p.res = residual; p.ldr = ldr; p.pre = pre; p.ldpre = ldpre; p.act = act;
-    return dtype == FAVAE_F32 ? gemm_run<float, float, false, false, S_REG>(p, (hipStream_t)stream)
-                              : gemm_run<bf16_t, bf16_t, false, false, S_REG>(p, (hipStream_t)stream);
+    return dtype == FAVAE_F32 ? gemm_run<float, float, false, false>(p, (hipStream_t)stream)
+                              : gemm_run<bf16_t, bf16_t, false, false>(p, (hipStream_t)stream);
 }
 
-extern "C" size_t favae_linear_act_bwd_scratch(long long M, int N, int K, int act, int dtype) {
+extern "C" size_t favae_linear_act_bwd_scratch(long long M, int N, int K, int act, int x_ckpt, int dtype) {
     if (lin_sizes("favae_linear_act_bwd_scratch", M, N, K, act, dtype) != FAVAE_OK) return 0;
-    return bwd_scratch(M, N, K, act, dtype).total;
+    return bwd_scratch(M, N, K, act, x_ckpt != 0, dtype).total;
 }
 
 extern "C" int favae_linear_act_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* xe, long long ldxe, const void* w,
@@ -787,7 +756,7 @@ extern "C" int favae_linear_act_bwd(const void* dy, long long lddy, const void* 
     FAVAE_CHECK_ARG(aligned(dy, es) && (xe || aligned(x, es)) && aligned(w, es) && (pe || aligned(pre, es)) && aligned(dx, es) &&
                         aligned(dw, dw_dtype == FAVAE_F32 ? 4 : 2),
                     "favae_linear_act_bwd: a pointer is not aligned to its type");
-    const BwdScratch sz = bwd_scratch(M, N, K, act, dtype);
+    const BwdScratch sz = bwd_scratch(M, N, K, act, xe && dw, dtype);
     FAVAE_CHECK_ARG(sz.total <= scratch_bytes && (sz.total == 0 || scratch) && aligned(scratch, 16), "favae_linear_act_bwd: scratch of %zu bytes, %zu needed",
                     scratch_bytes, sz.total);
     const hipStream_t st = (hipStream_t)stream;

@@ -31,7 +31,7 @@ _raw.favae_gn_act_bwd.argtypes = [_p, _ll, _ll, _p, _ll, _ll, _p, _p, _ll, _ll, 
 _raw.favae_linear_act_fwd_scratch.argtypes = [_ll, _i, _i, _i]
 _raw.favae_linear_act_fwd_scratch.restype = _sz
 _raw.favae_linear_act_fwd.argtypes = [_p, _ll, _p, _ll, _p, _p, _ll, _p, _ll, _p, _ll, _ll, _i, _i, _i, _p, _sz, _i, _p]
-_raw.favae_linear_act_bwd_scratch.argtypes = [_ll, _i, _i, _i, _i]
+_raw.favae_linear_act_bwd_scratch.argtypes = [_ll, _i, _i, _i, _i, _i]
 _raw.favae_linear_act_bwd_scratch.restype = _sz
 _raw.favae_linear_act_bwd.argtypes = [_p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _ll, _ll, _i, _i, _i, _p, _ll, _p, _ll, _i, _p, _p, _sz,
                                       _i, _p]
@@ -355,7 +355,7 @@ def linear_act_bwd(dy, x, w, act="none", pre=None, need=("x", "w", "b"), dw=None
     dx = dy.new_empty(x.shape) if "x" in need else None
     dw = None if "w" not in need else w.new_empty((n, k)) if dw is None else dw
     db = dy.new_empty(n, dtype=F32) if "b" in need else None
-    nbytes = _raw.favae_linear_act_bwd_scratch(m, n, k, a, code)
+    nbytes = _raw.favae_linear_act_bwd_scratch(m, n, k, a, xck and dw is not None, code)
     ws = _scratch(nbytes, dy)
     xp = x.q if xck else x
     pp = pre.q if pck else pre

@@ -638,7 +638,7 @@ int favae_linear_act_fwd(const void* x, long long ldx, const void* w, long long 
 /* Its gradients: du = dy act'(pre) rounded to dtype, dx [M][K] = du w (dtype), dw [N][K] = du^T x (dw_dtype: fp32 or dtype), db [N]
  * fp32 = column sums of du before its rounding; any of the three NULL to skip.  x and pre are tensors of dtype, or, with xe / pe
  * given, 8-bit checkpoints (x / pre point to q).  pre is not read with act none.  The gradient of residual is dy.  Deterministic. */
-size_t favae_linear_act_bwd_scratch(long long M, int N, int K, int act, int dtype);
+size_t favae_linear_act_bwd_scratch(long long M, int N, int K, int act, int x_ckpt /* x is a checkpoint and dw is wanted */, int dtype);
 int favae_linear_act_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* xe, long long ldxe, const void* w,
                          long long ldw, const void* pre, long long ldpre, const void* pe, long long ldpe, long long M, int N, int K,
                          int act, void* dx, long long lddx, void* dw, long long lddw, int dw_dtype, float* db, void* scratch,
