@@ -237,7 +237,7 @@ __global__ __launch_bounds__(512) void gn_param_grad_kernel(const float2* __rest
 
 // ---- geometry ------------------------------------------------------------------------------------------------------------
 
-GnPlan gn_plan(GnP& p, int es, int vec_max, bool backward) {
+GnPlan gn_plan(GnP& p, int es, int vec_max, bool backward, bool ckpt = false) {
     GnPlan pl;
     const int GT = backward ? GTB : GTF;
     // widest vector whose whole-group blocks (or pieces of one group) start on vector borders
@@ -273,7 +273,7 @@ GnPlan gn_plan(GnP& p, int es, int vec_max, bool backward) {
     lanes();
     // fewer channels side by side, down to 32 bytes, where a run of groups does not fit a workgroup's registers or where there would be
     // fewer workgroups than CUs (the blocks that share a cache line run on one XCD)
-    while (p.pieces == 1 && p.CB % 2 == 0 && (p.CB / 2) % unit == 0 && p.CB / 2 * es >= 32 &&
+    while (p.pieces == 1 && p.CB % 2 == 0 && (p.CB / 2) % unit == 0 && p.CB / 2 * es >= 32 && !(ckpt && p.CB % 64) &&
            (cdiv(p.S, p.P) > ITEMS_MAX || (p.S * (long long)p.CB > 16 * vec * 64 && cdivll(p.N, p.NSUB) * p.ncb < 512))) {
         p.CB /= 2;
         p.ncb = cdiv(p.C, p.CB);
@@ -356,7 +356,10 @@ extern "C" size_t favae_gn_act_scratch(long long N, long long S, int C, int G, i
         if (C % v) continue;
         GnP p = {};
         p.N = (int)N; p.S = (int)S; p.C = C; p.G = G; p.Cg = C / G;
-        need = std::max(need, gn_plan(p, dtype == FAVAE_F32 ? 4 : 2, v, backward != 0).part);
+        for (bool ckpt : {false, true}) {
+            GnP t = p;
+            need = std::max(need, gn_plan(t, dtype == FAVAE_F32 ? 4 : 2, v, backward != 0, ckpt).part);
+        }
     }
     return need * sizeof(float2);
 }
@@ -375,7 +378,7 @@ extern "C" int favae_gn_act_fwd(const void* x, long long xn, long long xs, long 
     p.x = x; p.xn = xn; p.xs = xs; p.y = y; p.yn = yn; p.ys = ys;
     p.gamma = gamma; p.beta = beta; p.mean = mean; p.rstd = rstd; p.part = (float2*)scratch;
     p.N = (int)N; p.S = (int)S; p.C = C; p.G = G; p.Cg = C / G; p.act = act; p.eps = eps;
-    const GnPlan pl = gn_plan(p, es, vec_of(p, es, false), false);
+    const GnPlan pl = gn_plan(p, es, vec_of(p, es, false), false, q != nullptr);
     FAVAE_CHECK_ARG(pl.part * sizeof(float2) <= scratch_bytes && (pl.part == 0 || scratch), "favae_gn_act_fwd: scratch of %zu bytes, %zu needed", scratch_bytes,
                     pl.part * sizeof(float2));
     if (q && S > 0) {

@@ -62,9 +62,12 @@ template <class T, int ROWS, bool CM, int BKE_ = 128 / (int)sizeof(T)> struct Ti
     static constexpr int CPR = CM ? ROWS / VE : BKE / VE;             // chunks of a row
     static constexpr int CHUNKS = ROWS * BKE / VE;
     static constexpr int BYTES = CHUNKS * 16;
+    static_assert(ROWS == 64 || ROWS == 128 || ROWS == 256, "swizzles");
+    // (rows of 128 bytes put rows r and r + 2 on one quarter)
+    __device__ static __forceinline__ int piece_swz(int row) { return ROWS == 64 ? (row >> 1) & 1 : row & 3; }
     __device__ static __forceinline__ int off(int row, int ch) {
         if constexpr (!CM) return row * RB + ((ch ^ ((row / (256 / RB)) & (CPR - 1))) << 4);
-        else if constexpr (sizeof(T) == 2) return row * (ROWS * 2) + ((((ch >> 2) ^ (row & 3)) << 2 | (ch & 3)) << 4);
+        else if constexpr (sizeof(T) == 2) return row * (ROWS * 2) + ((((ch >> 2) ^ piece_swz(row)) << 2 | (ch & 3)) << 4);
         else return row * (ROWS * 4) + ((ch ^ (row & 8)) << 4);
     }
     // inverse: which chunk of its row the 16-byte slot `slot` of that row holds
@@ -79,8 +82,8 @@ template <class T, int ROWS, bool CM, int BKE_ = 128 / (int)sizeof(T)> struct Ti
             f.v[0] = lo.x; f.v[1] = lo.y; f.v[2] = lo.z; f.v[3] = lo.w; f.v[4] = hi.x; f.v[5] = hi.y; f.v[6] = hi.z; f.v[7] = hi.w;
         } else if constexpr (sizeof(T) == 2) {
             const int i = lane & 15;
-            const int row = k0 + 8 * h + (i >> 2);                    // and row + 4: the same row & 3
-            const int ch = ((((rb >> 5) ^ (row & 3)) << 2) | (2 * ((lane >> 4) & 1) + ((i & 3) >> 1)));
+            const int row = k0 + 8 * h + (i >> 2);                    // and row + 4: the same swizzle
+            const int ch = ((((rb >> 5) ^ piece_swz(row)) << 2) | (2 * ((lane >> 4) & 1) + ((i & 3) >> 1)));
             const char* a = lds + row * (ROWS * 2) + ch * 16 + 8 * (i & 1);
             union { s16x4 s[2]; bf16x8 b; } c;
             c.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
@@ -477,6 +480,85 @@ template <class T, class OT> __global__ __launch_bounds__(256) void gemm_join_ke
     else epilogue8<T, OT, false>(p, f, bias, p.J - j, oo, op, orr);
 }
 
+// ---- few rows --------------------------------------------------------------------------------------------------------------
+// x w^T for M up to 64 rows (one to a few samples): bound by reading w once, so nothing is staged.  A block takes 16 columns (rows of w)
+// and all of K: its 16 waves take 32-deep (fp32: 16-deep) slices in turn and feed 16-byte loads straight into 16x16 MFMA, MT row tiles of
+// x against one of w; the waves' sums meet in LDS.  Rows of x or w that do not exist repeat the last one and are not stored.
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+template <class T> __device__ __forceinline__ uint4 load_chunk(const T* row, int k, int K) {     // 16 bytes from element k; past K zeros
+    constexpr int VE = 16 / sizeof(T);
+    uint4 t = make_uint4(0u, 0u, 0u, 0u);
+    if (k + VE <= K) __builtin_memcpy(&t, row + k, 16);
+    else {
+        T tmp[VE];
+#pragma unroll
+        for (int j = 0; j < VE; ++j) tmp[j] = k + j < K ? row[k + j] : (T)0;
+        __builtin_memcpy(&t, tmp, 16);
+    }
+    return t;
+}
+template <class T> __device__ __forceinline__ void mma16(f32x4_t& acc, const uint4& a, const uint4& b) {
+    if constexpr (sizeof(T) == 2) {
+        union { uint4 u; bf16x8 v; } x, y;
+        x.u = a; y.u = b;
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, y.v, acc, 0, 0, 0);
+    } else {
+        const unsigned ax[4] = {a.x, a.y, a.z, a.w}, bx[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ax[j]), __uint_as_float(bx[j]), acc, 0, 0, 0);
+    }
+}
+template <class T, int MT> __global__ __launch_bounds__(1024) void skinny_kernel(const GemmP p) {
+    constexpr int VE = 16 / sizeof(T), DEPTH = 4 * VE, AHEAD = MT == 4 ? 2 : 4;      // reduction elements of a slice; slices loaded together
+    __shared__ float red[16][MT * 256 + 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = lane >> 4;
+    const int j0 = blockIdx.x * 16, K = (int)p.Cn;
+    const T* w = (const T*)p.Q + (long long)min(j0 + r, p.J - 1) * p.ldq;
+    const T* x[MT];
+    f32x4_t acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        x[m] = (const T*)p.P + min((long long)(m * 16 + r), p.I - 1) * p.ldp;
+        acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int k0 = wave * DEPTH; k0 < K; k0 += 16 * DEPTH * AHEAD) {
+        uint4 a[AHEAD], b[AHEAD][MT];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int k = k0 + u * 16 * DEPTH + kq * VE;
+            a[u] = load_chunk(w, k, K);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) b[u][m] = load_chunk(x[m], k, K);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) mma16<T>(acc[m], a[u], b[u][m]);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) *(float4*)&red[wave][m * 256 + r * 16 + 4 * kq] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);   // [row of x][column]
+    __syncthreads();
+    for (int t = threadIdx.x; t < MT * 256; t += 1024) {
+        float s = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s += red[v][t];
+        red[0][t] = s;                                     // each thread its own column of red
+    }
+    __syncthreads();
+    if (threadIdx.x < MT * 32) {
+        const int i = threadIdx.x >> 1, j = j0 + (threadIdx.x & 1) * 8;
+        if (i < p.I && j < p.J) {
+            float f[8], bias[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = red[0][i * 16 + (threadIdx.x & 1) * 8 + k];
+            load_bias(p, bias, j);
+            const long long oo = i * p.ldo + j, op = i * p.ldpre + j, orr = i * p.ldr + j;
+            if (p.vec && j + 8 <= p.J) epilogue8<T, T, true>(p, f, bias, 8, oo, op, orr);
+            else epilogue8<T, T, false>(p, f, bias, p.J - j, oo, op, orr);
+        }
+    }
+}
+
 // ---- du = dy act'(u) and the column sums of du ---------------------------------------------------------------------------
 // A block takes DU_COLS = 256 columns of a run of rows: lane = 4 columns, 4 rows at a time; column sums (fp32) of the unrounded du go to
 // part[run][N].  du is rounded to T, the type of the matrix operands; with act == none it is dy itself and only the sums are taken.
@@ -552,23 +634,47 @@ __global__ __launch_bounds__(512) void col_join_kernel(const float* __restrict__
 // ---- host ----------------------------------------------------------------------------------------------------------------
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
-// Tiles of the product kernels.  WIDE for long reductions of KC operands with a tile for every CU; TALL where two workgroups of 8 waves
-// share a CU, so that the epilogue of one runs beside the MFMAs of the other; SMALL where tiles are few.
-// Measured, bf16 (us, WIDE / TALL): x w^T 16384 x 4096 x 4096 452 / 513, 65536 x 1024 x 1024 with gelu and residual 197 / 188; du w 65536 x 1024
-// x 1024 156 / 137; du^T x 1024 x 1024 x 65536 in 16 splits 172 / 151.
-enum Tile { WIDE = 0, TALL = 1, SMALL = 2 };
-constexpr int TILE_I[3] = {256, 128, 128}, TILE_J[3] = {256, 256, 128}, TILE_SLOTS[3] = {256, 512, 512};   // slots: workgroups the chip holds
+constexpr long long CUS = 256;
+int out_vec(const GemmP& p) {
+    return p.ldo % 8 == 0 && aligned(p.out, 16) && (!p.res || (p.ldr % 8 == 0 && aligned(p.res, 16))) && (!p.pre || (p.ldpre % 8 == 0 && aligned(p.pre, 16)));
+}
+constexpr int SKINNY_M = 16;
+
+// Tiles of the product kernels.  WIDE: long reductions of KC operands; TALL: two workgroups of 8 waves share a CU, so that the epilogue of
+// one runs beside the MFMAs of the other; SMALL and TINY where tiles are few; without DMA (odd sizes and strides) only the last two.
+// A reduction may be split over workgroups, whose fp32 sums a second launch joins.  Tile and splits are those with the least estimated
+// time, from what a step (128 bytes of reduction) was measured to take (us): alone on its CU, and as a share of a full one.
+//   bf16, KC operands     WIDE 1.73 / 1.73   TALL 1.3 / 0.97   SMALL 0.7 / 0.63   TINY 0.38 / 0.36
+//   bf16, a CM operand                       TALL 1.4 / 0.97   SMALL 1.2 / 0.73   TINY 0.38 / 0.26
+//   fp32                                                       SMALL 2.1 / 1.9    TINY 0.75 / 0.5
+//   without DMA                                                SMALL 1.2 / 0.85   TINY 1.0 / 0.4    (fp32: not less than with it)
+// Both sides, bf16 (us): x w^T 16384 x 4096 x 4096 WIDE 452, TALL 513; 65536 x 1024 x 1024 with gelu and residual 197, 188; du w 65536 x 1024 x
+// 1024 156, 137; 2048 x 2048 x 2048 TALL 47, SMALL 43, TINY 35; x w^T of that size 40, 26, 48; 1024 x 1024 x 1024 16, 12, 8.
+enum Tile { WIDE = 0, TALL = 1, SMALL = 2, TINY = 3 };
+constexpr int TILE_I[4] = {256, 128, 128, 64}, TILE_J[4] = {256, 256, 128, 64}, TILE_PER_CU[4] = {1, 2, 2, 4};   // workgroups that share a CU
 struct GemmPlan { Tile tile; int splits; };
-GemmPlan plan_gemm(long long I, int J, long long Cn, int es, bool both_kc) {
-    const auto tiles = [&](Tile t) { return cdivll(I, TILE_I[t]) * cdivll(J, TILE_J[t]); };
-    GemmPlan pl;
-    pl.tile = es == 2 && both_kc && Cn >= 2048 && tiles(WIDE) >= TILE_SLOTS[WIDE] ? WIDE : SMALL;
-    // a reduction is split over as many workgroups as fill the chip, at least 8 steps of 128 bytes each
-    const long long most = std::max<long long>(1, Cn * es / 1024);
-    if (pl.tile == SMALL && I >= 128 && J >= 256 && tiles(TALL) * most >= TILE_SLOTS[TALL]) pl.tile = TALL;
-    const long long n = std::max<long long>(1, tiles(pl.tile));
-    pl.splits = n >= TILE_SLOTS[pl.tile] ? 1 : (int)std::min<long long>(std::min<long long>(TILE_SLOTS[pl.tile] / n, most), 256);
-    return pl;
+GemmPlan plan_gemm(long long I, int J, long long Cn, int es, bool both_kc, bool dma) {
+    constexpr double KC_ALONE[4] = {1.73, 1.3, 0.7, 0.38}, KC_SHARE[4] = {1.73, 0.97, 0.63, 0.36};
+    constexpr double CM_ALONE[4] = {1.73, 1.4, 1.2, 0.38}, CM_SHARE[4] = {1.73, 0.97, 0.73, 0.26};
+    const long long steps = std::max<long long>(1, cdivll(Cn * es, 128));
+    GemmPlan best = {TINY, 1};
+    double least = 1e30;
+    for (int t = dma && es == 2 ? (both_kc ? WIDE : TALL) : SMALL; t <= TINY; ++t) {
+        double alone = es == 4 ? (t == SMALL ? 2.1 : 0.75) : (both_kc ? KC_ALONE : CM_ALONE)[t];
+        double share = es == 4 ? (t == SMALL ? 1.9 : 0.5) : (both_kc ? KC_SHARE : CM_SHARE)[t];
+        if (!dma) { alone = std::max(alone, t == SMALL ? 1.2 : 1.0); share = std::max(share, t == SMALL ? 0.85 : 0.4); }
+        const long long tiles = cdivll(I, TILE_I[t]) * cdivll(J, TILE_J[t]);
+        const double epilogue = TILE_I[t] * TILE_J[t] * 6e-5;                      // 1 us for 128 x 128
+        for (int s = 1; s <= 64; s += s < 4 ? 1 : s < 16 ? 4 : 16) {
+            if (s > 1 && (steps < 2 * s || tiles * s > 4096)) break;
+            const long long per_cu = cdivll(tiles * s, CUS), rounds = cdivll(per_cu, TILE_PER_CU[t]);
+            const double beside = (double)std::min<long long>(per_cu, TILE_PER_CU[t]);
+            const double us = rounds * (cdivll(steps, s) * std::max(alone, beside * share) + 1.5 + beside * epilogue) +
+                              (s > 1 ? 4.0 + s * (double)I * J * 2e-6 : 0.0);
+            if (us < least) { least = us; best = {(Tile)t, s}; }
+        }
+    }
+    return best;
 }
 
 template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int WPE>
@@ -582,24 +688,42 @@ void gemm_launch(const GemmP& p, unsigned blocks, hipStream_t st) {
 template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, hipStream_t st) {
     if (p.I == 0 || p.J == 0) return FAVAE_OK;
     constexpr int es = sizeof(T), VE = 16 / es;
-    GemmPlan pl = plan_gemm(p.I, p.J, p.Cn, es, !PCM && !QCM);
+    if constexpr (!PCM && !QCM) {
+        if (p.I <= SKINNY_M) {
+            p.splits = 1;
+            p.vec = out_vec(p);
+            const unsigned g = (unsigned)cdiv(p.J, 16);
+            if (p.I <= 16) skinny_kernel<T, 1><<<g, 1024, 0, st>>>(p);
+            else if (p.I <= 32) skinny_kernel<T, 2><<<g, 1024, 0, st>>>(p);
+            else skinny_kernel<T, 4><<<g, 1024, 0, st>>>(p);
+            FAVAE_LAUNCH_CHECK();
+            return FAVAE_OK;
+        }
+    }
     // DMA takes whole 16-byte chunks at 16-byte addresses, with 32-bit offsets inside a tile
     const auto chunks = [&](const char* a, long long ld, bool cm, long long outs) {
         return aligned(a, 16) && ld % VE == 0 && ld * es <= (1 << 22) && (cm ? outs : p.Cn) % VE == 0;
     };
     const bool dma = chunks(p.P, p.ldp, PCM, p.I) && chunks(p.Q, p.ldq, QCM, p.J);
-    if (!dma) pl.tile = SMALL;                   // (the split count of the planned tile stays: scratch is sized for it)
+    const GemmPlan pl = plan_gemm(p.I, p.J, p.Cn, es, !PCM && !QCM, dma);
     p.ti = (int)cdivll(p.I, TILE_I[pl.tile]);
     p.tj = cdiv(p.J, TILE_J[pl.tile]);
     const long long unit = 128 / es;
     p.cchunk = cdivll(cdivll(p.Cn, unit), pl.splits) * unit;
     p.splits = (int)std::max<long long>(1, cdivll(p.Cn, std::max<long long>(1, p.cchunk)));
-    p.vec = p.ldo % 8 == 0 && aligned(p.out, 16) && (!p.res || (p.ldr % 8 == 0 && aligned(p.res, 16))) && (!p.pre || (p.ldpre % 8 == 0 && aligned(p.pre, 16)));
+    p.vec = out_vec(p);
     const long long blocks = (long long)p.ti * p.tj * p.splits;
     FAVAE_CHECK_ARG(blocks <= 0x7fffffffLL, "favae_linear_act: too many rows for one launch");
     const unsigned g = (unsigned)blocks;
     if (!dma) {
-        gemm_kernel<T, OT, 128, 128, 2, 2, PCM, QCM><<<g, 256, 2 * (size_t)(TileImg<T, 128, PCM>::BYTES + TileImg<T, 128, QCM>::BYTES), st>>>(p);
+        if (pl.tile == TINY) {
+            constexpr size_t lds = std::max(2 * (size_t)(TileImg<T, 64, PCM>::BYTES + TileImg<T, 64, QCM>::BYTES), (size_t)4 * 32 * 36 * sizeof(float));
+            gemm_kernel<T, OT, 64, 64, 2, 2, PCM, QCM><<<g, 256, lds, st>>>(p);
+        } else {
+            gemm_kernel<T, OT, 128, 128, 2, 2, PCM, QCM><<<g, 256, 2 * (size_t)(TileImg<T, 128, PCM>::BYTES + TileImg<T, 128, QCM>::BYTES), st>>>(p);
+        }
+    } else if (pl.tile == TINY) {
+        gemm_launch<T, OT, 64, 64, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
     } else if constexpr (es == 4) {
         // fp32 MFMA runs at a sixteenth of the bf16 rate: the plain ring feeds it
         gemm_launch<T, OT, 128, 128, 2, 2, 32, 3, PCM, QCM, 1>(p, g, st);
@@ -620,8 +744,8 @@ template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, hipStream
 
 size_t round256(size_t a) { return (a + 255) & ~(size_t)255; }
 size_t split_bytes(long long I, int J, long long Cn, int es, bool both_kc) {
-    if (I == 0 || J == 0) return 0;
-    const int s = plan_gemm(I, J, Cn, es, both_kc).splits;
+    if (I == 0 || J == 0 || (both_kc && I <= SKINNY_M)) return 0;
+    const int s = std::max(plan_gemm(I, J, Cn, es, both_kc, true).splits, plan_gemm(I, J, Cn, es, both_kc, false).splits);
     return s > 1 ? round256((size_t)s * I * J * sizeof(float)) : 0;
 }
 constexpr int DU_RUNS = 256;

@@ -623,9 +623,10 @@ def test_refusals_on_the_gpu():
     with pytest.raises(ValueError, match="rows overlap"):
         b.linear_act(torch.randn(8, device=DEV).expand(4, 8), w)
     from favae_hip import lib as L
-    raw = L.raw()
-    y = torch.empty(2000, 64, device=DEV)
-    rc = b._raw.favae_linear_act_fwd(y.data_ptr(), 64, y.data_ptr(), 64, None, None, 0, None, 0, y.data_ptr(), 64, 64, 64, 100000, 0, None, 0, 0, None)
+    y, out = torch.zeros(512, 2048, device=DEV), torch.zeros(128, 64, device=DEV)
+    fwd = b._raw.favae_linear_act_fwd
+    rc = fwd(y.data_ptr(), 2047, y.data_ptr(), 2048, None, None, 0, None, 0, out.data_ptr(), 64, 128, 64, 2048, 0, None, 0, 0, None)
     assert rc < 0 and "row stride" in L.last_error()
-    rc = b._raw.favae_linear_act_fwd(y.data_ptr(), 4096, y.data_ptr(), 4096, None, None, 0, None, 0, y.data_ptr(), 64, 64, 64, 4096, 0, None, 0, 0, None)
+    assert b._raw.favae_linear_act_fwd_scratch(128, 64, 2048, 0) > 0
+    rc = fwd(y.data_ptr(), 2048, y.data_ptr(), 2048, None, None, 0, None, 0, out.data_ptr(), 64, 128, 64, 2048, 0, None, 0, 0, None)
     assert rc < 0 and "scratch" in L.last_error()
