@@ -10,6 +10,7 @@
 // transposed tile (Q rows x P columns): a lane then holds 4 neighbouring output columns of one row.
 #include "act8.h"
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 namespace {
@@ -40,12 +41,12 @@ struct GemmP {
     int ti, tj;                           // tiles
     // output
     void* out; long long ldo;
-    float* part;                          // splits > 1: [split][I][J]
+    float* part;                          // splits > 1: [split][I][ldpart]
+    int ldpart;                           // J rounded up to whole vectors of 8
     const float* bias;
     const void* res; long long ldr;
     void* pre; long long ldpre;
     int act;
-    int vec;                              // out, res and pre allow 16-byte accesses of 8 columns
 };
 
 
@@ -97,53 +98,15 @@ template <class T, int ROWS, bool CM, int BKE_ = 128 / (int)sizeof(T)> struct Ti
     }
 };
 
-// Staging of one operand's tile through registers: any alignment, any tail
-
-template <class T, int ROWS, bool CM, int NT, int BKE = 128 / (int)sizeof(T)> struct Stager {
-    typedef TileImg<T, ROWS, CM, BKE> Img;
-    static constexpr int NC = Img::CHUNKS / NT;
-    static_assert(Img::CHUNKS % NT == 0, "whole chunks per thread");
-    uint4 v[NC];
-    // o0: first output row of the tile, no: output rows that exist; c0: first reduction element, cn: end of this split
-    __device__ __forceinline__ void load(const char* base, long long ld, long long o0, long long no, long long c0, long long cn) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = (int)threadIdx.x + i * NT, row = c / Img::CPR, ch = c - row * Img::CPR;
-            // row / column position in memory: KC: rows are outputs; CM: rows are reduction elements
-            const long long rr = (CM ? c0 : o0) + row, rn = CM ? cn : no;
-            const long long cc = (CM ? o0 : c0) + ch * Img::VE, ce = CM ? no : cn;
-            uint4 t = make_uint4(0u, 0u, 0u, 0u);
-            if (rr < rn && cc < ce) {
-                const T* a = (const T*)base + rr * ld + cc;
-                if (cc + Img::VE <= ce) __builtin_memcpy(&t, a, 16);
-                else {
-                    T tmp[Img::VE];
-#pragma unroll
-                    for (int j = 0; j < Img::VE; ++j) tmp[j] = cc + j < ce ? a[j] : (T)0;
-                    __builtin_memcpy(&t, tmp, 16);
-                }
-            }
-            v[i] = t;
-        }
-    }
-    __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = (int)threadIdx.x + i * NT, row = c / Img::CPR, ch = c - row * Img::CPR;
-            *(uint4*)(lds + Img::off(row, ch)) = v[i];
-        }
-    }
-};
-
 // 8 neighbouring output columns of a row, `left` of which exist: bias, activation, residual, store.  oo, op, orr: element offsets in out, pre and
-// res.  FAST: all 8 exist and 16-byte accesses are allowed.
+// res.  FAST: all 8 exist.  (16-byte accesses at any alignment of the type: the memory system takes them, at a cost where they cross lines.)
 template <class T, class OT, bool FAST> __device__ __forceinline__ void epilogue8(const GemmP& p, float (&f)[8], const float (&bias)[8], int left, long long oo, long long op, long long orr) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] += bias[k];
     const auto put = [&](OT* o) __attribute__((always_inline)) {
-        if constexpr (FAST) {
-            if constexpr (sizeof(OT) == 2) { uint4 r; vec_put(r, f); *(uint4*)o = r; }
-            else { ((float4*)o)[0] = make_float4(f[0], f[1], f[2], f[3]); ((float4*)o)[1] = make_float4(f[4], f[5], f[6], f[7]); }
+        if (FAST || left >= 8) {
+            if constexpr (sizeof(OT) == 2) { uint4 r; vec_put(r, f); __builtin_memcpy(o, &r, 16); }
+            else { __builtin_memcpy(o, f, 16); __builtin_memcpy(o + 4, f + 4, 16); }
         } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) if (k < left) o[k] = from_f32<OT>(f[k]);
@@ -154,12 +117,9 @@ template <class T, class OT, bool FAST> __device__ __forceinline__ void epilogue
     if (p.res) {
         const T* a = (const T*)p.res + orr;
         float t[8];
-        if constexpr (FAST) {
-            if constexpr (sizeof(T) == 2) vec_get(t, *(const uint4*)a);
-            else {
-                const float4 lo = ((const float4*)a)[0], hi = ((const float4*)a)[1];
-                t[0] = lo.x; t[1] = lo.y; t[2] = lo.z; t[3] = lo.w; t[4] = hi.x; t[5] = hi.y; t[6] = hi.z; t[7] = hi.w;
-            }
+        if (FAST || left >= 8) {
+            if constexpr (sizeof(T) == 2) { uint4 r; __builtin_memcpy(&r, a, 16); vec_get(t, r); }
+            else { __builtin_memcpy(t, a, 16); __builtin_memcpy(t + 4, a + 4, 16); }
         } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) t[k] = k < left ? to_f32<T>(a[k]) : 0.f;
@@ -235,19 +195,13 @@ __device__ __forceinline__ void epilogue_rows(const GemmP& p, const float* tile,
     const long long i0 = i_lo + r0;
     long long oo = i0 * p.ldo + j, op = i0 * p.ldpre + j, orr = i0 * p.ldr + j;
     if (p.splits > 1) {
-        float* o = p.part + ((long long)split * p.I + i0) * p.J + j;
+        float* o = p.part + ((long long)split * p.I + i0) * p.ldpart + j;
 #pragma unroll FAST ? 4 : 1
         for (int e = 0; e < EL; ++e) {
             const float4 lo = *(const float4*)src, hi = *(const float4*)(src + 4);
-            if constexpr (FAST) { ((float4*)o)[0] = lo; ((float4*)o)[1] = hi; }
-            else {
-                const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                if (i0 + e * STEP < p.I)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) if (j + k < p.J) o[k] = f[k];
-            }
+            if (FAST || (i0 + e * STEP < p.I && j < p.J)) { ((float4*)o)[0] = lo; ((float4*)o)[1] = hi; }
             src += STEP * RS;
-            o += (long long)STEP * p.J;
+            o += (long long)STEP * p.ldpart;
         }
         return;
     }
@@ -267,7 +221,7 @@ __device__ __forceinline__ void gemm_epilogue(const GemmP& p, f32x16 (&acc)[NI][
     const int j = j0 + wj * WC + (lane % LPR) * 8;
     float bias[8];
     load_bias(p, bias, j);
-    const bool fast = p.vec && i0 + TI <= p.I && j0 + TJ <= p.J && (p.splits == 1 || p.J % 8 == 0);
+    const bool fast = i0 + TI <= p.I && j0 + TJ <= p.J;
     __syncthreads();
 #pragma unroll
     for (int a = 0; a < NI; ++a) {
@@ -284,67 +238,6 @@ __device__ __forceinline__ void gemm_epilogue(const GemmP& p, f32x16 (&acc)[NI][
     }
 }
 
-// T: type of the operands and the residual, OT: of the output (and pre).  TI x TJ output tile, WI x WJ waves.
-template <class T, class OT, int TI, int TJ, int WI, int WJ, bool PCM, bool QCM>
-__global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmP p) {
-    constexpr int NT = 64 * WI * WJ;
-    typedef TileImg<T, TI, PCM> PI;
-    typedef TileImg<T, TJ, QCM> QI;
-    constexpr int BKE = PI::BKE, STAGE = PI::BYTES + QI::BYTES;
-    constexpr int NI = TI / WI / 32, NJ = TJ / WJ / 32;
-    extern __shared__ char smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / WJ, wj = wave - wi * WJ;
-    int split, ti, tj;
-    gemm_tile(p, split, ti, tj);
-    const long long i0 = (long long)ti * TI;
-    const int j0 = tj * TJ;
-    const long long cb = split * p.cchunk, ce = min(p.Cn, cb + p.cchunk);
-
-    f32x16 acc[NI][NJ];
-#pragma unroll
-    for (int a = 0; a < NI; ++a)
-#pragma unroll
-        for (int c = 0; c < NJ; ++c)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[a][c][e] = 0.f;
-
-    Stager<T, TI, PCM, NT> sp;
-    Stager<T, TJ, QCM, NT> sq;
-    const int steps = (int)((ce - cb + BKE - 1) / BKE);
-    if (steps > 0) {
-        sp.load(p.P, p.ldp, i0, p.I, cb, ce);
-        sq.load(p.Q, p.ldq, j0, p.J, cb, ce);
-        sp.store(smem);
-        sq.store(smem + PI::BYTES);
-    }
-    for (int t = 0; t < steps; ++t) {
-        char* cur = smem + (t & 1) * STAGE;
-        __syncthreads();
-        if (t + 1 < steps) {
-            sp.load(p.P, p.ldp, i0, p.I, cb + (long long)(t + 1) * BKE, ce);
-            sq.load(p.Q, p.ldq, j0, p.J, cb + (long long)(t + 1) * BKE, ce);
-        }
-#pragma unroll
-        for (int k = 0; k < BKE; k += 16) {
-            Frag<T> fp[NI], fq[NJ];
-#pragma unroll
-            for (int a = 0; a < NI; ++a) PI::frag(fp[a], cur, wi * (TI / WI) + a * 32, k, lane);
-#pragma unroll
-            for (int c = 0; c < NJ; ++c) QI::frag(fq[c], cur + PI::BYTES, wj * (TJ / WJ) + c * 32, k, lane);
-#pragma unroll
-            for (int a = 0; a < NI; ++a)
-#pragma unroll
-                for (int c = 0; c < NJ; ++c) mma(acc[a][c], fq[c], fp[a]);
-        }
-        if (t + 1 < steps) {
-            char* nxt = smem + ((t + 1) & 1) * STAGE;
-            sp.store(nxt);
-            sq.store(nxt + PI::BYTES);
-        }
-    }
-    gemm_epilogue<T, OT, TI, TJ, WI, WJ>(p, acc, smem, i0, j0, split, lane, wi, wj, wave);
-}
-
 // Instruction order of a slice of M MFMAs with R LDS reads and `v` (0 or more) DMA loads: spread between the MFMAs
 template <int M, int R> __device__ __forceinline__ void slice_order(const int v) {
 #pragma unroll
@@ -356,7 +249,8 @@ template <int M, int R> __device__ __forceinline__ void slice_order(const int v)
     }
 }
 
-// The same product with both operands staged by DMA into a ring of STAGES tiles of BKE reduction
+// T: type of the operands and the residual, OT: of the output (and pre).  TI x TJ output tile, WI x WJ waves.
+// Both operands are staged by DMA into a ring of STAGES tiles of BKE reduction
 // elements.  At the top of step t one barrier makes tile t + 1 visible and frees tile t - 1, whose slot takes the DMA of tile
 // t + STAGES - 1; loads stay in flight over STAGES - 2 steps.  Fragments are read one 16-deep slice ahead of their MFMAs, across the
 // step border too, so that no MFMA waits for LDS behind a barrier.
@@ -455,7 +349,7 @@ __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP
 
 // Sum of the splits, then the epilogue
 template <class T, class OT> __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmP p) {
-    const int per_row = (p.J + 7) / 8;
+    const int per_row = p.ldpart / 8;
     const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
     const long long i = t / per_row;
     const int j = (int)(t - i * per_row) * 8;
@@ -463,27 +357,24 @@ template <class T, class OT> __global__ __launch_bounds__(256) void gemm_join_ke
     float f[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = 0.f;
+    const float* a = p.part + i * p.ldpart + j;
+#pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
-        const float* a = p.part + ((long long)s * p.I + i) * p.J + j;
-        if (p.J % 8 == 0) {
-            const float4 lo = ((const float4*)a)[0], hi = ((const float4*)a)[1];
-            f[0] += lo.x; f[1] += lo.y; f[2] += lo.z; f[3] += lo.w; f[4] += hi.x; f[5] += hi.y; f[6] += hi.z; f[7] += hi.w;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) if (j + k < p.J) f[k] += a[k];
-        }
+        const float4 lo = ((const float4*)a)[0], hi = ((const float4*)a)[1];
+        f[0] += lo.x; f[1] += lo.y; f[2] += lo.z; f[3] += lo.w; f[4] += hi.x; f[5] += hi.y; f[6] += hi.z; f[7] += hi.w;
+        a += p.I * p.ldpart;
     }
     float bias[8];
     load_bias(p, bias, j);
     const long long oo = i * p.ldo + j, op = i * p.ldpre + j, orr = i * p.ldr + j;
-    if (p.vec && j + 8 <= p.J) epilogue8<T, OT, true>(p, f, bias, 8, oo, op, orr);
-    else epilogue8<T, OT, false>(p, f, bias, p.J - j, oo, op, orr);
+    epilogue8<T, OT, false>(p, f, bias, p.J - j, oo, op, orr);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------------
-// x w^T for M up to 64 rows (one to a few samples): bound by reading w once, so nothing is staged.  A block takes 16 columns (rows of w)
-// and all of K: its 16 waves take 32-deep (fp32: 16-deep) slices in turn and feed 16-byte loads straight into 16x16 MFMA, MT row tiles of
-// x against one of w; the waves' sums meet in LDS.  Rows of x or w that do not exist repeat the last one and are not stored.
+// x w^T for M up to 16 rows (one to a few samples): bound by reading w once, so nothing is staged.  A block takes 16 columns (rows of w)
+// and all of K: its 16 waves take 32-deep (fp32: 16-deep) slices in turn and feed 16-byte loads straight into 16x16 MFMA; the waves' sums
+// meet in LDS.  Rows of x or w that do not exist repeat the last one and are not stored.  1 x 4096 x 4096 bf16: 8.2 us, 4.1 TB/s of w; the
+// tile kernels take 15.  (For 32 and 64 rows of 4096 x 4096, with 2 and 4 row tiles of x a wave, 14 and 22 us against their 15 and 16: not kept.)
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 template <class T> __device__ __forceinline__ uint4 load_chunk(const T* row, int k, int K) {     // 16 bytes from element k; past K zeros
     constexpr int VE = 16 / sizeof(T);
@@ -508,70 +399,74 @@ template <class T> __device__ __forceinline__ void mma16(f32x4_t& acc, const uin
         for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ax[j]), __uint_as_float(bx[j]), acc, 0, 0, 0);
     }
 }
-template <class T, int MT> __global__ __launch_bounds__(1024) void skinny_kernel(const GemmP p) {
-    constexpr int VE = 16 / sizeof(T), DEPTH = 4 * VE, AHEAD = MT == 4 ? 2 : 4;      // reduction elements of a slice; slices loaded together
-    __shared__ float red[16][MT * 256 + 4];
+constexpr int SKINNY_M = 16;
+template <class T> __global__ __launch_bounds__(1024) void skinny_kernel(const GemmP p) {
+    constexpr int VE = 16 / sizeof(T), DEPTH = 4 * VE, AHEAD = 4;      // reduction elements of a slice; slices loaded together
+    __shared__ float red[16][256 + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = lane >> 4;
     const int j0 = blockIdx.x * 16, K = (int)p.Cn;
     const T* w = (const T*)p.Q + (long long)min(j0 + r, p.J - 1) * p.ldq;
-    const T* x[MT];
-    f32x4_t acc[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        x[m] = (const T*)p.P + min((long long)(m * 16 + r), p.I - 1) * p.ldp;
-        acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
+    const T* x = (const T*)p.P + min((long long)r, p.I - 1) * p.ldp;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
     for (int k0 = wave * DEPTH; k0 < K; k0 += 16 * DEPTH * AHEAD) {
-        uint4 a[AHEAD], b[AHEAD][MT];
+        uint4 a[AHEAD], b[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int k = k0 + u * 16 * DEPTH + kq * VE;
             a[u] = load_chunk(w, k, K);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) b[u][m] = load_chunk(x[m], k, K);
+            b[u] = load_chunk(x, k, K);
         }
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) mma16<T>(acc[m], a[u], b[u][m]);
+        for (int u = 0; u < AHEAD; ++u) mma16<T>(acc, a[u], b[u]);
     }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) *(float4*)&red[wave][m * 256 + r * 16 + 4 * kq] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);   // [row of x][column]
+    *(float4*)&red[wave][r * 16 + 4 * kq] = make_float4(acc[0], acc[1], acc[2], acc[3]);   // [row of x][column]
     __syncthreads();
-    for (int t = threadIdx.x; t < MT * 256; t += 1024) {
+    if (threadIdx.x < 256) {
         float s = 0.f;
 #pragma unroll
-        for (int v = 0; v < 16; ++v) s += red[v][t];
-        red[0][t] = s;                                     // each thread its own column of red
+        for (int v = 0; v < 16; ++v) s += red[v][threadIdx.x];
+        red[0][threadIdx.x] = s;                           // (each thread its own column of red)
     }
     __syncthreads();
-    if (threadIdx.x < MT * 32) {
-        const int i = threadIdx.x >> 1, j = j0 + (threadIdx.x & 1) * 8;
+    if (threadIdx.x < 32) {
+        const int i = threadIdx.x >> 1, c = (threadIdx.x & 1) * 8, j = j0 + c;
         if (i < p.I && j < p.J) {
             float f[8], bias[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = red[0][i * 16 + (threadIdx.x & 1) * 8 + k];
+            for (int k = 0; k < 8; ++k) f[k] = red[0][i * 16 + c + k];
             load_bias(p, bias, j);
-            const long long oo = i * p.ldo + j, op = i * p.ldpre + j, orr = i * p.ldr + j;
-            if (p.vec && j + 8 <= p.J) epilogue8<T, T, true>(p, f, bias, 8, oo, op, orr);
-            else epilogue8<T, T, false>(p, f, bias, p.J - j, oo, op, orr);
+            epilogue8<T, T, false>(p, f, bias, p.J - j, i * p.ldo + j, i * p.ldpre + j, i * p.ldr + j);
         }
     }
 }
 
+// ---- operands for DMA ----------------------------------------------------------------------------------------------------
+// Copy of up to three operands [rows][cols] with any stride and alignment into [rows][ldo], ldo a multiple of 16 bytes, the rest of a row
+// zero: one pass over an odd operand costs less than staging it through registers would in every tile (x w^T 777 x 201 x 523 bf16: 14 us
+// against 10).
+struct PackP { const char* src[3]; long long ld[3]; char* dst[3]; long long rows[3], first[4]; int cols[3], cpr[3]; };   // cpr: 16-byte chunks of an output row; first: blocks
+template <class T> __global__ __launch_bounds__(256) void pack_kernel(const PackP p) {
+    const int j = (blockIdx.x >= p.first[1]) + (blockIdx.x >= p.first[2]);
+    const long long t = ((long long)blockIdx.x - p.first[j]) * 256 + threadIdx.x;
+    const long long row = t / p.cpr[j];
+    const int ch = (int)(t - row * p.cpr[j]);
+    if (row < p.rows[j]) ((uint4*)p.dst[j])[t] = load_chunk((const T*)p.src[j] + row * p.ld[j], ch * (16 / (int)sizeof(T)), p.cols[j]);
+}
+
 // ---- du = dy act'(u) and the column sums of du ---------------------------------------------------------------------------
-// A block takes DU_COLS = 256 columns of a run of rows: lane = 4 columns, 4 rows at a time; column sums (fp32) of the unrounded du go to
-// part[run][N].  du is rounded to T, the type of the matrix operands; with act == none it is dy itself and only the sums are taken.
+// A block takes 64 vectors of columns of a run of rows, 4 rows at a time; column sums (fp32) of the unrounded du go to part[run][N].  du is
+// rounded to T, the type of the matrix operands, and written with rows of ldu elements, zero past N.
 struct DuP {
     const void* dy; long long lddy;
     const void* pre; long long ldpre;
     const unsigned char *pq, *pe; long long ldpe;
-    void* du;                              // [M][N] contiguous
+    void* du; long long ldu;               // NULL: sums only
     float* part;                           // NULL: no sums
     long long M, rows;
     int N, act;
 };
-template <class T, int V, int SRC> __global__ __launch_bounds__(256) void act_bwd_kernel(const DuP p) {   // SRC: 0 no activation, 1 pre, 2 checkpoint
+template <class T, int SRC> __global__ __launch_bounds__(256) void act_bwd_kernel(const DuP p) {   // SRC: 0 no activation, 1 pre, 2 checkpoint
+    constexpr int V = 16 / sizeof(T);
     __shared__ float red[4][64 * V];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int j = blockIdx.x * (64 * V) + lane * V;
@@ -583,25 +478,34 @@ template <class T, int V, int SRC> __global__ __launch_bounds__(256) void act_bw
         with_act(SRC == 0 ? FAVAE_ACT_NONE : p.act, [&](auto a) __attribute__((always_inline)) {
 #pragma unroll 4
             for (long long i = r0 + w; i < r1; i += 4) {
-                typename VecOf<T, V>::raw rd;
+                uint4 rd = load_chunk((const T*)p.dy + i * p.lddy, j, p.N);
                 float d[V];
-                rd = *(const typename VecOf<T, V>::raw*)((const T*)p.dy + i * p.lddy + j);
-                vec_get(d, rd);
+                typename VecOf<T, V>::raw rv;
+                __builtin_memcpy(&rv, &rd, 16);
+                vec_get(d, rv);
                 if constexpr (SRC > 0) {
                     float z[V];
-                    if constexpr (SRC == 1) vec_get(z, *(const typename VecOf<T, V>::raw*)((const T*)p.pre + i * p.ldpre + j));
-                    else {
+                    if constexpr (SRC == 1) {
+                        const uint4 rz = load_chunk((const T*)p.pre + i * p.ldpre, j, p.N);
+                        __builtin_memcpy(&rv, &rz, 16);
+                        vec_get(z, rv);
+                    } else {
                         const float sc = ck_scale(p.pe[i * p.ldpe + (j >> 5)]);
                         const unsigned char* a8 = p.pq + i * p.ldpre + j;
                         unsigned wd[2] = {0u, 0u};
-                        __builtin_memcpy(wd, a8, V);
+                        if (j + V <= p.N) __builtin_memcpy(wd, a8, V);
+                        else
+#pragma unroll
+                            for (int k = 0; k < V; ++k) if (j + k < p.N) wd[k >> 2] |= (unsigned)a8[k] << (8 * (k & 3));
 #pragma unroll
                         for (int k = 0; k < V; ++k) z[k] = ck_value(wd[k >> 2], k & 3, sc);
                     }
-                    act_grad_mul<T, decltype(a)::value>(d, z);
-                    vec_put(rd, d);
-                    *(typename VecOf<T, V>::raw*)((T*)p.du + i * (long long)p.N + j) = rd;
+                    act_grad_mul<T, decltype(a)::value>(d, z);       // (past N: dy is 0, and z is 0 or, in a faulty block, NaN)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) d[k] = j + k < p.N ? d[k] : 0.f;
+                    vec_put(rv, d);
                 }
+                if (p.du) *(typename VecOf<T, V>::raw*)((T*)p.du + i * p.ldu + j) = rv;
 #pragma unroll
                 for (int k = 0; k < V; ++k) s[k] += d[k];
             }
@@ -635,34 +539,27 @@ __global__ __launch_bounds__(512) void col_join_kernel(const float* __restrict__
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 constexpr long long CUS = 256;
-int out_vec(const GemmP& p) {
-    return p.ldo % 8 == 0 && aligned(p.out, 16) && (!p.res || (p.ldr % 8 == 0 && aligned(p.res, 16))) && (!p.pre || (p.ldpre % 8 == 0 && aligned(p.pre, 16)));
-}
-constexpr int SKINNY_M = 16;
-
 // Tiles of the product kernels.  WIDE: long reductions of KC operands; TALL: two workgroups of 8 waves share a CU, so that the epilogue of
-// one runs beside the MFMAs of the other; SMALL and TINY where tiles are few; without DMA (odd sizes and strides) only the last two.
+// one runs beside the MFMAs of the other; SMALL and TINY where tiles are few.
 // A reduction may be split over workgroups, whose fp32 sums a second launch joins.  Tile and splits are those with the least estimated
 // time, from what a step (128 bytes of reduction) was measured to take (us): alone on its CU, and as a share of a full one.
 //   bf16, KC operands     WIDE 1.73 / 1.73   TALL 1.3 / 0.97   SMALL 0.7 / 0.63   TINY 0.38 / 0.36
-//   bf16, a CM operand                       TALL 1.4 / 0.97   SMALL 1.2 / 0.73   TINY 0.38 / 0.26
+//   bf16, a CM operand                       TALL 1.4 / 0.97   SMALL 1.2 / 0.73   TINY 0.9 / 0.26
 //   fp32                                                       SMALL 2.1 / 1.9    TINY 0.75 / 0.5
-//   without DMA                                                SMALL 1.2 / 0.85   TINY 1.0 / 0.4    (fp32: not less than with it)
 // Both sides, bf16 (us): x w^T 16384 x 4096 x 4096 WIDE 452, TALL 513; 65536 x 1024 x 1024 with gelu and residual 197, 188; du w 65536 x 1024 x
 // 1024 156, 137; 2048 x 2048 x 2048 TALL 47, SMALL 43, TINY 35; x w^T of that size 40, 26, 48; 1024 x 1024 x 1024 16, 12, 8.
 enum Tile { WIDE = 0, TALL = 1, SMALL = 2, TINY = 3 };
 constexpr int TILE_I[4] = {256, 128, 128, 64}, TILE_J[4] = {256, 256, 128, 64}, TILE_PER_CU[4] = {1, 2, 2, 4};   // workgroups that share a CU
 struct GemmPlan { Tile tile; int splits; };
-GemmPlan plan_gemm(long long I, int J, long long Cn, int es, bool both_kc, bool dma) {
+GemmPlan plan_gemm(long long I, int J, long long Cn, int es, bool both_kc) {
     constexpr double KC_ALONE[4] = {1.73, 1.3, 0.7, 0.38}, KC_SHARE[4] = {1.73, 0.97, 0.63, 0.36};
-    constexpr double CM_ALONE[4] = {1.73, 1.4, 1.2, 0.38}, CM_SHARE[4] = {1.73, 0.97, 0.73, 0.26};
+    constexpr double CM_ALONE[4] = {1.73, 1.4, 1.2, 0.9}, CM_SHARE[4] = {1.73, 0.97, 0.73, 0.26};
     const long long steps = std::max<long long>(1, cdivll(Cn * es, 128));
     GemmPlan best = {TINY, 1};
     double least = 1e30;
-    for (int t = dma && es == 2 ? (both_kc ? WIDE : TALL) : SMALL; t <= TINY; ++t) {
-        double alone = es == 4 ? (t == SMALL ? 2.1 : 0.75) : (both_kc ? KC_ALONE : CM_ALONE)[t];
-        double share = es == 4 ? (t == SMALL ? 1.9 : 0.5) : (both_kc ? KC_SHARE : CM_SHARE)[t];
-        if (!dma) { alone = std::max(alone, t == SMALL ? 1.2 : 1.0); share = std::max(share, t == SMALL ? 0.85 : 0.4); }
+    for (int t = es == 2 ? (both_kc ? WIDE : TALL) : SMALL; t <= TINY; ++t) {
+        const double alone = es == 4 ? (t == SMALL ? 2.1 : 0.75) : (both_kc ? KC_ALONE : CM_ALONE)[t];
+        const double share = es == 4 ? (t == SMALL ? 1.9 : 0.5) : (both_kc ? KC_SHARE : CM_SHARE)[t];
         const long long tiles = cdivll(I, TILE_I[t]) * cdivll(J, TILE_J[t]);
         const double epilogue = TILE_I[t] * TILE_J[t] * 6e-5;                      // 1 us for 128 x 128
         for (int s = 1; s <= 64; s += s < 4 ? 1 : s < 16 ? 4 : 16) {
@@ -685,68 +582,67 @@ void gemm_launch(const GemmP& p, unsigned blocks, hipStream_t st) {
     gemm_dma_kernel<T, OT, TI, TJ, WI, WJ, BKE, STAGES, PCM, QCM, WPE><<<blocks, 64 * WI * WJ, lds, st>>>(p);
 }
 
+// out = P Q^T over operands that DMA can take: 16-byte aligned rows, a whole number of chunks (the rest of a KC row zero), and 32-bit offsets
+// inside a tile
 template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, hipStream_t st) {
     if (p.I == 0 || p.J == 0) return FAVAE_OK;
-    constexpr int es = sizeof(T), VE = 16 / es;
-    if constexpr (!PCM && !QCM) {
-        if (p.I <= SKINNY_M) {
-            p.splits = 1;
-            p.vec = out_vec(p);
-            const unsigned g = (unsigned)cdiv(p.J, 16);
-            if (p.I <= 16) skinny_kernel<T, 1><<<g, 1024, 0, st>>>(p);
-            else if (p.I <= 32) skinny_kernel<T, 2><<<g, 1024, 0, st>>>(p);
-            else skinny_kernel<T, 4><<<g, 1024, 0, st>>>(p);
-            FAVAE_LAUNCH_CHECK();
-            return FAVAE_OK;
-        }
-    }
-    // DMA takes whole 16-byte chunks at 16-byte addresses, with 32-bit offsets inside a tile
-    const auto chunks = [&](const char* a, long long ld, bool cm, long long outs) {
-        return aligned(a, 16) && ld % VE == 0 && ld * es <= (1 << 22) && (cm ? outs : p.Cn) % VE == 0;
-    };
-    const bool dma = chunks(p.P, p.ldp, PCM, p.I) && chunks(p.Q, p.ldq, QCM, p.J);
-    const GemmPlan pl = plan_gemm(p.I, p.J, p.Cn, es, !PCM && !QCM, dma);
+    constexpr int es = sizeof(T);
+    const GemmPlan pl = plan_gemm(p.I, p.J, p.Cn, es, !PCM && !QCM);
     p.ti = (int)cdivll(p.I, TILE_I[pl.tile]);
     p.tj = cdiv(p.J, TILE_J[pl.tile]);
     const long long unit = 128 / es;
     p.cchunk = cdivll(cdivll(p.Cn, unit), pl.splits) * unit;
     p.splits = (int)std::max<long long>(1, cdivll(p.Cn, std::max<long long>(1, p.cchunk)));
-    p.vec = out_vec(p);
     const long long blocks = (long long)p.ti * p.tj * p.splits;
     FAVAE_CHECK_ARG(blocks <= 0x7fffffffLL, "favae_linear_act: too many rows for one launch");
+    p.ldpart = (p.J + 7) & ~7;
     const unsigned g = (unsigned)blocks;
-    if (!dma) {
-        if (pl.tile == TINY) {
-            constexpr size_t lds = std::max(2 * (size_t)(TileImg<T, 64, PCM>::BYTES + TileImg<T, 64, QCM>::BYTES), (size_t)4 * 32 * 36 * sizeof(float));
-            gemm_kernel<T, OT, 64, 64, 2, 2, PCM, QCM><<<g, 256, lds, st>>>(p);
-        } else {
-            gemm_kernel<T, OT, 128, 128, 2, 2, PCM, QCM><<<g, 256, 2 * (size_t)(TileImg<T, 128, PCM>::BYTES + TileImg<T, 128, QCM>::BYTES), st>>>(p);
-        }
-    } else if (pl.tile == TINY) {
-        gemm_launch<T, OT, 64, 64, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
-    } else if constexpr (es == 4) {
-        // fp32 MFMA runs at a sixteenth of the bf16 rate: the plain ring feeds it
-        gemm_launch<T, OT, 128, 128, 2, 2, 32, 3, PCM, QCM, 1>(p, g, st);
-    } else if (pl.tile == WIDE) {
-        if constexpr (!PCM && !QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, 2>(p, g, st);
-    } else if (pl.tile == TALL) {
-        gemm_launch<T, OT, 128, 256, 2, 4, 32, 3, PCM, QCM, 2>(p, g, st);
-    } else {
-        gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
-    }
+    if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
+    else if constexpr (es == 4) gemm_launch<T, OT, 128, 128, 2, 2, 32, 3, PCM, QCM, 1>(p, g, st);
+    else if (pl.tile == SMALL) gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
+    else if (pl.tile == TALL) gemm_launch<T, OT, 128, 256, 2, 4, 32, 3, PCM, QCM, 2>(p, g, st);
+    else if constexpr (!PCM && !QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, 2>(p, g, st);
     FAVAE_LAUNCH_CHECK();
     if (p.splits > 1) {
-        gemm_join_kernel<T, OT><<<(unsigned)cdivll(p.I * ((p.J + 7) / 8), 256), 256, 0, st>>>(p);
+        gemm_join_kernel<T, OT><<<(unsigned)cdivll(p.I * (p.ldpart / 8), 256), 256, 0, st>>>(p);
         FAVAE_LAUNCH_CHECK();
     }
     return FAVAE_OK;
 }
 
+// Operands as DMA takes them, or copies of them in the workspace
+struct Operand { const char* p; long long ld, rows; int cols; };
+bool even(const Operand& o, int es) { return aligned(o.p, 16) && (o.ld * es) % 16 == 0 && o.ld * es <= (1 << 22); }
+bool dma_ok(const Operand& o, int es) { return even(o, es) && (o.cols * es) % 16 == 0; }
+long long padded(long long cols, int es) { return cdivll(cols * es, 16) * 16 / es; }
+size_t pack_bytes(long long rows, int cols, int es);
+template <class T> int pack_operands(std::initializer_list<Operand*> ops, char*& ws, hipStream_t st) {
+    PackP k = {};
+    int n = 0;
+    for (Operand* o : ops) {
+        if (!o || o->rows == 0 || o->cols == 0 || dma_ok(*o, sizeof(T))) continue;
+        const long long ldo = padded(o->cols, sizeof(T));
+        k.src[n] = o->p; k.ld[n] = o->ld; k.dst[n] = ws; k.rows[n] = o->rows; k.cols[n] = o->cols; k.cpr[n] = (int)(ldo * (int)sizeof(T) / 16);
+        k.first[n + 1] = k.first[n] + cdivll(o->rows * k.cpr[n], 256);
+        *o = {ws, ldo, o->rows, o->cols};
+        ws += pack_bytes(o->rows, o->cols, sizeof(T));
+        ++n;
+    }
+    if (n == 0) return FAVAE_OK;
+    const long long blocks = k.first[n];
+    for (int j = n + 1; j < 4; ++j) k.first[j] = blocks;
+    FAVAE_CHECK_ARG(blocks <= 0x7fffffffLL, "favae_linear_act: too many rows for one launch");
+    pack_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(k);
+    FAVAE_LAUNCH_CHECK();
+    return FAVAE_OK;
+}
+
 size_t round256(size_t a) { return (a + 255) & ~(size_t)255; }
+size_t pack_bytes(long long rows, int cols, int es) { return round256((size_t)rows * padded(cols, es) * es); }
 size_t split_bytes(long long I, int J, long long Cn, int es, bool both_kc) {
-    if (I == 0 || J == 0 || (both_kc && I <= SKINNY_M)) return 0;
-    const int s = std::max(plan_gemm(I, J, Cn, es, both_kc, true).splits, plan_gemm(I, J, Cn, es, both_kc, false).splits);
-    return s > 1 ? round256((size_t)s * I * J * sizeof(float)) : 0;
+    if (I == 0 || J == 0) return 0;
+    const int s = plan_gemm(I, J, Cn, es, both_kc).splits;
+    return s > 1 ? round256((size_t)s * I * ((J + 7) & ~7) * sizeof(float)) : 0;
 }
 constexpr int DU_RUNS = 256;
 long long du_rows(long long M) { return std::max<long long>(16, cdivll(M, DU_RUNS)); }
@@ -754,75 +650,91 @@ long long du_rows(long long M) { return std::max<long long>(16, cdivll(M, DU_RUN
 int lin_sizes(const char* who, long long M, int N, int K, int act, int dtype) {
     FAVAE_CHECK_ARG(dtype == FAVAE_F32 || dtype == FAVAE_BF16, "%s: dtype is neither fp32 nor bf16", who);
     FAVAE_CHECK_ARG(act >= FAVAE_ACT_NONE && act <= FAVAE_ACT_GELU_TANH, "%s: unknown activation %d", who, act);
-    FAVAE_CHECK_ARG(M >= 0 && N >= 0 && K >= 0 && M <= 0x7fffffffLL && N <= (1 << 24) && K <= (1 << 24), "%s: a size is negative or too large", who);
+    FAVAE_CHECK_ARG(M >= 0 && N >= 0 && K >= 0 && M <= 0x7fffffffLL && N <= (1 << 20) && K <= (1 << 20), "%s: a size is negative or too large", who);
     return FAVAE_OK;
 }
 
-struct BwdScratch { size_t du, colp, split, x, total; };
-BwdScratch bwd_scratch(long long M, int N, int K, int act, bool x_ckpt, int dtype) {
-    const int es = dtype == FAVAE_F32 ? 4 : 2;
+// Whether the sizes alone (odd == 0: all pointers and row strides are 16-byte aligned) leave operand [..][cols] as DMA takes it
+bool whole(int cols, int es, int odd) { return !odd && (cols * es) % 16 == 0; }
+
+struct FwdScratch { size_t split, total; };
+FwdScratch fwd_scratch(long long M, int N, int K, int odd, int es) {
+    if (M == 0 || N == 0 || M <= SKINNY_M) return {0, 0};
+    FwdScratch s;
+    s.split = split_bytes(M, N, K, es, true);
+    s.total = s.split + (whole(K, es, odd) ? 0 : pack_bytes(M, K, es) + pack_bytes(N, K, es));
+    return s;
+}
+template <class T> int lin_fwd(GemmP p, Operand x, Operand w, char* scratch, const FwdScratch& sz, hipStream_t st) {
+    p.part = (float*)scratch;
+    if (x.rows <= SKINNY_M) {
+        p.P = x.p; p.ldp = x.ld; p.Q = w.p; p.ldq = w.ld;
+        p.splits = 1;
+        skinny_kernel<T><<<(unsigned)cdiv(p.J, 16), 1024, 0, st>>>(p);
+        FAVAE_LAUNCH_CHECK();
+        return FAVAE_OK;
+    }
+    char* ws = scratch + sz.split;
+    const int rc = pack_operands<T>({&x, &w}, ws, st);
+    if (rc != FAVAE_OK) return rc;
+    p.P = x.p; p.ldp = x.ld; p.Q = w.p; p.ldq = w.ld;
+    return gemm_run<T, T, false, false>(p, st);
+}
+
+struct BwdScratch { size_t du, colp, split, total; long long ldu; bool need_du; };
+BwdScratch bwd_scratch(long long M, int N, int K, int act, bool x_ckpt, int odd, int es) {
     BwdScratch s;
-    s.du = act == FAVAE_ACT_NONE ? 0 : round256((size_t)M * N * es);
+    s.ldu = padded(N, es);
+    s.need_du = act != FAVAE_ACT_NONE || !whole(N, es, odd);      // du, or dy as DMA takes it (then in either of two places)
+    s.du = s.need_du ? pack_bytes(M, N, es) : 0;
     s.colp = M > 0 ? round256((size_t)cdivll(M, du_rows(M)) * N * sizeof(float)) : 0;
     s.split = std::max(split_bytes(M, K, N, es, false), split_bytes(N, K, M, es, false));    // the two products run one after the other
-    s.x = x_ckpt ? round256((size_t)M * ((K + 7) & ~7) * es) : 0;
-    s.total = s.du + s.colp + s.split + s.x;
+    s.total = s.du + s.colp + s.split + (act == FAVAE_ACT_NONE ? s.du : 0) + (whole(K, es, odd) ? 0 : pack_bytes(N, K, es)) + (whole(K, es, odd) && !x_ckpt ? 0 : pack_bytes(M, K, es));
     return s;
 }
 
-template <class T> int lin_bwd(const void* dy, long long lddy, const void* x, long long ldx, const unsigned char* xe, long long ldxe, const void* w,
-                               long long ldw, const void* pre, long long ldpre, const unsigned char* pe, long long ldpe, long long M, int N, int K,
-                               int act, void* dx, long long lddx, void* dw, long long lddw, int dw_f32, float* db, char* scratch,
-                               const BwdScratch& sz, hipStream_t st) {
+template <class T> int lin_bwd(Operand dy, Operand x, const unsigned char* xe, long long ldxe, Operand w, const void* pre, long long ldpre,
+                               const unsigned char* pe, long long ldpe, long long M, int N, int K, int act, void* dx, long long lddx, void* dw,
+                               long long lddw, int dw_f32, float* db, char* scratch, const BwdScratch& sz, hipStream_t st) {
     constexpr int es = sizeof(T);
-    const T* du = (const T*)dy;
-    long long lddu = lddy;
     float* colp = (float*)(scratch + sz.du);
-    if (M > 0 && N > 0 && (act != FAVAE_ACT_NONE || db)) {
-        DuP d = {dy, lddy, pre, ldpre, (const unsigned char*)pre, pe, ldpe, scratch, db ? colp : nullptr, M, du_rows(M), N, act};
-        const int src = act == FAVAE_ACT_NONE ? 0 : pe ? 2 : 1;
-        constexpr int VW = 16 / es;
-        const bool wide = N % VW == 0 && lddy % VW == 0 && aligned(dy, 16) && (src != 1 || (ldpre % VW == 0 && aligned(pre, 16)));
-        const int v = wide ? VW : 1;
-        const dim3 g((unsigned)cdiv(N, 64 * v), (unsigned)cdivll(M, d.rows));
-        if (wide) {
-            if (src == 0) act_bwd_kernel<T, VW, 0><<<g, 256, 0, st>>>(d);
-            else if (src == 1) act_bwd_kernel<T, VW, 1><<<g, 256, 0, st>>>(d);
-            else act_bwd_kernel<T, VW, 2><<<g, 256, 0, st>>>(d);
-        } else {
-            if (src == 0) act_bwd_kernel<T, 1, 0><<<g, 256, 0, st>>>(d);
-            else if (src == 1) act_bwd_kernel<T, 1, 1><<<g, 256, 0, st>>>(d);
-            else act_bwd_kernel<T, 1, 2><<<g, 256, 0, st>>>(d);
-        }
+    float* part = (float*)(scratch + sz.du + sz.colp);
+    char* ws = scratch + sz.du + sz.colp + sz.split;
+    // du, or (beside the column sums) dy as DMA takes it
+    const bool want_du = (dx || dw) && (act != FAVAE_ACT_NONE || (db && !dma_ok(dy, es)));
+    if (M > 0 && N > 0 && (want_du || db)) {
+        DuP d = {dy.p, dy.ld, pre, ldpre, (const unsigned char*)pre, pe, ldpe, want_du ? scratch : nullptr, sz.ldu, db ? colp : nullptr, M, du_rows(M), N, act};
+        const dim3 g((unsigned)cdiv(N, 64 * (16 / es)), (unsigned)cdivll(M, d.rows));
+        if (act == FAVAE_ACT_NONE) act_bwd_kernel<T, 0><<<g, 256, 0, st>>>(d);
+        else if (!pe) act_bwd_kernel<T, 1><<<g, 256, 0, st>>>(d);
+        else act_bwd_kernel<T, 2><<<g, 256, 0, st>>>(d);
         FAVAE_LAUNCH_CHECK();
-        if (act != FAVAE_ACT_NONE) { du = (const T*)scratch; lddu = N; }
+        if (want_du) dy = {scratch, sz.ldu, M, N};
     }
     if (db && N > 0) {
         col_join_kernel<<<cdiv(N, 16), 512, 0, st>>>(colp, M > 0 ? cdivll(M, du_rows(M)) : 0, N, db);
         FAVAE_LAUNCH_CHECK();
     }
-    float* part = (float*)(scratch + sz.du + sz.colp);
-    if (dx) {
-        GemmP p = {};
-        p.P = (const char*)du; p.ldp = lddu; p.Q = (const char*)w; p.ldq = ldw; p.I = M; p.J = K; p.Cn = N;
-        p.out = dx; p.ldo = lddx; p.part = part; p.act = FAVAE_ACT_NONE;
-        const int rc = gemm_run<T, T, false, true>(p, st);
+    if (dw && xe && M > 0 && K > 0) {
+        // a checkpoint is decoded into the workspace first: 2 + 1 bytes a value, against decoding in the product's staging, which
+        // made du^T x 283 us instead of 12 + 135 (4096 x 1024 x 16384)
+        const long long ldt = padded(K, es);
+        const int rc = favae_ckpt8_unpack(x.p, x.ld, xe, ldxe, M, K, ws, ldt, es == 4 ? FAVAE_F32 : FAVAE_BF16, st);
         if (rc != FAVAE_OK) return rc;
+        x = {ws, ldt, M, K};
+        ws += pack_bytes(M, K, es);
+    }
+    const int rc = pack_operands<T>({(dx || dw) && !want_du ? &dy : nullptr, dw && !xe ? &x : nullptr, dx ? &w : nullptr}, ws, st);
+    if (rc != FAVAE_OK) return rc;
+    GemmP p = {};
+    p.P = dy.p; p.ldp = dy.ld; p.part = part; p.act = FAVAE_ACT_NONE;
+    if (dx) {
+        p.Q = w.p; p.ldq = w.ld; p.I = M; p.J = K; p.Cn = N; p.out = dx; p.ldo = lddx;
+        const int r2 = gemm_run<T, T, false, true>(p, st);
+        if (r2 != FAVAE_OK) return r2;
     }
     if (dw) {
-        if (xe && M > 0 && K > 0) {
-            // a checkpoint is decoded into the workspace first: 2 + 1 bytes a value, against decoding in the product's staging, which
-            // made du^T x 283 us instead of 12 + 135 (4096 x 1024 x 16384)
-            T* xt = (T*)(scratch + sz.du + sz.colp + sz.split);
-            const long long ldt = (K + 16 / es - 1) / (16 / es) * (16 / es);
-            const int rc = favae_ckpt8_unpack(x, ldx, xe, ldxe, M, K, xt, ldt, es == 4 ? FAVAE_F32 : FAVAE_BF16, st);
-            if (rc != FAVAE_OK) return rc;
-            x = xt;
-            ldx = ldt;
-        }
-        GemmP p = {};
-        p.P = (const char*)du; p.ldp = lddu; p.Q = (const char*)x; p.ldq = ldx; p.I = N; p.J = K; p.Cn = M;
-        p.out = dw; p.ldo = lddw; p.part = part; p.act = FAVAE_ACT_NONE;
+        p.Q = x.p; p.ldq = x.ld; p.I = N; p.J = K; p.Cn = M; p.out = dw; p.ldo = lddw;
         if constexpr (es == 2) {
             if (dw_f32) return gemm_run<T, float, true, true>(p, st);
         }
@@ -833,9 +745,9 @@ template <class T> int lin_bwd(const void* dy, long long lddy, const void* x, lo
 
 }  // namespace
 
-extern "C" size_t favae_linear_act_fwd_scratch(long long M, int N, int K, int dtype) {
+extern "C" size_t favae_linear_act_fwd_scratch(long long M, int N, int K, int odd, int dtype) {
     if (lin_sizes("favae_linear_act_fwd_scratch", M, N, K, FAVAE_ACT_NONE, dtype) != FAVAE_OK) return 0;
-    return split_bytes(M, N, K, dtype == FAVAE_F32 ? 4 : 2, true);
+    return fwd_scratch(M, N, K, odd, dtype == FAVAE_F32 ? 4 : 2).total;
 }
 
 extern "C" int favae_linear_act_fwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias, const void* residual,
@@ -848,18 +760,19 @@ extern "C" int favae_linear_act_fwd(const void* x, long long ldx, const void* w,
     FAVAE_CHECK_ARG(y && (K == 0 || (x && w)), "favae_linear_act_fwd: null pointer");
     FAVAE_CHECK_ARG(ldy >= N && ldx >= K && ldw >= K && (!residual || ldr >= N) && (!pre || ldpre >= N), "favae_linear_act_fwd: a row stride is below the row's length");
     FAVAE_CHECK_ARG(aligned(x, es) && aligned(w, es) && aligned(y, es) && aligned(residual, es) && aligned(pre, es), "favae_linear_act_fwd: a pointer is not aligned to its type");
-    const size_t need = split_bytes(M, N, K, es, true);
-    FAVAE_CHECK_ARG(need <= scratch_bytes && (need == 0 || scratch), "favae_linear_act_fwd: scratch of %zu bytes, %zu needed", scratch_bytes, need);
+    const Operand ox = {(const char*)x, ldx, M, K}, ow = {(const char*)w, ldw, N, K};
+    const FwdScratch sz = fwd_scratch(M, N, K, !(even(ox, es) && even(ow, es)), es);
+    FAVAE_CHECK_ARG(sz.total <= scratch_bytes && (sz.total == 0 || scratch) && aligned(scratch, 16), "favae_linear_act_fwd: scratch of %zu bytes, %zu needed", scratch_bytes, sz.total);
     GemmP p = {};
-    p.P = (const char*)x; p.ldp = ldx; p.Q = (const char*)w; p.ldq = ldw; p.I = M; p.J = N; p.Cn = K;
-    p.out = y; p.ldo = ldy; p.part = (float*)scratch; p.bias = bias; p.res = residual; p.ldr = ldr; p.pre = pre; p.ldpre = ldpre; p.act = act;
-    return dtype == FAVAE_F32 ? gemm_run<float, float, false, false>(p, (hipStream_t)stream)
-                              : gemm_run<bf16_t, bf16_t, false, false>(p, (hipStream_t)stream);
+    p.I = M; p.J = N; p.Cn = K;
+    p.out = y; p.ldo = ldy; p.bias = bias; p.res = residual; p.ldr = ldr; p.pre = pre; p.ldpre = ldpre; p.act = act;
+    return dtype == FAVAE_F32 ? lin_fwd<float>(p, ox, ow, (char*)scratch, sz, (hipStream_t)stream)
+                              : lin_fwd<bf16_t>(p, ox, ow, (char*)scratch, sz, (hipStream_t)stream);
 }
 
-extern "C" size_t favae_linear_act_bwd_scratch(long long M, int N, int K, int act, int x_ckpt, int dtype) {
+extern "C" size_t favae_linear_act_bwd_scratch(long long M, int N, int K, int act, int x_ckpt, int odd, int dtype) {
     if (lin_sizes("favae_linear_act_bwd_scratch", M, N, K, act, dtype) != FAVAE_OK) return 0;
-    return bwd_scratch(M, N, K, act, x_ckpt != 0, dtype).total;
+    return bwd_scratch(M, N, K, act, x_ckpt != 0, odd, dtype == FAVAE_F32 ? 4 : 2).total;
 }
 
 extern "C" int favae_linear_act_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* xe, long long ldxe, const void* w,
@@ -880,13 +793,14 @@ extern "C" int favae_linear_act_bwd(const void* dy, long long lddy, const void* 
     FAVAE_CHECK_ARG(aligned(dy, es) && (xe || aligned(x, es)) && aligned(w, es) && (pe || aligned(pre, es)) && aligned(dx, es) &&
                         aligned(dw, dw_dtype == FAVAE_F32 ? 4 : 2),
                     "favae_linear_act_bwd: a pointer is not aligned to its type");
-    const BwdScratch sz = bwd_scratch(M, N, K, act, xe && dw, dtype);
+    const Operand od = {(const char*)dy, lddy, M, N}, ox = {(const char*)x, ldx, M, K}, ow = {(const char*)w, ldw, N, K};
+    const bool odd = !(even(od, es) && (!dx || even(ow, es)) && (!dw || xe || even(ox, es)));
+    const BwdScratch sz = bwd_scratch(M, N, K, act, xe && dw, odd, es);
     FAVAE_CHECK_ARG(sz.total <= scratch_bytes && (sz.total == 0 || scratch) && aligned(scratch, 16), "favae_linear_act_bwd: scratch of %zu bytes, %zu needed",
                     scratch_bytes, sz.total);
     const hipStream_t st = (hipStream_t)stream;
-    return dtype == FAVAE_F32
-               ? lin_bwd<float>(dy, lddy, x, ldx, (const unsigned char*)xe, ldxe, w, ldw, pre, ldpre, (const unsigned char*)pe, ldpe, M, N, K, act, dx,
-                                lddx, dw, lddw, 1, db, (char*)scratch, sz, st)
-               : lin_bwd<bf16_t>(dy, lddy, x, ldx, (const unsigned char*)xe, ldxe, w, ldw, pre, ldpre, (const unsigned char*)pe, ldpe, M, N, K, act, dx,
-                                 lddx, dw, lddw, dw_dtype == FAVAE_F32, db, (char*)scratch, sz, st);
+    return dtype == FAVAE_F32 ? lin_bwd<float>(od, ox, (const unsigned char*)xe, ldxe, ow, pre, ldpre, (const unsigned char*)pe, ldpe, M, N, K, act, dx, lddx,
+                                               dw, lddw, 1, db, (char*)scratch, sz, st)
+                              : lin_bwd<bf16_t>(od, ox, (const unsigned char*)xe, ldxe, ow, pre, ldpre, (const unsigned char*)pe, ldpe, M, N, K, act, dx, lddx,
+                                                dw, lddw, dw_dtype == FAVAE_F32, db, (char*)scratch, sz, st);
 }

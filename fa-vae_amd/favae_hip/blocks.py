@@ -28,10 +28,10 @@ _raw.favae_gn_act_scratch.restype = _sz
 _raw.favae_gn_act_fwd.argtypes = [_p, _ll, _ll, _ll, _ll, _i, _i, _p, _p, ctypes.c_float, _i, _p, _ll, _ll, _p, _p, _p, _p, _p, _sz, _i, _p]
 _raw.favae_gn_act_bwd.argtypes = [_p, _ll, _ll, _p, _ll, _ll, _p, _p, _ll, _ll, _i, _i, _p, _p, _p, _p, _i, _p, _ll, _ll, _p, _p, _p, _sz,
                                   _i, _p]
-_raw.favae_linear_act_fwd_scratch.argtypes = [_ll, _i, _i, _i]
+_raw.favae_linear_act_fwd_scratch.argtypes = [_ll, _i, _i, _i, _i]
 _raw.favae_linear_act_fwd_scratch.restype = _sz
 _raw.favae_linear_act_fwd.argtypes = [_p, _ll, _p, _ll, _p, _p, _ll, _p, _ll, _p, _ll, _ll, _i, _i, _i, _p, _sz, _i, _p]
-_raw.favae_linear_act_bwd_scratch.argtypes = [_ll, _i, _i, _i, _i, _i]
+_raw.favae_linear_act_bwd_scratch.argtypes = [_ll, _i, _i, _i, _i, _i, _i]
 _raw.favae_linear_act_bwd_scratch.restype = _sz
 _raw.favae_linear_act_bwd.argtypes = [_p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _ll, _ll, _i, _i, _i, _p, _ll, _p, _ll, _i, _p, _p, _sz,
                                       _i, _p]
@@ -295,6 +295,12 @@ def group_norm_act_bwd(dy, x, groups, gamma, beta, mean, rstd, act="none", out=N
     return dx, dgamma, dbeta
 
 
+def _odd(t, ld, ptr):
+    """Whether the product has to copy t before it can read it in 16-byte pieces."""
+    row = ld * t.element_size()
+    return ptr % 16 != 0 or row % 16 != 0 or row > 1 << 22
+
+
 # ---- matrix product ------------------------------------------------------------------------------------------------------
 def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=None):
     """act(x w^T + bias) + residual: x [..., K], w [N, K], bias fp32 [N], residual and the result [..., N] of x's type, rows of any
@@ -317,9 +323,10 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
     y = _out(out, "out", x, shape, x.dtype, (x, w, bias, residual), residual)
     pre = x.new_empty(shape) if save_pre else None
     if m and n:
-        nbytes = _raw.favae_linear_act_fwd_scratch(m, n, k, code)
+        ldx, ldw, xp, wp = _rows(x, "x"), _rows(w, "w"), x.data_ptr(), w.data_ptr()
+        nbytes = _raw.favae_linear_act_fwd_scratch(m, n, k, _odd(x, ldx, xp) or _odd(w, ldw, wp), code)
         ws = _scratch(nbytes, x)
-        _call(dev, _raw.favae_linear_act_fwd, x.data_ptr(), _rows(x, "x"), w.data_ptr(), _rows(w, "w"), bp, _ptr(residual),
+        _call(dev, _raw.favae_linear_act_fwd, xp, ldx, wp, ldw, bp, _ptr(residual),
               0 if residual is None else _rows(residual, "residual"), _ptr(pre), n, y.data_ptr(), _rows(y, "out"), m, n, k, a, _ptr(ws), nbytes,
               code)
     return (y, pre) if save_pre else y
@@ -355,12 +362,14 @@ def linear_act_bwd(dy, x, w, act="none", pre=None, need=("x", "w", "b"), dw=None
     dx = dy.new_empty(x.shape) if "x" in need else None
     dw = None if "w" not in need else w.new_empty((n, k)) if dw is None else dw
     db = dy.new_empty(n, dtype=F32) if "b" in need else None
-    nbytes = _raw.favae_linear_act_bwd_scratch(m, n, k, a, xck and dw is not None, code)
-    ws = _scratch(nbytes, dy)
     xp = x.q if xck else x
     pp = pre.q if pck else pre
-    _call(dev, _raw.favae_linear_act_bwd, dy.data_ptr(), _rows(dy, "dy"), xp.data_ptr(), _rows(xp, "x"), x.e.data_ptr() if xck else None,
-          x.e.shape[-1] if xck else 0, w.data_ptr(), _rows(w, "w"), _ptr(pp), 0 if pp is None else _rows(pp, "pre"),
+    ldd, ldx, ldw = _rows(dy, "dy"), _rows(xp, "x"), _rows(w, "w")
+    odd = _odd(dy, ldd, dy.data_ptr()) or _odd(w, ldw, w.data_ptr()) or (not xck and _odd(x, ldx, x.data_ptr()))
+    nbytes = _raw.favae_linear_act_bwd_scratch(m, n, k, a, xck and dw is not None, odd, code)
+    ws = _scratch(nbytes, dy)
+    _call(dev, _raw.favae_linear_act_bwd, dy.data_ptr(), ldd, xp.data_ptr(), ldx, x.e.data_ptr() if xck else None,
+          x.e.shape[-1] if xck else 0, w.data_ptr(), ldw, _ptr(pp), 0 if pp is None else _rows(pp, "pre"),
           pre.e.data_ptr() if pck else None, pre.e.shape[-1] if pck else 0, m, n, k, a, _ptr(dx), k, _ptr(dw), k if dw is None else _rows(dw, "dw"),
           L.F32 if dw is not None and dw.dtype == F32 else code, _ptr(db), _ptr(ws), nbytes, code)
     return dx, dw, db

@@ -630,15 +630,17 @@ int favae_gn_act_bwd(const void* dy, long long dn, long long ds, const void* x, 
 
 /* y = act(u) + residual, u = x w^T + bias: x [M][K], w [N][K], y, residual and pre [M][N] of dtype, bias [N] fp32; bias, residual and
  * pre may be NULL.  pre receives u rounded to dtype.  Accumulation, bias, activation and residual in fp32, one rounding.  residual may
- * be y.  Row strides in elements. */
-size_t favae_linear_act_fwd_scratch(long long M, int N, int K, int dtype);
+ * be y.  Row strides in elements; N and K up to 2^20.  scratch: odd = 0 if x and w have 16-byte aligned pointers and row strides (of at
+ * most 4 MB), else 1. */
+size_t favae_linear_act_fwd_scratch(long long M, int N, int K, int odd, int dtype);
 int favae_linear_act_fwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias, const void* residual,
                          long long ldr, void* pre, long long ldpre, void* y, long long ldy, long long M, int N, int K, int act,
                          void* scratch, size_t scratch_bytes, int dtype, void* stream);
 /* Its gradients: du = dy act'(pre) rounded to dtype, dx [M][K] = du w (dtype), dw [N][K] = du^T x (dw_dtype: fp32 or dtype), db [N]
  * fp32 = column sums of du before its rounding; any of the three NULL to skip.  x and pre are tensors of dtype, or, with xe / pe
  * given, 8-bit checkpoints (x / pre point to q).  pre is not read with act none.  The gradient of residual is dy.  Deterministic. */
-size_t favae_linear_act_bwd_scratch(long long M, int N, int K, int act, int x_ckpt /* x is a checkpoint and dw is wanted */, int dtype);
+size_t favae_linear_act_bwd_scratch(long long M, int N, int K, int act, int x_ckpt /* x is a checkpoint and dw is wanted */,
+                                    int odd /* of dy, x, w, as above */, int dtype);
 int favae_linear_act_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* xe, long long ldxe, const void* w,
                          long long ldw, const void* pre, long long ldpre, const void* pe, long long ldpe, long long M, int N, int K,
                          int act, void* dx, long long lddx, void* dw, long long lddw, int dw_dtype, float* db, void* scratch,

@@ -627,6 +627,61 @@ def test_refusals_on_the_gpu():
     fwd = b._raw.favae_linear_act_fwd
     rc = fwd(y.data_ptr(), 2047, y.data_ptr(), 2048, None, None, 0, None, 0, out.data_ptr(), 64, 128, 64, 2048, 0, None, 0, 0, None)
     assert rc < 0 and "row stride" in L.last_error()
-    assert b._raw.favae_linear_act_fwd_scratch(128, 64, 2048, 0) > 0
+    assert b._raw.favae_linear_act_fwd_scratch(128, 64, 2048, 0, 0) > 0
     rc = fwd(y.data_ptr(), 2048, y.data_ptr(), 2048, None, None, 0, None, 0, out.data_ptr(), 64, 128, 64, 2048, 0, None, 0, 0, None)
     assert rc < 0 and "scratch" in L.last_error()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", [(17, 300, 8), (33, 201, 523), (200, 64, 64), (300, 1000, 301), (5, 7, 4096), (2000, 40, 72)])
+def test_scratch_is_what_the_size_functions_say(M, N, K, dtype):
+    """The C entry points with a workspace of exactly the stated size: what lies behind it stays as it was."""
+    from favae_hip import lib as L
+    raw = B()._raw
+    g = gen(M, N, K, 77)
+    code = L.F32 if dtype == F32 else L.BF16
+    x, w, dy, pre = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype), rnd(g, M, N, dtype=dtype), rnd(g, M, N, dtype=dtype)
+    y, dx, dw, db = torch.empty_like(dy), torch.empty_like(x), torch.empty_like(w), torch.empty(N, device=DEV)
+    ck = B().ckpt8_pack(x)
+    odd = int(K * x.element_size() % 16 != 0)
+    odd_b = int(odd or N * x.element_size() % 16 != 0)
+    st = torch.cuda.current_stream().cuda_stream
+
+    def run(n, f):
+        buf = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+        L.check(f(buf.data_ptr() if n else None, n))
+        assert (buf[n:] == 0xA5).all()
+
+    run(raw.favae_linear_act_fwd_scratch(M, N, K, odd, code),
+        lambda p, n: raw.favae_linear_act_fwd(x.data_ptr(), K, w.data_ptr(), K, None, None, 0, None, 0, y.data_ptr(), N, M, N, K, 2, p, n, code, st))
+    for act in (0, 2):
+        for xe in (None, ck):
+            xp = x if xe is None else ck.q
+            run(raw.favae_linear_act_bwd_scratch(M, N, K, act, int(xe is not None), odd_b, code),
+                lambda p, n: raw.favae_linear_act_bwd(dy.data_ptr(), N, xp.data_ptr(), K, None if xe is None else ck.e.data_ptr(), (K + 31) // 32, w.data_ptr(),
+                                                      K, pre.data_ptr(), N, None, 0, M, N, K, act, dx.data_ptr(), K, dw.data_ptr(), K, code, db.data_ptr(), p, n,
+                                                      code, st))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,S,C,G", GN)
+def test_group_norm_scratch_is_what_the_size_function_says(N, S, C, G, dtype):
+    from favae_hip import lib as L
+    raw = B()._raw
+    g = gen(N, S, C, G, 78)
+    code = L.F32 if dtype == F32 else L.BF16
+    x, dy, gamma, beta = rnd(g, N, S, C, dtype=dtype), rnd(g, N, S, C, dtype=dtype), rnd(g, C), rnd(g, C)
+    y, stat, grads = torch.empty_like(x), torch.empty(2, N, G, device=DEV), torch.empty(2, C, device=DEV)
+    st = torch.cuda.current_stream().cuda_stream
+    for back in (0, 1):
+        n = raw.favae_gn_act_scratch(N, S, C, G, back, code)
+        buf = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+        p = buf.data_ptr() if n else None
+        if back:
+            rc = raw.favae_gn_act_bwd(dy.data_ptr(), S * C, C, x.data_ptr(), S * C, C, None, None, N, S, C, G, gamma.data_ptr(), beta.data_ptr(), stat[0].data_ptr(),
+                                      stat[1].data_ptr(), 2, y.data_ptr(), S * C, C, grads[0].data_ptr(), grads[1].data_ptr(), p, n, code, st)
+        else:
+            rc = raw.favae_gn_act_fwd(x.data_ptr(), S * C, C, N, S, C, G, gamma.data_ptr(), beta.data_ptr(), 1e-5, 2, y.data_ptr(), S * C, C, stat[0].data_ptr(),
+                                      stat[1].data_ptr(), None, None, p, n, code, st)
+        L.check(rc)
+        assert (buf[n:] == 0xA5).all()
