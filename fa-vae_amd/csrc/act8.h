@@ -6,18 +6,11 @@
 #include "favae_hip.h"
 
 // ---- vectors -------------------------------------------------------------------------------------------------------------
-// VEC elements of T in registers as they lie in memory; converted to fp32 where they are used (half the registers for bf16)
-template <class T, int VEC> struct VecOf;
-template <> struct VecOf<float, 4> { typedef float4 raw; };
-template <> struct VecOf<float, 2> { typedef float2 raw; };
-template <> struct VecOf<float, 1> { typedef float raw; };
-template <> struct VecOf<bf16_t, 8> { typedef uint4 raw; };
-template <> struct VecOf<bf16_t, 2> { typedef unsigned raw; };
-template <> struct VecOf<bf16_t, 1> { typedef bf16_t raw; };
-
-__device__ __forceinline__ void vec_get(float (&f)[4], const float4& r) { f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w; }
-__device__ __forceinline__ void vec_get(float (&f)[2], const float2& r) { f[0] = r.x; f[1] = r.y; }
-__device__ __forceinline__ void vec_get(float (&f)[1], const float& r) { f[0] = r; }
+// 16 bytes of T in registers as they lie in memory; converted to fp32 where they are used (half the registers for bf16)
+template <class T> constexpr int VEC16 = 16 / (int)sizeof(T);
+__device__ __forceinline__ void vec_get(float (&f)[4], const uint4& r) {
+    f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
+}
 __device__ __forceinline__ void vec_get(float (&f)[8], const uint4& r) {
     const unsigned w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -26,20 +19,34 @@ __device__ __forceinline__ void vec_get(float (&f)[8], const uint4& r) {
         f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
     }
 }
-__device__ __forceinline__ void vec_get(float (&f)[2], const unsigned& r) {
-    f[0] = __uint_as_float(r << 16);
-    f[1] = __uint_as_float(r & 0xffff0000u);
+__device__ __forceinline__ void vec_put(uint4& r, const float (&f)[4]) {
+    r = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
 }
-__device__ __forceinline__ void vec_get(float (&f)[1], const bf16_t& r) { f[0] = bf16_to_f32(r); }
-
-__device__ __forceinline__ void vec_put(float4& r, const float (&f)[4]) { r = make_float4(f[0], f[1], f[2], f[3]); }
-__device__ __forceinline__ void vec_put(float2& r, const float (&f)[2]) { r = make_float2(f[0], f[1]); }
-__device__ __forceinline__ void vec_put(float& r, const float (&f)[1]) { r = f[0]; }
 __device__ __forceinline__ void vec_put(uint4& r, const float (&f)[8]) {
     r = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
-__device__ __forceinline__ void vec_put(unsigned& r, const float (&f)[2]) { r = pack_bf16x2(f[0], f[1]); }
-__device__ __forceinline__ void vec_put(bf16_t& r, const float (&f)[1]) { r = f32_to_bf16(f[0]); }
+// Loads and stores of 16 bytes at any alignment of T (the memory system takes them, at a cost where they cross lines), or of the first
+// nv elements of them: the end of a row
+template <class T> __device__ __forceinline__ uint4 load16(const T* a, int nv) {
+    uint4 t = make_uint4(0u, 0u, 0u, 0u);
+    if (nv >= VEC16<T>) __builtin_memcpy(&t, a, 16);
+    else {
+        T tmp[VEC16<T>];
+#pragma unroll
+        for (int j = 0; j < VEC16<T>; ++j) tmp[j] = j < nv ? a[j] : (T)0;
+        __builtin_memcpy(&t, tmp, 16);
+    }
+    return t;
+}
+template <class T> __device__ __forceinline__ void store16(T* a, const uint4& r, int nv) {
+    if (nv >= VEC16<T>) __builtin_memcpy(a, &r, 16);
+    else {
+        T tmp[VEC16<T>];
+        __builtin_memcpy(tmp, &r, 16);
+#pragma unroll
+        for (int j = 0; j < VEC16<T>; ++j) if (j < nv) a[j] = tmp[j];
+    }
+}
 
 // ---- activations ---------------------------------------------------------------------------------------------------------
 // sigmoid(t).  bf16 data: the hardware's exp2 and reciprocal (a few 2^-24 of relative error each, against a 2^-9 rounding of the
@@ -83,10 +90,6 @@ template <class F> __device__ __forceinline__ void with_act(int act, F&& f) {
     else f(std::integral_constant<int, FAVAE_ACT_NONE>());
 }
 
-template <int ACT, class F> __device__ __forceinline__ void act_choice(int act, F&& f) {
-    if constexpr (ACT >= 0) f(std::integral_constant<int, ACT>());
-    else with_act(act, f);
-}
 template <class F> void with_act_host(int act, F&& f) {
     if (act == FAVAE_ACT_SILU) f(std::integral_constant<int, FAVAE_ACT_SILU>());
     else if (act == FAVAE_ACT_GELU_TANH) f(std::integral_constant<int, FAVAE_ACT_GELU_TANH>());
@@ -111,10 +114,29 @@ __device__ __forceinline__ unsigned ck_code(unsigned amax_bits) {
     if (top > 127.f && e < 121) ++e;
     return (unsigned)(e + 127);
 }
-__device__ __forceinline__ int ck_round(float x, unsigned code) {
-    if (code == 255u) return 0;
-    const float q = rintf(x * __uint_as_float((254u - code) << 23));
-    return (int)fminf(fmaxf(q, -127.f), 127.f);
+// N values into N / 4 words of bytes: x / step + 1.5 * 2^23 rounds x / step to the nearest even integer, which is then the low byte of the
+// sum.  (The product is exact and |x / step| <= 128.)
+template <int N> __device__ __forceinline__ void ck_bytes(unsigned (&w)[N / 4], float (&f)[N], unsigned code) {
+    const float inv = __uint_as_float((254u - (code == 255u ? 127u : code)) << 23);
+    if (code == 248u) {                                          // the largest step cannot grow: 127 steps at most
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = fminf(fmaxf(f[j], -0x1.fcp127f), 0x1.fcp127f);
+    }
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) {
+        unsigned b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(fmaf(f[4 * k + j], inv, 12582912.f));
+        w[k] = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+        if (code == 255u) w[k] = 0u;
+    }
+}
+// largest |x| of N values, as bits
+template <int N> __device__ __forceinline__ unsigned ck_amax(const float (&f)[N]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
+    return m;
 }
 // value of byte j of w at step s: a conversion that selects and sign-extends its byte, and a product
 __device__ __forceinline__ float ck_value(unsigned w, int j, float s) { return (float)(signed char)(w >> (8 * j)) * s; }

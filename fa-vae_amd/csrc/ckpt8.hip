@@ -12,134 +12,99 @@ struct CkP {
     unsigned char* e; long long lde;
     void* out; long long ldo;
     long long R; int C, nb;              // nb = blocks of 32 channels in a row
-    long long items;
 };
 
-// Wide form: one lane takes 8 channels, 4 neighbouring lanes a block (C a multiple of 8, rows 16-byte aligned; lanes of a row's last
-// block that lie past C are idle).  U items a thread, all loads issued before the first use.
-template <class T, int U> __global__ __launch_bounds__(256) void ck_pack_wide(const CkP p) {
-    const int per_row = p.nb * 4;
-    const long long base = (long long)blockIdx.x * (256 * U);
-    const long long row0 = base / per_row;
-    const int off0 = (int)(base - row0 * per_row);
+// A lane takes 8 channels, 4 neighbouring lanes a block; lanes of a row's last block that lie past C are idle.  U vectors a thread, all
+// loads issued before the first use.  Rows of any stride and alignment; TAIL: C is no multiple of 8.
+template <class T> __device__ __forceinline__ void load8(float (&f)[8], const T* a, int nv) {
+    if constexpr (sizeof(T) == 2) vec_get(f, load16(a, nv));
+    else {
+        float lo[4], hi[4];
+        vec_get(lo, load16(a, nv));
+        vec_get(hi, load16(a + 4, nv - 4));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { f[j] = lo[j]; f[4 + j] = hi[j]; }
+    }
+}
+struct CkPlace { long long row; int c, nv; };
+template <bool TAIL> __device__ __forceinline__ CkPlace ck_place(const CkP& p, int u, long long row0, int off0) {
+    const unsigned per_row = (unsigned)p.nb * 4u, t = (unsigned)(off0 + u * 256) + threadIdx.x, dr = t / per_row;
+    CkPlace k;
+    k.row = row0 + dr;
+    k.c = (int)(t - dr * per_row) * 8;
+    k.nv = k.row < p.R ? p.C - k.c : 0;
+    if (!TAIL && k.nv > 0) k.nv = 8;
+    return k;
+}
+template <class T, int U, bool TAIL> __global__ __launch_bounds__(256) void ck_pack_kernel(const CkP p) {
+    const long long base = (long long)blockIdx.x * (256 * U), row0 = base / (p.nb * 4);
+    const int off0 = (int)(base - row0 * (p.nb * 4));
     float f[U][8];
-    long long row[U]; int c[U]; bool ok[U];
+    CkPlace k[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const unsigned t = (unsigned)(off0 + u * 256) + threadIdx.x;
-        const unsigned dr = t / (unsigned)per_row;
-        row[u] = row0 + dr;
-        c[u] = (int)(t - dr * (unsigned)per_row) * 8;
-        ok[u] = row[u] < p.R && c[u] < p.C;
+        k[u] = ck_place<TAIL>(p, u, row0, off0);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[u][j] = 0.f;
-        if (ok[u]) {
-            const T* s = (const T*)p.x + row[u] * p.ldx + c[u];
-            if constexpr (sizeof(T) == 2) vec_get(f[u], *(const uint4*)s);
-            else {
-                float lo[4], hi[4];
-                vec_get(lo, *(const float4*)s);
-                vec_get(hi, *(const float4*)(s + 4));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { f[u][j] = lo[j]; f[u][4 + j] = hi[j]; }
-            }
-        }
+        if (k[u].nv > 0) load8(f[u], (const T*)p.x + k[u].row * p.ldx + k[u].c, TAIL ? k[u].nv : 8);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        unsigned m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[u][j]) & 0x7fffffffu);
+        unsigned m = ck_amax(f[u]);
         m = max(m, (unsigned)__shfl_xor((int)m, 1, 64));
         m = max(m, (unsigned)__shfl_xor((int)m, 2, 64));
         const unsigned code = ck_code(m);
-        unsigned w[2] = {0u, 0u};
+        unsigned w[2];
+        ck_bytes(w, f[u], code);
+        unsigned char* q = p.q + k[u].row * p.ldq + k[u].c;
+        if (k[u].nv >= 8) __builtin_memcpy(q, w, 8);
+        else if constexpr (TAIL)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j >> 2] |= ((unsigned)ck_round(f[u][j], code) & 0xffu) << (8 * (j & 3));
-        if (ok[u]) {
-            *(uint2*)(p.q + row[u] * p.ldq + c[u]) = make_uint2(w[0], w[1]);
-            if ((c[u] & 31) == 0) p.e[row[u] * p.lde + (c[u] >> 5)] = (unsigned char)code;
-        }
+            for (int j = 0; j < 8; ++j) if (j < k[u].nv) q[j] = (unsigned char)(w[j >> 2] >> (8 * (j & 3)));
+        if (k[u].nv > 0 && (k[u].c & 31) == 0) p.e[k[u].row * p.lde + (k[u].c >> 5)] = (unsigned char)code;
     }
 }
 
-// Any width, stride and alignment: half a wave takes a block, one channel a lane
-template <class T, int U> __global__ __launch_bounds__(256) void ck_pack_any(const CkP p) {
-    const int lane = threadIdx.x & 31;
-    const long long b0 = (long long)blockIdx.x * (8 * U) + (threadIdx.x >> 5);
-    float f[U];
-    long long row[U]; int c[U]; bool ok[U];
+template <class T, int U, bool TAIL> __global__ __launch_bounds__(256) void ck_unpack_kernel(const CkP p) {
+    const long long base = (long long)blockIdx.x * (256 * U), row0 = base / (p.nb * 4);
+    const int off0 = (int)(base - row0 * (p.nb * 4));
+    unsigned w[U][2], code[U];
+    CkPlace k[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const long long b = b0 + 8 * u;
-        row[u] = b / p.nb;
-        c[u] = (int)(b - row[u] * p.nb) * 32 + lane;
-        ok[u] = row[u] < p.R && c[u] < p.C;
-        f[u] = ok[u] ? to_f32<T>(((const T*)p.x)[row[u] * p.ldx + c[u]]) : 0.f;
-    }
+        k[u] = ck_place<TAIL>(p, u, row0, off0);
+        w[u][0] = w[u][1] = code[u] = 0u;
+        if (k[u].nv > 0) {
+            const unsigned char* q = p.q + k[u].row * p.ldq + k[u].c;
+            if (!TAIL || k[u].nv >= 8) __builtin_memcpy(w[u], q, 8);
+            else
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        unsigned m = __float_as_uint(f[u]) & 0x7fffffffu;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-        const unsigned code = ck_code(m);
-        if (ok[u]) {
-            p.q[row[u] * p.ldq + c[u]] = (unsigned char)ck_round(f[u], code);
-            if (lane == 0) p.e[row[u] * p.lde + (c[u] >> 5)] = (unsigned char)code;
-        }
-    }
-}
-
-template <class T, int U> __global__ __launch_bounds__(256) void ck_unpack_wide(const CkP p) {
-    const int per_row = p.nb * 4;
-    const long long base = (long long)blockIdx.x * (256 * U);
-    const long long row0 = base / per_row;
-    const int off0 = (int)(base - row0 * per_row);
-    uint2 w[U]; unsigned code[U];
-    long long row[U]; int c[U]; bool ok[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const unsigned t = (unsigned)(off0 + u * 256) + threadIdx.x;
-        const unsigned dr = t / (unsigned)per_row;
-        row[u] = row0 + dr;
-        c[u] = (int)(t - dr * (unsigned)per_row) * 8;
-        ok[u] = row[u] < p.R && c[u] < p.C;
-        w[u] = make_uint2(0u, 0u);
-        code[u] = 0u;
-        if (ok[u]) {
-            w[u] = *(const uint2*)(p.q + row[u] * p.ldq + c[u]);
-            code[u] = p.e[row[u] * p.lde + (c[u] >> 5)];
+                for (int j = 0; j < 8; ++j) if (j < k[u].nv) w[u][j >> 2] |= (unsigned)q[j] << (8 * (j & 3));
+            code[u] = p.e[k[u].row * p.lde + (k[u].c >> 5)];
         }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        if (!ok[u]) continue;
+        if (k[u].nv <= 0) continue;
         const float s = ck_scale(code[u]);
         float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = ck_value(j < 4 ? w[u].x : w[u].y, j & 3, s);
-        T* o = (T*)p.out + row[u] * p.ldo + c[u];
-        if constexpr (sizeof(T) == 2) { uint4 r; vec_put(r, f); *(uint4*)o = r; }
-        else { *(float4*)o = make_float4(f[0], f[1], f[2], f[3]); *(float4*)(o + 4) = make_float4(f[4], f[5], f[6], f[7]); }
-    }
-}
-
-template <class T, int U> __global__ __launch_bounds__(256) void ck_unpack_any(const CkP p) {
-    const int lane = threadIdx.x & 31;
-    const long long b0 = (long long)blockIdx.x * (8 * U) + (threadIdx.x >> 5);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const long long b = b0 + 8 * u;
-        const long long row = b / p.nb;
-        const int c = (int)(b - row * p.nb) * 32 + lane;
-        if (row < p.R && c < p.C)
-            ((T*)p.out)[row * p.ldo + c] = from_f32<T>((float)(signed char)p.q[row * p.ldq + c] * ck_scale(p.e[row * p.lde + (c >> 5)]));
+        for (int j = 0; j < 8; ++j) f[j] = ck_value(w[u][j >> 2], j & 3, s);
+        T* o = (T*)p.out + k[u].row * p.ldo + k[u].c;
+        uint4 r;
+        const int nv = TAIL ? k[u].nv : 8;
+        if constexpr (sizeof(T) == 2) { vec_put(r, f); store16(o, r, nv); }
+        else {
+            const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+            vec_put(r, lo); store16(o, r, nv);
+            vec_put(r, hi); store16(o + 4, r, nv - 4);
+        }
     }
 }
 
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
-constexpr int U_WIDE = 4, U_ANY = 4;
+constexpr int U = 4;
 // a launch has at most 2^31 - 1 blocks
 template <class F> int launch_ck(long long blocks, const char* who, F&& f) {
     FAVAE_CHECK_ARG(blocks <= 0x7fffffffLL, "%s: too many rows for one launch", who);
@@ -159,17 +124,11 @@ extern "C" int favae_ckpt8_pack(const void* x, long long ldx, long long R, int C
     FAVAE_CHECK_ARG(C <= (1 << 28), "favae_ckpt8_pack: more than 2^28 channels");
     const int es = dtype == FAVAE_F32 ? 4 : 2;
     FAVAE_CHECK_ARG(aligned(x, es), "favae_ckpt8_pack: x is not aligned to its type");
-    CkP p = {x, ldx, (unsigned char*)q, ldq, (unsigned char*)e, lde, nullptr, 0, R, C, nb, 0};
+    CkP p = {x, ldx, (unsigned char*)q, ldq, (unsigned char*)e, lde, nullptr, 0, R, C, nb};
     const hipStream_t st = (hipStream_t)stream;
-    const bool wide = C % 8 == 0 && aligned(x, 16) && (ldx * es) % 16 == 0 && aligned(q, 8) && ldq % 8 == 0;
-    if (wide)
-        return launch_ck(cdivll(R * nb * 4, 256 * U_WIDE), "favae_ckpt8_pack", [&](unsigned g) {
-            if (dtype == FAVAE_F32) ck_pack_wide<float, U_WIDE><<<g, 256, 0, st>>>(p);
-            else ck_pack_wide<bf16_t, U_WIDE><<<g, 256, 0, st>>>(p);
-        });
-    return launch_ck(cdivll(R * nb, 8 * U_ANY), "favae_ckpt8_pack", [&](unsigned g) {
-        if (dtype == FAVAE_F32) ck_pack_any<float, U_ANY><<<g, 256, 0, st>>>(p);
-        else ck_pack_any<bf16_t, U_ANY><<<g, 256, 0, st>>>(p);
+    return launch_ck(cdivll(R * nb * 4, 256 * U), "favae_ckpt8_pack", [&](unsigned g) {
+        if (dtype == FAVAE_F32) C % 8 ? ck_pack_kernel<float, U, true><<<g, 256, 0, st>>>(p) : ck_pack_kernel<float, U, false><<<g, 256, 0, st>>>(p);
+        else C % 8 ? ck_pack_kernel<bf16_t, U, true><<<g, 256, 0, st>>>(p) : ck_pack_kernel<bf16_t, U, false><<<g, 256, 0, st>>>(p);
     });
 }
 
@@ -182,16 +141,10 @@ extern "C" int favae_ckpt8_unpack(const void* q, long long ldq, const void* e, l
     FAVAE_CHECK_ARG(C <= (1 << 28), "favae_ckpt8_unpack: more than 2^28 channels");
     const int es = dtype == FAVAE_F32 ? 4 : 2;
     FAVAE_CHECK_ARG(aligned(out, es), "favae_ckpt8_unpack: out is not aligned to its type");
-    CkP p = {nullptr, 0, (unsigned char*)q, ldq, (unsigned char*)e, lde, out, ldo, R, C, nb, 0};
+    CkP p = {nullptr, 0, (unsigned char*)q, ldq, (unsigned char*)e, lde, out, ldo, R, C, nb};
     const hipStream_t st = (hipStream_t)stream;
-    const bool wide = C % 8 == 0 && aligned(out, 16) && (ldo * es) % 16 == 0 && aligned(q, 8) && ldq % 8 == 0;
-    if (wide)
-        return launch_ck(cdivll(R * nb * 4, 256 * U_WIDE), "favae_ckpt8_unpack", [&](unsigned g) {
-            if (dtype == FAVAE_F32) ck_unpack_wide<float, U_WIDE><<<g, 256, 0, st>>>(p);
-            else ck_unpack_wide<bf16_t, U_WIDE><<<g, 256, 0, st>>>(p);
-        });
-    return launch_ck(cdivll(R * nb, 8 * U_ANY), "favae_ckpt8_unpack", [&](unsigned g) {
-        if (dtype == FAVAE_F32) ck_unpack_any<float, U_ANY><<<g, 256, 0, st>>>(p);
-        else ck_unpack_any<bf16_t, U_ANY><<<g, 256, 0, st>>>(p);
+    return launch_ck(cdivll(R * nb * 4, 256 * U), "favae_ckpt8_unpack", [&](unsigned g) {
+        if (dtype == FAVAE_F32) C % 8 ? ck_unpack_kernel<float, U, true><<<g, 256, 0, st>>>(p) : ck_unpack_kernel<float, U, false><<<g, 256, 0, st>>>(p);
+        else C % 8 ? ck_unpack_kernel<bf16_t, U, true><<<g, 256, 0, st>>>(p) : ck_unpack_kernel<bf16_t, U, false><<<g, 256, 0, st>>>(p);
     });
 }

@@ -4,9 +4,11 @@
 #include <algorithm>
 #include <type_traits>
 
-
 constexpr int GTF = 512, GTB = 256;     // threads of a workgroup, forward and backward
-constexpr int U = 4;                    // positions a thread has under way in the chunked form's second pass
+constexpr int GU = 4;                   // positions a thread has under way in the chunked forms
+constexpr int WAVE_ITEMS = 8, ITEMS_MAX = 16;
+
+enum GnForm { GN_WAVE, GN_HELD, GN_CHUNKED };
 
 struct GnP {
     const void *x, *dy;
@@ -17,16 +19,24 @@ struct GnP {
     const float *gamma, *beta;
     float *mean, *rstd;                 // [N][G]
     float2* part;                       // partial sums, see the kernels
+    float2* s12;                        // chunked backward: (s1, s2) / m of every group, [N][G]
     int N, S, C, G, Cg, act, nb;
     float eps;
-    // geometry.  A workgroup takes CB channels: whole groups (pieces == 1), or piece j of `pieces` of one group wider than it.
-    // LV lanes side by side cover the CB channels, P rows of lanes take P positions at once, NSUB samples share a workgroup.
+    // geometry.  A workgroup (a wave in the wave form) takes CB channels: whole groups (pieces == 1), or piece j of `pieces` of one group
+    // wider than it.  LV lanes side by side, 16 bytes each, cover the CB channels, P rows of lanes take P positions at once, NSUB samples share a
+    // workgroup.
     int LV, P, NSUB, CB, ncb, pieces, chunk, nchunk, shuf;
     long long blocks;
 };
 
-constexpr int ITEMS_MAX = 16;
-struct GnPlan { int vec; bool gs, held; int items; long long blocks; size_t part; };   // part: float2 entries of workspace
+struct GnPlan {
+    GnForm form;
+    int items, gpv;                     // 16-byte vectors a thread holds; groups a vector may touch (VEC: any)
+    bool tail;                          // a run of channels may end inside a vector, or start off the vector grid
+    int threads;
+    long long blocks, rows;             // rows of column sums (backward)
+    size_t part;                        // float2 entries of workspace
+};
 
 struct GnBlock { int c_lo, c_hi, g_lo, ng, cw, piece; };   // channels, groups, channels of a group inside this block
 __device__ __forceinline__ GnBlock gn_block(const GnP& p, int cb) {
@@ -61,11 +71,11 @@ template <int GT> __device__ __forceinline__ int pair_lanes(int pairs, int per) 
     return L;
 }
 
-// Sum of v over the threads of every (sample of the block, group of the block) pair into grp[].  A thread's NV values belong to
-// columns lv * NV + j of its row; a group is cpg neighbouring columns.  With p.shuf the 64 / LV rows of a wave are added by
+// Sum of v over the threads of every (sample of the block, group of the block) pair into grp[].  A thread's values j with own(j) belong
+// to columns col + j of its row; a group is cpg neighbouring columns.  With p.shuf the 64 / LV rows of a wave are added by
 // shuffles first.  Every thread of the block calls; values of idle threads are 0.
-template <int NV>
-__device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* red, float* grp, int lv, int r, int ng, int cpg) {
+template <int NV, class O>
+__device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* red, float* grp, int col, int r, int ng, int cpg, O&& own) {
     const int cols = p.LV * NV;
     int rows = p.P;
     if (p.shuf) {
@@ -75,10 +85,10 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
         rows = GTF / 64;
         if ((int)(threadIdx.x & 63) < p.LV)
 #pragma unroll
-            for (int j = 0; j < NV; ++j) red[(threadIdx.x >> 6) * cols + lv * NV + j] = v[j];
+            for (int j = 0; j < NV; ++j) if (own(j)) red[(threadIdx.x >> 6) * cols + col + j] = v[j];
     } else if (r < p.P * p.NSUB) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) red[r * cols + lv * NV + j] = v[j];
+        for (int j = 0; j < NV; ++j) if (own(j)) red[r * cols + col + j] = v[j];
     }
     __syncthreads();
     // L lanes take a pair: as many as there are threads for every pair at once, at most its values
@@ -99,71 +109,102 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
 // The values a thread holds are kept as they lie in memory and converted anew in every pass: without this the compiler keeps the fp32
 // values of the first pass for the next, twice the registers
 __device__ __forceinline__ void hold(uint4& r) { asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w)); }
-__device__ __forceinline__ void hold(float4& r) { asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w)); }
-__device__ __forceinline__ void hold(float2& r) { asm volatile("" : "+v"(r.x), "+v"(r.y)); }
 __device__ __forceinline__ void hold(unsigned& r) { asm volatile("" : "+v"(r)); }
 __device__ __forceinline__ void hold(float& r) { asm volatile("" : "+v"(r)); }
-__device__ __forceinline__ void hold(bf16_t& r) { asm volatile("" : "+v"(r)); }
 
-template <class T, int VEC> struct GnData {
-    typedef typename VecOf<T, VEC>::raw raw;
-    raw v;
-    __device__ __forceinline__ void load(const void* base, long long off) { v = *(const raw*)((const T*)base + off); }
+// A thread's channels: the vector from c0 on, of which elements j_lo .. j_hi - 1 are its own.  The last vector of a run that does not end on
+// the vector grid starts early, so that it is whole (its first elements then belong to the lane before it); a run narrower than a vector
+// is loaded element by element.
+template <class T, bool TAIL> struct GnLane {
+    static constexpr int VEC = VEC16<T>;
+    int c0, j_lo, j_hi;
+    __device__ __forceinline__ GnLane(int c_lo, int c_hi, int lv) {
+        c0 = c_lo + lv * VEC; j_lo = 0; j_hi = VEC;
+        if constexpr (TAIL) {
+            if (c_hi - c_lo < VEC) j_hi = c_hi - c_lo;
+            else if (c0 + VEC > c_hi) { j_lo = c0 - (c_hi - VEC); c0 = c_hi - VEC; }
+        }
+    }
+    __device__ __forceinline__ bool own(int j) const { return !TAIL || (j >= j_lo && j < j_hi); }
+    __device__ __forceinline__ void store(void* base, long long off, const uint4& r) const {
+        T* a = (T*)base + off;
+        if (!TAIL || j_hi - j_lo == VEC) __builtin_memcpy(a, &r, 16);
+        else {
+            T t[VEC];
+            __builtin_memcpy(t, &r, 16);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) if (own(j)) a[j] = t[j];
+        }
+    }
+};
+// A vector of a tensor
+template <class T, bool TAIL> struct GnData {
+    static constexpr int VEC = VEC16<T>;
+    uint4 v;
+    __device__ __forceinline__ void load(const void* base, long long off, const GnLane<T, TAIL>& l) { v = load16((const T*)base + off, TAIL ? l.j_hi : VEC); }
     __device__ __forceinline__ void get(float (&f)[VEC]) const { vec_get(f, v); }
     __device__ __forceinline__ void keep() { hold(v); }
 };
-// VEC values of an 8-bit checkpoint: they lie inside one block of 32 (VEC divides 32 and their first channel)
-template <int VEC> struct CkData {
-    unsigned w[VEC == 8 ? 2 : 1];
-    float s;
-    __device__ __forceinline__ void load(const unsigned char* q, const unsigned char* e, long long pos, int C, int nb, int c) {
-        const unsigned char* a = q + pos * C + c;
-        if constexpr (VEC == 8) { const uint2 t = *(const uint2*)a; w[0] = t.x; w[1] = t.y; }
-        else if constexpr (VEC == 4) w[0] = *(const unsigned*)a;
-        else if constexpr (VEC == 2) w[0] = *(const unsigned short*)a;
-        else w[0] = *a;
-        s = ck_scale(e[pos * nb + (c >> 5)]);
+// The same of an 8-bit checkpoint.  Without TAIL it lies inside one block of 32 channels, with it the elements from k0 on belong to the next.
+template <class T, bool TAIL> struct CkData {
+    static constexpr int VEC = VEC16<T>;
+    unsigned w[VEC / 4];
+    float s, s1;
+    int k0;
+    __device__ __forceinline__ void load(const unsigned char* q, const unsigned char* e, long long pos, int C, int nb, const GnLane<T, TAIL>& l) {
+        const unsigned char* a = q + pos * C + l.c0;
+        e += pos * nb + (l.c0 >> 5);
+        s = ck_scale(e[0]);
+        if constexpr (!TAIL) __builtin_memcpy(w, a, VEC);
+        else {
+            k0 = 32 - (l.c0 & 31);
+            s1 = ck_scale(e[k0 < l.j_hi ? 1 : 0]);
+            if (l.j_hi == VEC) __builtin_memcpy(w, a, VEC);
+            else {
+#pragma unroll
+                for (int j = 0; j < VEC / 4; ++j) w[j] = 0u;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) if (j < l.j_hi) w[j >> 2] |= (unsigned)a[j] << (8 * (j & 3));
+            }
+        }
     }
     __device__ __forceinline__ void get(float (&f)[VEC]) const {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = ck_value(w[j >> 2], j & 3, s);
+        for (int j = 0; j < VEC; ++j) f[j] = ck_value(w[j >> 2], j & 3, TAIL && j >= k0 ? s1 : s);
     }
     __device__ __forceinline__ void keep() {
-        hold(w[0]);
-        if constexpr (VEC == 8) hold(w[1]);
+#pragma unroll
+        for (int j = 0; j < VEC / 4; ++j) hold(w[j]);
         hold(s);
     }
 };
 
-// VEC values of a position into an 8-bit checkpoint: 32 / VEC neighbouring lanes hold a block (C a multiple of 32, all of them active)
-template <int VEC> __device__ __forceinline__ void ck_store(const GnP& p, const float (&f)[VEC], long long pos, int c) {
-    unsigned m = 0;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 1; o < 32 / VEC; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-    const unsigned code = ck_code(m);
-    unsigned w[2] = {0u, 0u};
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) w[j >> 2] |= ((unsigned)ck_round(f[j], code) & 0xffu) << (8 * (j & 3));
-    unsigned char* o = p.qo + pos * p.C + c;
-    if constexpr (VEC == 8) *(uint2*)o = make_uint2(w[0], w[1]);
-    else *(unsigned*)o = w[0];
-    if ((c & 31) == 0) p.eo[pos * p.nb + (c >> 5)] = (unsigned char)code;
-}
-
-// Per-channel constants of a thread.  GS: a vector lies inside one group, so that its mean and rstd are single values.
-template <int VEC, bool GS> struct GnStat {
-    float m[GS ? 1 : VEC], r[GS ? 1 : VEC];
-    __device__ __forceinline__ float mean(int j) const { return m[GS ? 0 : j]; }
-    __device__ __forceinline__ float rstd(int j) const { return r[GS ? 0 : j]; }
+// Mean and rstd of a thread's channels: GPV values a vector, VEC / GPV neighbouring channels each
+template <int VEC, int GPV> struct GnStat {
+    float m[GPV], r[GPV];
+    __device__ __forceinline__ float mean(int j) const { return m[j * GPV / VEC]; }
+    __device__ __forceinline__ float rstd(int j) const { return r[j * GPV / VEC]; }
 };
 
-#define GN_VEC(T, vec, F)                                                              \
-    do {                                                                               \
-        if constexpr (sizeof(T) == 4) { if ((vec) == 4) F(T, 4) else if ((vec) == 2) F(T, 2) else F(T, 1) } \
-        else { if ((vec) == 8) F(T, 8) else if ((vec) == 2) F(T, 2) else F(T, 1) }     \
-    } while (0)
+// f(integral_constant<GPV>, bool_constant<TAIL>) for the workgroup forms, where a vector touches one group or any
+template <class T, class F> int gn_variants(const GnPlan& pl, F&& f) {
+    if (pl.gpv == 1) return f(std::integral_constant<int, 1>(), std::false_type());
+    if (!pl.tail) return f(std::integral_constant<int, VEC16<T>>(), std::false_type());
+    return f(std::integral_constant<int, VEC16<T>>(), std::true_type());
+}
+// f(integral_constant<GPV>, integral_constant<ITEMS>) for the wave form
+template <class T, class F> int gn_wave_variants(const GnPlan& pl, F&& f) {
+    const auto items = [&](auto gpv) {
+        if (pl.items <= 1) return f(gpv, std::integral_constant<int, 1>());
+        if (pl.items <= 2) return f(gpv, std::integral_constant<int, 2>());
+        if (pl.items <= 4) return f(gpv, std::integral_constant<int, 4>());
+        return f(gpv, std::integral_constant<int, WAVE_ITEMS>());
+    };
+    if (pl.gpv == 1) return items(std::integral_constant<int, 1>());
+    if (pl.gpv == 2) return items(std::integral_constant<int, 2>());
+    if (pl.gpv == 4) return items(std::integral_constant<int, 4>());
+    return items(std::integral_constant<int, VEC16<T>>());
+}
 
 template <class K> int gn_launch(K k, const GnP& p, int threads, size_t lds, hipStream_t st) {
     FAVAE_CHECK_ARG(p.blocks <= 0x7fffffffLL, "favae_gn_act: too many samples for one launch");
@@ -172,6 +213,6 @@ template <class K> int gn_launch(K k, const GnP& p, int threads, size_t lds, hip
     return FAVAE_OK;
 }
 
-// backward kernels, one translation unit per type (gn_bwd_f32.hip, gn_bwd_bf16.hip)
-int gn_bwd_f32(const GnP& p, const GnPlan& pl, hipStream_t st);
-int gn_bwd_bf16(const GnP& p, const GnPlan& pl, hipStream_t st);
+// backward kernels, one translation unit per type (gn_bwd_f32.hip, gn_bwd_bf16.hip); dgamma and dbeta may be NULL
+int gn_bwd_f32(const GnP& p, const GnPlan& pl, float* dgamma, float* dbeta, hipStream_t st);
+int gn_bwd_bf16(const GnP& p, const GnPlan& pl, float* dgamma, float* dbeta, hipStream_t st);

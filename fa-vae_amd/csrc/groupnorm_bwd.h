@@ -1,14 +1,113 @@
-// Backward kernels of group norm with an activation (formulas and the two forms: groupnorm.hip).
+// Backward kernels of group norm with an activation (formulas and the three forms: groupnorm.hip).
 #pragma once
 #include "groupnorm.h"
 
 namespace {
 
+template <class T, bool TAIL, bool CK> using GnX = typename std::conditional<CK, CkData<T, TAIL>, GnData<T, TAIL>>::type;
+template <class T, bool TAIL, bool CK>
+__device__ __forceinline__ void gn_load(const GnP& p, GnX<T, TAIL, CK>& x, GnData<T, TAIL>& d, long long n, int s, const GnLane<T, TAIL>& l) {
+    if constexpr (CK) x.load(p.q, p.e, n * p.S + s, p.C, p.nb, l);
+    else x.load(p.x, n * p.xn + s * p.xs + l.c0, l);
+    d.load(p.dy, n * p.dn + s * p.ds + l.c0, l);
+}
 
-// ---- backward ------------------------------------------------------------------------------------------------------------
+// ---- wave form -----------------------------------------------------------------------------------------------------------
+// (lanes as in gn_wave_fwd_kernel.)  dz is held: its exp and reciprocal are half the work of a pass.  The sums over samples stay in each lane's
+// registers to the end; the waves of a workgroup then leave one row of them, part[row C + c].
+template <class T, int ITEMS, int GPV, bool CK> __global__ __launch_bounds__(256) void gn_wave_bwd_kernel(const GnP p) {
+    constexpr int VEC = VEC16<T>;
+    __shared__ float2 red[4][64][VEC + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const long long lb = xcd_order(blockIdx.x, p.blocks);
+    const int cb = (int)(lb % p.ncb);
+    const long long row = lb / p.ncb, rows = p.blocks / p.ncb;
+    const int lv = lane & (p.LV - 1), pos = lane / p.LV, gl = GPV == 1 ? p.Cg / VEC : 1;
+    const bool col_ok = cb * p.CB + lv * VEC < p.C;
+    const GnLane<T, false> ln(min(cb * p.CB + lv * VEC, p.C - VEC), p.C, 0);
+    const int c0 = ln.c0, g0 = c0 / p.Cg;
+    const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
+    float ga[VEC], be[VEC], sa[VEC], sb[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { ga[j] = p.gamma[c0 + j]; be[j] = p.beta[c0 + j]; sa[j] = sb[j] = 0.f; }
+    with_act(p.act, [&](auto act) __attribute__((always_inline)) {
+        for (long long n = row * waves + wave; n < p.N; n += rows * waves) {
+            GnX<T, false, CK> xv[ITEMS];
+            GnData<T, false> d[ITEMS];
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) gn_load<T, false, CK>(p, xv[i], d[i], n, min(pos + i * p.P, p.S - 1), ln);
+            GnStat<VEC, GPV> st;
+#pragma unroll
+            for (int j = 0; j < GPV; ++j) { st.m[j] = p.mean[n * p.G + g0 + j]; st.r[j] = p.rstd[n * p.G + g0 + j]; }
+            float dz[ITEMS][VEC], la[VEC], lb_[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) la[j] = lb_[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                float x[VEC], z[VEC];
+                if (pos + i * p.P >= p.S) d[i].v = make_uint4(0u, 0u, 0u, 0u);       // a position that is not there counts for nothing
+                xv[i].get(x);
+                d[i].get(dz[i]);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) { x[j] -= st.mean(j); z[j] = fmaf(x[j], ga[j] * st.rstd(j), be[j]); }
+                act_grad_mul<T, decltype(act)::value>(dz[i], z);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) { la[j] += dz[i][j]; lb_[j] = fmaf(dz[i][j], x[j], lb_[j]); }
+                xv[i].keep();
+                __builtin_amdgcn_sched_barrier(0);       // one item after the other: interleaved they need the registers of all
+            }
+            float s1[GPV], s2[GPV];
+#pragma unroll
+            for (int j = 0; j < GPV; ++j) s1[j] = s2[j] = 0.f;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                lb_[j] *= st.rstd(j);
+                sa[j] += la[j]; sb[j] += lb_[j];
+                s1[j * GPV / VEC] = fmaf(ga[j], la[j], s1[j * GPV / VEC]);
+                s2[j * GPV / VEC] = fmaf(ga[j], lb_[j], s2[j * GPV / VEC]);
+            }
+#pragma unroll
+            for (int j = 0; j < GPV; ++j) {
+                for (int o = p.LV; o < 64; o <<= 1) { s1[j] += __shfl_xor(s1[j], o, 64); s2[j] += __shfl_xor(s2[j], o, 64); }
+                if constexpr (GPV == 1)
+                    for (int o = 1; o < gl; o <<= 1) { s1[j] += __shfl_xor(s1[j], o, 64); s2[j] += __shfl_xor(s2[j], o, 64); }
+                s1[j] *= st.r[j] * inv_m;                                            // c1, c2
+                s2[j] *= st.r[j] * st.r[j] * inv_m;
+            }
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int s = pos + i * p.P;
+                float x[VEC], g[VEC];
+                xv[i].get(x);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) g[j] = fmaf(st.mean(j) - x[j], s2[j * GPV / VEC], fmaf(ga[j] * st.rstd(j), dz[i][j], -s1[j * GPV / VEC]));
+                uint4 o;
+                vec_put(o, g);
+                if (col_ok && s < p.S) ln.store(p.y, n * p.yn + s * p.ys + c0, o);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    });
+    for (int o = p.LV; o < 64; o <<= 1)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { sa[j] += __shfl_xor(sa[j], o, 64); sb[j] += __shfl_xor(sb[j], o, 64); }
+    if (pos == 0)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) red[wave][lv][j] = make_float2(sa[j], sb[j]);
+    __syncthreads();
+    if (wave == 0 && pos == 0 && col_ok)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float2 t = red[0][lv][j];
+            for (int w = 1; w < waves; ++w) { t.x += red[w][lv][j].x; t.y += red[w][lv][j].y; }
+            p.part[row * p.C + c0 + j] = t;
+        }
+}
+
+// ---- workgroup forms -----------------------------------------------------------------------------------------------------
 // Column sums (dz, dz xh) of a block's threads into tot[sub][CB] (float2).  red: [rows][CB] float2.
-template <int VEC>
-__device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float (&bq)[VEC], float2* red, float2* tot, int lv, int r) {
+template <int VEC, class O>
+__device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float (&bq)[VEC], float2* red, float2* tot, int col, int r, O&& own) {
     const int cols = p.LV * VEC;
     int rows = p.P;
     if (p.shuf) {
@@ -18,10 +117,10 @@ __device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float 
         rows = GTB / 64;
         if ((int)(threadIdx.x & 63) < p.LV)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) red[(threadIdx.x >> 6) * cols + lv * VEC + j] = make_float2(a[j], bq[j]);
+            for (int j = 0; j < VEC; ++j) if (own(j)) red[(threadIdx.x >> 6) * cols + col + j] = make_float2(a[j], bq[j]);
     } else if (r < p.P * p.NSUB) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) red[r * cols + lv * VEC + j] = make_float2(a[j], bq[j]);
+        for (int j = 0; j < VEC; ++j) if (own(j)) red[r * cols + col + j] = make_float2(a[j], bq[j]);
     }
     __syncthreads();
     for (int k = threadIdx.x; k < p.NSUB * cols; k += GTB) {
@@ -35,80 +134,84 @@ __device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float 
     }
     __syncthreads();
 }
+// gamma rstd and beta of a thread's channels
+template <int VEC, int GPV, bool TAIL>
+__device__ __forceinline__ void gn_affine(const GnP& p, const GnStat<VEC, GPV>& st, int c0, float (&a)[VEC], float (&be)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const int c = TAIL ? min(c0 + j, p.C - 1) : c0 + j;
+        a[j] = p.gamma[c] * st.rstd(j);
+        be[j] = p.beta[c];
+    }
+}
 
 // Held form: the block takes samples blockIdx, + gridDim, ...: dx, and its column sums over all of them in part[blockIdx C + c].
-// ACT: the activation, or -1: p.act (a choice inside the kernel costs the wide form its last registers).
+// ACT: the activation (chosen inside the kernel it would cost the last registers).
 // Lanes without a channel, a sample or a position read the last valid one instead and count for nothing, so that only stores are
 // under a lane mask.  Items are kept one after the other: interleaved by the compiler they would need the registers of all at once.
-template <class T, int VEC, int ITEMS, bool GS, bool CK, int ACT> __global__ __launch_bounds__(GTB) void gn_bwd_kernel(const GnP p) {
+template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ __launch_bounds__(GTB) void gn_bwd_kernel(const GnP p) {
     extern __shared__ float lds[];
+    constexpr int VEC = VEC16<T>;
     const int cols = p.LV * VEC;
     float2* red = (float2*)lds;
     float2* tot = red + (p.shuf ? (GTB / 64) * cols : p.P * p.NSUB * cols);
     float2* grp = tot + p.NSUB * cols;           // [NSUB][ng]
-    float2* acc = grp + p.NSUB * cols;           // [cols] (held form)
+    float2* acc = grp + p.NSUB * cols;           // [cols]
     const long long lb = xcd_order(blockIdx.x, p.blocks);
     const int cb = (int)(lb % p.ncb);
-    const long long t_ = lb / p.ncb;
-    const long long first = t_, stride = p.blocks / p.ncb;
+    const long long first = lb / p.ncb, stride = p.blocks / p.ncb;
     const GnBlock b = gn_block(p, cb);
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
     const int sub = r / p.P;
     int pos = r - sub * p.P;
     const int last = p.S - 1;
-    const bool col_ok = sub < p.NSUB && b.c_lo + lv * VEC < b.c_hi;
-    const int c0 = min(b.c_lo + lv * VEC, b.c_hi - VEC);
-    const int gl = (c0 - b.c_lo) / p.Cg;
+    const bool has = b.c_lo + lv * VEC < b.c_hi, col_ok = sub < p.NSUB && has;
+    const GnLane<T, TAIL> ln(b.c_lo, b.c_hi, min(lv, (b.c_hi - b.c_lo - 1) / VEC));
+    const int c0 = ln.c0;
+    const auto own = [&](int j) { return has && ln.own(j); };
+    int gi[GPV];
+#pragma unroll
+    for (int j = 0; j < GPV; ++j) gi[j] = min((c0 - b.c_lo + j) / p.Cg, b.ng - 1);
     for (int k = threadIdx.x; k < cols; k += GTB) acc[k] = make_float2(0.f, 0.f);
     const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
     for (long long nb0 = first; nb0 * p.NSUB < p.N; nb0 += stride) {
         const long long n0 = nb0 * p.NSUB + sub, n = min(n0, (long long)p.N - 1);
         const bool active = col_ok && n0 < p.N;
         asm volatile("" : "+v"(pos));            // the items' offsets are made where they are used, not kept over the samples
-        GnData<T, VEC> d[ITEMS];
-        typename std::conditional<CK, CkData<VEC>, GnData<T, VEC>>::type xv[ITEMS];
+        GnData<T, TAIL> d[ITEMS];
+        GnX<T, TAIL, CK> xv[ITEMS];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int s = min(pos + i * p.P, last);
-            if constexpr (CK) xv[i].load(p.q, p.e, n * p.S + s, p.C, p.nb, c0);
-            else xv[i].load(p.x, n * p.xn + s * p.xs + c0);
-            d[i].load(p.dy, n * p.dn + s * p.ds + c0);
-        }
-        GnStat<VEC, GS> st;
-        float a[VEC];                                // gamma rstd
-        float dz[ITEMS][VEC];             // held: its exp and reciprocal are half the work of a pass
+        for (int i = 0; i < ITEMS; ++i) gn_load<T, TAIL, CK>(p, xv[i], d[i], n, min(pos + i * p.P, last), ln);
+        GnStat<VEC, GPV> st;
+        float a[VEC];                            // gamma rstd
+        float dz[ITEMS][VEC];                    // held: its exp and reciprocal are half the work of a pass
         {
             float be[VEC], sa[VEC], sb[VEC];
 #pragma unroll
-            for (int j = 0; j < (GS ? 1 : VEC); ++j) {
-                const int g = b.g_lo + (GS ? gl : (c0 - b.c_lo + j) / p.Cg);
-                st.m[j] = p.mean[n * p.G + g];
-                st.r[j] = p.rstd[n * p.G + g];
+            for (int j = 0; j < GPV; ++j) { st.m[j] = p.mean[n * p.G + b.g_lo + gi[j]]; st.r[j] = p.rstd[n * p.G + b.g_lo + gi[j]]; }
+            gn_affine<VEC, GPV, TAIL>(p, st, c0, a, be);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) sa[j] = sb[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                float x[VEC], z[VEC], g[VEC];
+                if (!(active && pos + i * p.P <= last)) d[i].v = make_uint4(0u, 0u, 0u, 0u);
+                xv[i].get(x);
+                d[i].get(g);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) { x[j] -= st.mean(j); z[j] = fmaf(x[j], a[j], be[j]); }
+                act_grad_mul<T, ACT>(g, z);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    sa[j] += g[j]; sb[j] = fmaf(g[j], x[j], sb[j]);
+                    dz[i][j] = g[j];
+                }
+                xv[i].keep();
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) { a[j] = p.gamma[c0 + j] * st.rstd(j); be[j] = p.beta[c0 + j]; sa[j] = sb[j] = 0.f; }
-            act_choice<ACT>(p.act, [&](auto act) __attribute__((always_inline)) {
-#pragma unroll
-                for (int i = 0; i < ITEMS; ++i) {
-                    float x[VEC], z[VEC], g[VEC];
-                    if (!(active && pos + i * p.P <= last)) d[i].v = typename VecOf<T, VEC>::raw{};
-                    xv[i].get(x);
-                    d[i].get(g);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) { x[j] -= st.mean(j); z[j] = fmaf(x[j], a[j], be[j]); }
-                    act_grad_mul<T, decltype(act)::value>(g, z);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        sa[j] += g[j]; sb[j] = fmaf(g[j], x[j], sb[j]);
-                        dz[i][j] = g[j];
-                    }
-                    xv[i].keep();
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            });
-#pragma unroll
             for (int j = 0; j < VEC; ++j) sb[j] *= st.rstd(j);
-            gn_columns<VEC>(p, sa, sb, red, tot, lv, r);
+            gn_columns<VEC>(p, sa, sb, red, tot, c0 - b.c_lo, r, own);
         }
         for (int k = threadIdx.x; k < cols; k += GTB) {
             float2 t = acc[k];
@@ -130,10 +233,10 @@ template <class T, int VEC, int ITEMS, bool GS, bool CK, int ACT> __global__ __l
         }
         __syncthreads();
         asm volatile("" : "+v"(pos));
-        GnStat<VEC, GS> cc;                      // c1, c2 of the groups
+        GnStat<VEC, GPV> cc;                     // c1, c2 of the groups
 #pragma unroll
-        for (int j = 0; j < (GS ? 1 : VEC); ++j) {
-            const float2 t = grp[min(sub, p.NSUB - 1) * b.ng + (GS ? gl : (c0 - b.c_lo + j) / p.Cg)];
+        for (int j = 0; j < GPV; ++j) {
+            const float2 t = grp[min(sub, p.NSUB - 1) * b.ng + gi[j]];
             cc.m[j] = st.r[j] * t.x * inv_m;
             cc.r[j] = st.r[j] * st.r[j] * (t.y * inv_m);
         }
@@ -144,35 +247,29 @@ template <class T, int VEC, int ITEMS, bool GS, bool CK, int ACT> __global__ __l
             xv[i].get(x);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) g[j] = fmaf(st.mean(j) - x[j], cc.rstd(j), fmaf(a[j], dz[i][j], -cc.mean(j)));
-            typename VecOf<T, VEC>::raw o;
+            uint4 o;
             vec_put(o, g);
-            if (active && s <= last) *(typename VecOf<T, VEC>::raw*)((T*)p.y + n * p.yn + s * p.ys + c0) = o;
+            if (active && s <= last) ln.store(p.y, n * p.yn + s * p.ys + c0, o);
             __builtin_amdgcn_sched_barrier(0);
         }
-        __syncthreads();                              // red, tot and grp are free again
+        __syncthreads();                         // red, tot and grp are free again
     }
     for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTB) p.part[first * p.C + b.c_lo + k] = acc[k];
 }
 
-// f(x, dy, s) for positions s, s + P, ... below s_hi, U of them loaded at a time
-template <class T, int VEC, bool CK, class F> __device__ __forceinline__ void gn_walk(const GnP& p, long long n, int s, int s_hi, int c0, F&& f) {
-    for (; s < s_hi; s += U * p.P) {
-        typename std::conditional<CK, CkData<VEC>, GnData<T, VEC>>::type xv[U];
-        GnData<T, VEC> d[U];
+// f(x, dy, s) for positions s, s + P, ... below s_hi, GU of them loaded at a time
+template <class T, bool TAIL, bool CK, class F> __device__ __forceinline__ void gn_walk(const GnP& p, long long n, int s, int s_hi, const GnLane<T, TAIL>& l, F&& f) {
+    for (; s < s_hi; s += GU * p.P) {
+        GnX<T, TAIL, CK> xv[GU];
+        GnData<T, TAIL> d[GU];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < GU; ++u)
+            if (s + u * p.P < s_hi) gn_load<T, TAIL, CK>(p, xv[u], d[u], n, s + u * p.P, l);
+#pragma unroll
+        for (int u = 0; u < GU; ++u) {
             const int t = s + u * p.P;
             if (t < s_hi) {
-                if constexpr (CK) xv[u].load(p.q, p.e, n * p.S + t, p.C, p.nb, c0);
-                else xv[u].load(p.x, n * p.xn + t * p.xs + c0);
-                d[u].load(p.dy, n * p.dn + t * p.ds + c0);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int t = s + u * p.P;
-            if (t < s_hi) {
-                float x[VEC], g[VEC];
+                float x[VEC16<T>], g[VEC16<T>];
                 xv[u].get(x);
                 d[u].get(g);
                 f(x, g, t);
@@ -181,37 +278,42 @@ template <class T, int VEC, bool CK, class F> __device__ __forceinline__ void gn
     }
 }
 
+struct GnChunk { int cb, chunk; long long n; };
+__device__ __forceinline__ GnChunk gn_chunk(const GnP& p) {
+    const long long lb = xcd_order(blockIdx.x, p.blocks), t = lb / p.ncb;
+    return {(int)(lb % p.ncb), (int)(t % p.nchunk), t / p.nchunk};
+}
+
 // Chunked form, first launch: column sums of a chunk of positions in part[(n nchunk + chunk) C + c].
-template <class T, int VEC, bool GS, bool CK> __global__ __launch_bounds__(GTB) void gn_bwd_sums_kernel(const GnP p) {
+template <class T, int GPV, bool TAIL, bool CK> __global__ __launch_bounds__(GTB) void gn_bwd_sums_kernel(const GnP p) {
     extern __shared__ float lds[];
+    constexpr int VEC = VEC16<T>;
     const int cols = p.LV * VEC;
     float2* red = (float2*)lds;
     float2* tot = red + (p.shuf ? GTB / 64 : p.P) * cols;
-    const long long lb = xcd_order(blockIdx.x, p.blocks);
-    const int cb = (int)(lb % p.ncb);
-    const long long t_ = lb / p.ncb;
-    const int chunk = (int)(t_ % p.nchunk);
-    const long long n = t_ / p.nchunk;
-    const GnBlock b = gn_block(p, cb);
+    const GnChunk k_ = gn_chunk(p);
+    const GnBlock b = gn_block(p, k_.cb);
+    const long long n = k_.n;
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
-    const int c0 = b.c_lo + lv * VEC;
+    const bool has = b.c_lo + lv * VEC < b.c_hi;
+    const GnLane<T, TAIL> ln(b.c_lo, b.c_hi, lv);
+    const int c0 = ln.c0;
+    const auto own = [&](int j) { return has && ln.own(j); };
     float sa[VEC], sb[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) sa[j] = sb[j] = 0.f;
-    if (r < p.P && c0 < b.c_hi) {
-        GnStat<VEC, GS> st;
+    if (r < p.P && has) {
+        GnStat<VEC, GPV> st;
         float a[VEC], be[VEC];
 #pragma unroll
-        for (int j = 0; j < (GS ? 1 : VEC); ++j) {
-            const int g = b.g_lo + (p.pieces == 1 ? (lv * VEC + j) / p.Cg : 0);
+        for (int j = 0; j < GPV; ++j) {
+            const int g = b.g_lo + (p.pieces == 1 ? min((c0 - b.c_lo + j) / p.Cg, b.ng - 1) : 0);
             st.m[j] = p.mean[n * p.G + g];
             st.r[j] = p.rstd[n * p.G + g];
         }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) { a[j] = p.gamma[c0 + j] * st.rstd(j); be[j] = p.beta[c0 + j]; }
-        const int s_hi = min(p.S, (chunk + 1) * p.chunk);
+        gn_affine<VEC, GPV, TAIL>(p, st, c0, a, be);
         with_act(p.act, [&](auto act) __attribute__((always_inline)) {
-            gn_walk<T, VEC, CK>(p, n, chunk * p.chunk + r, s_hi, c0, [&](float (&x)[VEC], float (&g)[VEC], int s) __attribute__((always_inline)) {
+            gn_walk<T, TAIL, CK>(p, n, k_.chunk * p.chunk + r, min(p.S, (k_.chunk + 1) * p.chunk), ln, [&](float (&x)[VEC], float (&g)[VEC], int s) __attribute__((always_inline)) {
                 float z[VEC];
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) { x[j] -= st.mean(j); z[j] = fmaf(x[j], a[j], be[j]); }
@@ -223,89 +325,125 @@ template <class T, int VEC, bool GS, bool CK> __global__ __launch_bounds__(GTB) 
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sb[j] *= st.rstd(j);
     }
-    gn_columns<VEC>(p, sa, sb, red, tot, lv, r);
-    for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTB) p.part[(n * p.nchunk + chunk) * p.C + b.c_lo + k] = tot[k];
+    gn_columns<VEC>(p, sa, sb, red, tot, c0 - b.c_lo, r, own);
+    for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTB) p.part[(n * p.nchunk + k_.chunk) * p.C + b.c_lo + k] = tot[k];
 }
 
-// Chunked form, second launch: s1 and s2 of this block's groups from the column sums of every chunk, then dx.
-template <class T, int VEC, bool GS, bool CK> __global__ __launch_bounds__(GTB) void gn_bwd_apply_kernel(const GnP p) {
-    extern __shared__ float lds[];
-    float2* grp = (float2*)lds;
-    const long long lb = xcd_order(blockIdx.x, p.blocks);
-    const int cb = (int)(lb % p.ncb);
-    const long long t_ = lb / p.ncb;
-    const int chunk = (int)(t_ % p.nchunk);
-    const long long n = t_ / p.nchunk;
-    const GnBlock b = gn_block(p, cb);
-    const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
-    for (int g = threadIdx.x >> 6; g < b.ng; g += GTB / 64) {
-        float2 s = make_float2(0.f, 0.f);
-        for (int i = threadIdx.x & 63; i < p.nchunk * p.Cg; i += 64) {
-            const int ch = i / p.Cg, c = (b.g_lo + g) * p.Cg + (i - ch * p.Cg);
-            const float2 t = p.part[(n * p.nchunk + ch) * p.C + c];
-            const float w = p.gamma[c];
-            s.x = fmaf(w, t.x, s.x); s.y = fmaf(w, t.y, s.y);
-        }
-        s.x = wave_total(s.x); s.y = wave_total(s.y);
-        if ((threadIdx.x & 63) == 0) grp[g] = make_float2(s.x * inv_m, s.y * inv_m);
-    }
-    __syncthreads();
+// Chunked form, third launch: dx.
+template <class T, int GPV, bool TAIL, bool CK> __global__ __launch_bounds__(GTB) void gn_bwd_apply_kernel(const GnP p) {
+    constexpr int VEC = VEC16<T>;
+    const GnChunk k_ = gn_chunk(p);
+    const GnBlock b = gn_block(p, k_.cb);
+    const long long n = k_.n;
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
-    const int c0 = b.c_lo + lv * VEC;
-    if (r >= p.P || c0 >= b.c_hi) return;
-    GnStat<VEC, GS> st, cc;
+    if (r >= p.P || b.c_lo + lv * VEC >= b.c_hi) return;
+    const GnLane<T, TAIL> ln(b.c_lo, b.c_hi, lv);
+    const int c0 = ln.c0;
+    GnStat<VEC, GPV> st, cc;
 #pragma unroll
-    for (int j = 0; j < (GS ? 1 : VEC); ++j) {
-        const int g = p.pieces == 1 ? (lv * VEC + j) / p.Cg : 0;
-        st.m[j] = p.mean[n * p.G + b.g_lo + g];
-        st.r[j] = p.rstd[n * p.G + b.g_lo + g];
-        cc.m[j] = st.r[j] * grp[g].x; cc.r[j] = st.r[j] * st.r[j] * grp[g].y;
+    for (int j = 0; j < GPV; ++j) {
+        const long long g = n * p.G + b.g_lo + (p.pieces == 1 ? min((c0 - b.c_lo + j) / p.Cg, b.ng - 1) : 0);
+        st.m[j] = p.mean[g];
+        st.r[j] = p.rstd[g];
+        const float2 t = p.s12[g];
+        cc.m[j] = st.r[j] * t.x;
+        cc.r[j] = st.r[j] * st.r[j] * t.y;
     }
     float a[VEC], be[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) { a[j] = p.gamma[c0 + j] * st.rstd(j); be[j] = p.beta[c0 + j]; }
-    const int s_hi = min(p.S, (chunk + 1) * p.chunk);
+    gn_affine<VEC, GPV, TAIL>(p, st, c0, a, be);
     with_act(p.act, [&](auto act) __attribute__((always_inline)) {
-        gn_walk<T, VEC, CK>(p, n, chunk * p.chunk + r, s_hi, c0, [&](float (&x)[VEC], float (&g)[VEC], int s) __attribute__((always_inline)) {
+        gn_walk<T, TAIL, CK>(p, n, k_.chunk * p.chunk + r, min(p.S, (k_.chunk + 1) * p.chunk), ln, [&](float (&x)[VEC], float (&g)[VEC], int s) __attribute__((always_inline)) {
             float z[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) { x[j] -= st.mean(j); z[j] = fmaf(x[j], a[j], be[j]); }
             act_grad_mul<T, decltype(act)::value>(g, z);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) g[j] = fmaf(-x[j], cc.rstd(j), fmaf(a[j], g[j], -cc.mean(j)));
-            typename VecOf<T, VEC>::raw o;
+            uint4 o;
             vec_put(o, g);
-            *(typename VecOf<T, VEC>::raw*)((T*)p.y + n * p.yn + s * p.ys + c0) = o;
+            ln.store(p.y, n * p.yn + s * p.ys + c0, o);
         });
     });
 }
 
-template <class T, int VEC, bool GS, bool CK> int gn_bwd_t(const GnP& p, const GnPlan& pl, hipStream_t st) {
-    const int cols = p.LV * VEC;
-    const size_t lds = sizeof(float2) * ((size_t)(p.shuf ? GTB / 64 : p.P * p.NSUB) * cols + 2 * (size_t)p.NSUB * cols + cols);
-    if (!pl.held) {
-        const int rc = gn_launch(gn_bwd_sums_kernel<T, VEC, GS, CK>, p, GTB, lds, st);
-        if (rc != FAVAE_OK) return rc;
-        return gn_launch(gn_bwd_apply_kernel<T, VEC, GS, CK>, p, GTB, sizeof(float2) * cdiv(p.CB, std::min(p.Cg, p.CB)), st);
+// Sums over the rows of part [rows][C].  Blocks below gblocks (chunked form, second launch): (s1, s2) / m of a group a wave, from the
+// sample's nchunk rows.  The others: dbeta, dgamma of 4 channels, 256 rows at a time.
+__global__ __launch_bounds__(1024) void gn_join_kernel(const GnP p, long long rows, int gblocks, float* dgamma, float* dbeta) {
+    __shared__ float2 red[16][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if ((int)blockIdx.x < gblocks) {
+        const long long g = (long long)blockIdx.x * 16 + wave;
+        if (g >= (long long)p.N * p.G) return;
+        const long long n = g / p.G;
+        const int c0 = (int)(g - n * p.G) * p.Cg;
+        float2 s = make_float2(0.f, 0.f);
+        for (long long i = lane; i < (long long)p.nchunk * p.Cg; i += 64) {
+            const int ch = (int)(i / p.Cg), c = c0 + (int)(i - (long long)ch * p.Cg);
+            const float2 t = p.part[(n * p.nchunk + ch) * p.C + c];
+            const float w = p.gamma[c];
+            s.x = fmaf(w, t.x, s.x); s.y = fmaf(w, t.y, s.y);
+        }
+        s.x = wave_total(s.x); s.y = wave_total(s.y);
+        const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
+        if (lane == 0) p.s12[g] = make_float2(s.x * inv_m, s.y * inv_m);
+        return;
     }
-    if constexpr (VEC * sizeof(T) == 16) {
+    const int c = ((int)blockIdx.x - gblocks) * 4 + (threadIdx.x & 3);
+    float2 s = make_float2(0.f, 0.f);
+    if (c < p.C)
+#pragma unroll 4
+        for (long long i = threadIdx.x >> 2; i < rows; i += 256) {
+            const float2 t = p.part[i * p.C + c];
+            s.x += t.x; s.y += t.y;
+        }
+#pragma unroll
+    for (int o = 4; o < 64; o <<= 1) { s.x += __shfl_xor(s.x, o, 64); s.y += __shfl_xor(s.y, o, 64); }
+    if (lane < 4) red[wave][lane] = s;
+    __syncthreads();
+    if (threadIdx.x < 4 && c < p.C) {
+        float2 t = red[0][threadIdx.x];
+        for (int w = 1; w < 16; ++w) { t.x += red[w][threadIdx.x].x; t.y += red[w][threadIdx.x].y; }
+        if (dbeta) dbeta[c] = t.x;
+        if (dgamma) dgamma[c] = t.y;
+    }
+}
+
+template <class T, bool CK> int gn_bwd(const GnP& p, const GnPlan& pl, float* dgamma, float* dbeta, hipStream_t st) {
+    int rc = FAVAE_OK;
+    const int pblocks = dgamma || dbeta ? cdiv(p.C, 4) : 0;
+    const auto join = [&](int gblocks) {
+        if (gblocks + pblocks > 0) gn_join_kernel<<<gblocks + pblocks, 1024, 0, st>>>(p, pl.rows, gblocks, dgamma, dbeta);
+        FAVAE_LAUNCH_CHECK();
+        return FAVAE_OK;
+    };
+    if (pl.rows == 0) return join(0);                                    // no values: zero gradients
+    if (pl.form == GN_WAVE) {
+        rc = gn_wave_variants<T>(pl, [&](auto gpv, auto items) {
+            return gn_launch(gn_wave_bwd_kernel<T, decltype(items)::value, decltype(gpv)::value, CK>, p, pl.threads, 0, st);
+        });
+        return rc != FAVAE_OK ? rc : join(0);
+    }
+    const size_t cols = (size_t)p.LV * VEC16<T>, rows = p.shuf ? GTB / 64 : p.P * p.NSUB;
+    return gn_variants<T>(pl, [&](auto gpv, auto tail) {
+        constexpr int GPV = decltype(gpv)::value;
+        constexpr bool TAIL = decltype(tail)::value;
+        if (pl.form == GN_CHUNKED) {
+            int rc = gn_launch(gn_bwd_sums_kernel<T, GPV, TAIL, CK>, p, GTB, sizeof(float2) * (rows + 1) * cols, st);
+            if (rc != FAVAE_OK) return rc;
+            FAVAE_CHECK_ARG((long long)p.N * p.G <= 0x7fffffffLL, "favae_gn_act_bwd: too many groups for one launch");
+            rc = join((int)cdivll((long long)p.N * p.G, 16));
+            return rc != FAVAE_OK ? rc : gn_launch(gn_bwd_apply_kernel<T, GPV, TAIL, CK>, p, GTB, 0, st);
+        }
+        const size_t lds = sizeof(float2) * (rows + 2 * p.NSUB + 1) * cols;
         int rc = FAVAE_OK;
         with_act_host(p.act, [&](auto act) {
             constexpr int A = decltype(act)::value;
-            if (pl.items <= 4) rc = gn_launch(gn_bwd_kernel<T, VEC, 4, GS, CK, A>, p, GTB, lds, st);
-            else if (pl.items <= 8) rc = gn_launch(gn_bwd_kernel<T, VEC, 8, GS, CK, A>, p, GTB, lds, st);
-            else rc = gn_launch(gn_bwd_kernel<T, VEC, ITEMS_MAX, GS, CK, A>, p, GTB, lds, st);
+            if (pl.items <= 4) rc = gn_launch(gn_bwd_kernel<T, 4, GPV, TAIL, CK, A>, p, GTB, lds, st);
+            else if (pl.items <= 8) rc = gn_launch(gn_bwd_kernel<T, 8, GPV, TAIL, CK, A>, p, GTB, lds, st);
+            else rc = gn_launch(gn_bwd_kernel<T, ITEMS_MAX, GPV, TAIL, CK, A>, p, GTB, lds, st);
         });
-        return rc;
-    } else {
-        return pl.items <= 4 ? gn_launch(gn_bwd_kernel<T, VEC, 4, GS, CK, -1>, p, GTB, lds, st)
-                             : gn_launch(gn_bwd_kernel<T, VEC, ITEMS_MAX, GS, CK, -1>, p, GTB, lds, st);
-    }
-}
-template <class T, bool CK> int gn_bwd(const GnP& p, const GnPlan& pl, hipStream_t st) {
-#define GN_F(T_, V) { if constexpr (V == 1) return gn_bwd_t<T_, V, true, CK>(p, pl, st); else return pl.gs ? gn_bwd_t<T_, V, true, CK>(p, pl, st) : gn_bwd_t<T_, V, false, CK>(p, pl, st); }
-    GN_VEC(T, pl.vec, GN_F);
-#undef GN_F
+        return rc != FAVAE_OK ? rc : join(0);
+    });
 }
 
 }  // namespace

@@ -376,18 +376,7 @@ template <class T, class OT> __global__ __launch_bounds__(256) void gemm_join_ke
 // meet in LDS.  Rows of x or w that do not exist repeat the last one and are not stored.  1 x 4096 x 4096 bf16: 8.2 us, 4.1 TB/s of w; the
 // tile kernels take 15.  (For 32 and 64 rows of 4096 x 4096, with 2 and 4 row tiles of x a wave, 14 and 22 us against their 15 and 16: not kept.)
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
-template <class T> __device__ __forceinline__ uint4 load_chunk(const T* row, int k, int K) {     // 16 bytes from element k; past K zeros
-    constexpr int VE = 16 / sizeof(T);
-    uint4 t = make_uint4(0u, 0u, 0u, 0u);
-    if (k + VE <= K) __builtin_memcpy(&t, row + k, 16);
-    else {
-        T tmp[VE];
-#pragma unroll
-        for (int j = 0; j < VE; ++j) tmp[j] = k + j < K ? row[k + j] : (T)0;
-        __builtin_memcpy(&t, tmp, 16);
-    }
-    return t;
-}
+template <class T> __device__ __forceinline__ uint4 load_chunk(const T* row, int k, int K) { return load16(row + k, K - k); }     // from element k; past K zeros
 template <class T> __device__ __forceinline__ void mma16(f32x4_t& acc, const uint4& a, const uint4& b) {
     if constexpr (sizeof(T) == 2) {
         union { uint4 u; bf16x8 v; } x, y;
@@ -480,15 +469,11 @@ template <class T, int SRC> __global__ __launch_bounds__(256) void act_bwd_kerne
             for (long long i = r0 + w; i < r1; i += 4) {
                 uint4 rd = load_chunk((const T*)p.dy + i * p.lddy, j, p.N);
                 float d[V];
-                typename VecOf<T, V>::raw rv;
-                __builtin_memcpy(&rv, &rd, 16);
-                vec_get(d, rv);
+                vec_get(d, rd);
                 if constexpr (SRC > 0) {
                     float z[V];
                     if constexpr (SRC == 1) {
-                        const uint4 rz = load_chunk((const T*)p.pre + i * p.ldpre, j, p.N);
-                        __builtin_memcpy(&rv, &rz, 16);
-                        vec_get(z, rv);
+                        vec_get(z, load_chunk((const T*)p.pre + i * p.ldpre, j, p.N));
                     } else {
                         const float sc = ck_scale(p.pe[i * p.ldpe + (j >> 5)]);
                         const unsigned char* a8 = p.pq + i * p.ldpre + j;
@@ -503,9 +488,9 @@ template <class T, int SRC> __global__ __launch_bounds__(256) void act_bwd_kerne
                     act_grad_mul<T, decltype(a)::value>(d, z);       // (past N: dy is 0, and z is 0 or, in a faulty block, NaN)
 #pragma unroll
                     for (int k = 0; k < V; ++k) d[k] = j + k < p.N ? d[k] : 0.f;
-                    vec_put(rv, d);
+                    vec_put(rd, d);
                 }
-                if (p.du) *(typename VecOf<T, V>::raw*)((T*)p.du + i * p.ldu + j) = rv;
+                if (p.du) *(uint4*)((T*)p.du + i * p.ldu + j) = rd;
 #pragma unroll
                 for (int k = 0; k < V; ++k) s[k] += d[k];
             }
