@@ -7,8 +7,9 @@
 constexpr int GTF = 512, GTB = 256;     // threads of a workgroup, forward and backward
 constexpr int GU = 4;                   // positions a thread has under way in the chunked forms
 constexpr int WAVE_ITEMS = 8, ITEMS_MAX = 16;
+constexpr int GTP = 512, PIPED_ITEMS = 8;        // piped form
 
-enum GnForm { GN_WAVE, GN_HELD, GN_CHUNKED };
+enum GnForm { GN_WAVE, GN_PIPED, GN_HELD, GN_CHUNKED };
 
 struct GnP {
     const void *x, *dy;
@@ -58,6 +59,9 @@ __device__ __forceinline__ long long xcd_order(long long b, long long n) {
     return b < per * 8 ? (b & 7) * per + (b >> 3) : b;
 }
 
+// barrier for data in LDS: vector memory operations stay under way (__syncthreads waits for them)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 __device__ __forceinline__ float wave_total(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -90,7 +94,7 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
 #pragma unroll
         for (int j = 0; j < NV; ++j) if (own(j)) red[r * cols + col + j] = v[j];
     }
-    __syncthreads();
+    lds_barrier();
     // L lanes take a pair: as many as there are threads for every pair at once, at most its values
     const int pairs = p.NSUB * ng, per = rows * cpg, L = pair_lanes<GTF>(pairs, per), l = (int)threadIdx.x & (L - 1);
     for (int k = (int)threadIdx.x / L; k < pairs; k += GTF / L) {
@@ -103,7 +107,7 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
         for (int o = L >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
         if (l == 0) grp[k] = s;
     }
-    __syncthreads();
+    lds_barrier();
 }
 
 // The values a thread holds are kept as they lie in memory and converted anew in every pass: without this the compiler keeps the fp32
@@ -179,6 +183,20 @@ template <class T, bool TAIL> struct CkData {
     }
 };
 
+// ---- piped form: 16 bytes a lane between memory and LDS or registers through a buffer descriptor of one sample ---------------
+typedef unsigned gn_v4u __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* gn_lds;
+constexpr unsigned GN_NOWHERE = 0x80000000u;         // an offset outside every descriptor: loads give zeros, stores are dropped
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t gn_rsrc(const void* base, long long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + bytes), 0, 0x7fffffff, 0x00020000);
+}
+// items of a sample into buf[item][thread]: first offset `off`, `step` bytes between items, the first `mine` of them exist
+template <int ITEMS> __device__ __forceinline__ void gn_dma(char* buf, int wave, const __amdgpu_buffer_rsrc_t r, unsigned off, unsigned step, int mine) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (gn_lds)(buf + (i * GTP + wave * 64) * 16), 16, (int)(i < mine ? off + i * step : GN_NOWHERE), 0, 0, 0);
+}
+
 // Mean and rstd of a thread's channels: GPV values a vector, VEC / GPV neighbouring channels each
 template <int VEC, int GPV> struct GnStat {
     float m[GPV], r[GPV];
@@ -192,6 +210,13 @@ template <class T, class F> int gn_variants(const GnPlan& pl, F&& f) {
     if (!pl.tail) return f(std::integral_constant<int, VEC16<T>>(), std::false_type());
     return f(std::integral_constant<int, VEC16<T>>(), std::true_type());
 }
+// f(integral_constant<GPV>)
+template <class T, class F> int gn_gpv(const GnPlan& pl, F&& f) {
+    if (pl.gpv == 1) return f(std::integral_constant<int, 1>());
+    if (pl.gpv == 2) return f(std::integral_constant<int, 2>());
+    if (pl.gpv == 4) return f(std::integral_constant<int, 4>());
+    return f(std::integral_constant<int, VEC16<T>>());
+}
 // f(integral_constant<GPV>, integral_constant<ITEMS>) for the wave form
 template <class T, class F> int gn_wave_variants(const GnPlan& pl, F&& f) {
     const auto items = [&](auto gpv) {
@@ -200,10 +225,7 @@ template <class T, class F> int gn_wave_variants(const GnPlan& pl, F&& f) {
         if (pl.items <= 4) return f(gpv, std::integral_constant<int, 4>());
         return f(gpv, std::integral_constant<int, WAVE_ITEMS>());
     };
-    if (pl.gpv == 1) return items(std::integral_constant<int, 1>());
-    if (pl.gpv == 2) return items(std::integral_constant<int, 2>());
-    if (pl.gpv == 4) return items(std::integral_constant<int, 4>());
-    return items(std::integral_constant<int, VEC16<T>>());
+    return gn_gpv<T>(pl, items);
 }
 
 template <class K> int gn_launch(K k, const GnP& p, int threads, size_t lds, hipStream_t st) {

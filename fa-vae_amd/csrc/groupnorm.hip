@@ -7,10 +7,13 @@
 //   The kernels work with d = x - mean: z = fma(d, gamma rstd, beta), sum dz d, and dx = (gamma rstd) dz - c1 - d c2 with
 //   c1 = rstd s1 / m, c2 = rstd^2 s2 / m.
 //
-// Memory bounds both.  Three forms:
+// Memory bounds both.  Four forms:
 //   wave     the positions of a run of groups fit a wave's registers (up to 8 vectors of 16 bytes a lane; small maps): every wave works for
 //            itself, sums cross lanes by shuffles, there is no LDS and no barrier.
 //   held     they fit a workgroup's registers (up to 16 vectors a thread): the input is read once, sums meet in LDS.
+//   piped    (backward, up to 8 vectors a thread, 16-byte aligned tensors, enough samples) the same, and while the workgroup works on one sample
+//            the next is on its way into LDS, so that memory does not idle while a CU computes: 512 x 1024 x 128 bf16 silu 156 -> 97 us.
+//            (Forward two workgroups share a CU and cover each other: 68 us held, 81 piped, not kept.)
 //   chunked  they do not, or there are too few groups to fill the chip: a first launch leaves the partial sums of each chunk of positions,
 //            a later one joins them and makes the second pass over the data.
 // The variance is the sum of squared distances from the mean (no cancellation).  Sums are fp32 within a thread and joined in a fixed
@@ -292,7 +295,7 @@ template <class T, int GPV, bool TAIL> __global__ __launch_bounds__(GTF) void gn
             if (chunk == 0 && b.piece == 0) { p.mean[n * p.G + b.g_lo + g] = mean; p.rstd[n * p.G + b.g_lo + g] = rstd; }
         }
     }
-    __syncthreads();
+    lds_barrier();
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
     if (r >= p.P || b.c_lo + lv * VEC >= b.c_hi) return;
     const GnLane<T, TAIL> ln(b.c_lo, b.c_hi, lv);
@@ -339,7 +342,8 @@ template <class T, int GPV, bool TAIL> __global__ __launch_bounds__(GTF) void gn
 // ---- geometry ------------------------------------------------------------------------------------------------------------
 int pow2_floor(long long a) { int r = 1; while (2 * r <= a) r *= 2; return r; }
 
-GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt) {
+// even: 16-byte aligned rows
+GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
     GnPlan pl = {};
     const int vec = 16 / es, GT = backward ? GTB : GTF;
     const int S = std::max(1, p.S);
@@ -367,11 +371,28 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt) {
             return pl;
         }
     }
-    const int cap = GT * vec;
     const bool gs = p.Cg % vec == 0;
     long long unit = std::lcm((long long)p.Cg, (long long)vec);                          // whole groups that start on the vector grid
-    if (unit > cap) unit = p.Cg;
     pl.gpv = gs ? 1 : vec;
+    // piped form (backward): 32 lanes or fewer side by side (a power of two), at most 8 vectors a thread
+    if (backward && even && p.C % vec == 0 && unit <= 32 * vec) {
+        const auto fits = [&](int lv) { return (lv * vec) % unit == 0 && lv / 2 * vec < p.C && cdiv(S, GTP / lv) <= PIPED_ITEMS && S >= GTP / lv; };
+        int lv = 32;
+        while (lv > 1 && !fits(lv)) lv /= 2;
+        while (lv > 4 && cdiv(S, GTP / lv) > 4 && (long long)p.N * cdiv(p.C, lv * vec) < 1024 && fits(lv / 2)) lv /= 2;
+        if (lv > 1 && (long long)p.N * cdiv(p.C, lv * vec) >= 512) {
+            pl.form = GN_PIPED;
+            pl.gpv = gs ? 1 : vec % p.Cg == 0 ? vec / p.Cg : vec;
+            p.LV = lv; p.P = GTP / lv; p.CB = lv * vec; p.ncb = cdiv(p.C, p.CB);
+            pl.threads = GTP;
+            pl.rows = std::min<long long>(p.N, std::max(1, 256 / p.ncb));
+            pl.blocks = p.blocks = pl.rows * p.ncb;
+            pl.part = (size_t)pl.rows * p.C;
+            return pl;
+        }
+    }
+    const int cap = GT * vec;
+    if (unit > cap) unit = p.Cg;
     if (unit > cap) {                                       // a group wider than a workgroup's lanes
         p.CB = cap;
         p.pieces = cdiv(p.Cg, cap);
@@ -394,7 +415,7 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt) {
         p.shuf = p.NSUB == 1 && p.LV <= 32 && (p.LV & (p.LV - 1)) == 0 && p.P * p.LV == GT;
     };
     lanes();
-    // fewer channels side by side, down to 32 bytes, where a run of groups does not fit a workgroup's registers or where there would be
+    // fewer channels side by side, down to 32 bytes (64 x 4096 x 64 and 512 x 4096 x 64 bf16: 23 and 186 us so, chunked 25 and 212), where a run of groups does not fit a workgroup's registers or where there would be
     // fewer workgroups than CUs (the blocks that share a cache line run on one XCD)
     while (p.pieces == 1 && p.CB % 2 == 0 && (p.CB / 2) % unit == 0 && p.CB / 2 * es >= 32 && !(ckpt && p.CB % 64) &&
            (cdiv(S, p.P) > ITEMS_MAX || (S * (long long)p.CB > 16 * vec * 64 && cdivll(p.N, p.NSUB) * p.ncb < 512))) {
@@ -404,7 +425,7 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt) {
     }
     const long long held_blocks = cdivll(p.N, p.NSUB) * p.ncb;
     pl.threads = GT;
-    if (p.pieces == 1 && cdiv(S, p.P) <= ITEMS_MAX && (held_blocks >= 64 || cdiv(S, p.P) <= 4)) {
+    if (p.pieces == 1 && cdiv(S, p.P) <= ITEMS_MAX && (held_blocks >= (ckpt ? 256 : 64) || cdiv(S, p.P) <= 4)) {
         pl.form = GN_HELD;
         pl.items = cdiv(S, p.P);
         // backward: a workgroup goes over several samples and leaves one row of column sums
@@ -459,16 +480,20 @@ int gn_sizes(const char* who, long long N, long long S, int C, int G, int act, i
     return FAVAE_OK;
 }
 bool aligned(const void* a, int es) { return (uintptr_t)a % (size_t)es == 0; }
+// 16-byte aligned rows, and a sample within 31 bits
+bool even16(const void* a, long long n, long long s, long long S, int C, int es) {
+    return aligned(a, 16) && n * es % 16 == 0 && s * es % 16 == 0 && (S * s + C) * es < 0x70000000LL;
+}
 
 }  // namespace
 
 extern "C" size_t favae_gn_act_scratch(long long N, long long S, int C, int G, int backward, int dtype) {
     if (gn_sizes("favae_gn_act_scratch", N, S, C, G, FAVAE_ACT_NONE, dtype) != FAVAE_OK) return 0;
     size_t need = 0;
-    for (bool ckpt : {false, true}) {
+    for (bool either : {false, true}) {                     // forward: with a checkpoint or without; backward: aligned or not
         GnP p = {};
         p.N = (int)N; p.S = (int)S; p.C = C; p.G = G; p.Cg = C / G;
-        need = std::max(need, gn_plan(p, dtype == FAVAE_F32 ? 4 : 2, backward != 0, ckpt && !backward).part);
+        need = std::max(need, gn_plan(p, dtype == FAVAE_F32 ? 4 : 2, backward != 0, either && !backward, either && backward).part);
     }
     return need * sizeof(float2);
 }
@@ -488,7 +513,7 @@ extern "C" int favae_gn_act_fwd(const void* x, long long xn, long long xs, long 
     p.x = x; p.xn = xn; p.xs = xs; p.y = y; p.yn = yn; p.ys = ys;
     p.gamma = gamma; p.beta = beta; p.mean = mean; p.rstd = rstd; p.part = (float2*)scratch;
     p.N = (int)N; p.S = (int)S; p.C = C; p.G = G; p.Cg = C / G; p.act = act; p.eps = eps; p.nb = cdiv(C, CK_BLOCK);
-    const GnPlan pl = gn_plan(p, es, false, q != nullptr);
+    const GnPlan pl = gn_plan(p, es, false, q != nullptr, false);
     FAVAE_CHECK_ARG(pl.part * sizeof(float2) <= scratch_bytes && (pl.part == 0 || scratch), "favae_gn_act_fwd: scratch of %zu bytes, %zu needed", scratch_bytes,
                     pl.part * sizeof(float2));
     if (q && S > 0) {
@@ -524,7 +549,8 @@ extern "C" int favae_gn_act_bwd(const void* dy, long long dn, long long ds, cons
     p.N = (int)N; p.S = (int)S; p.C = C; p.G = G; p.Cg = C / G; p.act = act; p.nb = cdiv(C, CK_BLOCK);
     GnPlan pl = {};
     if (any) {
-        pl = gn_plan(p, es, true, false);
+        const bool even = (!x || even16(x, xn, xs, S, C, es)) && even16(dy, dn, ds, S, C, es) && even16(dx, dxn, dxs, S, C, es);
+        pl = gn_plan(p, es, true, false, even);
         FAVAE_CHECK_ARG(pl.part * sizeof(float2) <= scratch_bytes && scratch, "favae_gn_act_bwd: scratch of %zu bytes, %zu needed", scratch_bytes,
                         pl.part * sizeof(float2));
         p.s12 = p.part + (size_t)pl.rows * C;

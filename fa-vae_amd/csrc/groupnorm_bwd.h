@@ -94,7 +94,7 @@ template <class T, int ITEMS, int GPV, bool CK> __global__ __launch_bounds__(256
     if (pos == 0)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) red[wave][lv][j] = make_float2(sa[j], sb[j]);
-    __syncthreads();
+    lds_barrier();
     if (wave == 0 && pos == 0 && col_ok)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -102,6 +102,147 @@ template <class T, int ITEMS, int GPV, bool CK> __global__ __launch_bounds__(256
             for (int w = 1; w < waves; ++w) { t.x += red[w][lv][j].x; t.y += red[w][lv][j].y; }
             p.part[row * p.C + c0 + j] = t;
         }
+}
+
+// ---- piped form ----------------------------------------------------------------------------------------------------------
+// The block takes channel block blockIdx % ncb of samples blockIdx / ncb, + gridDim / ncb, ...  dy, and x unless it is a checkpoint, come through
+// LDS, where a wave reads back what its own DMA brought, so that only the sums need barriers; a checkpoint's 9 bytes a vector and the statistics
+// of the next sample wait in registers.  Stores go through a descriptor too, lanes without a position storing nowhere: the loads of the next
+// sample are then older than exactly ITEMS stores, and waiting for all but ITEMS operations waits for the loads alone.  Column sums over the
+// block's samples go to part[row C + c].
+template <class T, int GPV, bool CK, int ACT> __global__ __launch_bounds__(GTP) void gn_piped_bwd_kernel(const GnP p) {
+    extern __shared__ float lds[];
+    constexpr int VEC = VEC16<T>, ITEMS = PIPED_ITEMS;
+    constexpr long long ES = sizeof(T);
+    const int cols = p.LV * VEC;
+    char* dbuf = (char*)lds;
+    char* xbuf = dbuf + ITEMS * GTP * 16;
+    float2* red = (float2*)(xbuf + (CK ? 0 : ITEMS * GTP * 16));      // [GTP / 64][cols]
+    float2* tot = red + (GTP / 64) * cols;                            // [cols]
+    float2* grp = tot + cols;                                         // [ng]
+    float2* acc = grp + cols;                                         // [cols]
+    float* gam = (float*)(acc + cols);                                // [cols]
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const long long lb = xcd_order(blockIdx.x, p.blocks);
+    const int cb = (int)(lb % p.ncb);
+    const long long row = lb / p.ncb, stride = p.blocks / p.ncb;
+    const GnBlock b = gn_block(p, cb);
+    const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
+    const bool has = b.c_lo + lv * VEC < b.c_hi;
+    const GnLane<T, false> ln(min(b.c_lo + lv * VEC, b.c_hi - VEC), b.c_hi, 0);
+    const int c0 = ln.c0, mine = has ? (p.S - r + p.P - 1) / p.P : 0;
+    const unsigned dof = (unsigned)((r * p.ds + c0) * ES), dstep = (unsigned)(p.P * p.ds * ES);
+    const unsigned xof = (unsigned)((r * p.xs + c0) * ES), xstep = (unsigned)(p.P * p.xs * ES);
+    const unsigned yof = (unsigned)((r * p.ys + c0) * ES), ystep = (unsigned)(p.P * p.ys * ES);
+    int gi[GPV];
+#pragma unroll
+    for (int j = 0; j < GPV; ++j) gi[j] = (c0 - b.c_lo + j * (VEC / GPV)) / p.Cg;
+    float ga[VEC], be[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { ga[j] = p.gamma[c0 + j]; be[j] = p.beta[c0 + j]; }
+    for (int k = threadIdx.x; k < cols; k += GTP) {
+        acc[k] = make_float2(0.f, 0.f);
+        gam[k] = b.c_lo + k < b.c_hi ? p.gamma[b.c_lo + k] : 0.f;
+    }
+    const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
+    GnStat<VEC, GPV> nst;
+    CkData<T, false> nx[CK ? ITEMS : 1];
+    const auto fetch = [&](long long n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < GPV; ++j) { nst.m[j] = p.mean[n * p.G + b.g_lo + gi[j]]; nst.r[j] = p.rstd[n * p.G + b.g_lo + gi[j]]; }
+        if constexpr (CK) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) nx[i].load(p.q, p.e, n * p.S + min(r + i * p.P, p.S - 1), p.C, p.nb, ln);
+        } else gn_dma<ITEMS>(xbuf, wave, gn_rsrc(p.x, n * p.xn * ES), xof, xstep, mine);
+        gn_dma<ITEMS>(dbuf, wave, gn_rsrc(p.dy, n * p.dn * ES), dof, dstep, mine);
+    };
+    long long n = row;
+    fetch(n);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (; n < p.N; n += stride) {
+        GnData<T, false> d[ITEMS];
+        GnX<T, false, CK> xv[ITEMS];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            d[i].v = *(const uint4*)(dbuf + (i * GTP + (int)threadIdx.x) * 16);
+            if constexpr (CK) xv[i] = nx[i];
+            else xv[i].v = *(const uint4*)(xbuf + (i * GTP + (int)threadIdx.x) * 16);
+        }
+        const GnStat<VEC, GPV> st = nst;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the buffers are read: the next sample may come
+        if (n + stride < p.N) fetch(n + stride);
+        float a[VEC], dz[ITEMS][VEC];
+        {
+            float sa[VEC], sb[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) { a[j] = ga[j] * st.rstd(j); sa[j] = sb[j] = 0.f; }
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                float x[VEC], z[VEC], g[VEC];
+                xv[i].get(x);
+                d[i].get(g);                                          // (zeros where there is no position)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) { x[j] -= st.mean(j); z[j] = fmaf(x[j], a[j], be[j]); }
+                act_grad_mul<T, ACT>(g, z);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    sa[j] += g[j]; sb[j] = fmaf(g[j], x[j], sb[j]);
+                    dz[i][j] = g[j];
+                }
+                xv[i].keep();
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) sb[j] *= st.rstd(j);
+            // sums of the rows of a wave by shuffles, of the waves in LDS
+            for (int o = p.LV; o < 64; o <<= 1)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) { sa[j] += __shfl_xor(sa[j], o, 64); sb[j] += __shfl_xor(sb[j], o, 64); }
+            if ((int)(threadIdx.x & 63) < p.LV && has)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) red[wave * cols + lv * VEC + j] = make_float2(sa[j], sb[j]);
+        }
+        lds_barrier();
+        for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTP) {
+            float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < GTP / 64; ++w) { const float2 t = red[w * cols + k]; s.x += t.x; s.y += t.y; }
+            const float2 u = acc[k];
+            acc[k] = make_float2(u.x + s.x, u.y + s.y);
+            tot[k] = make_float2(gam[k] * s.x, gam[k] * s.y);
+        }
+        lds_barrier();
+        const int L = pair_lanes<GTP>(b.ng, b.cw), l = (int)threadIdx.x & (L - 1);
+        for (int g = (int)threadIdx.x / L; g < b.ng; g += GTP / L) {
+            float2 s = make_float2(0.f, 0.f);
+            for (int c = g * b.cw + l; c < (g + 1) * b.cw; c += L) { s.x += tot[c].x; s.y += tot[c].y; }
+            for (int o = L >> 1; o > 0; o >>= 1) { s.x += __shfl_xor(s.x, o, 64); s.y += __shfl_xor(s.y, o, 64); }
+            if (l == 0) grp[g] = s;
+        }
+        lds_barrier();
+        GnStat<VEC, GPV> cc;                                          // c1, c2 of the groups
+#pragma unroll
+        for (int j = 0; j < GPV; ++j) {
+            const float2 t = grp[gi[j]];
+            cc.m[j] = st.r[j] * t.x * inv_m;
+            cc.r[j] = st.r[j] * st.r[j] * (t.y * inv_m);
+        }
+        const __amdgpu_buffer_rsrc_t ry = gn_rsrc(p.y, n * p.yn * ES);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            float x[VEC], g[VEC];
+            xv[i].get(x);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) g[j] = fmaf(st.mean(j) - x[j], cc.rstd(j), fmaf(a[j], dz[i][j], -cc.mean(j)));
+            uint4 o;
+            vec_put(o, g);
+            __builtin_amdgcn_raw_buffer_store_b128(gn_v4u{o.x, o.y, o.z, o.w}, ry, (int)(i < mine ? yof + i * ystep : GN_NOWHERE), 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ITEMS) : "memory");
+    }
+    lds_barrier();
+    for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTP) p.part[row * p.C + b.c_lo + k] = acc[k];
 }
 
 // ---- workgroup forms -----------------------------------------------------------------------------------------------------
@@ -122,7 +263,7 @@ __device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float 
 #pragma unroll
         for (int j = 0; j < VEC; ++j) if (own(j)) red[r * cols + col + j] = make_float2(a[j], bq[j]);
     }
-    __syncthreads();
+    lds_barrier();
     for (int k = threadIdx.x; k < p.NSUB * cols; k += GTB) {
         const int sub = k / cols, c = k - sub * cols;
         float2 s = make_float2(0.f, 0.f);
@@ -132,7 +273,7 @@ __device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float 
         }
         tot[k] = s;
     }
-    __syncthreads();
+    lds_barrier();
 }
 // gamma rstd and beta of a thread's channels
 template <int VEC, int GPV, bool TAIL>
@@ -231,7 +372,7 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ _
             for (int o = L >> 1; o > 0; o >>= 1) { s.x += __shfl_xor(s.x, o, 64); s.y += __shfl_xor(s.y, o, 64); }
             if (l == 0) grp[k] = s;
         }
-        __syncthreads();
+        lds_barrier();
         asm volatile("" : "+v"(pos));
         GnStat<VEC, GPV> cc;                     // c1, c2 of the groups
 #pragma unroll
@@ -252,7 +393,7 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ _
             if (active && s <= last) ln.store(p.y, n * p.yn + s * p.ys + c0, o);
             __builtin_amdgcn_sched_barrier(0);
         }
-        __syncthreads();                         // red, tot and grp are free again
+        lds_barrier();                           // red, tot and grp are free again
     }
     for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTB) p.part[first * p.C + b.c_lo + k] = acc[k];
 }
@@ -399,7 +540,7 @@ __global__ __launch_bounds__(1024) void gn_join_kernel(const GnP p, long long ro
 #pragma unroll
     for (int o = 4; o < 64; o <<= 1) { s.x += __shfl_xor(s.x, o, 64); s.y += __shfl_xor(s.y, o, 64); }
     if (lane < 4) red[wave][lane] = s;
-    __syncthreads();
+    lds_barrier();
     if (threadIdx.x < 4 && c < p.C) {
         float2 t = red[0][threadIdx.x];
         for (int w = 1; w < 16; ++w) { t.x += red[w][threadIdx.x].x; t.y += red[w][threadIdx.x].y; }
@@ -420,6 +561,15 @@ template <class T, bool CK> int gn_bwd(const GnP& p, const GnPlan& pl, float* dg
     if (pl.form == GN_WAVE) {
         rc = gn_wave_variants<T>(pl, [&](auto gpv, auto items) {
             return gn_launch(gn_wave_bwd_kernel<T, decltype(items)::value, decltype(gpv)::value, CK>, p, pl.threads, 0, st);
+        });
+        return rc != FAVAE_OK ? rc : join(0);
+    }
+    if (pl.form == GN_PIPED) {
+        const size_t cols = (size_t)p.LV * VEC16<T>;
+        const size_t lds = (size_t)(CK ? 1 : 2) * PIPED_ITEMS * GTP * 16 + sizeof(float2) * (GTP / 64 + 3) * cols + sizeof(float) * cols;
+        with_act_host(p.act, [&](auto act) {
+            constexpr int A = decltype(act)::value;
+            rc = gn_gpv<T>(pl, [&](auto gpv) { return gn_launch(gn_piped_bwd_kernel<T, decltype(gpv)::value, CK, A>, p, GTP, lds, st); });
         });
         return rc != FAVAE_OK ? rc : join(0);
     }
