@@ -29,7 +29,14 @@ __device__ __forceinline__ void mma(f32x16& acc, const Frag<bf16_t>& a, const Fr
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, acc, 0, 0, 0);
 }
 
-typedef unsigned v4u __attribute__((ext_vector_type(4)));
+// Two transposing LDS loads, `second` bytes apart.  `restrict`: what it reads is not written while it runs, so that the compiler need not put a wait
+// for every DMA under way before it; the kernel's own waits order the two.
+__device__ __forceinline__ bf16x8 read_tr(const char* __restrict a, int second) {
+    union { s16x4 s[2]; bf16x8 b; } c;
+    c.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
+    c.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + second));
+    return c.b;
+}
 
 struct GemmP {
     const char *P, *Q;                    // operands
@@ -86,10 +93,7 @@ template <class T, int ROWS, bool CM, int BKE_ = 128 / (int)sizeof(T)> struct Ti
             const int row = k0 + 8 * h + (i >> 2);                    // and row + 4: the same swizzle
             const int ch = ((((rb >> 5) ^ piece_swz(row)) << 2) | (2 * ((lane >> 4) & 1) + ((i & 3) >> 1)));
             const char* a = lds + row * (ROWS * 2) + ch * 16 + 8 * (i & 1);
-            union { s16x4 s[2]; bf16x8 b; } c;
-            c.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
-            c.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 4 * ROWS * 2));
-            f.v = c.b;
+            f.v = read_tr(a, 4 * ROWS * 2);
         } else {
             const int ch = (rb + r) >> 2;
 #pragma unroll
@@ -98,9 +102,24 @@ template <class T, int ROWS, bool CM, int BKE_ = 128 / (int)sizeof(T)> struct Ti
     }
 };
 
-// 8 neighbouring output columns of a row, `left` of which exist: bias, activation, residual, store.  oo, op, orr: element offsets in out, pre and
-// res.  FAST: all 8 exist.  (16-byte accesses at any alignment of the type: the memory system takes them, at a cost where they cross lines.)
-template <class T, class OT, bool FAST> __device__ __forceinline__ void epilogue8(const GemmP& p, float (&f)[8], const float (&bias)[8], int left, long long oo, long long op, long long orr) {
+// 8 neighbouring elements of the residual, as they are in memory
+template <class T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
+// FAST: all 8 exist, else `left` of them (zeros behind).  16-byte accesses at any alignment of the type: the memory system takes them, at a
+// cost where they cross lines.
+template <class T, bool FAST> __device__ __forceinline__ Raw8<T> load_res(const T* a, int left) {
+    Raw8<T> r;
+    if (FAST || left >= 8) __builtin_memcpy(&r, a, sizeof(r));
+    else {
+        float t[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = k < left ? to_f32<T>(a[k]) : 0.f;
+        if constexpr (sizeof(T) == 2) vec_put(r.v[0], t);
+        else __builtin_memcpy(&r, t, sizeof(r));
+    }
+    return r;
+}
+// 8 neighbouring output columns of a row, `left` of which exist: bias, activation, residual, store.  oo, op: element offsets in out and pre
+template <class T, class OT, bool FAST> __device__ __forceinline__ void epilogue8(const GemmP& p, float (&f)[8], const float (&bias)[8], const Raw8<T>& res, int left, long long oo, long long op) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] += bias[k];
     const auto put = [&](OT* o) __attribute__((always_inline)) {
@@ -115,15 +134,9 @@ template <class T, class OT, bool FAST> __device__ __forceinline__ void epilogue
     if (p.pre) put((OT*)p.pre + op);
     with_act(p.act, [&](auto a) __attribute__((always_inline)) { act_apply<T, decltype(a)::value>(f); });
     if (p.res) {
-        const T* a = (const T*)p.res + orr;
         float t[8];
-        if (FAST || left >= 8) {
-            if constexpr (sizeof(T) == 2) { uint4 r; __builtin_memcpy(&r, a, 16); vec_get(t, r); }
-            else { __builtin_memcpy(t, a, 16); __builtin_memcpy(t + 4, a + 4, 16); }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = k < left ? to_f32<T>(a[k]) : 0.f;
-        }
+        if constexpr (sizeof(T) == 2) vec_get(t, res.v[0]);
+        else __builtin_memcpy(t, &res, sizeof(t));
 #pragma unroll
         for (int k = 0; k < 8; ++k) f[k] += t[k];
     }
@@ -186,42 +199,25 @@ __device__ __forceinline__ void gemm_tile(const GemmP& p, int& split, int& ti, i
 }
 
 // Output tile of a wave through LDS: 32 rows at a time in a region of its own, [32][NJ * 32 + 4] fp32, so that a lane ends up with 8
-// neighbouring columns of a row, 16 bytes of bf16; its columns are the same in every row it takes
-template <class T, class OT, bool FAST, int NJ, int EL>
-__device__ __forceinline__ void epilogue_rows(const GemmP& p, const float* tile, const float (&bias)[8], long long i_lo, int j, int split, int lane) {
-    constexpr int WC = NJ * 32, RS = WC + 4, LPR = WC / 8, STEP = 64 / LPR;
-    const int r0 = lane / LPR;
-    const float* src = tile + r0 * RS + (lane % LPR) * 8;
-    const long long i0 = i_lo + r0;
-    long long oo = i0 * p.ldo + j, op = i0 * p.ldpre + j, orr = i0 * p.ldr + j;
-    if (p.splits > 1) {
-        float* o = p.part + ((long long)split * p.I + i0) * p.ldpart + j;
-#pragma unroll FAST ? 4 : 1
-        for (int e = 0; e < EL; ++e) {
-            const float4 lo = *(const float4*)src, hi = *(const float4*)(src + 4);
-            if (FAST || (i0 + e * STEP < p.I && j < p.J)) { ((float4*)o)[0] = lo; ((float4*)o)[1] = hi; }
-            src += STEP * RS;
-            o += (long long)STEP * p.ldpart;
-        }
-        return;
-    }
-#pragma unroll FAST ? 2 : 1
-    for (int e = 0; e < EL; ++e) {
-        const float4 lo = *(const float4*)src, hi = *(const float4*)(src + 4);
-        float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        if (FAST || (i0 + e * STEP < p.I && j < p.J)) epilogue8<T, OT, FAST>(p, f, bias, p.J - j, oo, op, orr);
-        src += STEP * RS;
-        oo += STEP * p.ldo; op += STEP * p.ldpre; orr += STEP * p.ldr;
-    }
-}
-template <class T, class OT, int TI, int TJ, int WI, int WJ, int NI, int NJ>
-__device__ __forceinline__ void gemm_epilogue(const GemmP& p, f32x16 (&acc)[NI][NJ], char* smem, long long i0, int j0, int split, int lane, int wi, int wj, int wave) {
-    constexpr int WC = NJ * 32, RS = WC + 4, LPR = WC / 8, EL = 32 * LPR / 64;
-    float* tile = (float*)smem + wave * 32 * RS;
-    const int j = j0 + wj * WC + (lane % LPR) * 8;
+// neighbouring columns of a row, 16 bytes of bf16; its columns are the same in every row it takes.  The residual of the next 32 rows is on its
+// way while 32 are written (65536 x 1024 x 1024 with gelu and residual: 178 us, 203 with a load at each use).
+template <class T, class OT, int TI, int TJ, int WI, int WJ, int NI, int NJ, bool FAST>
+__device__ __forceinline__ void epilogue_tiles(const GemmP& p, f32x16 (&acc)[NI][NJ], float* tile, long long i0, int j, int split, int lane, int wi) {
+    constexpr int WC = NJ * 32, RS = WC + 4, LPR = WC / 8, EL = 32 * LPR / 64, STEP = 64 / LPR;
+    const int r0 = lane / LPR, left = p.J - j;
+    const long long i_lo = i0 + wi * (TI / WI) + r0;               // row of this lane; + 32 a + STEP e
     float bias[8];
     load_bias(p, bias, j);
-    const bool fast = i0 + TI <= p.I && j0 + TJ <= p.J;
+    const bool with_res = p.res && p.splits == 1;
+    Raw8<T> res[2][EL];
+    const auto fetch = [&](Raw8<T> (&r)[EL], int a) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < EL; ++e) {
+            const long long i = i_lo + 32 * a + STEP * e;
+            r[e] = load_res<T, FAST>((const T*)p.res + i * p.ldr + j, FAST || i < p.I ? left : 0);
+        }
+    };
+    if (with_res) fetch(res[0], 0);
     __syncthreads();
 #pragma unroll
     for (int a = 0; a < NI; ++a) {
@@ -231,11 +227,41 @@ __device__ __forceinline__ void gemm_epilogue(const GemmP& p, f32x16 (&acc)[NI][
             for (int e = 0; e < 4; ++e)
                 *(float4*)(tile + (lane & 31) * RS + c * 32 + 8 * e + 4 * (lane >> 5)) = make_float4(acc[a][c][4 * e], acc[a][c][4 * e + 1], acc[a][c][4 * e + 2], acc[a][c][4 * e + 3]);
         __builtin_amdgcn_wave_barrier();
-        const long long i_lo = i0 + wi * (TI / WI) + a * 32;
-        if (fast) epilogue_rows<T, OT, true, NJ, EL>(p, tile, bias, i_lo, j, split, lane);
-        else epilogue_rows<T, OT, false, NJ, EL>(p, tile, bias, i_lo, j, split, lane);
+        if (with_res && a + 1 < NI) fetch(res[(a + 1) & 1], a + 1);
+        const float* src = tile + r0 * RS + (lane % LPR) * 8;
+        const long long i = i_lo + 32 * a;
+        long long oo = i * p.ldo + j, op = i * p.ldpre + j;
+        if (p.splits > 1) {
+            float* o = p.part + ((long long)split * p.I + i) * p.ldpart + j;
+#pragma unroll FAST ? 4 : 1
+            for (int e = 0; e < EL; ++e) {
+                const float4 lo = *(const float4*)src, hi = *(const float4*)(src + 4);
+                if (FAST || (i + e * STEP < p.I && left > 0)) { ((float4*)o)[0] = lo; ((float4*)o)[1] = hi; }
+                src += STEP * RS;
+                o += (long long)STEP * p.ldpart;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < EL; ++e) {
+                const float4 lo = *(const float4*)src, hi = *(const float4*)(src + 4);
+                float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                if (FAST || (i + e * STEP < p.I && left > 0)) {
+                    epilogue8<T, OT, FAST>(p, f, bias, res[a & 1][e], left, oo, op);
+                }
+                src += STEP * RS;
+                oo += STEP * p.ldo; op += STEP * p.ldpre;
+            }
+        }
         __builtin_amdgcn_wave_barrier();
     }
+}
+template <class T, class OT, int TI, int TJ, int WI, int WJ, int NI, int NJ>
+__device__ __forceinline__ void gemm_epilogue(const GemmP& p, f32x16 (&acc)[NI][NJ], char* smem, long long i0, int j0, int split, int lane, int wi, int wj, int wave) {
+    constexpr int WC = NJ * 32;
+    float* tile = (float*)smem + wave * 32 * (WC + 4);
+    const int j = j0 + wj * WC + (lane % (WC / 8)) * 8;
+    if (i0 + TI <= p.I && j0 + TJ <= p.J) epilogue_tiles<T, OT, TI, TJ, WI, WJ, NI, NJ, true>(p, acc, tile, i0, j, split, lane, wi);
+    else epilogue_tiles<T, OT, TI, TJ, WI, WJ, NI, NJ, false>(p, acc, tile, i0, j, split, lane, wi);
 }
 
 // Instruction order of a slice of M MFMAs with R LDS reads and `v` (0 or more) DMA loads: spread between the MFMAs
@@ -250,10 +276,10 @@ template <int M, int R> __device__ __forceinline__ void slice_order(const int v)
 }
 
 // T: type of the operands and the residual, OT: of the output (and pre).  TI x TJ output tile, WI x WJ waves.
-// Both operands are staged by DMA into a ring of STAGES tiles of BKE reduction
-// elements.  At the top of step t one barrier makes tile t + 1 visible and frees tile t - 1, whose slot takes the DMA of tile
-// t + STAGES - 1; loads stay in flight over STAGES - 2 steps.  Fragments are read one 16-deep slice ahead of their MFMAs, across the
-// step border too, so that no MFMA waits for LDS behind a barrier.
+// Both operands are staged by DMA into a ring of STAGES tiles of BKE reduction elements.  A step has one barrier, before its last slice of 16:
+// there every wave has the fragments of the rest of tile t in registers, so that its slot takes the DMA of tile t + STAGES, and tile t + 1 is
+// waited for, whose first fragments are read beside the last slice's MFMAs.  So a load has STAGES - 1 steps to arrive, and no MFMA waits for LDS
+// behind a barrier.
 template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int WPE>
 __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP p) {
     constexpr int NT = 64 * WI * WJ;
@@ -262,7 +288,7 @@ __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP
     constexpr int STAGE = PI::BYTES + QI::BYTES, SL = BKE / 16;
     constexpr int NI = TI / WI / 32, NJ = TJ / WJ / 32;
     constexpr int LOADS = Dma<T, TI, PCM, BKE, NT>::NC + Dma<T, TJ, QCM, BKE, NT>::NC;   // DMA instructions of a wave per step
-    static_assert(STAGES >= 3 && SL >= 2 && SL % 2 == 0, "ring and slices");
+    static_assert(STAGES >= 2 && SL >= 2 && SL % 2 == 0, "ring and slices");
     extern __shared__ char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wi = wave / WJ, wj = wave - wi * WJ;
     int split, ti, tj;
@@ -296,33 +322,36 @@ __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP
         }
     };
     if (steps > 0) {
-        for (int t = 0; t < STAGES - 1 && t < steps; ++t) {
-            issue(smem + t * STAGE, t);
-        }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int t = 0; t < STAGES && t < steps; ++t) issue(smem + t * STAGE, t);
+        // tile 0 has landed
+        if (steps >= STAGES) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
         Frag<T> fp[2][NI], fq[2][NJ];
 #pragma unroll
         for (int a = 0; a < NI; ++a) PI::frag(fp[0][a], smem, pb + a * 32, 0, lane);
 #pragma unroll
         for (int c = 0; c < NJ; ++c) QI::frag(fq[0][c], smem + PI::BYTES, qb + c * 32, 0, lane);
-        int cur = 0, fill = (STAGES - 1) * STAGE;                            // byte offsets of the slots of tile t and of tile t + STAGES - 1
-        // FULL: another whole step to load; NONE: nothing left to load
+        char* cur = smem;
+        // FULL: another whole tile to load
         const auto step = [&](int t, auto full) __attribute__((always_inline)) {
             constexpr bool FULL = decltype(full)::value;
-            const int nxt = cur + STAGE == STAGES * STAGE ? 0 : cur + STAGE;
-            __builtin_amdgcn_sched_barrier(0);
-            // tile t + 1 has landed (younger loads may be under way), and every wave's reads of tile t - 1 are behind it
-            if (FULL || t + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 3) * LOADS) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            asm volatile("s_barrier" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (FULL) {
-                dp.template issue<true>(smem + fill, wave, BKE);
-                dq.template issue<true>(smem + fill + PI::BYTES, wave, BKE);
-            } else if (t + STAGES - 1 < steps) issue(smem + fill, t + STAGES - 1);
+            char* nxt = cur + STAGE == smem + STAGES * STAGE ? smem : cur + STAGE;
 #pragma unroll
             for (int k = 0; k < SL; ++k) {
-                const char* s = smem + (k + 1 < SL ? cur : nxt);
+                __builtin_amdgcn_sched_barrier(0);
+                if (k + 1 == SL) {
+                    // this wave's reads of tile t are done and its part of tile t + 1 has landed (younger loads may be under way)
+                    if (FULL || t + STAGES <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * LOADS) : "memory");
+                    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    asm volatile("s_barrier" ::: "memory");
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (FULL) {
+                        dp.template issue<true>(cur, wave, BKE);
+                        dq.template issue<true>(cur + PI::BYTES, wave, BKE);
+                    } else if (t + STAGES < steps) issue(cur, t + STAGES);
+                }
+                const char* s = k + 1 < SL ? cur : nxt;
                 const int k1 = k + 1 < SL ? (k + 1) * 16 : 0;
                 // (past the last tile this reads a slot that holds older values, and nothing uses them)
 #pragma unroll
@@ -333,15 +362,14 @@ __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP
                 for (int a = 0; a < NI; ++a)
 #pragma unroll
                     for (int c = 0; c < NJ; ++c) mma(acc[a][c], fq[k & 1][c], fp[k & 1][a]);
-                // order of the slice: an MFMA, then a share of the LDS reads and (first slice) of the DMA instructions, and so on
-                if constexpr (sizeof(T) == 2) slice_order<NI * NJ, (PCM ? 2 : 1) * NI + (QCM ? 2 : 1) * NJ>(k == 0 && FULL ? LOADS : 0);
-                __builtin_amdgcn_sched_barrier(0);
+                // order of the slice: an MFMA, then a share of the LDS reads and (last slice) of the DMA instructions, and so on
+                if constexpr (sizeof(T) == 2) slice_order<NI * NJ, (PCM ? 2 : 1) * NI + (QCM ? 2 : 1) * NJ>(k + 1 == SL && FULL ? LOADS : 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
             cur = nxt;
-            fill = fill + STAGE == STAGES * STAGE ? 0 : fill + STAGE;
         };
         int t = 0;
-        for (; t + STAGES < steps; ++t) step(t, std::true_type());
+        for (; t + STAGES + 1 < steps; ++t) step(t, std::true_type());
         for (; t < steps; ++t) step(t, std::false_type());
     }
     gemm_epilogue<T, OT, TI, TJ, WI, WJ>(p, acc, smem, i0, j0, split, lane, wi, wj, wave);
@@ -366,8 +394,9 @@ template <class T, class OT> __global__ __launch_bounds__(256) void gemm_join_ke
     }
     float bias[8];
     load_bias(p, bias, j);
-    const long long oo = i * p.ldo + j, op = i * p.ldpre + j, orr = i * p.ldr + j;
-    epilogue8<T, OT, false>(p, f, bias, p.J - j, oo, op, orr);
+    Raw8<T> res;
+    if (p.res) res = load_res<T, false>((const T*)p.res + i * p.ldr + j, p.J - j);
+    epilogue8<T, OT, false>(p, f, bias, res, p.J - j, i * p.ldo + j, i * p.ldpre + j);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------------
@@ -424,7 +453,9 @@ template <class T> __global__ __launch_bounds__(1024) void skinny_kernel(const G
 #pragma unroll
             for (int k = 0; k < 8; ++k) f[k] = red[0][i * 16 + c + k];
             load_bias(p, bias, j);
-            epilogue8<T, T, false>(p, f, bias, p.J - j, i * p.ldo + j, i * p.ldpre + j, i * p.ldr + j);
+            Raw8<T> res;
+            if (p.res) res = load_res<T, false>((const T*)p.res + i * p.ldr + j, p.J - j);
+            epilogue8<T, T, false>(p, f, bias, res, p.J - j, i * p.ldo + j, i * p.ldpre + j);
         }
     }
 }
@@ -524,29 +555,25 @@ __global__ __launch_bounds__(512) void col_join_kernel(const float* __restrict__
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 constexpr long long CUS = 256;
-// Tiles of the product kernels.  WIDE: long reductions of KC operands; TALL: two workgroups of 8 waves share a CU, so that the epilogue of
-// one runs beside the MFMAs of the other; SMALL and TINY where tiles are few.
+// Tiles of the product kernels: WIDE (bf16) where a CU has the one workgroup that its LDS takes, SMALL and TINY where tiles are few.
 // A reduction may be split over workgroups, whose fp32 sums a second launch joins.  Tile and splits are those with the least estimated
 // time, from what a step (128 bytes of reduction) was measured to take (us): alone on its CU, and as a share of a full one.
-//   bf16, KC operands     WIDE 1.73 / 1.73   TALL 1.3 / 0.97   SMALL 0.7 / 0.63   TINY 0.38 / 0.36
-//   bf16, a CM operand                       TALL 1.4 / 0.97   SMALL 1.2 / 0.73   TINY 0.9 / 0.26
-//   fp32                                                       SMALL 2.1 / 1.9    TINY 0.75 / 0.5
-// Both sides, bf16 (us): x w^T 16384 x 4096 x 4096 WIDE 452, TALL 513; 65536 x 1024 x 1024 with gelu and residual 197, 188; du w 65536 x 1024 x
-// 1024 156, 137; 2048 x 2048 x 2048 TALL 47, SMALL 43, TINY 35; x w^T of that size 40, 26, 48; 1024 x 1024 x 1024 16, 12, 8.
-enum Tile { WIDE = 0, TALL = 1, SMALL = 2, TINY = 3 };
-constexpr int TILE_I[4] = {256, 128, 128, 64}, TILE_J[4] = {256, 256, 128, 64}, TILE_PER_CU[4] = {1, 2, 2, 4};   // workgroups that share a CU
+//   bf16   WIDE 1.55 / 1.55   SMALL 0.66 / 0.63   TINY 0.33 / 0.2
+//   fp32                      SMALL 1.95 / 1.83   TINY 0.72 / 0.48
+// Both sides (us): x w^T, du w of 2048 x 2048 x 2048 bf16 SMALL 22, 22, TINY 28, 30; of 1024 x 1024 x 1024 11, 11 and 7.2, 7.3; of 2048 x 2048 x
+// 2048 fp32 128, 131 and 141, 146; of 1024 x 1024 x 1024 63, 65 and 23, 25.
+enum Tile { WIDE = 0, SMALL = 1, TINY = 2 };
+constexpr int TILE_I[3] = {256, 128, 64}, TILE_PER_CU[3] = {1, 2, 4};      // square; workgroups that share a CU
 struct GemmPlan { Tile tile; int splits; };
-GemmPlan plan_gemm(long long I, int J, long long Cn, int es, bool both_kc) {
-    constexpr double KC_ALONE[4] = {1.73, 1.3, 0.7, 0.38}, KC_SHARE[4] = {1.73, 0.97, 0.63, 0.36};
-    constexpr double CM_ALONE[4] = {1.73, 1.4, 1.2, 0.9}, CM_SHARE[4] = {1.73, 0.97, 0.73, 0.26};
+GemmPlan plan_gemm(long long I, int J, long long Cn, int es) {
+    constexpr double ALONE[2][3] = {{1.55, 0.66, 0.33}, {0, 1.95, 0.72}}, SHARE[2][3] = {{1.55, 0.63, 0.2}, {0, 1.83, 0.48}};
     const long long steps = std::max<long long>(1, cdivll(Cn * es, 128));
     GemmPlan best = {TINY, 1};
     double least = 1e30;
-    for (int t = es == 2 ? (both_kc ? WIDE : TALL) : SMALL; t <= TINY; ++t) {
-        const double alone = es == 4 ? (t == SMALL ? 2.1 : 0.75) : (both_kc ? KC_ALONE : CM_ALONE)[t];
-        const double share = es == 4 ? (t == SMALL ? 1.9 : 0.5) : (both_kc ? KC_SHARE : CM_SHARE)[t];
-        const long long tiles = cdivll(I, TILE_I[t]) * cdivll(J, TILE_J[t]);
-        const double epilogue = TILE_I[t] * TILE_J[t] * 6e-5;                      // 1 us for 128 x 128
+    for (int t = es == 2 ? WIDE : SMALL; t <= TINY; ++t) {
+        const double alone = ALONE[es == 4][t], share = SHARE[es == 4][t];
+        const long long tiles = cdivll(I, TILE_I[t]) * cdivll(J, TILE_I[t]);
+        const double epilogue = TILE_I[t] * TILE_I[t] * 1.2e-4;                     // 2 us for 128 x 128
         for (int s = 1; s <= 64; s += s < 4 ? 1 : s < 16 ? 4 : 16) {
             if (s > 1 && (steps < 2 * s || tiles * s > 4096)) break;
             const long long per_cu = cdivll(tiles * s, CUS), rounds = cdivll(per_cu, TILE_PER_CU[t]);
@@ -572,9 +599,9 @@ void gemm_launch(const GemmP& p, unsigned blocks, hipStream_t st) {
 template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, hipStream_t st) {
     if (p.I == 0 || p.J == 0) return FAVAE_OK;
     constexpr int es = sizeof(T);
-    const GemmPlan pl = plan_gemm(p.I, p.J, p.Cn, es, !PCM && !QCM);
+    const GemmPlan pl = plan_gemm(p.I, p.J, p.Cn, es);
     p.ti = (int)cdivll(p.I, TILE_I[pl.tile]);
-    p.tj = cdiv(p.J, TILE_J[pl.tile]);
+    p.tj = cdiv(p.J, TILE_I[pl.tile]);
     const long long unit = 128 / es;
     p.cchunk = cdivll(cdivll(p.Cn, unit), pl.splits) * unit;
     p.splits = (int)std::max<long long>(1, cdivll(p.Cn, std::max<long long>(1, p.cchunk)));
@@ -582,11 +609,14 @@ template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, hipStream
     FAVAE_CHECK_ARG(blocks <= 0x7fffffffLL, "favae_linear_act: too many rows for one launch");
     p.ldpart = (p.J + 7) & ~7;
     const unsigned g = (unsigned)blocks;
-    if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
-    else if constexpr (es == 4) gemm_launch<T, OT, 128, 128, 2, 2, 32, 3, PCM, QCM, 1>(p, g, st);
+    // steps of 128 bytes and two stages; one 64-byte steps and four where neither operand's steps leave half lines behind (x w^T 16384 x 4096 x
+    // 4096: 430 us, 452 with 64-byte steps; du w 423, 434; du^T x 409, 406; with 1024 rows and columns over 65536: 136, 131) and in SMALL, for
+    // loads that are longer under way (2048 x 2048 x 2048: 22.3 us, 26)
+    if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 128 / es, 2, PCM, QCM, 2>(p, g, st);
+    else if constexpr (es == 4) gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4>(p, g, st);
     else if (pl.tile == SMALL) gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
-    else if (pl.tile == TALL) gemm_launch<T, OT, 128, 256, 2, 4, 32, 3, PCM, QCM, 2>(p, g, st);
-    else if constexpr (!PCM && !QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, 2>(p, g, st);
+    else if constexpr (PCM && QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, 2>(p, g, st);
+    else gemm_launch<T, OT, 256, 256, 2, 4, 64, 2, PCM, QCM, 2>(p, g, st);
     FAVAE_LAUNCH_CHECK();
     if (p.splits > 1) {
         gemm_join_kernel<T, OT><<<(unsigned)cdivll(p.I * (p.ldpart / 8), 256), 256, 0, st>>>(p);
@@ -624,9 +654,9 @@ template <class T> int pack_operands(std::initializer_list<Operand*> ops, char*&
 
 size_t round256(size_t a) { return (a + 255) & ~(size_t)255; }
 size_t pack_bytes(long long rows, int cols, int es) { return round256((size_t)rows * padded(cols, es) * es); }
-size_t split_bytes(long long I, int J, long long Cn, int es, bool both_kc) {
+size_t split_bytes(long long I, int J, long long Cn, int es) {
     if (I == 0 || J == 0) return 0;
-    const int s = plan_gemm(I, J, Cn, es, both_kc).splits;
+    const int s = plan_gemm(I, J, Cn, es).splits;
     return s > 1 ? round256((size_t)s * I * ((J + 7) & ~7) * sizeof(float)) : 0;
 }
 constexpr int DU_RUNS = 256;
@@ -646,7 +676,7 @@ struct FwdScratch { size_t split, total; };
 FwdScratch fwd_scratch(long long M, int N, int K, int odd, int es) {
     if (M == 0 || N == 0 || M <= SKINNY_M) return {0, 0};
     FwdScratch s;
-    s.split = split_bytes(M, N, K, es, true);
+    s.split = split_bytes(M, N, K, es);
     s.total = s.split + (whole(K, es, odd) ? 0 : pack_bytes(M, K, es) + pack_bytes(N, K, es));
     return s;
 }
@@ -673,7 +703,7 @@ BwdScratch bwd_scratch(long long M, int N, int K, int act, bool x_ckpt, int odd,
     s.need_du = act != FAVAE_ACT_NONE || !whole(N, es, odd);      // du, or dy as DMA takes it (then in either of two places)
     s.du = s.need_du ? pack_bytes(M, N, es) : 0;
     s.colp = M > 0 ? round256((size_t)cdivll(M, du_rows(M)) * N * sizeof(float)) : 0;
-    s.split = std::max(split_bytes(M, K, N, es, false), split_bytes(N, K, M, es, false));    // the two products run one after the other
+    s.split = std::max(split_bytes(M, K, N, es), split_bytes(N, K, M, es));    // the two products run one after the other
     s.total = s.du + s.colp + s.split + (act == FAVAE_ACT_NONE ? s.du : 0) + (whole(K, es, odd) ? 0 : pack_bytes(N, K, es)) + (whole(K, es, odd) && !x_ckpt ? 0 : pack_bytes(M, K, es));
     return s;
 }
