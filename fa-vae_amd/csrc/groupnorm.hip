@@ -133,7 +133,7 @@ template <class T, int ITEMS, int GPV> __global__ __launch_bounds__(256) void gn
 template <class T, int ITEMS, int GPV, bool TAIL, bool STATS> __global__ __launch_bounds__(GTF, 4) void gn_fwd_kernel(const GnP p) {
     extern __shared__ float lds[];
     constexpr int VEC = VEC16<T>;
-    const long long lb = xcd_order(blockIdx.x, p.blocks);
+    const long long lb = xcd_order(STATS ? p.blocks - 1 - blockIdx.x : blockIdx.x, p.blocks);     // (from the back: GnChunk in groupnorm_bwd.h)
     const int cb = (int)(lb % p.ncb);
     const long long t_ = lb / p.ncb;
     const int chunk = (int)(t_ % p.nchunk);
@@ -415,9 +415,12 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
         p.shuf = p.NSUB == 1 && p.LV <= 32 && (p.LV & (p.LV - 1)) == 0 && p.P * p.LV == GT;
     };
     lanes();
-    // fewer channels side by side, down to 32 bytes (64 x 4096 x 64 and 512 x 4096 x 64 bf16: 23 and 186 us so, chunked 25 and 212), where a run of groups does not fit a workgroup's registers or where there would be
-    // fewer workgroups than CUs (the blocks that share a cache line run on one XCD)
-    while (p.pieces == 1 && p.CB % 2 == 0 && (p.CB / 2) % unit == 0 && p.CB / 2 * es >= 32 && !(ckpt && p.CB % 64) &&
+    // fewer channels side by side, down to 32 bytes, where a run of groups does not fit a workgroup's registers or where there would be fewer
+    // workgroups than CUs (the blocks that share a cache line run on one XCD).  Forward, 32 bytes so and chunked: 64, 512 x 4096 x 64 bf16 23, 185 us
+    // and 28, 199; 64 x 4096 x 64 fp32 36 and 44.  fp32 that passes the 256 MB cache is the other way round (512 x 4096 x 64 349 and 311, x 128 679
+    // and 587): down to 64 bytes there.
+    const int narrow = es == 4 && (long long)p.N * S * p.C * es >= 1LL << 28 ? 64 : 32;
+    while (p.pieces == 1 && p.CB % 2 == 0 && (p.CB / 2) % unit == 0 && p.CB / 2 * es >= narrow && !(ckpt && p.CB % 64) &&
            (cdiv(S, p.P) > ITEMS_MAX || (S * (long long)p.CB > 16 * vec * 64 && cdivll(p.N, p.NSUB) * p.ncb < 512))) {
         p.CB /= 2;
         p.ncb = cdiv(p.C, p.CB);

@@ -419,9 +419,11 @@ template <class T, bool TAIL, bool CK, class F> __device__ __forceinline__ void 
     }
 }
 
+// The first launch goes over the chunks from the back: what was written last, and for the launch that comes after it what was read last, is still in
+// the 256 MB cache (512 x 4096 x 64 bf16 in a loop: 110 and 139 us, 127 and 150 with both from the front).
 struct GnChunk { int cb, chunk; long long n; };
-__device__ __forceinline__ GnChunk gn_chunk(const GnP& p) {
-    const long long lb = xcd_order(blockIdx.x, p.blocks), t = lb / p.ncb;
+__device__ __forceinline__ GnChunk gn_chunk(const GnP& p, bool back) {
+    const long long lb = xcd_order(back ? p.blocks - 1 - blockIdx.x : blockIdx.x, p.blocks), t = lb / p.ncb;
     return {(int)(lb % p.ncb), (int)(t % p.nchunk), t / p.nchunk};
 }
 
@@ -432,7 +434,7 @@ template <class T, int GPV, bool TAIL, bool CK> __global__ __launch_bounds__(GTB
     const int cols = p.LV * VEC;
     float2* red = (float2*)lds;
     float2* tot = red + (p.shuf ? GTB / 64 : p.P) * cols;
-    const GnChunk k_ = gn_chunk(p);
+    const GnChunk k_ = gn_chunk(p, true);
     const GnBlock b = gn_block(p, k_.cb);
     const long long n = k_.n;
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
@@ -473,7 +475,7 @@ template <class T, int GPV, bool TAIL, bool CK> __global__ __launch_bounds__(GTB
 // Chunked form, third launch: dx.
 template <class T, int GPV, bool TAIL, bool CK> __global__ __launch_bounds__(GTB) void gn_bwd_apply_kernel(const GnP p) {
     constexpr int VEC = VEC16<T>;
-    const GnChunk k_ = gn_chunk(p);
+    const GnChunk k_ = gn_chunk(p, false);
     const GnBlock b = gn_block(p, k_.cb);
     const long long n = k_.n;
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
