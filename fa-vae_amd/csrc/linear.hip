@@ -151,7 +151,6 @@ __device__ __forceinline__ void load_bias(const GemmP& p, float (&b)[8], int j) 
 // neighbouring 16-byte slots, so the swizzle is applied to the addresses: the lane that fills slot s of a row loads the chunk that
 // belongs there.  The buffer descriptor's range check turns what lies outside the operand into zeros: lanes whose output row (or
 // column) does not exist, or whose chunk lies past the end of the reduction, carry an offset with bit 31 set.
-typedef unsigned v4u_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
 template <class T, int ROWS, bool CM, int BKE, int NT> struct Dma {
     typedef TileImg<T, ROWS, CM, BKE> Img;

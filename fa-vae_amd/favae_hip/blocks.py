@@ -160,6 +160,16 @@ def _apart(out, name, ins, may_be=None):
             raise ValueError("%s overlaps an input" % name)
 
 
+def _distinct(t, name):
+    """Every element of t, which a call writes, has a place of its own."""
+    span = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st < span:
+            raise ValueError("%s overlaps itself" % name)
+        span = st * n                                        # (at least: strides that interleave otherwise are refused too)
+    return t
+
+
 def _out(out, name, like, shape, dtype, ins, may_be=None):
     if out is None:
         return like.new_empty(shape, dtype=dtype)
@@ -167,7 +177,7 @@ def _out(out, name, like, shape, dtype, ins, may_be=None):
     if out.dtype != dtype or out.shape != torch.Size(shape) or out.device != dev:
         raise ValueError("%s: %s %s on %s" % (name, dtype, list(shape), dev))
     _apart(out, name, ins, may_be)
-    return out
+    return out if out.is_contiguous() or out.numel() == 0 else _distinct(out, name)
 
 
 _stream_of, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice    # torch.cuda.current_stream builds an object: 2 us

@@ -390,6 +390,28 @@ def test_linear_act_large_tiles(M, N, K, dtype):
     lin_bwd_check(b, M, N, K, dtype, "none", False, gen(M, N, K, 3))
 
 
+# every tile, alone and split, with rows, columns and reductions that end inside one: 128 wide; 256 wide in y and dw, dx split; 256 wide over one
+# step; dw split over 256 wide tiles; 128 wide and split in fp32
+@pytest.mark.parametrize("M,N,K,dtype", [(2040, 2056, 2056, BF16), (1030, 8200, 2056, BF16), (5000, 2056, 8, BF16), (60000, 1016, 1024, BF16), (2056, 2056, 2056, F32)])
+def test_linear_act_every_tile(M, N, K, dtype):
+    b = B()
+    g = gen(M, N, K, 4)
+    x, w = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype, scale=K ** -0.5)
+    bias, res = rnd(g, N, scale=0.3), rnd(g, M, N, dtype=dtype)
+    u = x.double() @ w.double().t() + bias.double()
+    u_err = lin_bound(x, w, bias)
+    v = act64(u, "silu")[0]
+    err = SLOPE * u_err + (u.abs() + 8) * 4 * U * v.abs()
+    v = v + res.double()
+    close(b.linear_act(x, w, bias, act="silu", residual=res), v, err + U * v.abs())
+    r = res.clone()
+    assert b.linear_act(x, w, bias, act="silu", residual=r, out=r) is r          # in place
+    close(r, v, err + U * v.abs())
+    del u, u_err, v, err, r
+    lin_bwd_check(b, M, N, K, dtype, "gelu_tanh", False, gen(M, N, K, 5), None)
+    lin_bwd_check(b, M, N, K, dtype, "none", False, gen(M, N, K, 6), F32)
+
+
 def test_linear_act_bwd_long_reduction():
     lin_bwd_check(B(), 9001, 72, 136, BF16, "silu", True, gen(5), F32)
     lin_bwd_check(B(), 20000, 64, 64, F32, "none", False, gen(6))
@@ -616,6 +638,14 @@ def test_refusals_on_the_gpu():
         b.linear_act(x, w, residual=big[:4], out=big[1:])
     with pytest.raises(ValueError, match="overlaps"):
         b.group_norm_act(x, 2, torch.ones(8, device=DEV), torch.zeros(8, device=DEV), ckpt=True, out=x)
+    ones, zeros, maps = torch.ones(8, device=DEV), torch.zeros(8, device=DEV), torch.randn(3, 5, 8, device=DEV)
+    with pytest.raises(ValueError, match="itself"):                               # one sample's memory for all of them
+        b.group_norm_act(maps, 2, ones, zeros, out=torch.zeros(1, 5, 8, device=DEV).expand(3, 5, 8))
+    with pytest.raises(ValueError, match="itself"):
+        b.group_norm_act(maps, 2, ones, zeros, out=torch.zeros(64, device=DEV).as_strided((3, 5, 8), (8, 8, 1)))
+    between = torch.zeros(5, 3, 8, device=DEV).transpose(0, 1)                    # samples between each other's positions: taken
+    y = b.group_norm_act(maps, 2, ones, zeros, out=between)[0]
+    assert y is between and torch.equal(y, b.group_norm_act(maps, 2, ones, zeros)[0])
     with pytest.raises(ValueError, match="device"):
         b.linear_act(x, w, bias=torch.randn(6))
     with pytest.raises(ValueError, match="contiguous"):
