@@ -122,7 +122,7 @@ def _maps(t, name):
 
 
 def _vec(t, n, name, dev):
-    if t.dtype != F32 or t.dim() != 1 or t.shape[0] != n:
+    if t.dtype != F32 or t.shape != (n,):
         raise ValueError("%s: float32 [%d]" % (name, n))
     if t.device != dev or not t.is_contiguous():
         raise ValueError("%s: contiguous and on the device of the call" % name)
@@ -263,9 +263,12 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError("eps: not negative")
-    xn, xs = _maps(x, "x")
-    y = _out(out, "out", x, x.shape, x.dtype, (x, gamma, beta), None if ckpt else x)
-    yn, ys = _maps(y, "out")
+    xn, xs = (s * c, c) if x.is_contiguous() else _maps(x, "x")
+    if out is None:
+        y, yn, ys = x.new_empty(x.shape), s * c, c
+    else:
+        y = _out(out, "out", x, x.shape, x.dtype, (x, gamma, beta), None if ckpt else x)
+        yn, ys = _maps(y, "out")
     mean, rstd = x.new_empty((2, n, groups), dtype=F32).unbind()
     ck = _new_ckpt(x) if ckpt else None
     if ckpt and xn != s * xs and n > 1 and s > 1:
@@ -292,10 +295,13 @@ def group_norm_act_bwd(dy, x, groups, gamma, beta, mean, rstd, act="none", out=N
     for t, name in ((mean, "mean"), (rstd, "rstd")):
         if t.dtype != F32 or t.shape != (n, groups) or not t.is_contiguous():
             raise ValueError("%s: contiguous float32 [%d, %d]" % (name, n, groups))
-    dn, ds = _maps(dy, "dy")
-    xn, xs = (0, 0) if ck else _maps(x, "x")
-    dx = _out(out, "out", dy, dy.shape, dy.dtype, (dy, x.q, x.e, gamma, beta, mean, rstd) if ck else (dy, x, gamma, beta, mean, rstd), dy)
-    dxn, dxs = _maps(dx, "out")
+    dn, ds = (s * c, c) if dy.is_contiguous() else _maps(dy, "dy")
+    xn, xs = (0, 0) if ck else (s * c, c) if x.is_contiguous() else _maps(x, "x")
+    if out is None:
+        dx, dxn, dxs = dy.new_empty(dy.shape), s * c, c
+    else:
+        dx = _out(out, "out", dy, dy.shape, dy.dtype, (dy, x.q, x.e, gamma, beta, mean, rstd) if ck else (dy, x, gamma, beta, mean, rstd), dy)
+        dxn, dxs = _maps(dx, "out")
     dgamma, dbeta = dy.new_empty((2, c), dtype=F32).unbind()
     nbytes = _raw.favae_gn_act_scratch(n, s, c, groups, 1, code)
     ws = _scratch(nbytes, dy)
@@ -330,15 +336,20 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("residual: %s %s" % (x.dtype, list(shape)))
     bp = None if bias is None else _vec(bias, n, "bias", dev)
-    y = _out(out, "out", x, shape, x.dtype, (x, w, bias, residual), residual)
+    if out is None:
+        y, ldy = x.new_empty(shape), n
+    else:
+        y = _out(out, "out", x, shape, x.dtype, (x, w, bias, residual), residual)
+        ldy = _rows(y, "out")
     pre = x.new_empty(shape) if save_pre else None
     if m and n:
-        ldx, ldw, xp, wp = _rows(x, "x"), _rows(w, "w"), x.data_ptr(), w.data_ptr()
+        ldx = k if x.is_contiguous() else _rows(x, "x")
+        ldw = k if w.is_contiguous() else _rows(w, "w")
+        xp, wp = x.data_ptr(), w.data_ptr()
         nbytes = _raw.favae_linear_act_fwd_scratch(m, n, k, _odd(x, ldx, xp) or _odd(w, ldw, wp), code)
         ws = _scratch(nbytes, x)
         _call(dev, _raw.favae_linear_act_fwd, xp, ldx, wp, ldw, bp, _ptr(residual),
-              0 if residual is None else _rows(residual, "residual"), _ptr(pre), n, y.data_ptr(), _rows(y, "out"), m, n, k, a, _ptr(ws), nbytes,
-              code)
+              0 if residual is None else _rows(residual, "residual"), _ptr(pre), n, y.data_ptr(), ldy, m, n, k, a, _ptr(ws), nbytes, code)
     return (y, pre) if save_pre else y
 
 
