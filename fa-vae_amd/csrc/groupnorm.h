@@ -54,9 +54,20 @@ __device__ __forceinline__ GnBlock gn_block(const GnP& p, int cb) {
 }
 // consecutive logical blocks (the channel blocks of one sample read the same cache lines) go to one XCD: the launch deals blocks to
 // the 8 XCDs in turn
-__device__ __forceinline__ long long xcd_order(long long b, long long n) {
-    const long long per = n / 8;
+__device__ __forceinline__ unsigned xcd_order(unsigned b, unsigned n) {
+    const unsigned per = n / 8;
     return b < per * 8 ? (b & 7) * per + (b >> 3) : b;
+}
+// groups of elements c, c + STEP, ... (counted from a group's start), at most `last`; STEP <= Cg.  Divisions are 32 bits wide and few: a 64-bit
+// one is 100 to 150 instructions.
+template <int STEP, int N> __device__ __forceinline__ void group_of(int (&g)[N], int c, int Cg, int last) {
+    int q = c / Cg, r = c - q * Cg;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        g[j] = min(q, last);
+        r += STEP;
+        if (r >= Cg) { r -= Cg; ++q; }
+    }
 }
 
 // barrier for data in LDS: vector memory operations stay under way (__syncthreads waits for them)
@@ -95,13 +106,30 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
         for (int j = 0; j < NV; ++j) if (own(j)) red[r * cols + col + j] = v[j];
     }
     lds_barrier();
+    const int pairs = p.NSUB * ng;
+    if (!p.shuf) {
+        // many rows: the columns first (with a division for each value, and partial vectors stored element by element, 512 x 195 x 210 bf16 took 45 us, now 41)
+        const int all = p.NSUB * cols, L = pair_lanes<GTF>(all, rows), l = (int)threadIdx.x & (L - 1);
+        float* tot = grp + pairs;
+        for (int k = (int)threadIdx.x / L; k < all; k += GTF / L) {
+            const int sub = k / cols;
+            const float* a = red + (sub * rows + l) * cols + k - sub * cols;
+            float s = 0.f;
+            for (int i = l; i < rows; i += L) { s += *a; a += L * cols; }
+            for (int o = L >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+            if (l == 0) tot[k] = s;
+        }
+        lds_barrier();
+        red = tot;
+        rows = 1;
+    }
     // L lanes take a pair: as many as there are threads for every pair at once, at most its values
-    const int pairs = p.NSUB * ng, per = rows * cpg, L = pair_lanes<GTF>(pairs, per), l = (int)threadIdx.x & (L - 1);
+    const int per = rows * cpg, L = pair_lanes<GTF>(pairs, per), l = (int)threadIdx.x & (L - 1);
     for (int k = (int)threadIdx.x / L; k < pairs; k += GTF / L) {
         const int sub = k / ng, g = k - sub * ng;
         float s = 0.f;
         for (int i = l; i < per; i += L) {
-            const int row = i / cpg, c = i - row * cpg;
+            const int row = rows == 1 ? 0 : i / cpg, c = i - row * cpg;
             s += red[(sub * rows + row) * cols + g * cpg + c];
         }
         for (int o = L >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -130,6 +158,9 @@ template <class T, bool TAIL> struct GnLane {
         }
     }
     __device__ __forceinline__ bool own(int j) const { return !TAIL || (j >= j_lo && j < j_hi); }
+    // the whole vector, with the elements that the lane before writes too, to the same values: where every thread of the block has read
+    // what it needs (`out` may be the input)
+    __device__ __forceinline__ void store_whole(void* base, long long off, const uint4& r) const { store16((T*)base + off, r, TAIL ? j_hi : VEC); }
     __device__ __forceinline__ void store(void* base, long long off, const uint4& r) const {
         T* a = (T*)base + off;
         if (!TAIL || j_hi - j_lo == VEC) __builtin_memcpy(a, &r, 16);

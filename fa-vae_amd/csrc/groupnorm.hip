@@ -41,9 +41,9 @@ template <int VEC> __device__ __forceinline__ void ck_store(const GnP& p, float 
 template <class T, int ITEMS, int GPV> __global__ __launch_bounds__(256) void gn_wave_fwd_kernel(const GnP p) {
     constexpr int VEC = VEC16<T>;
     const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
-    const long long lb = xcd_order(blockIdx.x, p.blocks);
-    const int cb = (int)(lb % p.ncb);
-    const long long row = lb / p.ncb, rows = p.blocks / p.ncb;
+    const unsigned lb = xcd_order(blockIdx.x, (unsigned)p.blocks), row_ = lb / (unsigned)p.ncb;
+    const int cb = (int)(lb - row_ * p.ncb);
+    const long long row = row_, rows = (unsigned)p.blocks / (unsigned)p.ncb;
     const int lv = lane & (p.LV - 1), pos = lane / p.LV, gl = GPV == 1 ? p.Cg / VEC : 1;
     const bool col_ok = cb * p.CB + lv * VEC < p.C;
     const GnLane<T, false> ln(min(cb * p.CB + lv * VEC, p.C - VEC), p.C, 0);
@@ -133,11 +133,10 @@ template <class T, int ITEMS, int GPV> __global__ __launch_bounds__(256) void gn
 template <class T, int ITEMS, int GPV, bool TAIL, bool STATS> __global__ __launch_bounds__(GTF, 4) void gn_fwd_kernel(const GnP p) {
     extern __shared__ float lds[];
     constexpr int VEC = VEC16<T>;
-    const long long lb = xcd_order(STATS ? p.blocks - 1 - blockIdx.x : blockIdx.x, p.blocks);     // (from the back: GnChunk in groupnorm_bwd.h)
-    const int cb = (int)(lb % p.ncb);
-    const long long t_ = lb / p.ncb;
-    const int chunk = (int)(t_ % p.nchunk);
-    const long long nb0 = t_ / p.nchunk;
+    const unsigned lb = xcd_order(STATS ? (unsigned)p.blocks - 1u - blockIdx.x : blockIdx.x, (unsigned)p.blocks);     // (from the back: GnChunk in groupnorm_bwd.h)
+    const unsigned t_ = lb / (unsigned)p.ncb, nb_ = STATS ? t_ / (unsigned)p.nchunk : t_;
+    const int cb = (int)(lb - t_ * p.ncb), chunk = STATS ? (int)(t_ - nb_ * p.nchunk) : 0;
+    const long long nb0 = nb_;
     const GnBlock b = gn_block(p, cb);
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
     const int sub = r / p.P, pos = r - sub * p.P;
@@ -151,11 +150,10 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool STATS> __global__ __launc
     float* grp = lds + GTF * GPV;
 
     GnData<T, TAIL> d[ITEMS];
+    const long long x0 = n * p.xn + (s_lo + pos) * p.xs + c0, y0 = n * p.yn + (s_lo + pos) * p.ys + c0;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const int s = s_lo + pos + i * p.P;
-        if (active && s < s_hi) d[i].load(p.x, n * p.xn + s * p.xs + c0, ln);
-    }
+    for (int i = 0; i < ITEMS; ++i)
+        if (active && s_lo + pos + i * p.P < s_hi) d[i].load(p.x, x0 + i * (p.P * p.xs), ln);
     float v[GPV];
 #pragma unroll
     for (int j = 0; j < GPV; ++j) v[j] = 0.f;
@@ -174,9 +172,10 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool STATS> __global__ __launc
     const float inv = s_hi > s_lo ? 1.f / ((float)(s_hi - s_lo) * (float)b.cw) : 0.f;
     GnStat<VEC, GPV> st;
     int gl[GPV];
+    group_of<1>(gl, active && p.pieces == 1 ? c0 - b.c_lo : 0, p.Cg, b.ng - 1);       // (an element past a narrow run: any group)
 #pragma unroll
     for (int j = 0; j < GPV; ++j) {
-        gl[j] = active ? sub * b.ng + (p.pieces == 1 ? min((c0 - b.c_lo + j) / p.Cg, b.ng - 1) : 0) : 0;     // (an element past a narrow run: any group)
+        gl[j] = active ? sub * b.ng + gl[j] : 0;
         st.m[j] = grp[gl[j]] * inv;
         v[j] = 0.f;
     }
@@ -256,7 +255,7 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool STATS> __global__ __launc
                     act_apply<T, decltype(act)::value>(f);
                     uint4 o;
                     vec_put(o, f);
-                    ln.store(p.y, n * p.yn + s * p.ys + c0, o);
+                    ln.store_whole(p.y, y0 + i * (p.P * p.ys), o);
                 }
             }
         });
@@ -267,11 +266,9 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool STATS> __global__ __launc
 template <class T, int GPV, bool TAIL> __global__ __launch_bounds__(GTF) void gn_apply_kernel(const GnP p) {
     extern __shared__ float lds[];
     constexpr int VEC = VEC16<T>;
-    const long long lb = xcd_order(blockIdx.x, p.blocks);
-    const int cb = (int)(lb % p.ncb);
-    const long long t_ = lb / p.ncb;
-    const int chunk = (int)(t_ % p.nchunk);
-    const long long n = t_ / p.nchunk;
+    const unsigned lb = xcd_order(blockIdx.x, (unsigned)p.blocks), t_ = lb / (unsigned)p.ncb, n_ = t_ / (unsigned)p.nchunk;
+    const int cb = (int)(lb - t_ * p.ncb), chunk = (int)(t_ - n_ * p.nchunk);
+    const long long n = n_;
     const GnBlock b = gn_block(p, cb);
     const int parts = p.nchunk * p.pieces;
     float2* stat = (float2*)lds;                 // [ng] (mean, rstd)
@@ -301,9 +298,11 @@ template <class T, int GPV, bool TAIL> __global__ __launch_bounds__(GTF) void gn
     const GnLane<T, TAIL> ln(b.c_lo, b.c_hi, lv);
     const int c0 = ln.c0;
     GnStat<VEC, GPV> st;
+    int gi[GPV];
+    group_of<1>(gi, p.pieces == 1 ? c0 - b.c_lo : 0, p.Cg, b.ng - 1);
 #pragma unroll
     for (int j = 0; j < GPV; ++j) {
-        const float2 t = stat[p.pieces == 1 ? min((c0 - b.c_lo + j) / p.Cg, b.ng - 1) : 0];
+        const float2 t = stat[gi[j]];
         st.m[j] = t.x; st.r[j] = t.y;
     }
     float ga[VEC], be[VEC];
@@ -465,7 +464,7 @@ template <class T> int gn_fwd(const GnP& p, const GnPlan& pl, hipStream_t st) {
         constexpr int GPV = decltype(gpv)::value;
         constexpr bool TAIL = decltype(tail)::value;
         const int gpb = cdiv(p.CB, std::min(p.Cg, p.CB));
-        const size_t lds = sizeof(float) * ((size_t)GTF * GPV + (size_t)p.NSUB * gpb);
+        const size_t lds = sizeof(float) * ((size_t)GTF * GPV + (size_t)p.NSUB * (gpb + (p.shuf ? 0 : p.LV * GPV)));
         if (pl.form == GN_HELD)
             return pl.items <= 4 ? gn_launch(gn_fwd_kernel<T, 4, GPV, TAIL, false>, p, GTF, lds, st)
                                  : gn_launch(gn_fwd_kernel<T, ITEMS_MAX, GPV, TAIL, false>, p, GTF, lds, st);

@@ -19,9 +19,9 @@ template <class T, int ITEMS, int GPV, bool CK> __global__ __launch_bounds__(256
     constexpr int VEC = VEC16<T>;
     __shared__ float2 red[4][64][VEC + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const long long lb = xcd_order(blockIdx.x, p.blocks);
-    const int cb = (int)(lb % p.ncb);
-    const long long row = lb / p.ncb, rows = p.blocks / p.ncb;
+    const unsigned lb = xcd_order(blockIdx.x, (unsigned)p.blocks), row_ = lb / (unsigned)p.ncb;
+    const int cb = (int)(lb - row_ * p.ncb);
+    const long long row = row_, rows = (unsigned)p.blocks / (unsigned)p.ncb;
     const int lv = lane & (p.LV - 1), pos = lane / p.LV, gl = GPV == 1 ? p.Cg / VEC : 1;
     const bool col_ok = cb * p.CB + lv * VEC < p.C;
     const GnLane<T, false> ln(min(cb * p.CB + lv * VEC, p.C - VEC), p.C, 0);
@@ -123,9 +123,9 @@ template <class T, int GPV, bool CK, int ACT> __global__ __launch_bounds__(GTP) 
     float2* acc = grp + cols;                                         // [cols]
     float* gam = (float*)(acc + cols);                                // [cols]
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const long long lb = xcd_order(blockIdx.x, p.blocks);
-    const int cb = (int)(lb % p.ncb);
-    const long long row = lb / p.ncb, stride = p.blocks / p.ncb;
+    const unsigned lb = xcd_order(blockIdx.x, (unsigned)p.blocks), row_ = lb / (unsigned)p.ncb;
+    const int cb = (int)(lb - row_ * p.ncb);
+    const long long row = row_, stride = (unsigned)p.blocks / (unsigned)p.ncb;
     const GnBlock b = gn_block(p, cb);
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
     const bool has = b.c_lo + lv * VEC < b.c_hi;
@@ -135,8 +135,7 @@ template <class T, int GPV, bool CK, int ACT> __global__ __launch_bounds__(GTP) 
     const unsigned xof = (unsigned)((r * p.xs + c0) * ES), xstep = (unsigned)(p.P * p.xs * ES);
     const unsigned yof = (unsigned)((r * p.ys + c0) * ES), ystep = (unsigned)(p.P * p.ys * ES);
     int gi[GPV];
-#pragma unroll
-    for (int j = 0; j < GPV; ++j) gi[j] = (c0 - b.c_lo + j * (VEC / GPV)) / p.Cg;
+    group_of<VEC / GPV>(gi, c0 - b.c_lo, p.Cg, b.ng - 1);
     float ga[VEC], be[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) { ga[j] = p.gamma[c0 + j]; be[j] = p.beta[c0 + j]; }
@@ -298,9 +297,9 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ _
     float2* tot = red + (p.shuf ? (GTB / 64) * cols : p.P * p.NSUB * cols);
     float2* grp = tot + p.NSUB * cols;           // [NSUB][ng]
     float2* acc = grp + p.NSUB * cols;           // [cols]
-    const long long lb = xcd_order(blockIdx.x, p.blocks);
-    const int cb = (int)(lb % p.ncb);
-    const long long first = lb / p.ncb, stride = p.blocks / p.ncb;
+    const unsigned lb = xcd_order(blockIdx.x, (unsigned)p.blocks), row_ = lb / (unsigned)p.ncb;
+    const int cb = (int)(lb - row_ * p.ncb);
+    const long long first = row_, stride = (unsigned)p.blocks / (unsigned)p.ncb;
     const GnBlock b = gn_block(p, cb);
     const int r = (int)threadIdx.x / p.LV, lv = (int)threadIdx.x - r * p.LV;
     const int sub = r / p.P;
@@ -311,8 +310,7 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ _
     const int c0 = ln.c0;
     const auto own = [&](int j) { return has && ln.own(j); };
     int gi[GPV];
-#pragma unroll
-    for (int j = 0; j < GPV; ++j) gi[j] = min((c0 - b.c_lo + j) / p.Cg, b.ng - 1);
+    group_of<1>(gi, c0 - b.c_lo, p.Cg, b.ng - 1);
     for (int k = threadIdx.x; k < cols; k += GTB) acc[k] = make_float2(0.f, 0.f);
     const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
     for (long long nb0 = first; nb0 * p.NSUB < p.N; nb0 += stride) {
@@ -390,7 +388,7 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ _
             for (int j = 0; j < VEC; ++j) g[j] = fmaf(st.mean(j) - x[j], cc.rstd(j), fmaf(a[j], dz[i][j], -cc.mean(j)));
             uint4 o;
             vec_put(o, g);
-            if (active && s <= last) ln.store(p.y, n * p.yn + s * p.ys + c0, o);
+            if (active && s <= last) ln.store_whole(p.y, n * p.yn + s * p.ys + c0, o);
             __builtin_amdgcn_sched_barrier(0);
         }
         lds_barrier();                           // red, tot and grp are free again
@@ -423,8 +421,8 @@ template <class T, bool TAIL, bool CK, class F> __device__ __forceinline__ void 
 // the 256 MB cache (512 x 4096 x 64 bf16 in a loop: 110 and 139 us, 127 and 150 with both from the front).
 struct GnChunk { int cb, chunk; long long n; };
 __device__ __forceinline__ GnChunk gn_chunk(const GnP& p, bool back) {
-    const long long lb = xcd_order(back ? p.blocks - 1 - blockIdx.x : blockIdx.x, p.blocks), t = lb / p.ncb;
-    return {(int)(lb % p.ncb), (int)(t % p.nchunk), t / p.nchunk};
+    const unsigned lb = xcd_order(back ? (unsigned)p.blocks - 1u - blockIdx.x : blockIdx.x, (unsigned)p.blocks), t = lb / (unsigned)p.ncb, n = t / (unsigned)p.nchunk;
+    return {(int)(lb - t * p.ncb), (int)(t - n * p.nchunk), (long long)n};
 }
 
 // Chunked form, first launch: column sums of a chunk of positions in part[(n nchunk + chunk) C + c].
@@ -448,9 +446,11 @@ template <class T, int GPV, bool TAIL, bool CK> __global__ __launch_bounds__(GTB
     if (r < p.P && has) {
         GnStat<VEC, GPV> st;
         float a[VEC], be[VEC];
+        int gi[GPV];
+        group_of<1>(gi, p.pieces == 1 ? c0 - b.c_lo : 0, p.Cg, b.ng - 1);
 #pragma unroll
         for (int j = 0; j < GPV; ++j) {
-            const int g = b.g_lo + (p.pieces == 1 ? min((c0 - b.c_lo + j) / p.Cg, b.ng - 1) : 0);
+            const int g = b.g_lo + gi[j];
             st.m[j] = p.mean[n * p.G + g];
             st.r[j] = p.rstd[n * p.G + g];
         }
@@ -483,9 +483,11 @@ template <class T, int GPV, bool TAIL, bool CK> __global__ __launch_bounds__(GTB
     const GnLane<T, TAIL> ln(b.c_lo, b.c_hi, lv);
     const int c0 = ln.c0;
     GnStat<VEC, GPV> st, cc;
+    int gi[GPV];
+    group_of<1>(gi, p.pieces == 1 ? c0 - b.c_lo : 0, p.Cg, b.ng - 1);
 #pragma unroll
     for (int j = 0; j < GPV; ++j) {
-        const long long g = n * p.G + b.g_lo + (p.pieces == 1 ? min((c0 - b.c_lo + j) / p.Cg, b.ng - 1) : 0);
+        const long long g = n * p.G + b.g_lo + gi[j];
         st.m[j] = p.mean[g];
         st.r[j] = p.rstd[g];
         const float2 t = p.s12[g];
@@ -517,14 +519,17 @@ __global__ __launch_bounds__(1024) void gn_join_kernel(const GnP p, long long ro
     if ((int)blockIdx.x < gblocks) {
         const long long g = (long long)blockIdx.x * 16 + wave;
         if (g >= (long long)p.N * p.G) return;
-        const long long n = g / p.G;
-        const int c0 = (int)(g - n * p.G) * p.Cg;
+        const long long n = (unsigned)g / (unsigned)p.G;
+        const int c0 = (int)(g - n * p.G) * p.Cg, dch = 64 / p.Cg, dc = 64 - dch * p.Cg;
+        int ch = lane / p.Cg, c1 = lane - ch * p.Cg;
         float2 s = make_float2(0.f, 0.f);
-        for (long long i = lane; i < (long long)p.nchunk * p.Cg; i += 64) {
-            const int ch = (int)(i / p.Cg), c = c0 + (int)(i - (long long)ch * p.Cg);
+        while (ch < p.nchunk) {
+            const int c = c0 + c1;
             const float2 t = p.part[(n * p.nchunk + ch) * p.C + c];
             const float w = p.gamma[c];
             s.x = fmaf(w, t.x, s.x); s.y = fmaf(w, t.y, s.y);
+            ch += dch; c1 += dc;
+            if (c1 >= p.Cg) { c1 -= p.Cg; ++ch; }
         }
         s.x = wave_total(s.x); s.y = wave_total(s.y);
         const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
@@ -592,6 +597,7 @@ template <class T, bool CK> int gn_bwd(const GnP& p, const GnPlan& pl, float* dg
             constexpr int A = decltype(act)::value;
             if (pl.items <= 4) rc = gn_launch(gn_bwd_kernel<T, 4, GPV, TAIL, CK, A>, p, GTB, lds, st);
             else if (pl.items <= 8) rc = gn_launch(gn_bwd_kernel<T, 8, GPV, TAIL, CK, A>, p, GTB, lds, st);
+            else if (pl.items <= 12) rc = gn_launch(gn_bwd_kernel<T, 12, GPV, TAIL, CK, A>, p, GTB, lds, st);
             else rc = gn_launch(gn_bwd_kernel<T, ITEMS_MAX, GPV, TAIL, CK, A>, p, GTB, lds, st);
         });
         return rc != FAVAE_OK ? rc : join(0);
