@@ -371,7 +371,8 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
         }
     }
     const bool gs = p.Cg % vec == 0;
-    long long unit = std::lcm((long long)p.Cg, (long long)vec);                          // whole groups that start on the vector grid
+    // whole groups that start on the vector grid; where rows do not end on it anyway, any whole groups
+    long long unit = p.C % vec ? p.Cg : std::lcm((long long)p.Cg, (long long)vec);
     pl.gpv = gs ? 1 : vec;
     // piped form (backward): 32 lanes or fewer side by side (a power of two), at most 8 vectors a thread
     if (backward && even && p.C % vec == 0 && unit <= 32 * vec) {
@@ -406,6 +407,15 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
         p.ncb = cdiv(p.C, p.CB);
         pl.tail = p.C % vec != 0 || unit % vec != 0;
     }
+    // off the grid: blocks of nearly equal numbers of groups, the last one a whole vector wide too
+    const auto even_out = [&]() {
+        if (!pl.tail || p.pieces > 1) return;
+        int per = cdiv(p.G, cdiv(p.G, p.CB / p.Cg));
+        while (per < p.G && (p.G - (cdiv(p.G, per) - 1) * per) * p.Cg < vec) ++per;
+        p.CB = per * p.Cg;
+        p.ncb = cdiv(p.G, per);
+    };
+    even_out();
     const auto lanes = [&]() {
         p.LV = cdiv(p.CB, vec);
         p.P = GT / p.LV;
@@ -419,11 +429,16 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
     // and 28, 199; 64 x 4096 x 64 fp32 36 and 44.  fp32 that passes the 256 MB cache is the other way round (512 x 4096 x 64 349 and 311, x 128 679
     // and 587): down to 64 bytes there.
     const int narrow = es == 4 && (long long)p.N * S * p.C * es >= 1LL << 28 ? 64 : 32;
-    while (p.pieces == 1 && p.CB % 2 == 0 && (p.CB / 2) % unit == 0 && p.CB / 2 * es >= narrow && !(ckpt && p.CB % 64) &&
+    const auto halves = [&]() { return pl.tail ? p.CB > p.Cg && cdiv(p.CB / p.Cg, 2) * p.Cg * es >= narrow
+                                               : p.CB % 2 == 0 && (p.CB / 2) % unit == 0 && p.CB / 2 * es >= narrow && !(ckpt && p.CB % 64); };
+    while (p.pieces == 1 && halves() &&
            (cdiv(S, p.P) > ITEMS_MAX || (S * (long long)p.CB > 16 * vec * 64 && cdivll(p.N, p.NSUB) * p.ncb < 512))) {
-        p.CB /= 2;
+        const int before = p.CB;
+        p.CB = pl.tail ? cdiv(p.CB / p.Cg, 2) * p.Cg : p.CB / 2;
         p.ncb = cdiv(p.C, p.CB);
+        even_out();
         lanes();
+        if (p.CB == before) break;
     }
     const long long held_blocks = cdivll(p.N, p.NSUB) * p.ncb;
     pl.threads = GT;
@@ -437,7 +452,7 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
     } else {
         pl.form = GN_CHUNKED;
         while (p.pieces == 1 && p.CB * es < 128 && p.CB * 2 <= std::min(cap, p.C)) p.CB *= 2;   // whole cache lines again
-        if (p.pieces == 1) { p.ncb = cdiv(p.C, p.CB); p.LV = cdiv(p.CB, vec); }
+        if (p.pieces == 1) { p.ncb = cdiv(p.C, p.CB); even_out(); p.LV = cdiv(p.CB, vec); }
         p.NSUB = 1;
         p.P = std::max(1, GT / p.LV);
         p.shuf = p.LV <= 32 && (p.LV & (p.LV - 1)) == 0 && p.P * p.LV == GT;
