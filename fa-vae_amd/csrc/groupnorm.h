@@ -4,7 +4,7 @@
 #include <algorithm>
 #include <type_traits>
 
-constexpr int GTF = 512, GTB = 256;     // threads of a workgroup, forward and backward
+constexpr int GTF = 512, GTB = 256;     // threads of a workgroup, forward and backward, at most
 constexpr int GU = 4;                   // positions a thread has under way in the chunked forms
 constexpr int WAVE_ITEMS = 8, ITEMS_MAX = 16;
 constexpr int GTP = 512, PIPED_ITEMS = 8;        // piped form
@@ -26,7 +26,7 @@ struct GnP {
     // geometry.  A workgroup (a wave in the wave form) takes CB channels: whole groups (pieces == 1), or piece j of `pieces` of one group
     // wider than it.  LV lanes side by side, 16 bytes each, cover the CB channels, P rows of lanes take P positions at once, NSUB samples share a
     // workgroup.
-    int LV, P, NSUB, CB, ncb, pieces, chunk, nchunk, shuf;
+    int LV, P, NSUB, CB, ncb, pieces, chunk, nchunk, shuf, nt;      // nt: threads
     long long blocks;
 };
 
@@ -79,11 +79,11 @@ __device__ __forceinline__ float wave_total(float v) {
     return v;
 }
 
-// lanes (a power of two up to 64) that add the `per` values of each of `pairs` sums side by side
-template <int GT> __device__ __forceinline__ int pair_lanes(int pairs, int per) {
-    int L = 64;
-    while (L > 1 && (pairs * L > GT || L / 2 >= per)) L >>= 1;
-    return L;
+// log2 of the lanes (up to 64) that add the `per` values of each of `pairs` sums side by side
+__device__ __forceinline__ int pair_lanes_log2(int threads, int pairs, int per) {
+    int s = 6;
+    while (s > 0 && (pairs << s > threads || 1 << (s - 1) >= per)) --s;
+    return s;
 }
 
 // Sum of v over the threads of every (sample of the block, group of the block) pair into grp[].  A thread's values j with own(j) belong
@@ -97,7 +97,7 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
         for (int o = p.LV; o < 64; o <<= 1)
 #pragma unroll
             for (int j = 0; j < NV; ++j) v[j] += __shfl_xor(v[j], o, 64);
-        rows = GTF / 64;
+        rows = p.nt / 64;
         if ((int)(threadIdx.x & 63) < p.LV)
 #pragma unroll
             for (int j = 0; j < NV; ++j) if (own(j)) red[(threadIdx.x >> 6) * cols + col + j] = v[j];
@@ -109,9 +109,9 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
     const int pairs = p.NSUB * ng;
     if (!p.shuf) {
         // many rows: the columns first (with a division for each value, and partial vectors stored element by element, 512 x 195 x 210 bf16 took 45 us, now 41)
-        const int all = p.NSUB * cols, L = pair_lanes<GTF>(all, rows), l = (int)threadIdx.x & (L - 1);
+        const int all = p.NSUB * cols, ls = pair_lanes_log2(p.nt, all, rows), L = 1 << ls, l = (int)threadIdx.x & (L - 1);
         float* tot = grp + pairs;
-        for (int k = (int)threadIdx.x / L; k < all; k += GTF / L) {
+        for (int k = (int)threadIdx.x >> ls; k < all; k += p.nt >> ls) {
             const int sub = k / cols;
             const float* a = red + (sub * rows + l) * cols + k - sub * cols;
             float s = 0.f;
@@ -124,8 +124,8 @@ __device__ __forceinline__ void gn_reduce(const GnP& p, float (&v)[NV], float* r
         rows = 1;
     }
     // L lanes take a pair: as many as there are threads for every pair at once, at most its values
-    const int per = rows * cpg, L = pair_lanes<GTF>(pairs, per), l = (int)threadIdx.x & (L - 1);
-    for (int k = (int)threadIdx.x / L; k < pairs; k += GTF / L) {
+    const int per = rows * cpg, ls = pair_lanes_log2(p.nt, pairs, per), L = 1 << ls, l = (int)threadIdx.x & (L - 1);
+    for (int k = (int)threadIdx.x >> ls; k < pairs; k += p.nt >> ls) {
         const int sub = k / ng, g = k - sub * ng;
         float s = 0.f;
         for (int i = l; i < per; i += L) {

@@ -147,7 +147,7 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool STATS> __global__ __launc
     const bool has = b.c_lo + lv * VEC < b.c_hi, active = sub < p.NSUB && n < p.N && has;
     const auto own = [&](int j) { return has && ln.own(j); };
     float* red = lds;
-    float* grp = lds + GTF * GPV;
+    float* grp = lds + p.nt * GPV;
 
     GnData<T, TAIL> d[ITEMS];
     const long long x0 = n * p.xn + (s_lo + pos) * p.xs + c0, y0 = n * p.yn + (s_lo + pos) * p.ys + c0;
@@ -181,9 +181,9 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool STATS> __global__ __launc
     }
     float keep_mean = 0.f;                       // a pair's mean, by the thread that stores it
     const int pairs = p.NSUB * b.ng;
-    if ((int)threadIdx.x < pairs && pairs <= GTF) keep_mean = grp[threadIdx.x] * inv;
-    if (pairs > GTF)                             // more pairs than threads: through memory at once (grp is reused below)
-        for (int k = threadIdx.x; k < pairs; k += GTF) {
+    if ((int)threadIdx.x < pairs && pairs <= p.nt) keep_mean = grp[threadIdx.x] * inv;
+    if (pairs > p.nt)                             // more pairs than threads: through memory at once (grp is reused below)
+        for (int k = threadIdx.x; k < pairs; k += p.nt) {
             const long long nn = nb0 * p.NSUB + k / b.ng;
             if (nn < p.N) {
                 if constexpr (STATS) p.part[((nn * p.G + b.g_lo + k % b.ng) * p.nchunk + chunk) * p.pieces + b.piece].x = grp[k] * inv;
@@ -204,16 +204,16 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool STATS> __global__ __launc
         }
     }
     gn_reduce<GPV>(p, v, red, grp, col, r, b.ng, cpg, own);
-    for (int k = threadIdx.x; k < pairs; k += GTF) {
+    for (int k = threadIdx.x; k < pairs; k += p.nt) {
         const long long nn = nb0 * p.NSUB + k / b.ng;
         const int g = b.g_lo + k % b.ng;
         if (nn < p.N) {
             if constexpr (STATS) {
                 float2* o = p.part + ((nn * p.G + g) * p.nchunk + chunk) * p.pieces + b.piece;
-                if (pairs <= GTF) o->x = keep_mean;
+                if (pairs <= p.nt) o->x = keep_mean;
                 o->y = grp[k];
             } else {
-                if (pairs <= GTF) p.mean[nn * p.G + g] = keep_mean;
+                if (pairs <= p.nt) p.mean[nn * p.G + g] = keep_mean;
                 p.rstd[nn * p.G + g] = 1.f / sqrtf(grp[k] * inv + p.eps);
             }
         }
@@ -272,7 +272,7 @@ template <class T, int GPV, bool TAIL> __global__ __launch_bounds__(GTF) void gn
     const GnBlock b = gn_block(p, cb);
     const int parts = p.nchunk * p.pieces;
     float2* stat = (float2*)lds;                 // [ng] (mean, rstd)
-    for (int g = threadIdx.x >> 6; g < b.ng; g += GTF / 64) {
+    for (int g = threadIdx.x >> 6; g < b.ng; g += p.nt / 64) {
         const float2* a = p.part + (n * p.G + b.g_lo + g) * parts;
         const float m = (float)p.S * (float)p.Cg;
         const auto count = [&](int i) {
@@ -345,6 +345,7 @@ int pow2_floor(long long a) { int r = 1; while (2 * r <= a) r *= 2; return r; }
 GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
     GnPlan pl = {};
     const int vec = 16 / es, GT = backward ? GTB : GTF;
+    p.nt = GT;
     const int S = std::max(1, p.S);
     p.pieces = 1; p.nchunk = 1; p.chunk = S; p.NSUB = 1; p.shuf = 0;
     // wave form: groups that are a power of two below a vector, or a power of two of whole vectors
@@ -418,10 +419,10 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
     even_out();
     const auto lanes = [&]() {
         p.LV = cdiv(p.CB, vec);
-        p.P = GT / p.LV;
+        p.P = p.nt / p.LV;
         p.NSUB = 1;
-        if (p.P > S) { p.P = S; p.NSUB = std::min(GT / (p.LV * p.P), std::max(1, p.N)); }
-        p.shuf = p.NSUB == 1 && p.LV <= 32 && (p.LV & (p.LV - 1)) == 0 && p.P * p.LV == GT;
+        if (p.P > S) { p.P = S; p.NSUB = std::min(p.nt / (p.LV * p.P), std::max(1, p.N)); }
+        p.shuf = p.NSUB == 1 && p.LV <= 32 && (p.LV & (p.LV - 1)) == 0 && p.P * p.LV == p.nt;
     };
     lanes();
     // fewer channels side by side, down to 32 bytes, where a run of groups does not fit a workgroup's registers or where there would be fewer
@@ -440,8 +441,16 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
         lanes();
         if (p.CB == before) break;
     }
+    // forward, vectors of several groups: what a thread does besides its vectors costs as much as some 8 of them, so smaller workgroups of up to 8
+    // vectors a thread while the chip keeps 4 waves a CU (300 x 50 x 231 bf16: 14 us, 23 with 512 threads; not with one group a vector, 64 x 1024 x
+    // 64: 12.5 and 9.6, nor backward, 300 x 50 x 231 fp32: 26 and 24)
+    while (!backward && !gs && p.pieces == 1 && p.nt > 64 && p.nt / 2 >= p.LV) {
+        const GnP before = p;
+        p.nt /= 2;
+        lanes();
+        if (cdiv(S, p.P) > 8 || cdivll(p.N, p.NSUB) * p.ncb * (p.nt / 64) < 1024) { p = before; break; }
+    }
     const long long held_blocks = cdivll(p.N, p.NSUB) * p.ncb;
-    pl.threads = GT;
     if (p.pieces == 1 && cdiv(S, p.P) <= ITEMS_MAX && (held_blocks >= (ckpt ? 256 : 64) || cdiv(S, p.P) <= 4)) {
         pl.form = GN_HELD;
         pl.items = cdiv(S, p.P);
@@ -454,6 +463,7 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
         while (p.pieces == 1 && p.CB * es < 128 && p.CB * 2 <= std::min(cap, p.C)) p.CB *= 2;   // whole cache lines again
         if (p.pieces == 1) { p.ncb = cdiv(p.C, p.CB); even_out(); p.LV = cdiv(p.CB, vec); }
         p.NSUB = 1;
+        p.nt = GT;
         p.P = std::max(1, GT / p.LV);
         p.shuf = p.LV <= 32 && (p.LV & (p.LV - 1)) == 0 && p.P * p.LV == GT;
         pl.items = ITEMS_MAX;
@@ -466,6 +476,7 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
         pl.rows = (long long)p.N * p.nchunk;
         pl.part = backward ? (size_t)pl.rows * p.C + (size_t)p.N * p.G : (size_t)p.N * p.G * p.nchunk * p.pieces;
     }
+    pl.threads = p.nt;
     p.blocks = pl.blocks;
     return pl;
 }
@@ -479,13 +490,13 @@ template <class T> int gn_fwd(const GnP& p, const GnPlan& pl, hipStream_t st) {
         constexpr int GPV = decltype(gpv)::value;
         constexpr bool TAIL = decltype(tail)::value;
         const int gpb = cdiv(p.CB, std::min(p.Cg, p.CB));
-        const size_t lds = sizeof(float) * ((size_t)GTF * GPV + (size_t)p.NSUB * (gpb + (p.shuf ? 0 : p.LV * GPV)));
+        const size_t lds = sizeof(float) * ((size_t)p.nt * GPV + (size_t)p.NSUB * (gpb + (p.shuf ? 0 : p.LV * GPV)));
         if (pl.form == GN_HELD)
-            return pl.items <= 4 ? gn_launch(gn_fwd_kernel<T, 4, GPV, TAIL, false>, p, GTF, lds, st)
-                                 : gn_launch(gn_fwd_kernel<T, ITEMS_MAX, GPV, TAIL, false>, p, GTF, lds, st);
-        const int rc = gn_launch(gn_fwd_kernel<T, ITEMS_MAX, GPV, TAIL, true>, p, GTF, lds, st);
+            return pl.items <= 4 ? gn_launch(gn_fwd_kernel<T, 4, GPV, TAIL, false>, p, p.nt, lds, st)
+                                 : gn_launch(gn_fwd_kernel<T, ITEMS_MAX, GPV, TAIL, false>, p, p.nt, lds, st);
+        const int rc = gn_launch(gn_fwd_kernel<T, ITEMS_MAX, GPV, TAIL, true>, p, p.nt, lds, st);
         if (rc != FAVAE_OK) return rc;
-        return gn_launch(gn_apply_kernel<T, GPV, TAIL>, p, GTF, sizeof(float2) * gpb, st);
+        return gn_launch(gn_apply_kernel<T, GPV, TAIL>, p, p.nt, sizeof(float2) * gpb, st);
     });
 }
 

@@ -211,8 +211,8 @@ template <class T, int GPV, bool CK, int ACT> __global__ __launch_bounds__(GTP) 
             tot[k] = make_float2(gam[k] * s.x, gam[k] * s.y);
         }
         lds_barrier();
-        const int L = pair_lanes<GTP>(b.ng, b.cw), l = (int)threadIdx.x & (L - 1);
-        for (int g = (int)threadIdx.x / L; g < b.ng; g += GTP / L) {
+        const int ls = pair_lanes_log2(GTP, b.ng, b.cw), L = 1 << ls, l = (int)threadIdx.x & (L - 1);
+        for (int g = (int)threadIdx.x >> ls; g < b.ng; g += GTP >> ls) {
             float2 s = make_float2(0.f, 0.f);
             for (int c = g * b.cw + l; c < (g + 1) * b.cw; c += L) { s.x += tot[c].x; s.y += tot[c].y; }
             for (int o = L >> 1; o > 0; o >>= 1) { s.x += __shfl_xor(s.x, o, 64); s.y += __shfl_xor(s.y, o, 64); }
@@ -254,7 +254,7 @@ __device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float 
         for (int o = p.LV; o < 64; o <<= 1)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) { a[j] += __shfl_xor(a[j], o, 64); bq[j] += __shfl_xor(bq[j], o, 64); }
-        rows = GTB / 64;
+        rows = p.nt / 64;
         if ((int)(threadIdx.x & 63) < p.LV)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) if (own(j)) red[(threadIdx.x >> 6) * cols + col + j] = make_float2(a[j], bq[j]);
@@ -263,7 +263,7 @@ __device__ __forceinline__ void gn_columns(const GnP& p, float (&a)[VEC], float 
         for (int j = 0; j < VEC; ++j) if (own(j)) red[r * cols + col + j] = make_float2(a[j], bq[j]);
     }
     lds_barrier();
-    for (int k = threadIdx.x; k < p.NSUB * cols; k += GTB) {
+    for (int k = threadIdx.x; k < p.NSUB * cols; k += p.nt) {
         const int sub = k / cols, c = k - sub * cols;
         float2 s = make_float2(0.f, 0.f);
         for (int i = 0; i < rows; ++i) {
@@ -294,7 +294,7 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ _
     constexpr int VEC = VEC16<T>;
     const int cols = p.LV * VEC;
     float2* red = (float2*)lds;
-    float2* tot = red + (p.shuf ? (GTB / 64) * cols : p.P * p.NSUB * cols);
+    float2* tot = red + (p.shuf ? (p.nt / 64) * cols : p.P * p.NSUB * cols);
     float2* grp = tot + p.NSUB * cols;           // [NSUB][ng]
     float2* acc = grp + p.NSUB * cols;           // [cols]
     const unsigned lb = xcd_order(blockIdx.x, (unsigned)p.blocks), row_ = lb / (unsigned)p.ncb;
@@ -311,7 +311,7 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ _
     const auto own = [&](int j) { return has && ln.own(j); };
     int gi[GPV];
     group_of<1>(gi, c0 - b.c_lo, p.Cg, b.ng - 1);
-    for (int k = threadIdx.x; k < cols; k += GTB) acc[k] = make_float2(0.f, 0.f);
+    for (int k = threadIdx.x; k < cols; k += p.nt) acc[k] = make_float2(0.f, 0.f);
     const float inv_m = 1.f / ((float)p.S * (float)p.Cg);
     for (long long nb0 = first; nb0 * p.NSUB < p.N; nb0 += stride) {
         const long long n0 = nb0 * p.NSUB + sub, n = min(n0, (long long)p.N - 1);
@@ -352,14 +352,14 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ _
             for (int j = 0; j < VEC; ++j) sb[j] *= st.rstd(j);
             gn_columns<VEC>(p, sa, sb, red, tot, c0 - b.c_lo, r, own);
         }
-        for (int k = threadIdx.x; k < cols; k += GTB) {
+        for (int k = threadIdx.x; k < cols; k += p.nt) {
             float2 t = acc[k];
             for (int u = 0; u < p.NSUB; ++u) { t.x += tot[u * cols + k].x; t.y += tot[u * cols + k].y; }
             acc[k] = t;
         }
         const int pairs = p.NSUB * b.ng;
-        const int L = pair_lanes<GTB>(pairs, b.cw), l = (int)threadIdx.x & (L - 1);
-        for (int k = (int)threadIdx.x / L; k < pairs; k += GTB / L) {
+        const int ls = pair_lanes_log2(p.nt, pairs, b.cw), L = 1 << ls, l = (int)threadIdx.x & (L - 1);
+        for (int k = (int)threadIdx.x >> ls; k < pairs; k += p.nt >> ls) {
             const int u = k / b.ng, g = k - u * b.ng;
             float2 s = make_float2(0.f, 0.f);
             for (int c = g * b.cw + l; c < (g + 1) * b.cw; c += L) {
@@ -393,7 +393,7 @@ template <class T, int ITEMS, int GPV, bool TAIL, bool CK, int ACT> __global__ _
         }
         lds_barrier();                           // red, tot and grp are free again
     }
-    for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTB) p.part[first * p.C + b.c_lo + k] = acc[k];
+    for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += p.nt) p.part[first * p.C + b.c_lo + k] = acc[k];
 }
 
 // f(x, dy, s) for positions s, s + P, ... below s_hi, GU of them loaded at a time
@@ -431,7 +431,7 @@ template <class T, int GPV, bool TAIL, bool CK> __global__ __launch_bounds__(GTB
     constexpr int VEC = VEC16<T>;
     const int cols = p.LV * VEC;
     float2* red = (float2*)lds;
-    float2* tot = red + (p.shuf ? GTB / 64 : p.P) * cols;
+    float2* tot = red + (p.shuf ? p.nt / 64 : p.P) * cols;
     const GnChunk k_ = gn_chunk(p, true);
     const GnBlock b = gn_block(p, k_.cb);
     const long long n = k_.n;
@@ -469,7 +469,7 @@ template <class T, int GPV, bool TAIL, bool CK> __global__ __launch_bounds__(GTB
         for (int j = 0; j < VEC; ++j) sb[j] *= st.rstd(j);
     }
     gn_columns<VEC>(p, sa, sb, red, tot, c0 - b.c_lo, r, own);
-    for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += GTB) p.part[(n * p.nchunk + k_.chunk) * p.C + b.c_lo + k] = tot[k];
+    for (int k = threadIdx.x; k < b.c_hi - b.c_lo; k += p.nt) p.part[(n * p.nchunk + k_.chunk) * p.C + b.c_lo + k] = tot[k];
 }
 
 // Chunked form, third launch: dx.
@@ -580,25 +580,25 @@ template <class T, bool CK> int gn_bwd(const GnP& p, const GnPlan& pl, float* dg
         });
         return rc != FAVAE_OK ? rc : join(0);
     }
-    const size_t cols = (size_t)p.LV * VEC16<T>, rows = p.shuf ? GTB / 64 : p.P * p.NSUB;
+    const size_t cols = (size_t)p.LV * VEC16<T>, rows = p.shuf ? p.nt / 64 : p.P * p.NSUB;
     return gn_variants<T>(pl, [&](auto gpv, auto tail) {
         constexpr int GPV = decltype(gpv)::value;
         constexpr bool TAIL = decltype(tail)::value;
         if (pl.form == GN_CHUNKED) {
-            int rc = gn_launch(gn_bwd_sums_kernel<T, GPV, TAIL, CK>, p, GTB, sizeof(float2) * (rows + 1) * cols, st);
+            int rc = gn_launch(gn_bwd_sums_kernel<T, GPV, TAIL, CK>, p, p.nt, sizeof(float2) * (rows + 1) * cols, st);
             if (rc != FAVAE_OK) return rc;
             FAVAE_CHECK_ARG((long long)p.N * p.G <= 0x7fffffffLL, "favae_gn_act_bwd: too many groups for one launch");
             rc = join((int)cdivll((long long)p.N * p.G, 16));
-            return rc != FAVAE_OK ? rc : gn_launch(gn_bwd_apply_kernel<T, GPV, TAIL, CK>, p, GTB, 0, st);
+            return rc != FAVAE_OK ? rc : gn_launch(gn_bwd_apply_kernel<T, GPV, TAIL, CK>, p, p.nt, 0, st);
         }
         const size_t lds = sizeof(float2) * (rows + 2 * p.NSUB + 1) * cols;
         int rc = FAVAE_OK;
         with_act_host(p.act, [&](auto act) {
             constexpr int A = decltype(act)::value;
-            if (pl.items <= 4) rc = gn_launch(gn_bwd_kernel<T, 4, GPV, TAIL, CK, A>, p, GTB, lds, st);
-            else if (pl.items <= 8) rc = gn_launch(gn_bwd_kernel<T, 8, GPV, TAIL, CK, A>, p, GTB, lds, st);
-            else if (pl.items <= 12) rc = gn_launch(gn_bwd_kernel<T, 12, GPV, TAIL, CK, A>, p, GTB, lds, st);
-            else rc = gn_launch(gn_bwd_kernel<T, ITEMS_MAX, GPV, TAIL, CK, A>, p, GTB, lds, st);
+            if (pl.items <= 4) rc = gn_launch(gn_bwd_kernel<T, 4, GPV, TAIL, CK, A>, p, p.nt, lds, st);
+            else if (pl.items <= 8) rc = gn_launch(gn_bwd_kernel<T, 8, GPV, TAIL, CK, A>, p, p.nt, lds, st);
+            else if (pl.items <= 12) rc = gn_launch(gn_bwd_kernel<T, 12, GPV, TAIL, CK, A>, p, p.nt, lds, st);
+            else rc = gn_launch(gn_bwd_kernel<T, ITEMS_MAX, GPV, TAIL, CK, A>, p, p.nt, lds, st);
         });
         return rc != FAVAE_OK ? rc : join(0);
     });
