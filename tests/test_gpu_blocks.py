@@ -212,6 +212,50 @@ def test_group_norm_act_bwd(N, S, C, G, dtype):
             gn_bwd_check(B(), N, S, C, G, dtype, act, ck, gen(N, S, C, G, ck))
 
 
+# channel counts off the vector grid: blocks of groups with a short last one, several of one sample's blocks, small workgroups, several samples in
+# one, rows narrower than a vector, chunks
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,S,C,G", [(2, 4000, 945, 945), (300, 50, 231, 33), (100, 700, 165, 5), (64, 1023, 99, 33), (500, 9, 66, 2), (40, 12, 7, 7),
+                                     (600, 3, 5, 1), (3, 20, 20, 4), (1, 20000, 33, 3), (260, 64, 1023, 31)])
+def test_group_norm_odd_channels(N, S, C, G, dtype):
+    b = B()
+    g = gen(N, S, C, G, 1)
+    x = rnd(g, N, S, C, dtype=dtype, scale=1.7, shift=3.0)
+    gamma, beta = rnd(g, C, scale=0.3, shift=1.0), rnd(g, C, scale=0.5)
+    y, mean, rstd = b.group_norm_act(x, G, gamma, beta, act="silu")
+    want, m, r, z, z_err, m_err, r_rel = gn_ref(x, gamma, beta, G, "silu")
+    close(mean, m, m_err)
+    close(rstd, r, r * r_rel)
+    close(y, want, SLOPE * z_err + (z.abs() + 8) * 4 * U * want.abs())
+    xi = x.clone()
+    assert torch.equal(b.group_norm_act(xi, G, gamma, beta, act="silu", out=xi)[0], y)           # in place
+    dy = rnd(g, N, S, C, dtype=dtype)
+    dx = b.group_norm_act_bwd(dy, x, G, gamma, beta, mean, rstd, act="silu")[0]
+    di = dy.clone()
+    assert torch.equal(b.group_norm_act_bwd(di, x, G, gamma, beta, mean, rstd, act="silu", out=di)[0], dx)
+    for ck in (False, True):
+        gn_bwd_check(b, N, S, C, G, dtype, "silu", ck, gen(N, S, C, G, 2 + ck))
+
+
+@pytest.mark.parametrize("N,S,C,G", [(3, 50, 210, 30), (300, 50, 231, 33), (2, 2000, 99, 33), (1, 30000, 33, 11)])
+def test_group_norm_nan_stays_in_its_group_with_odd_channels(N, S, C, G):
+    b = B()
+    g = gen(N, S, C, G, 9)
+    x, dy = rnd(g, N, S, C, dtype=BF16), rnd(g, N, S, C, dtype=BF16)
+    gamma, beta = torch.ones(C, device=DEV), torch.zeros(C, device=DEV)
+    cg = C // G
+    bad = torch.zeros(N, S, C, dtype=torch.bool, device=DEV)
+    for grp in (0, G // 2, G - 1):
+        x[N - 1, S - 1, grp * cg + cg - 1] = float("nan")
+        bad[N - 1, :, grp * cg:(grp + 1) * cg] = True
+    y, m, r = b.group_norm_act(x, G, gamma, beta, act="silu")
+    assert torch.isnan(y[bad]).all() and torch.isfinite(y[~bad]).all()
+    dx, dg, db = b.group_norm_act_bwd(dy, x, G, gamma, beta, m, r, act="silu")
+    assert torch.isnan(dx[bad]).all() and torch.isfinite(dx[~bad]).all()
+    cols = bad.flatten(0, 1).any(0)
+    assert torch.isnan(dg[cols]).all() and torch.isfinite(dg[~cols]).all() and torch.isnan(db[cols]).all() and torch.isfinite(db[~cols]).all()
+
+
 def test_group_norm_gradients_against_differences():
     """dx, dgamma, dbeta of the kernels against central differences of the fp64 forward formula along random directions."""
     b = B()
