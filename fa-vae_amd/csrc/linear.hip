@@ -152,10 +152,12 @@ __device__ __forceinline__ void load_bias(const GemmP& p, float (&b)[8], int j) 
 // belongs there.  The buffer descriptor's range check turns what lies outside the operand into zeros: lanes whose output row (or
 // column) does not exist, or whose chunk lies past the end of the reduction, carry an offset with bit 31 set.
 typedef __attribute__((address_space(3))) void* lds_ptr;
-template <class T, int ROWS, bool CM, int BKE, int NT> struct Dma {
+// B: bytes that a lane brings, 16, or 4 for fp32 operands of any alignment and width (a wave's load brings
+// 256 bytes then: 4001 x 4003 x 4005 953 us, 4004 x 4004 x 4004 931; 777 x 201 x 523 8.3 us, 10.5 and a copy of 3 with 16 bytes).
+template <class T, int ROWS, bool CM, int BKE, int NT, int B> struct Dma {
     typedef TileImg<T, ROWS, CM, BKE> Img;
-    static constexpr int NC = Img::CHUNKS / NT;
-    static_assert(Img::CHUNKS % NT == 0, "whole chunks per thread");
+    static constexpr int PER = 16 / B, VB = B / (int)sizeof(T), NC = Img::CHUNKS * PER / NT;      // lanes of a chunk, elements of a lane
+    static_assert(Img::CHUNKS * PER % NT == 0 && (B == 16 || B == 4) && VB > 0, "whole chunks per thread");
     unsigned voff[NC];
     const char* base;                 // element (o0, first reduction element of this split), KC; (first, o0), CM
     long long step;                   // bytes between steps
@@ -164,9 +166,9 @@ template <class T, int ROWS, bool CM, int BKE, int NT> struct Dma {
         step = CM ? (long long)BKE * ld * (long long)sizeof(T) : (long long)Img::RB;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int c = (int)threadIdx.x + i * NT, row = c / Img::CPR, slot = c - row * Img::CPR, ch = Img::chunk_at(row, slot);
-            const bool ok = CM ? o0 + ch * Img::VE < no : o0 + row < no;
-            voff[i] = ok ? (unsigned)row * (unsigned)(ld * (int)sizeof(T)) + (unsigned)ch * 16u : 0x80000000u;
+            const int c = ((int)threadIdx.x + i * NT) / PER, d = (int)threadIdx.x % PER, row = c / Img::CPR, e = Img::chunk_at(row, c - row * Img::CPR) * Img::VE + d * VB;
+            const bool ok = CM ? o0 + e < no : o0 + row < no;
+            voff[i] = ok ? (unsigned)row * (unsigned)(ld * (int)sizeof(T)) + (unsigned)e * (unsigned)sizeof(T) : 0x80000000u;
         }
     }
     // FULL: BKE reduction elements are left; otherwise `left` of them, the rest reads as zero
@@ -176,10 +178,11 @@ template <class T, int ROWS, bool CM, int BKE, int NT> struct Dma {
         for (int i = 0; i < NC; ++i) {
             unsigned v = voff[i];
             if constexpr (!FULL) {
-                const int c = (int)threadIdx.x + i * NT, row = c / Img::CPR, slot = c - row * Img::CPR;
-                v = (CM ? row : Img::chunk_at(row, slot) * Img::VE) < left ? v : 0x80000000u;
+                const int c = ((int)threadIdx.x + i * NT) / PER, row = c / Img::CPR;
+                v = (CM ? row : Img::chunk_at(row, c - row * Img::CPR) * Img::VE + (int)threadIdx.x % PER * VB) < left ? v : 0x80000000u;
             }
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (wave * 64 + i * NT) * 16), 16, (int)v, 0, 0, 0);
+            if constexpr (B == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (wave * 64 + i * NT) * 16), 16, (int)v, 0, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (wave * 64 + i * NT) * 4), 4, (int)v, 0, 0, 0);
         }
         base += step;
     }
@@ -280,14 +283,14 @@ template <int M, int R> __device__ __forceinline__ void slice_order(const int v)
 // waited for, whose first fragments are read beside the last slice's MFMAs.  So a load has STAGES - 1 steps to arrive, and no MFMA waits for LDS
 // behind a barrier.  Bound by the matrix units and, close behind, LDS (a wave's 128 x 64 tile reads 6 fragments for 8 MFMAs): 16384 x 4096 x 4096
 // bf16 430 us, 1280 TFLOP/s; 4096 x 4096 x 4096 fp32 940 us, 146.
-template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int WPE>
+template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int WPE, int B>
 __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP p) {
     constexpr int NT = 64 * WI * WJ;
     typedef TileImg<T, TI, PCM, BKE> PI;
     typedef TileImg<T, TJ, QCM, BKE> QI;
     constexpr int STAGE = PI::BYTES + QI::BYTES, SL = BKE / 16;
     constexpr int NI = TI / WI / 32, NJ = TJ / WJ / 32;
-    constexpr int LOADS = Dma<T, TI, PCM, BKE, NT>::NC + Dma<T, TJ, QCM, BKE, NT>::NC;   // DMA instructions of a wave per step
+    constexpr int LOADS = Dma<T, TI, PCM, BKE, NT, B>::NC + Dma<T, TJ, QCM, BKE, NT, B>::NC;   // DMA instructions of a wave per step
     static_assert(STAGES >= 2 && SL >= 2 && SL % 2 == 0, "ring and slices");
     extern __shared__ char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wi = wave / WJ, wj = wave - wi * WJ;
@@ -305,8 +308,8 @@ __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[a][c][e] = 0.f;
 
-    Dma<T, TI, PCM, BKE, NT> dp;
-    Dma<T, TJ, QCM, BKE, NT> dq;
+    Dma<T, TI, PCM, BKE, NT, B> dp;
+    Dma<T, TJ, QCM, BKE, NT, B> dq;
     dp.init(p.P, p.ldp, i0, p.I, cb);
     dq.init(p.Q, p.ldq, j0, p.J, cb);
     const int steps = (int)((ce - cb + BKE - 1) / BKE);
@@ -462,8 +465,8 @@ template <class T> __global__ __launch_bounds__(1024) void skinny_kernel(const G
 
 // ---- operands for DMA ----------------------------------------------------------------------------------------------------
 // Copy of up to three operands [rows][cols] with any stride and alignment into [rows][ldo], ldo a multiple of 16 bytes, the rest of a row
-// zero: one pass over an odd operand costs less than staging it through registers would in every tile (x w^T 777 x 201 x 523 bf16: 14 us
-// against 10).
+// zero: bf16 rows that are not 16-byte aligned, and rows more than 4 MB apart.  One pass over an odd operand costs less than staging it through
+// registers would in every tile (x w^T 777 x 201 x 523 bf16: 14 us against 10).
 struct PackP { const char* src[3]; long long ld[3]; char* dst[3]; long long rows[3], first[4]; int cols[3], cpr[3]; };   // cpr: 16-byte chunks of an output row; first: blocks
 template <class T> __global__ __launch_bounds__(256) void pack_kernel(const PackP p) {
     const int j = (blockIdx.x >= p.first[1]) + (blockIdx.x >= p.first[2]);
@@ -587,17 +590,17 @@ GemmPlan plan_gemm(long long I, int J, long long Cn, int es) {
     return best;
 }
 
-template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int WPE>
+template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int WPE, int B = 16>
 void gemm_launch(const GemmP& p, unsigned blocks, hipStream_t st) {
     constexpr size_t ring = STAGES * (size_t)(TileImg<T, TI, PCM, BKE>::BYTES + TileImg<T, TJ, QCM, BKE>::BYTES);
     constexpr size_t lds = std::max(ring, (size_t)WI * WJ * 32 * (TJ / WJ + 4) * sizeof(float));
     static_assert(lds <= 160 * 1024, "LDS of a CU");
-    gemm_dma_kernel<T, OT, TI, TJ, WI, WJ, BKE, STAGES, PCM, QCM, WPE><<<blocks, 64 * WI * WJ, lds, st>>>(p);
+    gemm_dma_kernel<T, OT, TI, TJ, WI, WJ, BKE, STAGES, PCM, QCM, WPE, B><<<blocks, 64 * WI * WJ, lds, st>>>(p);
 }
 
 // out = P Q^T over operands that DMA can take: 16-byte aligned rows, a whole number of chunks (the rest of a KC row zero), and 32-bit offsets
-// inside a tile
-template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, hipStream_t st) {
+// inside a tile; odd (fp32): any alignment and width
+template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, bool odd, hipStream_t st) {
     if (p.I == 0 || p.J == 0) return FAVAE_OK;
     constexpr int es = sizeof(T);
     const GemmPlan pl = plan_gemm(p.I, p.J, p.Cn, es);
@@ -613,8 +616,12 @@ template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, hipStream
     // steps of 128 bytes and two stages; one 64-byte steps and four where neither operand's steps leave half lines behind (x w^T 16384 x 4096 x
     // 4096: 430 us, 452 with 64-byte steps; du w 423, 434; du^T x 409, 406; with 1024 rows and columns over 65536: 136, 131) and in SMALL, for
     // loads that are longer under way (2048 x 2048 x 2048: 22.3 us, 26)
-    if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 128 / es, 2, PCM, QCM, 2>(p, g, st);
-    else if constexpr (es == 4) gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4>(p, g, st);
+    if constexpr (es == 4) {
+        if (pl.tile == TINY && odd) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2, 4>(p, g, st);
+        else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2>(p, g, st);
+        else if (odd) gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4, 4>(p, g, st);
+        else gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4>(p, g, st);
+    } else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 64, 2, PCM, QCM, 2>(p, g, st);
     else if (pl.tile == SMALL) gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
     else if constexpr (PCM && QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, 2>(p, g, st);
     else gemm_launch<T, OT, 256, 256, 2, 4, 64, 2, PCM, QCM, 2>(p, g, st);
@@ -626,10 +633,12 @@ template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, hipStream
     return FAVAE_OK;
 }
 
-// Operands as DMA takes them, or copies of them in the workspace
-struct Operand { const char* p; long long ld, rows; int cols; };
-bool even(const Operand& o, int es) { return aligned(o.p, 16) && (o.ld * es) % 16 == 0 && o.ld * es <= (1 << 22); }
-bool dma_ok(const Operand& o, int es) { return even(o, es) && (o.cols * es) % 16 == 0; }
+// Operands as DMA takes them, or copies of them in the workspace (`ours`: rows padded to 16 bytes).  odd: 1 if a row is not 16-byte aligned, 2 if
+// rows are more than 4 MB apart.
+struct Operand { const char* p; long long ld, rows; int cols; bool ours = false; };
+int odd_of(const Operand& o, int es) { return o.ld * es > 1 << 22 ? 2 : !aligned(o.p, 16) || (o.ld * es) % 16 != 0; }
+bool dma16(const Operand& o, int es) { return o.ours || (odd_of(o, es) == 0 && (o.cols * es) % 16 == 0); }
+bool dma_ok(const Operand& o, int es) { return dma16(o, es) || (es == 4 && odd_of(o, es) < 2); }
 long long padded(long long cols, int es) { return cdivll(cols * es, 16) * 16 / es; }
 size_t pack_bytes(long long rows, int cols, int es);
 template <class T> int pack_operands(std::initializer_list<Operand*> ops, char*& ws, hipStream_t st) {
@@ -640,7 +649,7 @@ template <class T> int pack_operands(std::initializer_list<Operand*> ops, char*&
         const long long ldo = padded(o->cols, sizeof(T));
         k.src[n] = o->p; k.ld[n] = o->ld; k.dst[n] = ws; k.rows[n] = o->rows; k.cols[n] = o->cols; k.cpr[n] = (int)(ldo * (int)sizeof(T) / 16);
         k.first[n + 1] = k.first[n] + cdivll(o->rows * k.cpr[n], 256);
-        *o = {ws, ldo, o->rows, o->cols};
+        *o = {ws, ldo, o->rows, o->cols, true};
         ws += pack_bytes(o->rows, o->cols, sizeof(T));
         ++n;
     }
@@ -670,8 +679,8 @@ int lin_sizes(const char* who, long long M, int N, int K, int act, int dtype) {
     return FAVAE_OK;
 }
 
-// Whether the sizes alone (odd == 0: all pointers and row strides are 16-byte aligned) leave operand [..][cols] as DMA takes it
-bool whole(int cols, int es, int odd) { return !odd && (cols * es) % 16 == 0; }
+// Whether operands [..][cols] need no copy, from their width and the largest of their `odd`
+bool whole(int cols, int es, int odd) { return es == 4 ? odd < 2 : !odd && (cols * es) % 16 == 0; }
 
 struct FwdScratch { size_t split, total; };
 FwdScratch fwd_scratch(long long M, int N, int K, int odd, int es) {
@@ -694,7 +703,7 @@ template <class T> int lin_fwd(GemmP p, Operand x, Operand w, char* scratch, con
     const int rc = pack_operands<T>({&x, &w}, ws, st);
     if (rc != FAVAE_OK) return rc;
     p.P = x.p; p.ldp = x.ld; p.Q = w.p; p.ldq = w.ld;
-    return gemm_run<T, T, false, false>(p, st);
+    return gemm_run<T, T, false, false>(p, !(dma16(x, sizeof(T)) && dma16(w, sizeof(T))), st);
 }
 
 struct BwdScratch { size_t du, colp, split, total; long long ldu; bool need_du; };
@@ -725,7 +734,7 @@ template <class T> int lin_bwd(Operand dy, Operand x, const unsigned char* xe, l
         else if (!pe) act_bwd_kernel<T, 1><<<g, 256, 0, st>>>(d);
         else act_bwd_kernel<T, 2><<<g, 256, 0, st>>>(d);
         FAVAE_LAUNCH_CHECK();
-        if (want_du) dy = {scratch, sz.ldu, M, N};
+        if (want_du) dy = {scratch, sz.ldu, M, N, true};
     }
     if (db && N > 0) {
         col_join_kernel<<<cdiv(N, 16), 512, 0, st>>>(colp, M > 0 ? cdivll(M, du_rows(M)) : 0, N, db);
@@ -737,7 +746,7 @@ template <class T> int lin_bwd(Operand dy, Operand x, const unsigned char* xe, l
         const long long ldt = padded(K, es);
         const int rc = favae_ckpt8_unpack(x.p, x.ld, xe, ldxe, M, K, ws, ldt, es == 4 ? FAVAE_F32 : FAVAE_BF16, st);
         if (rc != FAVAE_OK) return rc;
-        x = {ws, ldt, M, K};
+        x = {ws, ldt, M, K, true};
         ws += pack_bytes(M, K, es);
     }
     const int rc = pack_operands<T>({(dx || dw) && !want_du ? &dy : nullptr, dw && !xe ? &x : nullptr, dx ? &w : nullptr}, ws, st);
@@ -746,15 +755,16 @@ template <class T> int lin_bwd(Operand dy, Operand x, const unsigned char* xe, l
     p.P = dy.p; p.ldp = dy.ld; p.part = part; p.act = FAVAE_ACT_NONE;
     if (dx) {
         p.Q = w.p; p.ldq = w.ld; p.I = M; p.J = K; p.Cn = N; p.out = dx; p.ldo = lddx;
-        const int r2 = gemm_run<T, T, false, true>(p, st);
+        const int r2 = gemm_run<T, T, false, true>(p, !(dma16(dy, es) && dma16(w, es)), st);
         if (r2 != FAVAE_OK) return r2;
     }
     if (dw) {
         p.Q = x.p; p.ldq = x.ld; p.I = N; p.J = K; p.Cn = M; p.out = dw; p.ldo = lddw;
+        const bool odd = !(dma16(dy, es) && dma16(x, es));
         if constexpr (es == 2) {
-            if (dw_f32) return gemm_run<T, float, true, true>(p, st);
+            if (dw_f32) return gemm_run<T, float, true, true>(p, odd, st);
         }
-        return gemm_run<T, T, true, true>(p, st);
+        return gemm_run<T, T, true, true>(p, odd, st);
     }
     return FAVAE_OK;
 }
@@ -777,7 +787,7 @@ extern "C" int favae_linear_act_fwd(const void* x, long long ldx, const void* w,
     FAVAE_CHECK_ARG(ldy >= N && ldx >= K && ldw >= K && (!residual || ldr >= N) && (!pre || ldpre >= N), "favae_linear_act_fwd: a row stride is below the row's length");
     FAVAE_CHECK_ARG(aligned(x, es) && aligned(w, es) && aligned(y, es) && aligned(residual, es) && aligned(pre, es), "favae_linear_act_fwd: a pointer is not aligned to its type");
     const Operand ox = {(const char*)x, ldx, M, K}, ow = {(const char*)w, ldw, N, K};
-    const FwdScratch sz = fwd_scratch(M, N, K, !(even(ox, es) && even(ow, es)), es);
+    const FwdScratch sz = fwd_scratch(M, N, K, std::max(odd_of(ox, es), odd_of(ow, es)), es);
     FAVAE_CHECK_ARG(sz.total <= scratch_bytes && (sz.total == 0 || scratch) && aligned(scratch, 16), "favae_linear_act_fwd: scratch of %zu bytes, %zu needed", scratch_bytes, sz.total);
     GemmP p = {};
     p.I = M; p.J = N; p.Cn = K;
@@ -810,7 +820,7 @@ extern "C" int favae_linear_act_bwd(const void* dy, long long lddy, const void* 
                         aligned(dw, dw_dtype == FAVAE_F32 ? 4 : 2),
                     "favae_linear_act_bwd: a pointer is not aligned to its type");
     const Operand od = {(const char*)dy, lddy, M, N}, ox = {(const char*)x, ldx, M, K}, ow = {(const char*)w, ldw, N, K};
-    const bool odd = !(even(od, es) && (!dx || even(ow, es)) && (!dw || xe || even(ox, es)));
+    const int odd = std::max({odd_of(od, es), dx ? odd_of(ow, es) : 0, dw && !xe ? odd_of(ox, es) : 0});
     const BwdScratch sz = bwd_scratch(M, N, K, act, xe && dw, odd, es);
     FAVAE_CHECK_ARG(sz.total <= scratch_bytes && (sz.total == 0 || scratch) && aligned(scratch, 16), "favae_linear_act_bwd: scratch of %zu bytes, %zu needed",
                     scratch_bytes, sz.total);

@@ -312,9 +312,9 @@ def group_norm_act_bwd(dy, x, groups, gamma, beta, mean, rstd, act="none", out=N
 
 
 def _odd(t, ld, ptr):
-    """Whether the product has to copy t before it can read it in 16-byte pieces."""
+    """How t lies: 0 in 16-byte aligned rows, 1 not, 2 in rows more than 4 MB apart (the size of a product's workspace depends on it)."""
     row = ld * t.element_size()
-    return ptr % 16 != 0 or row % 16 != 0 or row > 1 << 22
+    return 2 if row > 1 << 22 else 1 if ptr % 16 or row % 16 else 0
 
 
 # ---- matrix product ------------------------------------------------------------------------------------------------------
@@ -346,7 +346,7 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
         ldx = k if x.is_contiguous() else _rows(x, "x")
         ldw = k if w.is_contiguous() else _rows(w, "w")
         xp, wp = x.data_ptr(), w.data_ptr()
-        nbytes = _raw.favae_linear_act_fwd_scratch(m, n, k, _odd(x, ldx, xp) or _odd(w, ldw, wp), code)
+        nbytes = _raw.favae_linear_act_fwd_scratch(m, n, k, max(_odd(x, ldx, xp), _odd(w, ldw, wp)), code)
         ws = _scratch(nbytes, x)
         _call(dev, _raw.favae_linear_act_fwd, xp, ldx, wp, ldw, bp, _ptr(residual),
               0 if residual is None else _rows(residual, "residual"), _ptr(pre), n, y.data_ptr(), ldy, m, n, k, a, _ptr(ws), nbytes, code)
@@ -386,7 +386,7 @@ def linear_act_bwd(dy, x, w, act="none", pre=None, need=("x", "w", "b"), dw=None
     xp = x.q if xck else x
     pp = pre.q if pck else pre
     ldd, ldx, ldw = _rows(dy, "dy"), _rows(xp, "x"), _rows(w, "w")
-    odd = _odd(dy, ldd, dy.data_ptr()) or _odd(w, ldw, w.data_ptr()) or (not xck and _odd(x, ldx, x.data_ptr()))
+    odd = max(_odd(dy, ldd, dy.data_ptr()), _odd(w, ldw, w.data_ptr()), 0 if xck else _odd(x, ldx, x.data_ptr()))
     nbytes = _raw.favae_linear_act_bwd_scratch(m, n, k, a, xck and dw is not None, odd, code)
     ws = _scratch(nbytes, dy)
     _call(dev, _raw.favae_linear_act_bwd, dy.data_ptr(), ldd, xp.data_ptr(), ldx, x.e.data_ptr() if xck else None,

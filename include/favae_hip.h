@@ -630,8 +630,8 @@ int favae_gn_act_bwd(const void* dy, long long dn, long long ds, const void* x, 
 
 /* y = act(u) + residual, u = x w^T + bias: x [M][K], w [N][K], y, residual and pre [M][N] of dtype, bias [N] fp32; bias, residual and
  * pre may be NULL.  pre receives u rounded to dtype.  Accumulation, bias, activation and residual in fp32, one rounding.  residual may
- * be y.  Row strides in elements; N and K up to 2^20.  scratch: odd = 0 if x and w have 16-byte aligned pointers and row strides (of at
- * most 4 MB), else 1. */
+ * be y.  Row strides in elements; N and K up to 2^20.  scratch: odd = 0 if x and w have 16-byte aligned pointers and row strides, 1 if one
+ * has not, 2 if a row stride is above 4 MB. */
 size_t favae_linear_act_fwd_scratch(long long M, int N, int K, int odd, int dtype);
 int favae_linear_act_fwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias, const void* residual,
                          long long ldr, void* pre, long long ldpre, void* y, long long ldy, long long M, int N, int K, int act,

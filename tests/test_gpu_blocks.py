@@ -456,6 +456,37 @@ def test_linear_act_every_tile(M, N, K, dtype):
     lin_bwd_check(b, M, N, K, dtype, "none", False, gen(M, N, K, 6), F32)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N,K,ld", [(2049, 2051, 2047, 2050), (777, 201, 523, 523), (19, 70, 33, (1 << 21) + 8)])
+def test_linear_odd_rows(M, N, K, ld, dtype):
+    """Operands that start one element off and end inside a chunk, with faults around them; rows more than 4 MB apart."""
+    b = B()
+    g = gen(M, N, K, 8)
+
+    def within(t, lead):
+        buf = torch.empty(t.shape[0] * lead + 64, dtype=dtype, device=DEV)
+        if buf.numel() < 1 << 24:
+            buf.fill_(float("nan"))
+        v = buf[1:].as_strided(t.shape, (lead, 1))
+        v.copy_(t)
+        return v
+    x, w, dy, pre = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype, scale=K ** -0.5), rnd(g, M, N, dtype=dtype), rnd(g, M, N, dtype=dtype, scale=2.0)
+    bias = rnd(g, N, scale=0.3)
+    xo, wo, do = within(x, ld), within(w, K + 3), within(dy, N + 5)
+    u = x.double() @ w.double().t() + bias.double()
+    v = act64(u, "silu")[0]
+    close(b.linear_act(xo, wo, bias, act="silu"), v, SLOPE * lin_bound(x, w, bias) + (u.abs() + 8) * 4 * U * v.abs())
+    for act in ("none", "silu"):
+        dx, dw, db = b.linear_act_bwd(do, xo, wo, act=act, pre=None if act == "none" else within(pre, N + 1))
+        slope = act64(pre.double(), act)[1]
+        du = dy.double() * slope
+        du_err = dy.double().abs() * (pre.double().abs() + 8) * 4 * U if act != "none" else torch.zeros_like(du)
+        close(db, du.sum(0), du_err.sum(0) + (SUM + (M / 256 / 4 + 16) * U) * du.abs().sum(0))
+        du_r = du_err + (half(dtype) * du.abs() if act != "none" else 0.0)
+        close(dx, du @ w.double(), du_r @ w.double().abs() + (N + 8) * U * (du.abs() @ w.double().abs()))
+        close(dw, du.t() @ x.double(), du_r.t() @ x.double().abs() + (M + 300) * U * (du.abs().t() @ x.double().abs()))
+
+
 def test_linear_act_bwd_long_reduction():
     lin_bwd_check(B(), 9001, 72, 136, BF16, "silu", True, gen(5), F32)
     lin_bwd_check(B(), 20000, 64, 64, F32, "none", False, gen(6))
