@@ -412,7 +412,9 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
     const auto even_out = [&]() {
         if (!pl.tail || p.pieces > 1) return;
         int per = cdiv(p.G, cdiv(p.G, p.CB / p.Cg));
-        while (per < p.G && (p.G - (cdiv(p.G, per) - 1) * per) * p.Cg < vec) ++per;
+        const auto thin = [&]() { return per < p.G && (p.G - (cdiv(p.G, per) - 1) * per) * p.Cg < vec; };
+        while (thin() && (per + 1) * p.Cg <= cap) ++per;
+        while (thin() && per > 1) --per;
         p.CB = per * p.Cg;
         p.ncb = cdiv(p.G, per);
     };
@@ -470,7 +472,7 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
         // forward: chunks of what a workgroup holds, shorter where that leaves the chip empty; backward: about 2048 workgroups
         long long chunk = backward ? cdivll(cdivll((long long)p.N * p.ncb * S, 2048), GU * p.P) * GU * p.P : (long long)p.P * ITEMS_MAX;
         while (chunk > GU * p.P && (long long)p.N * p.ncb * cdivll(S, chunk) < 512) chunk = cdivll(chunk / 2, p.P) * p.P;
-        p.chunk = (int)std::min<long long>(chunk, S);
+        p.chunk = (int)std::max<long long>(1, std::min<long long>(chunk, S));          // (an empty batch has chunks too)
         p.nchunk = cdiv(S, p.chunk);
         pl.blocks = (long long)p.N * p.ncb * p.nchunk;
         pl.rows = (long long)p.N * p.nchunk;
@@ -504,7 +506,7 @@ int gn_sizes(const char* who, long long N, long long S, int C, int G, int act, i
     FAVAE_CHECK_ARG(dtype == FAVAE_F32 || dtype == FAVAE_BF16, "%s: dtype is neither fp32 nor bf16", who);
     FAVAE_CHECK_ARG(act >= FAVAE_ACT_NONE && act <= FAVAE_ACT_GELU_TANH, "%s: unknown activation %d", who, act);
     FAVAE_CHECK_ARG(N >= 0 && S >= 0 && C >= 1 && G >= 1 && C % G == 0, "%s: C = %d channels do not divide into G = %d groups, or a negative size", who, C, G);
-    FAVAE_CHECK_ARG(N <= 0x7fffffff && S <= 0x3fffffff && C <= (1 << 24), "%s: N, S or C too large", who);
+    FAVAE_CHECK_ARG(N <= 0x7fffffff && S <= 0x3fffffff && N * S <= (1LL << 38) && C <= (1 << 24), "%s: N, S or C too large", who);
     return FAVAE_OK;
 }
 bool aligned(const void* a, int es) { return (uintptr_t)a % (size_t)es == 0; }

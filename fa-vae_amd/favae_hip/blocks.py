@@ -258,7 +258,8 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
     0 and variance 0.  out may be x (without ckpt)."""
     n, s, c = _gn_sizes(x.shape, groups)
     code, a, dev = _code(x, "x"), _act(act), x.device
-    _on(dev)
+    if dev.type != "cuda":
+        _on(dev)
     g, b = _vec(gamma, c, "gamma", dev), _vec(beta, c, "beta", dev)
     eps = float(eps)
     if not eps >= 0.0:
@@ -269,7 +270,7 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
     else:
         y = _out(out, "out", x, x.shape, x.dtype, (x, gamma, beta), None if ckpt else x)
         yn, ys = _maps(y, "out")
-    mean, rstd = x.new_empty((2, n, groups), dtype=F32).unbind()
+    mean, rstd = gamma.new_empty((2, n, groups)).unbind()
     ck = _new_ckpt(x) if ckpt else None
     if ckpt and xn != s * xs and n > 1 and s > 1:
         x = x.contiguous()                                   # a checkpoint is of one run of rows
@@ -290,11 +291,12 @@ def group_norm_act_bwd(dy, x, groups, gamma, beta, mean, rstd, act="none", out=N
     ck = isinstance(x, Ckpt8)
     if x.shape != dy.shape or x.dtype != dy.dtype:
         raise ValueError("x: %s %s, as dy" % (dy.dtype, list(dy.shape)))
-    _on(dev, x=x, mean=mean, rstd=rstd)
+    if dev.type != "cuda" or x.device != dev or mean.device != dev or rstd.device != dev:
+        _on(dev, x=x, mean=mean, rstd=rstd)
     g, b = _vec(gamma, c, "gamma", dev), _vec(beta, c, "beta", dev)
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t.dtype != F32 or t.shape != (n, groups) or not t.is_contiguous():
-            raise ValueError("%s: contiguous float32 [%d, %d]" % (name, n, groups))
+    stat = (n, groups)
+    if not (mean.dtype == rstd.dtype == F32 and mean.shape == rstd.shape == stat and mean.is_contiguous() and rstd.is_contiguous()):
+        raise ValueError("mean and rstd: contiguous float32 [%d, %d]" % stat)
     dn, ds = (s * c, c) if dy.is_contiguous() else _maps(dy, "dy")
     xn, xs = (0, 0) if ck else (s * c, c) if x.is_contiguous() else _maps(x, "x")
     if out is None:
@@ -302,7 +304,7 @@ def group_norm_act_bwd(dy, x, groups, gamma, beta, mean, rstd, act="none", out=N
     else:
         dx = _out(out, "out", dy, dy.shape, dy.dtype, (dy, x.q, x.e, gamma, beta, mean, rstd) if ck else (dy, x, gamma, beta, mean, rstd), dy)
         dxn, dxs = _maps(dx, "out")
-    dgamma, dbeta = dy.new_empty((2, c), dtype=F32).unbind()
+    dgamma, dbeta = gamma.new_empty((2, c)).unbind()
     nbytes = _raw.favae_gn_act_scratch(n, s, c, groups, 1, code)
     ws = _scratch(nbytes, dy)
     _call(dev, _raw.favae_gn_act_bwd, dy.data_ptr(), dn, ds, None if ck else x.data_ptr(), xn, xs, x.q.data_ptr() if ck else None,
@@ -327,7 +329,8 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
     code, a, dev = _code(x, "x"), _act(act), x.device
     if w.dtype != x.dtype:
         raise TypeError("w: %s, as x" % x.dtype)
-    _on(dev, w=w, residual=residual)
+    if dev.type != "cuda" or w.device != dev or residual is not None:
+        _on(dev, w=w, residual=residual)
     n, k = w.shape
     m = 1
     for v in x.shape[:-1]:

@@ -100,3 +100,16 @@ def test_c_entry_points_refuse_without_a_gpu():
                        (lambda: r.favae_linear_act_fwd(None, 8, None, 8, None, None, 0, None, 0, None, 6, 4, 6, 8, 0, None, 0, 5, None), "dtype"),
                        (lambda: r.favae_linear_act_bwd(None, 6, None, 8, None, 0, None, 8, None, 0, None, 0, 4, 6, 8, 0, None, 8, None, 8, 0, None, None, 0, 0, None), "dy")):
         assert call() < 0 and text in L.last_error(), L.last_error()
+
+
+def test_group_norm_plans_for_any_channel_count():
+    """The workspace size, and with it the choice of a kernel, for channel counts around every limit of a workgroup."""
+    from favae_hip import blocks as b
+    from favae_hip import lib as L
+    for dtype in (L.F32, L.BF16):
+        for backward in (0, 1):
+            for c, g in [(1047553, 1047553), (1 << 24, 1), (1 << 24, 1 << 24), ((1 << 24) - 1, 1), ((1 << 24) - 1, (1 << 24) - 1), (4097, 1), (4097 * 3, 3),
+                         (1023 * 1021, 1023), (7, 7), (1, 1)]:
+                for n, s in [(1, 1), (1, 5000), (300, 17), (0, 4), (2, 0)]:
+                    assert b._raw.favae_gn_act_scratch(n, s, c, g, backward, dtype) >= 0
+    assert L.last_error() is not None

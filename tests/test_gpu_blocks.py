@@ -318,6 +318,12 @@ def test_group_norm_layouts_in_place_and_empty():
         st = torch.zeros(t.shape[0], 4, device=DEV)
         dx, dg, db = b.group_norm_act_bwd(t, t, 4, gamma, beta, st, st)
         assert dx.shape == t.shape and (dg == 0).all() and (db == 0).all()
+    for wide in ((0, 5, 4099), (0, 5, 8192)):                 # an empty batch of what would go in chunks
+        t, v = torch.empty(wide, device=DEV), torch.ones(wide[-1], device=DEV)
+        st = torch.zeros(0, 1, device=DEV)
+        assert b.group_norm_act(t, 1, v, v)[0].shape == wide
+        dx, dg, db = b.group_norm_act_bwd(t, t, 1, v, v, st, st)
+        assert dx.shape == wide and (dg == 0).all() and (db == 0).all()
     # a constant group: variance 0
     y, m, r = b.group_norm_act(torch.full((2, 9, 32), 5.0, device=DEV), 4, gamma, beta)
     assert (m == 5).all() and torch.equal(y, beta.expand(2, 9, 32))
