@@ -615,13 +615,15 @@ template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, bool odd,
     const unsigned g = (unsigned)blocks;
     // steps of 128 bytes and two stages; one 64-byte steps and four where neither operand's steps leave half lines behind (x w^T 16384 x 4096 x
     // 4096: 430 us, 452 with 64-byte steps; du w 423, 434; du^T x 409, 406; with 1024 rows and columns over 65536: 136, 131) and in SMALL, for
-    // loads that are longer under way (2048 x 2048 x 2048: 22.3 us, 26)
+    // loads that are longer under way (2048 x 2048 x 2048: 22.3 us, 26).  TINY with a CU to itself: four stages, where two leave too little of w
+    // under way (64 x 4096 x 4096 13 us, 15.5; fp32 33 either way); with neighbours 30 us, 34 (du w 2048 x 2048 x 2048) the other way round.
     if constexpr (es == 4) {
         if (pl.tile == TINY && odd) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2, 4>(p, g, st);
         else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2>(p, g, st);
         else if (odd) gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4, 4>(p, g, st);
         else gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4>(p, g, st);
-    } else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 64, 2, PCM, QCM, 2>(p, g, st);
+    } else if (pl.tile == TINY && blocks <= CUS) gemm_launch<T, OT, 64, 64, 2, 2, 64, 4, PCM, QCM, 2>(p, g, st);
+    else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 64, 2, PCM, QCM, 2>(p, g, st);
     else if (pl.tile == SMALL) gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
     else if constexpr (PCM && QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, 2>(p, g, st);
     else gemm_launch<T, OT, 256, 256, 2, 4, 64, 2, PCM, QCM, 2>(p, g, st);
