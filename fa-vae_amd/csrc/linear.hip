@@ -672,7 +672,8 @@ size_t split_bytes(long long I, int J, long long Cn, int es) {
     return s > 1 ? round256((size_t)s * I * ((J + 7) & ~7) * sizeof(float)) : 0;
 }
 constexpr int DU_RUNS = 256;
-long long du_rows(long long M) { return std::max<long long>(16, cdivll(M, DU_RUNS)); }
+// rows of a run; up to 64 rows are one run, whose sums are db: no launch to join them
+long long du_rows(long long M) { return M <= 64 ? 64 : std::max<long long>(16, cdivll(M, DU_RUNS)); }
 
 int lin_sizes(const char* who, long long M, int N, int K, int act, int dtype) {
     FAVAE_CHECK_ARG(dtype == FAVAE_F32 || dtype == FAVAE_BF16, "%s: dtype is neither fp32 nor bf16", who);
@@ -729,8 +730,9 @@ template <class T> int lin_bwd(Operand dy, Operand x, const unsigned char* xe, l
     char* ws = scratch + sz.du + sz.colp + sz.split;
     // du, or (beside the column sums) dy as DMA takes it
     const bool want_du = (dx || dw) && (act != FAVAE_ACT_NONE || (db && !dma_ok(dy, es)));
+    const bool one_run = M > 0 && M <= du_rows(M);
     if (M > 0 && N > 0 && (want_du || db)) {
-        DuP d = {dy.p, dy.ld, pre, ldpre, (const unsigned char*)pre, pe, ldpe, want_du ? scratch : nullptr, sz.ldu, db ? colp : nullptr, M, du_rows(M), N, act};
+        DuP d = {dy.p, dy.ld, pre, ldpre, (const unsigned char*)pre, pe, ldpe, want_du ? scratch : nullptr, sz.ldu, db ? (one_run ? db : colp) : nullptr, M, du_rows(M), N, act};
         const dim3 g((unsigned)cdiv(N, 64 * (16 / es)), (unsigned)cdivll(M, d.rows));
         if (act == FAVAE_ACT_NONE) act_bwd_kernel<T, 0><<<g, 256, 0, st>>>(d);
         else if (!pe) act_bwd_kernel<T, 1><<<g, 256, 0, st>>>(d);
@@ -738,7 +740,7 @@ template <class T> int lin_bwd(Operand dy, Operand x, const unsigned char* xe, l
         FAVAE_LAUNCH_CHECK();
         if (want_du) dy = {scratch, sz.ldu, M, N, true};
     }
-    if (db && N > 0) {
+    if (db && N > 0 && !one_run) {
         col_join_kernel<<<cdiv(N, 16), 512, 0, st>>>(colp, M > 0 ? cdivll(M, du_rows(M)) : 0, N, db);
         FAVAE_LAUNCH_CHECK();
     }

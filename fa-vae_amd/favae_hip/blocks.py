@@ -356,7 +356,10 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
     return (y, pre) if save_pre else y
 
 
-def linear_act_bwd(dy, x, w, act="none", pre=None, need=("x", "w", "b"), dw=None):
+_ALL = ("x", "w", "b")
+
+
+def linear_act_bwd(dy, x, w, act="none", pre=None, need=_ALL, dw=None):
     """Gradients of linear_act: (dx, dw, db), None for what `need` leaves out.  x and pre: tensors or Ckpt8; pre is needed unless act
     is "none".  dx [..., K] is of dy's type, dw [N, K] of w's type or, into a float32 `dw`, unrounded, db fp32 [N].  The gradient of
     the residual is dy."""
@@ -365,7 +368,7 @@ def linear_act_bwd(dy, x, w, act="none", pre=None, need=("x", "w", "b"), dw=None
         raise ValueError("dy [..., N], x [..., K], w [N, K], not %s, %s, %s" % (list(dy.shape), list(x.shape), list(w.shape)))
     if w.dtype != dy.dtype or x.dtype != dy.dtype:
         raise TypeError("x and w: %s, as dy" % dy.dtype)
-    if not set(need) <= {"x", "w", "b"}:
+    if need is not _ALL and not set(need) <= set(_ALL):
         raise ValueError("need: of 'x', 'w', 'b'")
     if act == "none":
         pre = None
@@ -373,27 +376,33 @@ def linear_act_bwd(dy, x, w, act="none", pre=None, need=("x", "w", "b"), dw=None
         raise ValueError("pre: the gradient of %s needs the pre-activation" % act)
     elif pre.shape != dy.shape or pre.dtype != dy.dtype:
         raise ValueError("pre: %s %s, as dy" % (dy.dtype, list(dy.shape)))
-    _on(dev, x=x, w=w, pre=pre)
+    if dev.type != "cuda" or x.device != dev or w.device != dev or pre is not None:
+        _on(dev, x=x, w=w, pre=pre)
     n, k = w.shape
     m = 1
     for v in dy.shape[:-1]:
         m *= v
     xck, pck = isinstance(x, Ckpt8), isinstance(pre, Ckpt8)
+    lddw = k
     if dw is not None and "w" in need:
         if dw.dtype not in (F32, w.dtype) or dw.shape != w.shape or dw.device != dev:
             raise ValueError("dw: float32 or %s, %s" % (w.dtype, list(w.shape)))
+        lddw = _rows(dw, "dw")
         _apart(dw, "dw", (dy, w) + ((x.q, x.e) if xck else (x,)) + ((pre.q, pre.e) if pck else (pre,)))
     dx = dy.new_empty(x.shape) if "x" in need else None
     dw = None if "w" not in need else w.new_empty((n, k)) if dw is None else dw
     db = dy.new_empty(n, dtype=F32) if "b" in need else None
     xp = x.q if xck else x
     pp = pre.q if pck else pre
-    ldd, ldx, ldw = _rows(dy, "dy"), _rows(xp, "x"), _rows(w, "w")
-    odd = max(_odd(dy, ldd, dy.data_ptr()), _odd(w, ldw, w.data_ptr()), 0 if xck else _odd(x, ldx, x.data_ptr()))
+    ldd = n if dy.is_contiguous() else _rows(dy, "dy")
+    ldx = k if xp.is_contiguous() else _rows(xp, "x")
+    ldw = k if w.is_contiguous() else _rows(w, "w")
+    dyp, wp, xptr = dy.data_ptr(), w.data_ptr(), xp.data_ptr()
+    odd = max(_odd(dy, ldd, dyp), _odd(w, ldw, wp), 0 if xck else _odd(x, ldx, xptr))
     nbytes = _raw.favae_linear_act_bwd_scratch(m, n, k, a, xck and dw is not None, odd, code)
     ws = _scratch(nbytes, dy)
-    _call(dev, _raw.favae_linear_act_bwd, dy.data_ptr(), ldd, xp.data_ptr(), ldx, x.e.data_ptr() if xck else None,
-          x.e.shape[-1] if xck else 0, w.data_ptr(), ldw, _ptr(pp), 0 if pp is None else _rows(pp, "pre"),
-          pre.e.data_ptr() if pck else None, pre.e.shape[-1] if pck else 0, m, n, k, a, _ptr(dx), k, _ptr(dw), k if dw is None else _rows(dw, "dw"),
+    _call(dev, _raw.favae_linear_act_bwd, dyp, ldd, xptr, ldx, x.e.data_ptr() if xck else None,
+          x.e.shape[-1] if xck else 0, wp, ldw, _ptr(pp), 0 if pp is None else _rows(pp, "pre"),
+          pre.e.data_ptr() if pck else None, pre.e.shape[-1] if pck else 0, m, n, k, a, _ptr(dx), k, _ptr(dw), lddw,
           L.F32 if dw is not None and dw.dtype == F32 else code, _ptr(db), _ptr(ws), nbytes, code)
     return dx, dw, db
