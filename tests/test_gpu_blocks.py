@@ -498,6 +498,21 @@ def test_linear_act_bwd_long_reduction():
     lin_bwd_check(B(), 20000, 64, 64, F32, "none", False, gen(6))
 
 
+@pytest.mark.parametrize("M", [1, 3, 4, 63, 64, 65, 129])
+def test_linear_bias_gradient_of_few_rows(M):
+    """One run of rows, whose sums are the gradient, and two of them; without dx and dw too."""
+    b = B()
+    g = gen(M, 12)
+    for dtype, n in ((BF16, 200), (F32, 201)):
+        dy, x, w, pre = rnd(g, M, n, dtype=dtype), rnd(g, M, 40, dtype=dtype), rnd(g, n, 40, dtype=dtype), rnd(g, M, n, dtype=dtype)
+        for act in ("none", "silu"):
+            du = dy.double() * act64(pre.double(), act)[1]
+            err = (SUM * du.abs() + dy.double().abs() * (pre.double().abs() + 8) * 4 * U).sum(0)
+            p = None if act == "none" else pre
+            close(b.linear_act_bwd(dy, x, w, act=act, pre=p)[2], du.sum(0), err)
+            close(b.linear_act_bwd(dy, x, w, act=act, pre=p, need=("b",))[2], du.sum(0), err)
+
+
 def test_linear_gradients_against_differences():
     b = B()
     g = gen(43)
