@@ -208,7 +208,7 @@ def _new_ckpt(x):
     shape = x.shape
     ck = Ckpt8.__new__(Ckpt8)                                # right by construction
     ck.q = x.new_empty(shape, dtype=torch.int8)
-    ck.e = x.new_empty(shape[:-1] + ((shape[-1] + CKPT_BLOCK - 1) // CKPT_BLOCK,), dtype=torch.uint8)
+    ck.e = x.new_empty(shape[:-1] + (-(-shape[-1] // CKPT_BLOCK),), dtype=torch.uint8)
     ck.dtype = x.dtype
     return ck
 
@@ -216,26 +216,35 @@ def _new_ckpt(x):
 def ckpt8_pack(x):
     """x [..., C] (fp32 or bf16, rows of any stride) -> Ckpt8."""
     code, ld, dev = _code(x, "x"), _rows(x, "x"), x.device
-    _on(dev)
+    if dev.type != "cuda":
+        _on(dev)
     c = x.shape[-1]
     ck = _new_ckpt(x)
-    if x.numel():
-        _call(dev, _raw.favae_ckpt8_pack, x.data_ptr(), ld, x.numel() // c, c, ck.q.data_ptr(), c, ck.e.data_ptr(), ck.e.shape[-1], code)
+    n = x.numel()
+    if n:
+        _call(dev, _raw.favae_ckpt8_pack, x.data_ptr(), ld, n // c, c, ck.q.data_ptr(), c, ck.e.data_ptr(), -(-c // CKPT_BLOCK), code)
     return ck
 
 
 def ckpt8_unpack(ck, dtype=None, out=None):
     """The values of a checkpoint, in the type it was packed from or in `dtype`; out: rows of any stride."""
+    q, e = ck.q, ck.e
     dtype = ck.dtype if dtype is None and out is None else out.dtype if dtype is None else dtype
     if dtype not in (F32, BF16):
         raise TypeError("dtype: float32 or bfloat16")
-    dev = ck.device
-    _on(dev)
-    out = _out(out, "out", ck.q, ck.shape, dtype, (ck.q, ck.e))
-    c = ck.shape[-1]
-    if out.numel():
-        _call(dev, _raw.favae_ckpt8_unpack, ck.q.data_ptr(), c, ck.e.data_ptr(), ck.e.shape[-1], out.numel() // c, c, out.data_ptr(),
-              _rows(out, "out"), _code(out, "out"))
+    dev = q.device
+    if dev.type != "cuda":
+        _on(dev)
+    c = q.shape[-1]
+    if out is None:
+        out, ld = q.new_empty(q.shape, dtype=dtype), c
+    else:
+        out = _out(out, "out", q, q.shape, dtype, (q, e))
+        ld = _rows(out, "out")
+    n = q.numel()
+    if n:
+        _call(dev, _raw.favae_ckpt8_unpack, q.data_ptr(), c, e.data_ptr(), -(-c // CKPT_BLOCK), n // c, c, out.data_ptr(), ld,
+              L.F32 if dtype == F32 else L.BF16)
     return out
 
 
