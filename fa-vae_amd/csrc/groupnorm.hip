@@ -453,7 +453,9 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
         if (cdiv(S, p.P) > 8 || cdivll(p.N, p.NSUB) * p.ncb * (p.nt / 64) < 1024) { p = before; break; }
     }
     const long long held_blocks = cdivll(p.N, p.NSUB) * p.ncb;
-    if (p.pieces == 1 && cdiv(S, p.P) <= ITEMS_MAX && (held_blocks >= (ckpt ? 256 : 64) || cdiv(S, p.P) <= 4)) {
+    // held with fewer workgroups than CUs, and chunked: 64 of them (8 x 4096 x 64 fp32, 16 x 4096 x 64 bf16) 18.1, 17.7 us and 14.4, 14.1; 192 (24 x 4096 x 64
+    // fp32) 23.3 and 28.8; 64 and 100 off the grid (64 x 1000 x 33, 100 x 1500 x 15 bf16) 14.0, 13.6 and 19.9, 18.2
+    if (p.pieces == 1 && cdiv(S, p.P) <= ITEMS_MAX && (held_blocks >= (ckpt ? 256 : pl.tail ? 64 : 96) || cdiv(S, p.P) <= 4)) {
         pl.form = GN_HELD;
         pl.items = cdiv(S, p.P);
         // backward: a workgroup goes over several samples and leaves one row of column sums
@@ -543,7 +545,7 @@ extern "C" int favae_gn_act_fwd(const void* x, long long xn, long long xs, long 
     p.x = x; p.xn = xn; p.xs = xs; p.y = y; p.yn = yn; p.ys = ys;
     p.gamma = gamma; p.beta = beta; p.mean = mean; p.rstd = rstd; p.part = (float2*)scratch;
     p.N = (int)N; p.S = (int)S; p.C = C; p.G = G; p.Cg = C / G; p.act = act; p.eps = eps; p.nb = cdiv(C, CK_BLOCK);
-    const GnPlan pl = gn_plan(p, es, false, q != nullptr, false);
+    const GnPlan pl = gn_plan(p, es, false, q && C % CK_BLOCK == 0, false);       // (other widths are packed in a launch of their own)
     FAVAE_CHECK_ARG(pl.part * sizeof(float2) <= scratch_bytes && (pl.part == 0 || scratch), "favae_gn_act_fwd: scratch of %zu bytes, %zu needed", scratch_bytes,
                     pl.part * sizeof(float2));
     if (q && S > 0) {
