@@ -23,7 +23,7 @@
 
 namespace {
 
-// VEC values of a position into an 8-bit checkpoint: 32 / VEC neighbouring lanes hold a block (C a multiple of 32, all of them active)
+// VEC values of a position into an 8-bit checkpoint: 32 / VEC neighbouring lanes hold a block (ck_in_kernel), all of them active
 template <int VEC> __device__ __forceinline__ void ck_store(const GnP& p, float (&f)[VEC], long long pos, int c) {
     unsigned m = ck_amax(f);
 #pragma unroll
@@ -341,6 +341,13 @@ template <class T, int GPV, bool TAIL> __global__ __launch_bounds__(GTF) void gn
 // ---- geometry ------------------------------------------------------------------------------------------------------------
 int pow2_floor(long long a) { int r = 1; while (2 * r <= a) r *= 2; return r; }
 
+// Whether the kernels of a plan can write the checkpoint with y: a wave's lanes then hold whole blocks of 32 channels.  Widths are multiples of 32,
+// and every run of channels starts on one: runs of whole groups begin at a multiple of CB, the pieces of a group wider than a workgroup where
+// the group does.
+bool ck_in_kernel(const GnP& p, const GnPlan& pl) {
+    return !pl.tail && p.C % CK_BLOCK == 0 && p.CB % CK_BLOCK == 0 && (p.pieces == 1 || p.Cg % CK_BLOCK == 0);
+}
+
 // even: 16-byte aligned rows
 GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
     GnPlan pl = {};
@@ -549,8 +556,8 @@ extern "C" int favae_gn_act_fwd(const void* x, long long xn, long long xs, long 
     FAVAE_CHECK_ARG(pl.part * sizeof(float2) <= scratch_bytes && (pl.part == 0 || scratch), "favae_gn_act_fwd: scratch of %zu bytes, %zu needed", scratch_bytes,
                     pl.part * sizeof(float2));
     if (q && S > 0) {
-        // the checkpoint leaves with y where the lanes of a wave hold whole blocks of 32 channels; otherwise a launch of its own first
-        if (!pl.tail && C % CK_BLOCK == 0 && p.CB % CK_BLOCK == 0) {
+        // the checkpoint leaves with y, or in a launch of its own first
+        if (ck_in_kernel(p, pl)) {
             p.qo = (unsigned char*)q;
             p.eo = (unsigned char*)e;
         } else {

@@ -811,3 +811,16 @@ def test_group_norm_scratch_is_what_the_size_function_says(N, S, C, G, dtype):
                                       stat[1].data_ptr(), None, None, p, n, code, st)
         L.check(rc)
         assert (buf[n:] == 0xA5).all()
+
+
+# ---- checkpoints of the forward pass, further shapes ------------------------------------------------------------------------
+# groups wider than a workgroup: whole vectors but no whole blocks of 32 channels wide (4104, 2056, 4112), off the vector grid, whole blocks (8192)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,S,C,G", [(2, 16, 16416, 4), (2, 16, 16416, 8), (2, 5, 8224, 4), (2, 5, 8224, 2), (1, 3, 8224, 1), (1, 3, 12299, 1), (2, 5, 8192, 1)])
+def test_group_norm_checkpoint_of_wide_groups_is_the_input_packed(N, S, C, G, dtype):
+    b = B()
+    # every channel of another size, so that neighbouring blocks have other steps
+    x = (rnd(gen(31, N, C, G), N, S, C) * torch.exp2(torch.randint(-12, 12, (C,), generator=gen(32, C), device=DEV).float())).to(dtype)
+    ck = b.group_norm_act(x, G, torch.ones(C, device=DEV), torch.zeros(C, device=DEV), act="silu", ckpt=True)[3]
+    ref = b.ckpt8_pack(x)
+    assert torch.equal(ck.e, ref.e) and torch.equal(ck.q, ref.q)
