@@ -274,7 +274,7 @@ template <class T, int GPV, bool TAIL> __global__ __launch_bounds__(GTF) void gn
     float2* stat = (float2*)lds;                 // [ng] (mean, rstd)
     for (int g = threadIdx.x >> 6; g < b.ng; g += p.nt / 64) {
         const float2* a = p.part + (n * p.G + b.g_lo + g) * parts;
-        const float m = (float)p.S * (float)p.Cg;
+        const float m = p.S > 0 ? (float)p.S * (float)p.Cg : 1.f;       // (no positions: both sums are 0, and so are mean and variance)
         const auto count = [&](int i) {
             const int ch = i / p.pieces, pc = i - ch * p.pieces;
             return (float)(min(p.S, (ch + 1) * p.chunk) - ch * p.chunk) * (float)(p.pieces == 1 ? p.Cg : min(p.Cg, (pc + 1) * p.CB) - pc * p.CB);

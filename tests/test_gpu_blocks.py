@@ -824,3 +824,17 @@ def test_group_norm_checkpoint_of_wide_groups_is_the_input_packed(N, S, C, G, dt
     ck = b.group_norm_act(x, G, torch.ones(C, device=DEV), torch.zeros(C, device=DEV), act="silu", ckpt=True)[3]
     ref = b.ckpt8_pack(x)
     assert torch.equal(ck.e, ref.e) and torch.equal(ck.q, ref.q)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,C,G", [(2, 8192, 1), (2, 4099, 1), (3, 16416, 2), (1, 1 << 20, 4)])
+def test_group_norm_of_no_positions_in_wide_groups(N, C, G, dtype):
+    """Mean 0 and variance 0, also where a group is wider than a workgroup."""
+    b = B()
+    e, one, zero = torch.empty(N, 0, C, dtype=dtype, device=DEV), torch.ones(C, device=DEV), torch.zeros(C, device=DEV)
+    for eps in (1e-5, 1.0):
+        y, m, r = b.group_norm_act(e, G, one, zero, eps=eps)
+        assert y.shape == e.shape and (m == 0).all()
+        close(r, torch.full((N, G), eps, device=DEV, dtype=F64).rsqrt(), 3 * U * eps ** -0.5)      # eps as fp32, the root and the division
+    dx, dg, db = b.group_norm_act_bwd(e, e, G, one, zero, m, r)
+    assert dx.shape == e.shape and (dg == 0).all() and (db == 0).all()
