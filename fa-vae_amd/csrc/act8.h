@@ -138,5 +138,8 @@ template <int N> __device__ __forceinline__ unsigned ck_amax(const float (&f)[N]
     for (int j = 0; j < N; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
     return m;
 }
+// host, ckpt8.hip: x [N][S][C] with any strides of a sample and of a position (N, S, C > 0, S < 2^31 for N > 1) -> q, e of N S rows
+int ck_pack_samples(const void* x, long long xn, long long xs, long long N, long long S, int C, void* q, long long ldq, void* e, long long lde, int dtype,
+                    hipStream_t st);
 // value of byte j of w at step s: a conversion that selects and sign-extends its byte, and a product
 __device__ __forceinline__ float ck_value(unsigned w, int j, float s) { return (float)(signed char)(w >> (8 * j)) * s; }

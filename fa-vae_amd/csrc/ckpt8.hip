@@ -8,6 +8,7 @@ namespace {
 
 struct CkP {
     const void* x; long long ldx;
+    long long xn; unsigned S;            // pack, samples of S rows each that are not one run: stride of a sample (ldx: of a row in it)
     unsigned char* q; long long ldq;
     unsigned char* e; long long lde;
     void* out; long long ldo;
@@ -36,9 +37,11 @@ template <bool TAIL> __device__ __forceinline__ CkPlace ck_place(const CkP& p, i
     if (!TAIL && k.nv > 0) k.nv = 8;
     return k;
 }
-template <class T, int U, bool TAIL> __global__ __launch_bounds__(256) void ck_pack_kernel(const CkP p) {
+// SAMPLES: x lies in samples of p.S rows, q and e in one run all the same
+template <class T, int U, bool TAIL, bool SAMPLES> __global__ __launch_bounds__(256) void ck_pack_kernel(const CkP p) {
     const long long base = (long long)blockIdx.x * (256 * U), row0 = base / (p.nb * 4);
     const int off0 = (int)(base - row0 * (p.nb * 4));
+    const long long n0 = SAMPLES ? row0 / p.S : 0;
     float f[U][8];
     CkPlace k[U];
 #pragma unroll
@@ -46,7 +49,12 @@ template <class T, int U, bool TAIL> __global__ __launch_bounds__(256) void ck_p
         k[u] = ck_place<TAIL>(p, u, row0, off0);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[u][j] = 0.f;
-        if (k[u].nv > 0) load8(f[u], (const T*)p.x + k[u].row * p.ldx + k[u].c, TAIL ? k[u].nv : 8);
+        long long off = k[u].row * p.ldx;
+        if constexpr (SAMPLES) {                                 // (rows since the start of sample n0: below S + 256 + 1)
+            const unsigned r = (unsigned)(k[u].row - n0 * p.S), dn = r / p.S;
+            off = (n0 + dn) * p.xn + (long long)(r - dn * p.S) * p.ldx;
+        }
+        if (k[u].nv > 0) load8(f[u], (const T*)p.x + off + k[u].c, TAIL ? k[u].nv : 8);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -115,21 +123,31 @@ template <class F> int launch_ck(long long blocks, const char* who, F&& f) {
 
 }  // namespace
 
+int ck_pack_samples(const void* x, long long xn, long long xs, long long N, long long S, int C, void* q, long long ldq, void* e, long long lde, int dtype,
+                    hipStream_t st) {
+    const int nb = cdiv(C, CK_BLOCK);
+    const bool run = N == 1 || S == 1 || xn == S * xs;
+    const CkP p = {x, S == 1 && N > 1 ? xn : xs, xn, (unsigned)S, (unsigned char*)q, ldq, (unsigned char*)e, lde, nullptr, 0, N * S, C, nb};
+    return launch_ck(cdivll(p.R * nb * 4, 256 * U), "favae_ckpt8_pack", [&](unsigned g) {
+        const auto go = [&](auto t, auto tail) {
+            constexpr bool TAIL = decltype(tail)::value;
+            if (run) ck_pack_kernel<decltype(t), U, TAIL, false><<<g, 256, 0, st>>>(p);
+            else ck_pack_kernel<decltype(t), U, TAIL, true><<<g, 256, 0, st>>>(p);
+        };
+        if (dtype == FAVAE_F32) C % 8 ? go(0.f, std::true_type()) : go(0.f, std::false_type());
+        else C % 8 ? go(bf16_t(0), std::true_type()) : go(bf16_t(0), std::false_type());
+    });
+}
+
 extern "C" int favae_ckpt8_pack(const void* x, long long ldx, long long R, int C, void* q, long long ldq, void* e, long long lde, int dtype,
                                 void* stream) {
     FAVAE_CHECK_ARG(R >= 0 && C >= 0 && (dtype == FAVAE_F32 || dtype == FAVAE_BF16), "favae_ckpt8_pack: bad sizes or dtype");
     if (R == 0 || C == 0) return FAVAE_OK;
-    const int nb = cdiv(C, CK_BLOCK);
-    FAVAE_CHECK_ARG(x && q && e && ldx >= C && ldq >= C && lde >= nb, "favae_ckpt8_pack: null pointer or a row stride below the row's length");
     FAVAE_CHECK_ARG(C <= (1 << 28), "favae_ckpt8_pack: more than 2^28 channels");
+    FAVAE_CHECK_ARG(x && q && e && ldx >= C && ldq >= C && lde >= cdiv(C, CK_BLOCK), "favae_ckpt8_pack: null pointer or a row stride below the row's length");
     const int es = dtype == FAVAE_F32 ? 4 : 2;
     FAVAE_CHECK_ARG(aligned(x, es), "favae_ckpt8_pack: x is not aligned to its type");
-    CkP p = {x, ldx, (unsigned char*)q, ldq, (unsigned char*)e, lde, nullptr, 0, R, C, nb};
-    const hipStream_t st = (hipStream_t)stream;
-    return launch_ck(cdivll(R * nb * 4, 256 * U), "favae_ckpt8_pack", [&](unsigned g) {
-        if (dtype == FAVAE_F32) C % 8 ? ck_pack_kernel<float, U, true><<<g, 256, 0, st>>>(p) : ck_pack_kernel<float, U, false><<<g, 256, 0, st>>>(p);
-        else C % 8 ? ck_pack_kernel<bf16_t, U, true><<<g, 256, 0, st>>>(p) : ck_pack_kernel<bf16_t, U, false><<<g, 256, 0, st>>>(p);
-    });
+    return ck_pack_samples(x, 0, ldx, 1, R, C, q, ldq, e, lde, dtype, (hipStream_t)stream);
 }
 
 extern "C" int favae_ckpt8_unpack(const void* q, long long ldq, const void* e, long long lde, long long R, int C, void* out, long long ldo,
@@ -141,7 +159,7 @@ extern "C" int favae_ckpt8_unpack(const void* q, long long ldq, const void* e, l
     FAVAE_CHECK_ARG(C <= (1 << 28), "favae_ckpt8_unpack: more than 2^28 channels");
     const int es = dtype == FAVAE_F32 ? 4 : 2;
     FAVAE_CHECK_ARG(aligned(out, es), "favae_ckpt8_unpack: out is not aligned to its type");
-    CkP p = {nullptr, 0, (unsigned char*)q, ldq, (unsigned char*)e, lde, out, ldo, R, C, nb};
+    CkP p = {nullptr, 0, 0, 0, (unsigned char*)q, ldq, (unsigned char*)e, lde, out, ldo, R, C, nb};
     const hipStream_t st = (hipStream_t)stream;
     return launch_ck(cdivll(R * nb * 4, 256 * U), "favae_ckpt8_unpack", [&](unsigned g) {
         if (dtype == FAVAE_F32) C % 8 ? ck_unpack_kernel<float, U, true><<<g, 256, 0, st>>>(p) : ck_unpack_kernel<float, U, false><<<g, 256, 0, st>>>(p);

@@ -561,8 +561,7 @@ extern "C" int favae_gn_act_fwd(const void* x, long long xn, long long xs, long 
             p.qo = (unsigned char*)q;
             p.eo = (unsigned char*)e;
         } else {
-            FAVAE_CHECK_ARG(N == 1 || S == 1 || xn == S * xs, "favae_gn_act_fwd: a checkpoint of x needs one stride between all its rows");
-            const int r2 = favae_ckpt8_pack(x, S == 1 ? xn : xs, N * S, C, q, C, e, p.nb, dtype, stream);
+            const int r2 = ck_pack_samples(x, xn, xs, N, S, C, q, C, e, p.nb, dtype, (hipStream_t)stream);
             if (r2 != FAVAE_OK) return r2;
         }
     }

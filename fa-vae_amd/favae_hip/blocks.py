@@ -281,9 +281,6 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
         yn, ys = _maps(y, "out")
     mean, rstd = gamma.new_empty((2, n, groups)).unbind()
     ck = _new_ckpt(x) if ckpt else None
-    if ckpt and xn != s * xs and n > 1 and s > 1:
-        x = x.contiguous()                                   # a checkpoint is of one run of rows
-        xn, xs = s * c, c
     if n:
         nbytes = _raw.favae_gn_act_scratch(n, s, c, groups, 0, code)
         ws = _scratch(nbytes, x)

@@ -838,3 +838,43 @@ def test_group_norm_of_no_positions_in_wide_groups(N, C, G, dtype):
         close(r, torch.full((N, G), eps, device=DEV, dtype=F64).rsqrt(), 3 * U * eps ** -0.5)      # eps as fp32, the root and the division
     dx, dg, db = b.group_norm_act_bwd(e, e, G, one, zero, m, r)
     assert dx.shape == e.shape and (dg == 0).all() and (db == 0).all()
+
+
+def checkpoint_layouts(g, C, dtype):
+    wide = rnd(g, 5, 12, C + 24, dtype=dtype)
+    one = rnd(g, 1, 7, C, dtype=dtype)
+    return {"cropped": wide[:, 2:9, :C], "cropped and shifted": wide[:, :7, 3:C + 3], "every other sample": wide[::2, :, :C], "one position": wide[:, 4, :C],
+            "one sample for all": one.expand(4, 7, C), "one position for all": one[:, :1].expand(4, 1, C), "one row for all": one[0, 0].expand(4, C),
+            "samples between each other's positions": wide.transpose(0, 1)[:7, :, :C]}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("C,G", [(40, 5), (64, 8), (33, 3), (4104, 1)])
+def test_group_norm_checkpoint_of_any_layout(C, G, dtype):
+    b = B()
+    gamma, beta = torch.ones(C, device=DEV), torch.zeros(C, device=DEV)
+    for name, x in checkpoint_layouts(gen(33, C), C, dtype).items():
+        y, m, r, ck = b.group_norm_act(x, G, gamma, beta, act="silu", ckpt=True)
+        ref = b.ckpt8_pack(x.contiguous())
+        assert torch.equal(ck.q, ref.q) and torch.equal(ck.e, ref.e), name
+        want, m2, r2, z, z_err, m_err, r_rel = gn_ref(x.contiguous(), gamma, beta, G, "silu")
+        close(y.reshape(want.shape), want, SLOPE * z_err + (z.abs() + 8) * 4 * U * want.abs())
+        close(m, m2, m_err)
+
+
+@pytest.mark.parametrize("C,G", [(64, 8), (72, 9), (66, 3)])
+def test_group_norm_checkpoint_makes_no_copy_of_its_input(C, G):
+    """A cropped map with a checkpoint: outputs, checkpoint and workspace are all that is allocated."""
+    b = B()
+    wide = rnd(gen(34), 64, 33, 32, C + 24, dtype=BF16)
+    x = wide[:, :32, :, :C].flatten(1, 2)
+    assert x.data_ptr() == wide.data_ptr() and not x.is_contiguous() and x.stride(0) != 1024 * x.stride(1)
+    gamma, beta = torch.ones(C, device=DEV), torch.zeros(C, device=DEV)
+    b.group_norm_act(x, G, gamma, beta, act="silu", ckpt=True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = b.group_norm_act(x, G, gamma, beta, act="silu", ckpt=True)
+    held = torch.cuda.memory_allocated() - before
+    assert torch.cuda.max_memory_allocated() - before - held < x.numel()       # half of what a copy takes
+    del out
