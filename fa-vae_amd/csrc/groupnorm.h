@@ -260,7 +260,6 @@ template <class T, class F> int gn_wave_variants(const GnPlan& pl, F&& f) {
 }
 
 template <class K> int gn_launch(K k, const GnP& p, int threads, size_t lds, hipStream_t st) {
-    FAVAE_CHECK_ARG(p.blocks <= 0x7fffffffLL, "favae_gn_act: too many samples for one launch");
     if (p.blocks > 0) k<<<(unsigned)p.blocks, threads, lds, st>>>(p);
     FAVAE_LAUNCH_CHECK();
     return FAVAE_OK;

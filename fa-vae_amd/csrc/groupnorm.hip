@@ -518,6 +518,14 @@ int gn_sizes(const char* who, long long N, long long S, int C, int G, int act, i
     FAVAE_CHECK_ARG(N <= 0x7fffffff && S <= 0x3fffffff && N * S <= (1LL << 38) && C <= (1 << 24), "%s: N, S or C too large", who);
     return FAVAE_OK;
 }
+// limits of the launches, checked before the first of them
+int gn_fits(const char* who, const GnP& p, const GnPlan& pl, size_t scratch_bytes) {
+    FAVAE_CHECK_ARG(pl.blocks <= 0x7fffffffLL, "%s: too many samples for one launch", who);
+    FAVAE_CHECK_ARG(pl.form != GN_CHUNKED || (long long)p.N * p.G <= 0x7fffffffLL, "%s: too many groups for one launch", who);
+    FAVAE_CHECK_ARG(pl.part * sizeof(float2) <= scratch_bytes && (pl.part == 0 || p.part), "%s: scratch of %zu bytes, %zu needed", who, scratch_bytes,
+                    pl.part * sizeof(float2));
+    return FAVAE_OK;
+}
 bool aligned(const void* a, int es) { return (uintptr_t)a % (size_t)es == 0; }
 // 16-byte aligned rows, and a sample within 31 bits
 bool even16(const void* a, long long n, long long s, long long S, int C, int es) {
@@ -553,8 +561,8 @@ extern "C" int favae_gn_act_fwd(const void* x, long long xn, long long xs, long 
     p.gamma = gamma; p.beta = beta; p.mean = mean; p.rstd = rstd; p.part = (float2*)scratch;
     p.N = (int)N; p.S = (int)S; p.C = C; p.G = G; p.Cg = C / G; p.act = act; p.eps = eps; p.nb = cdiv(C, CK_BLOCK);
     const GnPlan pl = gn_plan(p, es, false, q && C % CK_BLOCK == 0, false);       // (other widths are packed in a launch of their own)
-    FAVAE_CHECK_ARG(pl.part * sizeof(float2) <= scratch_bytes && (pl.part == 0 || scratch), "favae_gn_act_fwd: scratch of %zu bytes, %zu needed", scratch_bytes,
-                    pl.part * sizeof(float2));
+    const int fit = gn_fits("favae_gn_act_fwd", p, pl, scratch_bytes);
+    if (fit != FAVAE_OK) return fit;
     if (q && S > 0) {
         // the checkpoint leaves with y, or in a launch of its own first
         if (ck_in_kernel(p, pl)) {
@@ -589,8 +597,8 @@ extern "C" int favae_gn_act_bwd(const void* dy, long long dn, long long ds, cons
     if (any) {
         const bool even = (!x || even16(x, xn, xs, S, C, es)) && even16(dy, dn, ds, S, C, es) && even16(dx, dxn, dxs, S, C, es);
         pl = gn_plan(p, es, true, false, even);
-        FAVAE_CHECK_ARG(pl.part * sizeof(float2) <= scratch_bytes && scratch, "favae_gn_act_bwd: scratch of %zu bytes, %zu needed", scratch_bytes,
-                        pl.part * sizeof(float2));
+        const int fit = gn_fits("favae_gn_act_bwd", p, pl, scratch_bytes);
+        if (fit != FAVAE_OK) return fit;
         p.s12 = p.part + (size_t)pl.rows * C;
     }
     return dtype == FAVAE_F32 ? gn_bwd_f32(p, pl, dgamma, dbeta, (hipStream_t)stream) : gn_bwd_bf16(p, pl, dgamma, dbeta, (hipStream_t)stream);

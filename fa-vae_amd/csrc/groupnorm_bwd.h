@@ -587,7 +587,6 @@ template <class T, bool CK> int gn_bwd(const GnP& p, const GnPlan& pl, float* dg
         if (pl.form == GN_CHUNKED) {
             int rc = gn_launch(gn_bwd_sums_kernel<T, GPV, TAIL, CK>, p, p.nt, sizeof(float2) * (rows + 1) * cols, st);
             if (rc != FAVAE_OK) return rc;
-            FAVAE_CHECK_ARG((long long)p.N * p.G <= 0x7fffffffLL, "favae_gn_act_bwd: too many groups for one launch");
             rc = join((int)cdivll((long long)p.N * p.G, 16));
             return rc != FAVAE_OK ? rc : gn_launch(gn_bwd_apply_kernel<T, GPV, TAIL, CK>, p, p.nt, 0, st);
         }

@@ -609,24 +609,22 @@ template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, bool odd,
     const long long unit = 128 / es;
     p.cchunk = cdivll(cdivll(p.Cn, unit), pl.splits) * unit;
     p.splits = (int)std::max<long long>(1, cdivll(p.Cn, std::max<long long>(1, p.cchunk)));
-    const long long blocks = (long long)p.ti * p.tj * p.splits;
-    FAVAE_CHECK_ARG(blocks <= 0x7fffffffLL, "favae_linear_act: too many rows for one launch");
+    const unsigned blocks = (unsigned)p.ti * (unsigned)p.tj * (unsigned)p.splits;
     p.ldpart = (p.J + 7) & ~7;
-    const unsigned g = (unsigned)blocks;
     // steps of 128 bytes and two stages; one 64-byte steps and four where neither operand's steps leave half lines behind (x w^T 16384 x 4096 x
     // 4096: 430 us, 452 with 64-byte steps; du w 423, 434; du^T x 409, 406; with 1024 rows and columns over 65536: 136, 131) and in SMALL, for
     // loads that are longer under way (2048 x 2048 x 2048: 22.3 us, 26).  TINY with a CU to itself: four stages, where two leave too little of w
     // under way (64 x 4096 x 4096 13 us, 15.5; fp32 33 either way); with neighbours 30 us, 34 (du w 2048 x 2048 x 2048) the other way round.
     if constexpr (es == 4) {
-        if (pl.tile == TINY && odd) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2, 4>(p, g, st);
-        else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2>(p, g, st);
-        else if (odd) gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4, 4>(p, g, st);
-        else gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4>(p, g, st);
-    } else if (pl.tile == TINY && blocks <= CUS) gemm_launch<T, OT, 64, 64, 2, 2, 64, 4, PCM, QCM, 2>(p, g, st);
-    else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 64, 2, PCM, QCM, 2>(p, g, st);
-    else if (pl.tile == SMALL) gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, 2>(p, g, st);
-    else if constexpr (PCM && QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, 2>(p, g, st);
-    else gemm_launch<T, OT, 256, 256, 2, 4, 64, 2, PCM, QCM, 2>(p, g, st);
+        if (pl.tile == TINY && odd) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2, 4>(p, blocks, st);
+        else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2>(p, blocks, st);
+        else if (odd) gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4, 4>(p, blocks, st);
+        else gemm_launch<T, OT, 128, 128, 2, 4, 32, 2, PCM, QCM, 4>(p, blocks, st);
+    } else if (pl.tile == TINY && blocks <= CUS) gemm_launch<T, OT, 64, 64, 2, 2, 64, 4, PCM, QCM, 2>(p, blocks, st);
+    else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 64, 2, PCM, QCM, 2>(p, blocks, st);
+    else if (pl.tile == SMALL) gemm_launch<T, OT, 128, 128, 2, 2, 32, 4, PCM, QCM, 2>(p, blocks, st);
+    else if constexpr (PCM && QCM) gemm_launch<T, OT, 256, 256, 2, 4, 32, 4, PCM, QCM, 2>(p, blocks, st);
+    else gemm_launch<T, OT, 256, 256, 2, 4, 64, 2, PCM, QCM, 2>(p, blocks, st);
     FAVAE_LAUNCH_CHECK();
     if (p.splits > 1) {
         gemm_join_kernel<T, OT><<<(unsigned)cdivll(p.I * (p.ldpart / 8), 256), 256, 0, st>>>(p);
@@ -656,10 +654,8 @@ template <class T> int pack_operands(std::initializer_list<Operand*> ops, char*&
         ++n;
     }
     if (n == 0) return FAVAE_OK;
-    const long long blocks = k.first[n];
-    for (int j = n + 1; j < 4; ++j) k.first[j] = blocks;
-    FAVAE_CHECK_ARG(blocks <= 0x7fffffffLL, "favae_linear_act: too many rows for one launch");
-    pack_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(k);
+    for (int j = n + 1; j < 4; ++j) k.first[j] = k.first[n];
+    pack_kernel<T><<<(unsigned)k.first[n], 256, 0, st>>>(k);
     FAVAE_LAUNCH_CHECK();
     return FAVAE_OK;
 }
@@ -679,6 +675,9 @@ int lin_sizes(const char* who, long long M, int N, int K, int act, int dtype) {
     FAVAE_CHECK_ARG(dtype == FAVAE_F32 || dtype == FAVAE_BF16, "%s: dtype is neither fp32 nor bf16", who);
     FAVAE_CHECK_ARG(act >= FAVAE_ACT_NONE && act <= FAVAE_ACT_GELU_TANH, "%s: unknown activation %d", who, act);
     FAVAE_CHECK_ARG(M >= 0 && N >= 0 && K >= 0 && M <= 0x7fffffffLL && N <= (1 << 20) && K <= (1 << 20), "%s: a size is negative or too large", who);
+    // 512 GB of bf16: no tensor of the card, and every launch below stays under 2^31 workgroups (operands copied 256 chunks of 16 bytes at a time: two of
+    // 2^38 fp32 and a w of 2^40 are 1.5 * 2^30; tiles of 64 x 64: 2^28)
+    FAVAE_CHECK_ARG(M * std::max(N, K) <= 1LL << 38, "%s: %lld rows of %d and %d columns are too large", who, M, N, K);
     return FAVAE_OK;
 }
 

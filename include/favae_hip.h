@@ -616,7 +616,7 @@ int favae_ckpt8_unpack(const void* q, long long ldq, const void* e, long long ld
 
 /* y = act(gamma (x - mean) rstd + beta) over x [N][S][C] in G groups of C / G neighbouring channels; mean, rstd [N][G] fp32 out,
  * rstd = (population variance + eps)^-1/2.  Strides of a sample and of a position in elements, channels contiguous.  S = 0: mean 0,
- * variance 0.  y may be x.  q, e: x as an 8-bit checkpoint (contiguous, R = N * S rows), or both NULL. */
+ * variance 0.  y may be x.  q, e: x as an 8-bit checkpoint (contiguous, R = N * S rows), or both NULL.  N S up to 2^38, C up to 2^24. */
 size_t favae_gn_act_scratch(long long N, long long S, int C, int G, int backward, int dtype);
 int favae_gn_act_fwd(const void* x, long long xn, long long xs, long long N, long long S, int C, int G, const float* gamma,
                      const float* beta, float eps, int act, void* y, long long yn, long long ys, float* mean, float* rstd, void* q, void* e,
@@ -630,7 +630,7 @@ int favae_gn_act_bwd(const void* dy, long long dn, long long ds, const void* x, 
 
 /* y = act(u) + residual, u = x w^T + bias: x [M][K], w [N][K], y, residual and pre [M][N] of dtype, bias [N] fp32; bias, residual and
  * pre may be NULL.  pre receives u rounded to dtype.  Accumulation, bias, activation and residual in fp32, one rounding.  residual may
- * be y.  Row strides in elements; N and K up to 2^20.  scratch: odd = 0 if x and w have 16-byte aligned pointers and row strides, 1 if one
+ * be y.  Row strides in elements; N and K up to 2^20, M max(N, K) up to 2^38.  scratch: odd = 0 if x and w have 16-byte aligned pointers and row strides, 1 if one
  * has not, 2 if a row stride is above 4 MB. */
 size_t favae_linear_act_fwd_scratch(long long M, int N, int K, int odd, int dtype);
 int favae_linear_act_fwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias, const void* residual,

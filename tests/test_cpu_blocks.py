@@ -113,3 +113,23 @@ def test_group_norm_plans_for_any_channel_count():
                 for n, s in [(1, 1), (1, 5000), (300, 17), (0, 4), (2, 0)]:
                     assert b._raw.favae_gn_act_scratch(n, s, c, g, backward, dtype) >= 0
     assert L.last_error() is not None
+
+
+def test_limits_are_checked_before_anything_is_launched():
+    """Sizes past a limit, with pointers that no launch would survive: the argument error (-1), never that of a launch (-2)."""
+    if torch.cuda.is_available():
+        pytest.skip("a launch would be seen by its error, which needs a machine without a GPU")
+    from favae_hip import blocks as b
+    from favae_hip import lib as L
+    r, p, big = b._raw, 4096, 1 << 60
+    calls = {
+        # groups of all samples together, backward in chunks
+        "groups": lambda: r.favae_gn_act_bwd(p, 64 << 13, 64, p, 64 << 13, 64, None, None, 1 << 25, 1 << 13, 64, 64, p, p, p, p, 0, p, 64 << 13, 64, p, p, p, big, L.BF16, None),
+        # workgroups of the norm, whose checkpoint goes first
+        "samples": lambda: r.favae_gn_act_fwd(p, 8201, 8201, 1 << 30, 1, 8201, 8201, p, p, 1e-5, 0, p, 8201, 8201, p, p, p, p, p, big, L.BF16, None),
+        # operands of the products, whose du goes first
+        "too large": lambda: r.favae_linear_act_bwd(p, 1 << 20, p, 1 << 20, None, 0, p, 1 << 20, p, 1 << 20, None, 0, 1 << 22, 1 << 20, 1 << 20, 2, p, 1 << 20, p, 1 << 20,
+                                                    L.BF16, p, p, big, L.BF16, None)}
+    for text, call in calls.items():
+        assert call() == -1 and text in L.last_error(), (text, L.last_error())
+    assert r.favae_linear_act_bwd(p, 8, p, 8, None, 0, p, 8, None, 0, None, 0, 4, 8, 8, 0, p, 8, None, 8, L.BF16, None, p, big, L.BF16, None) == -2      # (a launch)
