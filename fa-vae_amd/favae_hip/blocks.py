@@ -11,7 +11,7 @@ linear.hip, ckpt8.hip).
 Tensors are fp32 or bf16 (one type per call), scale, shift, bias and statistics fp32.  Every call is asynchronous on the current
 stream of its tensors' device, may be captured into a graph, and takes its workspace from torch's allocator on that stream.
 Activations: "none", "lrelu" (slope 0.01), "silu", "gelu_tanh".  Wrong arguments raise ValueError or TypeError before anything is
-launched; there is no CPU fallback.
+launched (sizes past a limit of the library: lib.FavaeArgError, a ValueError and a FavaeHipError); there is no CPU fallback.
 """
 import ctypes
 
@@ -191,6 +191,8 @@ def _call(dev, fn, *args):
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _stream_of(i))
+    if rc == L.ERR_ARG:
+        raise L.FavaeArgError(L.last_error())
     if rc:
         L.check(rc)
 

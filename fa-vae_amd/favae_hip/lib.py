@@ -11,6 +11,7 @@ import torch
 F32, BF16 = 0, 1
 RAW_BF16, DACT_BF16, OUT_BF16 = 0x10, 0x20, 0x40      # storage flags of include/favae_hip.h
 NOT_SPD = 1
+ERR_ARG = -1
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_PATH = os.path.join(_HERE, "libfavae_hip.so")
@@ -18,6 +19,10 @@ _LIB_PATH = os.path.join(_HERE, "libfavae_hip.so")
 
 class FavaeHipError(RuntimeError):
     pass
+
+
+class FavaeArgError(FavaeHipError, ValueError):
+    """An argument that the library refuses (FAVAE_ERR_ARG), for callers that promise ValueError."""
 
 
 def _load():

@@ -878,3 +878,19 @@ def test_group_norm_checkpoint_makes_no_copy_of_its_input(C, G):
     held = torch.cuda.memory_allocated() - before
     assert torch.cuda.max_memory_allocated() - before - held < x.numel()       # half of what a copy takes
     del out
+
+
+def test_sizes_past_a_limit_are_value_errors():
+    """What only the library refuses arrives as the errors of wrong arguments do, and as the library's own."""
+    from favae_hip import lib as L
+    b = B()
+    k = (1 << 20) + 8
+    x, w = torch.zeros(2, k, dtype=BF16, device=DEV), torch.zeros(3, k, dtype=BF16, device=DEV)
+    c = (1 << 24) + 8
+    m, v = torch.zeros(1, 1, c, dtype=BF16, device=DEV), torch.zeros(c, device=DEV)
+    st = torch.zeros(1, 1, device=DEV)
+    for call, text in ((lambda: b.linear_act(x, w), "too large"), (lambda: b.linear_act_bwd(torch.zeros(2, 3, dtype=BF16, device=DEV), x, w), "too large"),
+                       (lambda: b.group_norm_act(m, 1, v, v), "too large"), (lambda: b.group_norm_act_bwd(m, m, 1, v, v, st, st), "too large")):
+        for err in (ValueError, L.FavaeHipError):
+            with pytest.raises(err, match=text):
+                call()
