@@ -12,6 +12,10 @@ Tensors are fp32 or bf16 (one type per call), scale, shift, bias and statistics 
 stream of its tensors' device, may be captured into a graph, and takes its workspace from torch's allocator on that stream.
 Activations: "none", "lrelu" (slope 0.01), "silu", "gelu_tanh".  Wrong arguments raise ValueError or TypeError before anything is
 launched (sizes past a limit of the library: lib.FavaeArgError, a ValueError and a FavaeHipError); there is no CPU fallback.
+
+Nothing here enters an autograd graph: gradients come from the *_bwd calls, made by hand under torch.no_grad() or from an
+autograd.Function.  With grad mode on and an input that requires a gradient, the values are the same, differentiating them raises, and
+`out` is refused.  What a *_bwd call or ckpt8_unpack returns is a constant.
 """
 import ctypes
 
@@ -180,6 +184,21 @@ def _out(out, name, like, shape, dtype, ins, may_be=None):
     return out if out.is_contiguous() or out.numel() == 0 else _distinct(out, name)
 
 
+def _no_out(out):
+    """An output of the caller's is refused where autograd would follow the inputs, as torch's own operators do."""
+    if out is not None:
+        raise ValueError("out: takes no part in autograd, and an input requires a gradient (call under torch.no_grad())")
+
+
+def _no_graph(name, outs, *ins):
+    """The outputs, with a node of autograd that raises: to be differentiated they would have to come from a graph, and there is none."""
+    leaf = next(t for t in ins if t is not None and t.requires_grad)
+    node = torch._C._functions.DelayedError("%s leaves no autograd graph: its gradients are %s_bwd's (call both under torch.no_grad(), or from an "
+                                            "autograd.Function)" % (name, name), len(outs) + 1)
+    return node(*outs, leaf)[:-1]
+
+
+_grad_mode = torch.is_grad_enabled
 _stream_of, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice    # torch.cuda.current_stream builds an object: 2 us
 
 
@@ -275,6 +294,9 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError("eps: not negative")
+    cut = _grad_mode() and (x.requires_grad or gamma.requires_grad or beta.requires_grad)
+    if cut:
+        _no_out(out)
     xn, xs = (s * c, c) if x.is_contiguous() else _maps(x, "x")
     if out is None:
         y, yn, ys = x.new_empty(x.shape), s * c, c
@@ -288,6 +310,8 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
         ws = _scratch(nbytes, x)
         _call(dev, _raw.favae_gn_act_fwd, x.data_ptr(), xn, xs, n, s, c, groups, g, b, eps, a, y.data_ptr(), yn, ys, mean.data_ptr(),
               rstd.data_ptr(), ck.q.data_ptr() if ckpt else None, ck.e.data_ptr() if ckpt else None, _ptr(ws), nbytes, code)
+    if cut:
+        y, mean, rstd = _no_graph("group_norm_act", (y, mean, rstd), x, gamma, beta)
     return (y, mean, rstd, ck) if ckpt else (y, mean, rstd)
 
 
@@ -347,6 +371,10 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("residual: %s %s" % (x.dtype, list(shape)))
     bp = None if bias is None else _vec(bias, n, "bias", dev)
+    cut = _grad_mode() and (x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad) or
+                            (residual is not None and residual.requires_grad))
+    if cut:
+        _no_out(out)
     if out is None:
         y, ldy = x.new_empty(shape), n
     else:
@@ -361,6 +389,10 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
         ws = _scratch(nbytes, x)
         _call(dev, _raw.favae_linear_act_fwd, xp, ldx, wp, ldw, bp, _ptr(residual),
               0 if residual is None else _rows(residual, "residual"), _ptr(pre), n, y.data_ptr(), ldy, m, n, k, a, _ptr(ws), nbytes, code)
+    if cut:
+        if save_pre:
+            return _no_graph("linear_act", (y, pre), x, w, bias, residual)
+        return _no_graph("linear_act", (y,), x, w, bias, residual)[0]
     return (y, pre) if save_pre else y
 
 

@@ -894,3 +894,63 @@ def test_sizes_past_a_limit_are_value_errors():
         for err in (ValueError, L.FavaeHipError):
             with pytest.raises(err, match=text):
                 call()
+
+
+def test_a_lost_gradient_is_an_error():
+    """Inputs that require gradients: the values are those of no_grad, and differentiating them says where the gradients are instead of leaving them out."""
+    b = B()
+    g = gen(51)
+    x, w = rnd(g, 6, 5, 32), torch.nn.Parameter(rnd(g, 24, 32))
+    gamma, beta, bias, res = torch.nn.Parameter(rnd(g, 32)), rnd(g, 32), rnd(g, 24), rnd(g, 6, 5, 24)
+    norm = lambda **k: b.group_norm_act(x, 4, gamma, beta, act="silu", **k)
+    lin = lambda **k: b.linear_act(x, w, bias, act="silu", **k)
+    with torch.no_grad():
+        want = list(norm()) + list(lin(save_pre=True)) + [lin()]
+    assert not any(t.requires_grad for t in want)
+    got = list(norm(ckpt=True)[:3]) + list(lin(save_pre=True)) + [lin()]
+    for k, (a, t) in enumerate(zip(got, want)):
+        assert torch.equal(a, t) and a.dtype == t.dtype
+        with pytest.raises(RuntimeError, match="group_norm_act_bwd" if k < 3 else "linear_act_bwd"):
+            (2 * a).sum().backward()
+    assert w.grad is None and gamma.grad is None
+    for t in (x, beta):
+        t.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="linear_act_bwd"):
+        b.linear_act(x, w.detach()).sum().backward()
+    with pytest.raises(RuntimeError, match="linear_act_bwd"):
+        b.linear_act(x.detach(), w.detach(), residual=res.clone().requires_grad_(True)).sum().backward()
+    with pytest.raises(RuntimeError, match="group_norm_act_bwd"):
+        b.group_norm_act(x.detach(), 4, gamma.detach(), beta)[0].sum().backward()
+    # an output of the caller's, as with torch's own operators
+    buf, y = torch.empty(6, 5, 24, device=DEV), torch.empty(6, 5, 32, device=DEV)
+    for call in (lambda: lin(out=buf), lambda: norm(out=y)):
+        with pytest.raises(ValueError, match="out"):
+            call()
+    with torch.no_grad():
+        assert lin(out=buf) is buf and torch.equal(buf, want[5]) and norm(out=y)[0] is y and torch.equal(y, want[0])
+    # gradients are constants, and so is what was packed
+    grads = b.linear_act_bwd(res, x, w)
+    assert not any(t.requires_grad for t in grads) and not b.ckpt8_unpack(b.ckpt8_pack(x)).requires_grad
+
+
+def test_operators_inside_an_autograd_function():
+    b = B()
+    g = gen(52)
+
+    class Linear(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w, bias):
+            y, pre = b.linear_act(x, w, bias, act="silu", save_pre=True)
+            ctx.save_for_backward(x, w, pre)
+            return y
+
+        @staticmethod
+        def backward(ctx, dy):
+            x, w, pre = ctx.saved_tensors
+            return b.linear_act_bwd(dy, x, w, act="silu", pre=pre)
+    x, w, bias = rnd(g, 20, 32).requires_grad_(True), rnd(g, 24, 32).requires_grad_(True), rnd(g, 24).requires_grad_(True)
+    dy = rnd(g, 20, 24)
+    Linear.apply(x, w, bias).backward(dy)
+    pre = b.linear_act(x.detach(), w.detach(), bias.detach(), act="silu", save_pre=True)[1]
+    for a, t in zip((x, w, bias), b.linear_act_bwd(dy, x.detach(), w.detach(), act="silu", pre=pre)):
+        assert torch.equal(a.grad, t)
