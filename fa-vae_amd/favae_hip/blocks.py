@@ -18,6 +18,7 @@ autograd.Function.  With grad mode on and an input that requires a gradient, the
 `out` is refused.  What a *_bwd call or ckpt8_unpack returns is a constant.
 """
 import ctypes
+import math
 
 import torch
 
@@ -153,6 +154,22 @@ def _same_place(a, b):
     return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
 
 
+def _beside(a, b):
+    """Whether a and b, whose spans meet, are different columns of one buffer: modulo the largest pitch that all their strides but the last
+    are multiples of, the bytes of their rows do not meet."""
+    pitch, width = 0, []
+    for t in (a, b):
+        es, inner = t.element_size(), t.dim() - 1
+        for k in range(inner):
+            if t.shape[k] > 1:
+                pitch = math.gcd(pitch, t.stride(k) * es)
+        width.append(((t.shape[inner] - 1) * t.stride(inner) + 1) * es)
+    if pitch == 0:
+        return False
+    d = (b.data_ptr() - a.data_ptr()) % pitch
+    return width[0] <= d and d + width[1] <= pitch
+
+
 def _apart(out, name, ins, may_be=None):
     """`out` shares no memory with the inputs, but that it may be `may_be` itself."""
     lo, hi = _span(out)
@@ -160,7 +177,7 @@ def _apart(out, name, ins, may_be=None):
         if t is None or (t is may_be and _same_place(out, t)):
             continue
         a, b = _span(t)
-        if lo < b and a < hi:
+        if lo < b and a < hi and not _beside(out, t):
             raise ValueError("%s overlaps an input" % name)
 
 

@@ -133,3 +133,49 @@ def test_limits_are_checked_before_anything_is_launched():
     for text, call in calls.items():
         assert call() == -1 and text in L.last_error(), (text, L.last_error())
     assert r.favae_linear_act_bwd(p, 8, p, 8, None, 0, p, 8, None, 0, None, 0, 4, 8, 8, 0, p, 8, None, 8, L.BF16, None, p, big, L.BF16, None) == -2      # (a launch)
+
+
+def test_outputs_beside_an_input_in_one_buffer():
+    """Memory spans that meet without an element in common: columns of one buffer, and what only looks so."""
+    import random
+    b = _b()
+    big = torch.zeros(6, 5, 40)
+    x = big[:, :, :24]
+    apart = lambda out, *ins: b._apart(out, "out", ins)
+    for out in (big[:, :, 24:], big[:, :, 24:32], big[1:, :, 24:], big[:, 2:, 30:], big[::2, :, 24:], big[3, :, 24:]):
+        apart(out, x)
+        apart(x, out)
+    apart(torch.zeros(3, 8)[:, 4:], torch.zeros(3, 8))
+    rows = torch.zeros(64).as_strided((3, 8), (20, 1), 0)
+    apart(torch.zeros(0), rows)
+    for out in (big[:, :, 23:], big[:, :, 10:20], big[2:, :, 23:30], big.view(6, 200)[:, 20:50], big.view(-1)[24:60], big[..., ::2], big.transpose(1, 2)[:, 24:]):
+        with pytest.raises(ValueError, match="overlaps"):
+            apart(out, x)
+        with pytest.raises(ValueError, match="overlaps"):
+            apart(x, out)
+    # another pitch, another type's view, and a pitch that is no multiple
+    base = torch.zeros(400)
+    a = base.as_strided((8, 4), (10, 1), 0)
+    for out in (base.as_strided((4, 4), (15, 1), 5), base.as_strided((8, 4), (12, 1), 5), base.as_strided((8, 8), (10, 1), 4), base.as_strided((4, 2, 3), (20, 7, 1), 5)):
+        with pytest.raises(ValueError, match="overlaps"):
+            apart(out, a)
+    apart(base.as_strided((3, 2, 4), (40, 20, 1), 5), a)
+    apart(base.as_strided((4, 4), (20, 1), 5), a)
+    apart(base.view(torch.bfloat16).as_strided((8, 8), (20, 1), 10), a)
+    # never two tensors with an element in common
+    rng, taken = random.Random(1), 0
+    for _ in range(2000):
+        pitch = rng.randint(4, 9)
+        pair = []
+        for _ in range(2):
+            k, c = rng.choice([1, 1, 2]), rng.randint(1, 5)
+            sh, st = (rng.randint(1, 4), rng.randint(1, 4), c), (pitch * rng.randint(0, 3), pitch * k + rng.choice([0, 0, 0, 1]), 1)
+            pair.append(base.as_strided(sh, st, rng.randint(0, 2 * pitch)))
+        one, two = (set(torch.arange(400).as_strided(t.shape, t.stride(), t.storage_offset()).flatten().tolist()) for t in pair)
+        try:
+            apart(*pair)
+            taken += 1
+            assert not one & two
+        except ValueError:
+            pass
+    assert taken > 200

@@ -954,3 +954,20 @@ def test_operators_inside_an_autograd_function():
     pre = b.linear_act(x.detach(), w.detach(), bias.detach(), act="silu", save_pre=True)[1]
     for a, t in zip((x, w, bias), b.linear_act_bwd(dy, x.detach(), w.detach(), act="silu", pre=pre)):
         assert torch.equal(a.grad, t)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_outputs_into_other_columns_of_the_input_s_buffer(dtype):
+    b = B()
+    g = gen(61)
+    start = rnd(g, 4, 9, 80, dtype=dtype)
+    gamma, beta, w = rnd(g, 32), rnd(g, 32), rnd(g, 40, 32, dtype=dtype, scale=0.2)
+    for off in (32, 37):
+        big = start.clone()
+        y = b.group_norm_act(big[..., :32], 4, gamma, beta, act="silu", out=big[..., off:off + 32])[0]
+        assert torch.equal(y, b.group_norm_act(start[..., :32].clone(), 4, gamma, beta, act="silu", out=torch.empty_like(start)[..., off:off + 32])[0])
+        z = b.linear_act(big[..., :32], w, act="silu", out=big[..., off:off + 40])
+        assert torch.equal(z, b.linear_act(start[..., :32], w, act="silu"))
+        ck = b.ckpt8_pack(start[..., :32])
+        b.ckpt8_unpack(ck, out=big[..., off:off + 32])
+        assert torch.equal(big[..., :32], start[..., :32]) and torch.equal(big[..., off + 40:], start[..., off + 40:])
