@@ -545,6 +545,18 @@ extern "C" size_t favae_gn_act_scratch(long long N, long long S, int C, int G, i
     return need * sizeof(float2);
 }
 
+extern "C" int favae_debug_gn_act_plan(long long N, long long S, int C, int G, int backward, int either, int dtype, int* out12) {
+    const int rc = gn_sizes("favae_debug_gn_act_plan", N, S, C, G, FAVAE_ACT_NONE, dtype);
+    if (rc != FAVAE_OK) return rc;
+    FAVAE_CHECK_ARG(out12, "favae_debug_gn_act_plan: null pointer");
+    GnP p = {};
+    p.N = (int)N; p.S = (int)S; p.C = C; p.G = G; p.Cg = C / G;
+    const GnPlan pl = gn_plan(p, dtype == FAVAE_F32 ? 4 : 2, backward != 0, !backward && either && C % CK_BLOCK == 0, backward && either);
+    const int v[12] = {pl.form, pl.items, pl.gpv, pl.tail, p.pieces, p.NSUB, p.P, p.ncb, p.nchunk, p.CB, (int)std::min<long long>(pl.rows, 0x7fffffff), ck_in_kernel(p, pl)};
+    std::copy(v, v + 12, out12);
+    return FAVAE_OK;
+}
+
 extern "C" int favae_gn_act_fwd(const void* x, long long xn, long long xs, long long N, long long S, int C, int G, const float* gamma,
                                 const float* beta, float eps, int act, void* y, long long yn, long long ys, float* mean, float* rstd,
                                 void* q, void* e, void* scratch, size_t scratch_bytes, int dtype, void* stream) {

@@ -621,6 +621,11 @@ size_t favae_gn_act_scratch(long long N, long long S, int C, int G, int backward
 int favae_gn_act_fwd(const void* x, long long xn, long long xs, long long N, long long S, int C, int G, const float* gamma,
                      const float* beta, float eps, int act, void* y, long long yn, long long ys, float* mean, float* rstd, void* q, void* e,
                      void* scratch, size_t scratch_bytes, int dtype, void* stream);
+/* Test hook: what the rules choose for a shape.  either: a checkpoint is wanted (forward), all tensors have 16-byte aligned rows (backward).
+ * form (0 wave, 1 piped, 2 held, 3 chunked), vectors a thread, groups a vector may touch, runs that end inside a vector, pieces of a group,
+ * samples of a workgroup, positions side by side, channel blocks, chunks, channels of a block, rows of column sums, the kernel may write a
+ * checkpoint. */
+int favae_debug_gn_act_plan(long long N, long long S, int C, int G, int backward, int either, int dtype, int* out12);
 /* Its gradients from dy and either x or its checkpoint (q, e as above with R = N * S contiguous rows; mean and rstd stay those of the
  * forward pass): dx (dtype; may be dy), dgamma and dbeta [C] fp32 (NULL to skip).  Deterministic. */
 int favae_gn_act_bwd(const void* dy, long long dn, long long ds, const void* x, long long xn, long long xs, const void* q, const void* e,

@@ -179,3 +179,66 @@ def test_outputs_beside_an_input_in_one_buffer():
         except ValueError:
             pass
     assert taken > 200
+
+
+def norm_form(n, s, c, g, backward, dtype, even=1):
+    """(form, vectors a thread up to the kernel's own number, groups a vector may touch, runs that end inside a vector), and what is ragged about it."""
+    import ctypes
+    from favae_hip import blocks as b
+    from favae_hip import lib as L
+    v = (ctypes.c_int * 12)()
+    assert b._raw.favae_debug_gn_act_plan(ctypes.c_longlong(n), ctypes.c_longlong(s), c, g, backward, even if backward else 0, dtype, v) == 0
+    form, items, gpv, tail, pieces, nsub, p, ncb, nchunk, cb, rows, _ = v
+    name, vec = ("wave", "piped", "held", "chunked")[form], 4 if dtype == L.F32 else 8
+    sizes = {"wave": (1, 2, 4, 8), "held": (4, 8, 12, 16) if backward else (4, 16)}.get(name, (1 << 30,))
+    if name in ("held", "chunked"):
+        gpv = gpv if gpv == 1 else vec
+        tail = tail if gpv > 1 else 0
+    ragged = {k for k, is_so in (("channels", c % cb), ("positions", p and s % p), ("samples", rows and n > rows and n % rows)) if is_so}
+    return (name, min(t for t in sizes if t >= items) if name in ("wave", "held") else 0, gpv, tail), ragged
+
+
+def test_every_form_of_the_norm_has_a_shape_among_the_gpu_tests():
+    import test_gpu_blocks as t
+    from favae_hip import lib as L
+    for dtype, vec in ((L.F32, 4), (L.BF16, 8)):
+        gpvs = [1, 2, 4, 8][:vec.bit_length()]
+        for backward in (0, 1):
+            got = [norm_form(*shape, backward, dtype) for shape in t.GN_FORMS]
+            kinds = [(1, 0), (vec, 0), (vec, 1)]
+            want = {("wave", i, k, 0) for i in (1, 2, 4, 8) for k in gpvs} | {("chunked", 0) + k for k in kinds}
+            want |= {("held", i) + k for i in ((4, 8, 12, 16) if backward else (4, 16)) for k in kinds}
+            if backward:
+                want |= {("piped", 0, k, 0) for k in gpvs}
+            assert want == {k for k, _ in got}, want ^ {k for k, _ in got}
+            for form in ("wave", "held", "chunked") + (("piped",) if backward else ()):
+                ragged = set().union(*(r for (f, *_), r in got if f == form))
+                assert {"positions", "channels"} <= ragged and (form not in ("piped", "wave") or not backward or "samples" in ragged), (form, ragged)
+
+
+def test_shapes_of_the_piped_backward_are_piped():
+    import test_gpu_blocks as t
+    from favae_hip import lib as L
+    for mark in t.test_group_norm_piped_backward.pytestmark:
+        for dtype, *shape in mark.args[1]:
+            (form, *_), _ = norm_form(*shape, 1, L.F32 if dtype == torch.float32 else L.BF16)
+            assert form == "piped", shape
+
+
+def test_checkpoints_are_written_by_the_norm_where_its_runs_start_on_their_blocks():
+    """Whatever the plan, a run of channels that a kernel packs starts and ends on a block of 32."""
+    import ctypes
+    import random
+    from favae_hip import blocks as b
+    rng, v, seen = random.Random(3), (ctypes.c_int * 12)(), set()
+    for _ in range(20000):
+        cg = rng.choice([1, 2, 4, 8, 12, 16, 24, 32, 40, 64, 2056, 2080, 4104, 4128, 8192, rng.randint(1, 9000)])
+        g = rng.choice([1, 2, 4, 8, 32, rng.randint(1, 40)])
+        dtype, c = rng.randint(0, 1), cg * g
+        assert b._raw.favae_debug_gn_act_plan(ctypes.c_longlong(rng.choice([1, 3, 64, 700])), ctypes.c_longlong(rng.choice([0, 1, 5, 64, 1000, 5000])), c, g, 0, 1, dtype, v) == 0
+        form, pieces, cb, packs = v[0], v[4], v[9], v[11]
+        if packs:
+            starts = [k * cg + j * cb for k in range(g) for j in range(pieces)] if pieces > 1 else range(0, c, cb)
+            assert c % 32 == 0 and all(t % 32 == 0 for t in starts), (cg, g, pieces, cb)
+        seen.add((bool(packs), pieces > 1, c % 32 == 0))
+    assert {(True, True, True), (False, True, True), (True, False, True)} <= seen

@@ -971,3 +971,81 @@ def test_outputs_into_other_columns_of_the_input_s_buffer(dtype):
         ck = b.ckpt8_pack(start[..., :32])
         b.ckpt8_unpack(ck, out=big[..., off:off + 32])
         assert torch.equal(big[..., :32], start[..., :32]) and torch.equal(big[..., off + 40:], start[..., off + 40:])
+
+
+# ---- every form of the norm --------------------------------------------------------------------------------------------------
+# Each kernel variant that the rules choose between (test_cpu_blocks.py holds the list to it), in both types: wave with 1, 2, 4, 8 vectors a lane and 1 to
+# 8 groups a vector; held with up to 4, 8, 12, 16 vectors a thread; piped with 1 to 8 groups a vector; chunked; last channel blocks that are partial,
+# positions that are no multiple of what a workgroup takes at once, samples that workgroups take unequal numbers of.
+GN_FORMS = [(1, 1, 24, 12), (1, 1, 24, 6), (1, 5, 40, 5), (1, 9, 40, 20), (1, 5, 72, 9), (1, 11, 432, 9), (1, 1, 12, 12), (1, 131, 24, 12), (1, 140, 24, 3),
+            (1, 17, 16, 16), (1, 33, 16, 16), (1, 348, 33, 11), (1, 151, 16, 16), (1, 518, 8, 8), (1, 5, 40, 20), (1, 5, 80, 20), (1, 9, 72, 9), (1, 17, 40, 20),
+            (1, 9, 80, 20), (1, 344, 72, 3), (1, 144, 24, 6), (1, 44, 60, 20), (1, 1031, 40, 20), (1, 33, 32, 32), (1, 2140, 1, 1), (1, 237, 35, 5),
+            (72, 2061, 1, 1), (1, 9, 20, 20), (1, 17, 20, 20), (1, 131, 12, 12), (1, 132, 12, 6), (1, 142, 12, 3), (1, 25, 240, 20), (72, 1313, 1, 1),
+            (34, 1049, 44, 11), (1, 698, 35, 5), (33, 85, 216, 9), (25, 1055, 64, 64), (1, 513, 96, 3), (20, 1698, 72, 9), (1, 1067, 80, 20), (32, 1257, 15, 3),
+            (12, 205, 320, 64), (306, 281, 40, 20), (297, 284, 40, 5), (32, 426, 35, 5), (98, 1549, 16, 16), (558, 291, 16, 16), (21, 1119, 72, 9), (37, 693, 35, 5),
+            (236, 261, 80, 20), (68, 102, 100, 20), (20, 1780, 36, 9), (275, 279, 20, 20), (126, 85, 240, 20), (266, 211, 60, 20), (177, 303, 100, 20),
+            (4999, 2, 32, 8)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,S,C,G", GN_FORMS)
+def test_group_norm_every_form(N, S, C, G, dtype):
+    b = B()
+    g = gen(N, S, C, G, 5)
+    x = rnd(g, N, S, C, dtype=dtype, scale=1.7, shift=3.0)
+    gamma, beta = rnd(g, C, scale=0.3, shift=1.0), rnd(g, C, scale=0.5)
+    for act in ACTS:
+        want, m, r, z, z_err, m_err, r_rel = gn_ref(x, gamma, beta, G, act)
+        for ckpt in (False, True):
+            y, mean, rstd, *ck = b.group_norm_act(x, G, gamma, beta, act=act, ckpt=ckpt)
+            close(mean, m, m_err)
+            close(rstd, r, r * r_rel)
+            close(y, want, SLOPE * z_err + (z.abs() + 8) * 4 * U * want.abs())
+            if ckpt:
+                ref = b.ckpt8_pack(x)
+                assert torch.equal(ck[0].q, ref.q) and torch.equal(ck[0].e, ref.e)
+    for act in ACTS:
+        for ck in (False, True):
+            gn_bwd_check(b, N, S, C, G, dtype, act, ck, gen(N, S, C, G, 6 + ck))
+
+
+# the piped backward: 1, 2, 4 and 8 groups a vector, 8 vectors a thread, unequal numbers of samples
+@pytest.mark.parametrize("dtype,N,S,C,G", [(F32, 275, 279, 20, 20), (F32, 306, 281, 40, 20), (F32, 297, 284, 40, 5), (F32, 600, 101, 128, 1), (F32, 300, 500, 64, 8),
+                                           (BF16, 558, 291, 16, 16), (BF16, 306, 281, 40, 20), (BF16, 236, 261, 80, 20), (BF16, 297, 284, 40, 5),
+                                           (BF16, 600, 101, 256, 1), (BF16, 300, 1000, 64, 8)])
+def test_group_norm_piped_backward(dtype, N, S, C, G):
+    b = B()
+    g = gen(N, S, C, G, 8)
+    pad = 16 // torch.finfo(dtype).bits * 8                    # elements of 16 bytes
+    wide = rnd(g, N, S + 1, C + pad, dtype=dtype, scale=1.7, shift=3.0)
+    x, dy = wide[:, :S, :C], rnd(g, N, S + 2, C + 2 * pad, dtype=dtype)[:, 1:S + 1, pad:C + pad]
+    gamma, beta = rnd(g, C, scale=0.3, shift=1.0), rnd(g, C, scale=0.5)
+    mean, rstd = b.group_norm_act(x, G, gamma, beta, act="silu")[1:]
+    ck = b.ckpt8_pack(x.contiguous())
+    for src in (x, ck):
+        one = b.group_norm_act_bwd(dy.contiguous(), x.contiguous() if src is x else ck, G, gamma, beta, mean, rstd, act="silu")
+        # strided rows, the gradient over dy, into rows with others between them: the same kernel, the same bits
+        buf = torch.full((N, S + 1, C + pad), 7.0, dtype=dtype, device=DEV)
+        for out in (None, dy.clone(), buf[:, :S, :C]):
+            d = out if out is not None and out.is_contiguous() else dy
+            two = b.group_norm_act_bwd(d, src, G, gamma, beta, mean, rstd, act="silu", out=out)
+            assert out is None or two[0] is out
+            for a, t in zip(two, one):
+                assert torch.equal(a, t)
+        assert (buf[:, S:] == 7).all() and (buf[..., C:] == 7).all()
+    # a fault stays in its sample and group, and in the groups that share its block of a checkpoint
+    cg = C // G
+    x = x.contiguous()
+    for n, i, c in ((N - 1, S - 1, C - 1), (N // 2, 0, 0), (N // 3, S // 2, (G // 2) * cg)):
+        x[n, i, c] = float("nan")
+    ck = b.ckpt8_pack(x)
+    mean, rstd = b.group_norm_act(x, G, gamma, beta, act="silu")[1:]
+    assert torch.isnan(mean).sum() == 3
+    for src, v in ((x, x), (ck, b.ckpt8_unpack(ck))):
+        dx, dg, db = b.group_norm_act_bwd(dy, src, G, gamma, beta, mean, rstd, act="silu")
+        z = torch.isnan(v) | torch.isnan(mean).repeat_interleave(cg, 1)[:, None, :]
+        bad = z.reshape(N, S, G, cg).any(3).any(1).repeat_interleave(cg, 1)[:, None, :].expand(N, S, C)
+        assert torch.isnan(dx[bad]).all() and torch.isfinite(dx[~bad]).all()
+        cols = z.any(0).any(0)
+        for t in (dg, db):
+            assert torch.isnan(t[cols]).all() and torch.isfinite(t[~cols]).all()
