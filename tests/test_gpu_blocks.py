@@ -1049,3 +1049,39 @@ def test_group_norm_piped_backward(dtype, N, S, C, G):
         cols = z.any(0).any(0)
         for t in (dg, db):
             assert torch.isnan(t[cols]).all() and torch.isfinite(t[~cols]).all()
+
+
+# 128-wide fp32 tiles alone (y; dx; dw), and in bf16 128-wide ones split (dw), 64-wide ones split with two stages (dx; y)
+@pytest.mark.parametrize("M,N,K,dtype", [(4311, 1080, 4, F32), (2638, 4, 1657, F32), (19, 1418, 2903, F32), (5201, 73, 2073, BF16), (1484, 2568, 5, BF16),
+                                         (2638, 4, 1657, BF16)])
+def test_linear_act_tiles_alone_and_split(M, N, K, dtype):
+    b = B()
+    g = gen(M, N, K, 13)
+    x, w = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype, scale=K ** -0.5)
+    bias, res = rnd(g, N, scale=0.3), rnd(g, M, N, dtype=dtype)
+    y, pre = b.linear_act(x, w, bias, act="gelu_tanh", residual=res, save_pre=True)
+    u = x.double() @ w.double().t() + bias.double()
+    u_err = lin_bound(x, w, bias)
+    v = act64(u, "gelu_tanh")[0]
+    err = SLOPE * u_err + (u.abs() + 8) * 4 * U * v.abs()
+    v = v + res.double()
+    close(pre, u, u_err)
+    close(y, v, err + U * v.abs())
+    for ck in (False, True):
+        lin_bwd_check(b, M, N, K, dtype, "silu", ck, gen(M, N, K, 14 + ck))
+    lin_bwd_check(b, M, N, K, dtype, "none", False, gen(M, N, K, 16), F32)
+
+
+@pytest.mark.parametrize("M,N,K", [(65536, 1024, 1024), (16384, 4096, 1024)])
+def test_large_product_gradients_repeat_bit_for_bit(M, N, K):
+    """Ring of tiles, split reductions and their joins at full size, other work between the runs."""
+    b = B()
+    g = gen(M, N, K, 17)
+    dy, x, pre, w = rnd(g, M, N, dtype=BF16), rnd(g, M, K, dtype=BF16), rnd(g, M, N, dtype=BF16), rnd(g, N, K, dtype=BF16, scale=K ** -0.5)
+    x8, pre8 = b.ckpt8_pack(x), b.ckpt8_pack(pre)
+    for src, p in ((x, pre), (x8, pre8)):
+        first = b.linear_act_bwd(dy, src, w, act="gelu_tanh", pre=p)
+        for _ in range(4):
+            b.linear_act(x, w, act="silu")
+            for a, t in zip(b.linear_act_bwd(dy, src, w, act="gelu_tanh", pre=p), first):
+                assert torch.equal(a, t)
