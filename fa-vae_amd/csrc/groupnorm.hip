@@ -461,8 +461,10 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
     }
     const long long held_blocks = cdivll(p.N, p.NSUB) * p.ncb;
     // held with fewer workgroups than CUs, and chunked: 64 of them (8 x 4096 x 64 fp32, 16 x 4096 x 64 bf16) 18.1, 17.7 us and 14.4, 14.1; 192 (24 x 4096 x 64
-    // fp32) 23.3 and 28.8; 64 and 100 off the grid (64 x 1000 x 33, 100 x 1500 x 15 bf16) 14.0, 13.6 and 19.9, 18.2
-    if (p.pieces == 1 && cdiv(S, p.P) <= ITEMS_MAX && (held_blocks >= (ckpt ? 256 : pl.tail ? 64 : 96) || cdiv(S, p.P) <= 4)) {
+    // fp32) 23.3 and 28.8; 64 and 100 off the grid (64 x 1000 x 33, 100 x 1500 x 15 bf16) 14.0, 13.6 and 19.9, 18.2.  With a checkpoint, whose runs are 32
+    // channels wide at least (halves()) and so twice as long a thread: 96 (48 x 2048 x 64 bf16) 23.9 and 20.0, 128 (64 x 1024 x 64 bf16, fp32) 16.7, 25.9 and
+    // 15.6, 22.6; 192 (24 x 512 x 256 fp32) 16.8 and 20.2, 200 (200 x 1500 x 32 bf16) 23.2 and 28.9
+    if (p.pieces == 1 && cdiv(S, p.P) <= ITEMS_MAX && (held_blocks >= (ckpt ? 160 : pl.tail ? 64 : 96) || cdiv(S, p.P) <= 4)) {
         pl.form = GN_HELD;
         pl.items = cdiv(S, p.P);
         // backward: a workgroup goes over several samples and leaves one row of column sums

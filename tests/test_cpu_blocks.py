@@ -242,3 +242,16 @@ def test_checkpoints_are_written_by_the_norm_where_its_runs_start_on_their_block
             assert c % 32 == 0 and all(t % 32 == 0 for t in starts), (cg, g, pieces, cb)
         seen.add((bool(packs), pieces > 1, c % 32 == 0))
     assert {(True, True, True), (False, True, True), (True, False, True)} <= seen
+
+
+def test_forward_form_with_a_checkpoint():
+    """Held from 160 workgroups on, chunked below, where a thread would have more than 4 vectors; without a checkpoint from 96 on."""
+    import ctypes
+    from favae_hip import blocks as b
+    from favae_hip import lib as L
+    v = (ctypes.c_int * 12)()
+    for shape, dtype, ckpt, form in (((64, 1024, 64, 8), L.BF16, 1, 3), ((48, 2048, 64, 8), L.BF16, 1, 3), ((200, 1500, 32, 4), L.BF16, 1, 2), ((24, 512, 256, 32), L.F32, 1, 2),
+                                     ((64, 1024, 64, 8), L.BF16, 0, 2), ((8, 4096, 64, 8), L.BF16, 0, 3)):
+        n, s, c, g = shape
+        assert b._raw.favae_debug_gn_act_plan(ctypes.c_longlong(n), ctypes.c_longlong(s), c, g, 0, ckpt, dtype, v) == 0
+        assert v[0] == form and (not ckpt or v[11]), (shape, ckpt, list(v))

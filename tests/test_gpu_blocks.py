@@ -1085,3 +1085,19 @@ def test_large_product_gradients_repeat_bit_for_bit(M, N, K):
             b.linear_act(x, w, act="silu")
             for a, t in zip(b.linear_act_bwd(dy, src, w, act="gelu_tanh", pre=p), first):
                 assert torch.equal(a, t)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,S,C,G", [(200, 1500, 32, 4), (24, 512, 256, 32), (48, 2048, 64, 8)])
+def test_group_norm_checkpoint_on_either_side_of_its_limit(N, S, C, G, dtype):
+    b = B()
+    g = gen(N, S, C, G, 18)
+    x = rnd(g, N, S, C, dtype=dtype, scale=1.7, shift=3.0)
+    gamma, beta = rnd(g, C, scale=0.3, shift=1.0), rnd(g, C, scale=0.5)
+    y, mean, rstd, ck = b.group_norm_act(x, G, gamma, beta, act="silu", ckpt=True)
+    want, m, r, z, z_err, m_err, r_rel = gn_ref(x, gamma, beta, G, "silu")
+    close(mean, m, m_err)
+    close(rstd, r, r * r_rel)
+    close(y, want, SLOPE * z_err + (z.abs() + 8) * 4 * U * want.abs())
+    ref = b.ckpt8_pack(x)
+    assert torch.equal(ck.q, ref.q) and torch.equal(ck.e, ref.e)
