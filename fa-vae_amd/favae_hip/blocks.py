@@ -303,7 +303,8 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
     """y = act(gamma * (x - mean) * rstd + beta) over x [N, ..., C], channels last, per sample and group of C / groups neighbouring
     channels.  Returns y, mean [N, groups], rstd [N, groups] (fp32) and, with ckpt, x as a Ckpt8.  A sample of no positions has mean
     0 and variance 0.  out may be x (without ckpt)."""
-    n, s, c = _gn_sizes(x.shape, groups)
+    shape = x.shape
+    n, s, c = _gn_sizes(shape, groups)
     code, a, dev = _code(x, "x"), _act(act), x.device
     if dev.type != "cuda":
         _on(dev)
@@ -316,9 +317,9 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
         _no_out(out)
     xn, xs = (s * c, c) if x.is_contiguous() else _maps(x, "x")
     if out is None:
-        y, yn, ys = x.new_empty(x.shape), s * c, c
+        y, yn, ys = x.new_empty(shape), s * c, c
     else:
-        y = _out(out, "out", x, x.shape, x.dtype, (x, gamma, beta), None if ckpt else x)
+        y = _out(out, "out", x, shape, x.dtype, (x, gamma, beta), None if ckpt else x)
         yn, ys = _maps(y, "out")
     mean, rstd = gamma.new_empty((2, n, groups)).unbind()
     ck = _new_ckpt(x) if ckpt else None
@@ -373,18 +374,20 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
     """act(x w^T + bias) + residual: x [..., K], w [N, K], bias fp32 [N], residual and the result [..., N] of x's type, rows of any
     stride.  Sums, bias, activation and residual are fp32, the result is rounded once.  With save_pre returns (y, pre), pre = x w^T +
     bias rounded to x's type, for linear_act_bwd.  out may be residual."""
-    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
-        raise ValueError("x [..., K] and w [N, K], not %s and %s" % (list(x.shape), list(w.shape)))
+    xsh, wsh = x.shape, w.shape
+    if len(wsh) != 2 or not xsh or xsh[-1] != wsh[1]:
+        raise ValueError("x [..., K] and w [N, K], not %s and %s" % (list(xsh), list(wsh)))
     code, a, dev = _code(x, "x"), _act(act), x.device
     if w.dtype != x.dtype:
         raise TypeError("w: %s, as x" % x.dtype)
     if dev.type != "cuda" or w.device != dev or residual is not None:
         _on(dev, w=w, residual=residual)
-    n, k = w.shape
+    n, k = wsh
+    lead = xsh[:-1]
     m = 1
-    for v in x.shape[:-1]:
+    for v in lead:
         m *= v
-    shape = x.shape[:-1] + (n,)
+    shape = lead + (n,)
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("residual: %s %s" % (x.dtype, list(shape)))
     bp = None if bias is None else _vec(bias, n, "bias", dev)
