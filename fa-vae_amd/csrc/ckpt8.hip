@@ -1,7 +1,7 @@
 // Activation checkpoints in 8 bits: pack and unpack.
 //
 // q [R][C] int8 and one code byte per 32 channels of a row; the format is defined in act8.h.  Both directions are one pass over the
-// data and bound by memory: pack reads 2 or 4 bytes a value and writes 33/32, unpack the reverse.  65536 x 1024 bf16 there and back 74 us, 5.4 TB/s.
+// data and bound by memory: pack reads 2 or 4 bytes a value and writes 33/32, unpack the reverse.  65536 x 1024 bf16 there and back 75 us, 5.4 TB/s.
 #include "act8.h"
 
 namespace {

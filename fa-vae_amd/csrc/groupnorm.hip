@@ -11,8 +11,8 @@
 //   wave     the positions of a run of groups fit a wave's registers (up to 8 vectors of 16 bytes a lane; small maps): every wave works for
 //            itself, sums cross lanes by shuffles, there is no LDS and no barrier.
 //   held     they fit a workgroup's registers (up to 16 vectors a thread): the input is read once, sums meet in LDS.
-//   piped    (backward, up to 8 vectors a thread, 16-byte aligned tensors, enough samples) the same, and while the workgroup works on one sample
-//            the next is on its way into LDS, so that memory does not idle while a CU computes: 512 x 1024 x 128 bf16 silu 156 -> 97 us.
+//   piped    (backward, up to 8 vectors a thread, 16-byte aligned tensors, enough samples) the same, and during the first pass over one sample
+//            the next is on its way into LDS, so that memory does not idle while a CU computes: 512 x 1024 x 128 bf16 silu 156 -> 95 us.
 //            (Forward two workgroups share a CU and cover each other: 68 us held, 81 piped, not kept.)
 //   chunked  they do not, or there are too few groups to fill the chip: a first launch leaves the partial sums of each chunk of positions,
 //            a later one joins them and makes the second pass over the data.
@@ -390,7 +390,7 @@ GnPlan gn_plan(GnP& p, int es, bool backward, bool ckpt, bool even) {
         while (lv > 4 && cdiv(S, GTP / lv) > 4 && (long long)p.N * cdiv(p.C, lv * vec) < 1024 && fits(lv / 2)) lv /= 2;
         if (lv > 1 && (long long)p.N * cdiv(p.C, lv * vec) >= 512) {
             pl.form = GN_PIPED;
-            pl.gpv = gs ? 1 : vec % p.Cg == 0 ? vec / p.Cg : vec;
+            pl.gpv = gs ? 1 : vec / p.Cg;                            // (unit is vec times a power of two: so is Cg, or it divides vec)
             p.LV = lv; p.P = GTP / lv; p.CB = lv * vec; p.ncb = cdiv(p.C, p.CB);
             pl.threads = GTP;
             pl.rows = std::min<long long>(p.N, std::max(1, 256 / p.ncb));

@@ -282,7 +282,9 @@ template <int M, int R> __device__ __forceinline__ void slice_order(const int v)
 // there every wave has the fragments of the rest of tile t in registers, so that its slot takes the DMA of tile t + STAGES, and tile t + 1 is
 // waited for, whose first fragments are read beside the last slice's MFMAs.  So a load has STAGES - 1 steps to arrive, and no MFMA waits for LDS
 // behind a barrier.  Bound by the matrix units and, close behind, LDS (a wave's 128 x 64 tile reads 6 fragments for 8 MFMAs): 16384 x 4096 x 4096
-// bf16 430 us, 1280 TFLOP/s; 4096 x 4096 x 4096 fp32 940 us, 146.
+// bf16 418 to 430 us, 1280 to 1315 TFLOP/s; 4096 x 4096 x 4096 fp32 940 us, 146.
+// (fp32 with a row operand: the two 16-byte LDS loads of a fragment are no builtins with `restrict`, and the compiler waits for every DMA under way
+// before them, so that a load has part of a step to arrive.)
 template <class T, class OT, int TI, int TJ, int WI, int WJ, int BKE, int STAGES, bool PCM, bool QCM, int WPE, int B>
 __global__ __launch_bounds__(64 * WI * WJ, WPE) void gemm_dma_kernel(const GemmP p) {
     constexpr int NT = 64 * WI * WJ;
@@ -478,8 +480,10 @@ template <class T> __global__ __launch_bounds__(256) void pack_kernel(const Pack
 
 // ---- du = dy act'(u) and the column sums of du ---------------------------------------------------------------------------
 // A block takes 64 vectors of columns of a run of rows, 4 rows at a time; column sums (fp32) of the unrounded du go to part[run][N].  du is
-// rounded to T, the type of the matrix operands, and written with rows of ldu elements, zero past N.  Bound by memory: 65536 x 1024 bf16 gelu
-// 81 us, 5.0 TB/s; 16384 x 4096 from a checkpoint 67 us.
+// rounded to T, since the matrix units read operands of that type, and written with rows of ldu elements, zero past N.  For bf16 that makes the error
+// of dx and dw 0.0023 of their norm, 0.0017 with an unrounded du (the rounding of the result), at 65536 x 1024 x 1024; a du of two bf16 parts would
+// take both products twice, 270 us more.  Against the formula with du rounded once, 0.03 to 0.2 % of the values are one step off.  Bound by memory: 65536 x 1024 bf16 gelu
+// 81 to 88 us, 4.6 to 5.0 TB/s; 16384 x 4096 from a checkpoint 67 to 69 us.
 struct DuP {
     const void* dy; long long lddy;
     const void* pre; long long ldpre;
@@ -614,7 +618,7 @@ template <class T, class OT, bool PCM, bool QCM> int gemm_run(GemmP p, bool odd,
     // steps of 128 bytes and two stages; one 64-byte steps and four where neither operand's steps leave half lines behind (x w^T 16384 x 4096 x
     // 4096: 430 us, 452 with 64-byte steps; du w 423, 434; du^T x 409, 406; with 1024 rows and columns over 65536: 136, 131) and in SMALL, for
     // loads that are longer under way (2048 x 2048 x 2048: 22.3 us, 26).  TINY with a CU to itself: four stages, where two leave too little of w
-    // under way (64 x 4096 x 4096 13 us, 15.5; fp32 33 either way); with neighbours 30 us, 34 (du w 2048 x 2048 x 2048) the other way round.
+    // under way (64 x 4096 x 4096 13 us, 15.5; fp32 33 either way, for the wait named at gemm_dma_kernel); with neighbours 30 us, 34 (du w 2048 x 2048 x 2048) the other way round.
     if constexpr (es == 4) {
         if (pl.tile == TINY && odd) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2, 4>(p, blocks, st);
         else if (pl.tile == TINY) gemm_launch<T, OT, 64, 64, 2, 2, 32, 2, PCM, QCM, 2>(p, blocks, st);

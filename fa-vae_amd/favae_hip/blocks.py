@@ -421,8 +421,8 @@ _ALL = ("x", "w", "b")
 
 def linear_act_bwd(dy, x, w, act="none", pre=None, need=_ALL, dw=None):
     """Gradients of linear_act: (dx, dw, db), None for what `need` leaves out.  x and pre: tensors or Ckpt8; pre is needed unless act
-    is "none".  dx [..., K] is of dy's type, dw [N, K] of w's type or, into a float32 `dw`, unrounded, db fp32 [N].  The gradient of
-    the residual is dy."""
+    is "none".  dx [..., K] is of dy's type, dw [N, K] of w's type or, into a float32 `dw`, as it was summed, db fp32 [N].  Both products
+    read du = dy act'(pre) rounded once to dy's type (db sums it unrounded).  The gradient of the residual is dy."""
     code, a, dev = _code(dy, "dy"), _act(act), dy.device
     if w.dim() != 2 or dy.dim() < 1 or dy.shape[-1] != w.shape[0] or x.shape != dy.shape[:-1] + (w.shape[1],):
         raise ValueError("dy [..., N], x [..., K], w [N, K], not %s, %s, %s" % (list(dy.shape), list(x.shape), list(w.shape)))
