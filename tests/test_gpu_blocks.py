@@ -1101,3 +1101,35 @@ def test_group_norm_checkpoint_on_either_side_of_its_limit(N, S, C, G, dtype):
     close(y, want, SLOPE * z_err + (z.abs() + 8) * 4 * U * want.abs())
     ref = b.ckpt8_pack(x)
     assert torch.equal(ck.q, ref.q) and torch.equal(ck.e, ref.e)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,S,C,G", [(64, 1024, 64, 8), (200, 1500, 32, 4), (3, 64, 64, 8), (2, 16, 16416, 4), (5, 195, 210, 30), (2, 4096, 64, 16), (300, 500, 64, 8),
+                                     (1, 20000, 33, 3)])
+def test_group_norm_scratch_with_a_checkpoint_and_with_odd_rows(N, S, C, G, dtype):
+    """As above, for the forward pass with a checkpoint and for rows that are not 16-byte aligned, whose forms differ; the checkpoint's own ends too."""
+    from favae_hip import lib as L
+    raw = B()._raw
+    g = gen(N, S, C, G, 79)
+    code = L.F32 if dtype == F32 else L.BF16
+    nb = (C + 31) // 32
+    st = torch.cuda.current_stream().cuda_stream
+    gamma, beta = rnd(g, C), rnd(g, C)
+    for lead in (0, 1):                                        # elements before the first
+        x, dy, y = (rnd(g, N * S * C + 1, dtype=dtype)[lead:lead + N * S * C] for _ in range(3))
+        stat, grads = torch.empty(2, N, G, device=DEV), torch.empty(2, C, device=DEV)
+        q, e = torch.full((N * S * C + 64,), 9, dtype=torch.int8, device=DEV), torch.full((N * S * nb + 64,), 9, dtype=torch.uint8, device=DEV)
+        for back in (0, 1):
+            n = raw.favae_gn_act_scratch(N, S, C, G, back, code)
+            buf = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+            p = buf.data_ptr() if n else None
+            if back:
+                rc = raw.favae_gn_act_bwd(dy.data_ptr(), S * C, C, x.data_ptr(), S * C, C, None, None, N, S, C, G, gamma.data_ptr(), beta.data_ptr(),
+                                          stat[0].data_ptr(), stat[1].data_ptr(), 2, y.data_ptr(), S * C, C, grads[0].data_ptr(), grads[1].data_ptr(), p, n, code, st)
+            else:
+                rc = raw.favae_gn_act_fwd(x.data_ptr(), S * C, C, N, S, C, G, gamma.data_ptr(), beta.data_ptr(), 1e-5, 2, y.data_ptr(), S * C, C,
+                                          stat[0].data_ptr(), stat[1].data_ptr(), q.data_ptr(), e.data_ptr(), p, n, code, st)
+            L.check(rc)
+            assert (buf[n:] == 0xA5).all() and (q[N * S * C:] == 9).all() and (e[N * S * nb:] == 9).all()
+        ref = B().ckpt8_pack(x.view(N * S, C))
+        assert torch.equal(q[:N * S * C].view(N * S, C), ref.q) and torch.equal(e[:N * S * nb].view(N * S, nb), ref.e)
