@@ -207,12 +207,12 @@ def _no_out(out):
         raise ValueError("out: takes no part in autograd, and an input requires a gradient (call under torch.no_grad())")
 
 
-def _no_graph(name, outs, *ins):
-    """The outputs, with a node of autograd that raises: to be differentiated they would have to come from a graph, and there is none."""
-    leaf = next(t for t in ins if t is not None and t.requires_grad)
+def _no_graph(name, *outs):
+    """The outputs, with a node of autograd that raises: to be differentiated they would have to come from a graph, and there is none.  The node
+    hangs on a leaf of its own, so that an output that lives on keeps nothing of the caller's."""
     node = torch._C._functions.DelayedError("%s leaves no autograd graph: its gradients are %s_bwd's (call both under torch.no_grad(), or from an "
                                             "autograd.Function)" % (name, name), len(outs) + 1)
-    return node(*outs, leaf)[:-1]
+    return node(*outs, torch.empty(0, device="cpu", requires_grad=True))[:-1]
 
 
 _grad_mode = torch.is_grad_enabled
@@ -329,7 +329,7 @@ def group_norm_act(x, groups, gamma, beta, act="none", eps=1e-5, ckpt=False, out
         _call(dev, _raw.favae_gn_act_fwd, x.data_ptr(), xn, xs, n, s, c, groups, g, b, eps, a, y.data_ptr(), yn, ys, mean.data_ptr(),
               rstd.data_ptr(), ck.q.data_ptr() if ckpt else None, ck.e.data_ptr() if ckpt else None, _ptr(ws), nbytes, code)
     if cut:
-        y, mean, rstd = _no_graph("group_norm_act", (y, mean, rstd), x, gamma, beta)
+        y, mean, rstd = _no_graph("group_norm_act", y, mean, rstd)
     return (y, mean, rstd, ck) if ckpt else (y, mean, rstd)
 
 
@@ -410,9 +410,7 @@ def linear_act(x, w, bias=None, act="none", residual=None, save_pre=False, out=N
         _call(dev, _raw.favae_linear_act_fwd, xp, ldx, wp, ldw, bp, _ptr(residual),
               0 if residual is None else _rows(residual, "residual"), _ptr(pre), n, y.data_ptr(), ldy, m, n, k, a, _ptr(ws), nbytes, code)
     if cut:
-        if save_pre:
-            return _no_graph("linear_act", (y, pre), x, w, bias, residual)
-        return _no_graph("linear_act", (y,), x, w, bias, residual)[0]
+        return _no_graph("linear_act", y, pre) if save_pre else _no_graph("linear_act", y)[0]
     return (y, pre) if save_pre else y
 
 

@@ -1133,3 +1133,33 @@ def test_group_norm_scratch_with_a_checkpoint_and_with_odd_rows(N, S, C, G, dtyp
             assert (buf[n:] == 0xA5).all() and (q[N * S * C:] == 9).all() and (e[N * S * nb:] == 9).all()
         ref = B().ckpt8_pack(x.view(N * S, C))
         assert torch.equal(q[:N * S * C].view(N * S, C), ref.q) and torch.equal(e[:N * S * nb].view(N * S, nb), ref.e)
+
+
+def test_the_node_that_raises_keeps_no_parameter():
+    """An output that lives on holds no node of the caller's leaves: their gradients may be captured into a graph meanwhile."""
+    b = B()
+    g = gen(53)
+    x, w = rnd(g, 6, 32).requires_grad_(True), torch.nn.Parameter(rnd(g, 24, 32))
+    gamma, beta = torch.nn.Parameter(rnd(g, 32)), rnd(g, 32)
+    mine = [x, w, gamma]
+    for y in (b.linear_act(x, w), b.group_norm_act(x.view(1, 6, 32), 4, gamma, beta)[0]):
+        todo, seen = [y.grad_fn], 0
+        while todo:
+            node = todo.pop()
+            seen += 1
+            assert not any(getattr(node, "variable", None) is t for t in mine)
+            todo += [f for f, _ in node.next_functions if f is not None]
+        assert seen
+    # and the calls are captured in grad mode as they are under no_grad
+    want = b.linear_act(x.detach(), w.detach(), act="silu")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b.linear_act(x, w, act="silu")
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        y = b.linear_act(x, w, act="silu")
+    for _ in range(3):
+        y.detach().fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(y, want)
